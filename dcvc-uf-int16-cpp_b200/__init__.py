@@ -690,3 +690,7 @@ class StreamCodec:
         d = bytes(digest)
         return {"frames": frames.value, "packets": packets.value,
                 "sha256": [d[32 * b: 32 * b + 32].hex() for b in range(self.batch)]}
+
+
+# Latent attention: rotary positions, the 8-bit paged cache and attention over it.
+from .attention import KVCache, KVForkPlan, KVPlan, Rotary  # noqa: E402,F401

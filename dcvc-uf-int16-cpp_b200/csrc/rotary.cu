@@ -1,0 +1,215 @@
+// Rotary positions over several axes (ufb_rotary).
+//
+// A head's pair j = (a, b) belongs to one axis and turns by the angle of its
+// token's position there:  a' = a c - b s,  b' = a s + b c  (inverse: s -> -s).
+// (c, s) come from a table of float pairs, one row for each position of an
+// axis, computed once in 64 bits: large positions cost no accuracy and the
+// kernel no sine.
+//
+// Bound by HBM: every element is read once and written once.  A thread owns one
+// 16-byte column of a head (8 or 4 elements), reads that column's (c, s) once
+// and applies them to several heads of the same token, since the table bytes of
+// a column are four times its data in 16 bits.  In the half layout the partner
+// column lies n elements away and n need not be a multiple of the column: it is
+// read as the two aligned columns around it and shifted into place, so every
+// access stays 16 bytes wide whatever the pair counts are.
+#include "attention.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace ufb {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T>
+struct Column;  // 16 bytes of T as floats
+
+template <>
+struct Column<float> {
+    static constexpr int n = 4;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[4]) {
+        f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
+        f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
+        return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+};
+
+template <>
+struct Column<__half> {
+    static constexpr int n = 8;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            f[2 * i] = p.x, f[2 * i + 1] = p.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+template <>
+struct Column<__nv_bfloat16> {
+    static constexpr int n = 8;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&f)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// 16 bytes that start at byte `at` (a multiple of the element size, possibly
+// negative or past the row) of a row of `columns` aligned 16-byte columns;
+// bytes outside the row are undefined and never used by the caller.
+__device__ __forceinline__ uint4 window16(const uint4* row, int at, int columns) {
+    const int first = at >> 4, rest = at & 15;
+    const uint4 lo = row[min(max(first, 0), columns - 1)];
+    if (rest == 0) return lo;
+    const uint4 hi = row[min(max(first + 1, 0), columns - 1)];
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (rest & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (rest & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    if (rest & 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Thread = (token, group of `per` heads, column).
+template <typename T, int LAYOUT>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, int columns, int groups, int per,
+                                                          int* status) {
+    constexpr int N = Column<T>::n;
+    const long long id = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
+    const int col = static_cast<int>(id % columns);
+    const long long unit = id / columns;
+    const int group = static_cast<int>(unit % groups);
+    const long long token = unit / groups;
+    if (token >= a.tokens) return;
+
+    // this column's (cos, +-sin); sin's sign and the partner's side by element
+    float c[N], s[N];
+    const int e0 = col * N;
+    bool bad = false;
+    long long row[UFB_ROTARY_MAX_AXES];
+#pragma unroll
+    for (int ax = 0; ax < UFB_ROTARY_MAX_AXES; ++ax) {
+        row[ax] = 0;
+        if (ax < a.axes) {
+            const int p = a.positions[token * a.axes + ax];
+            bad |= p < 0 || p >= a.extent[ax];
+            row[ax] = a.base[ax] + static_cast<long long>(bad ? 0 : p) * (a.first[ax + 1] - a.first[ax]) - a.first[ax];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = e0 + i;
+        const int pair = LAYOUT == UFB_ROTARY_HALF ? (e < a.pairs ? e : e - a.pairs) : e >> 1;
+        const bool second = LAYOUT == UFB_ROTARY_HALF ? e >= a.pairs : (e & 1);
+        c[i] = 1.0f, s[i] = -0.0f;  // x * 1 + 0 * -0 is x, zeros of both signs included
+        if (pair < a.pairs) {
+            long long r = row[0];
+#pragma unroll
+            for (int ax = 1; ax < UFB_ROTARY_MAX_AXES; ++ax)
+                if (ax < a.axes && pair >= a.first[ax]) r = row[ax];
+            const float2 t = __ldg(a.table + r + pair);
+            c[i] = t.x;
+            s[i] = second != (a.inverse != 0) ? t.y : -t.y;
+        }
+        if (bad) c[i] = s[i] = __int_as_float(0x7fffffff);
+    }
+    if (bad && col == 0 && group == 0) atomicCAS(status, 0, kStatusPosition);
+
+    const int total = a.x[0].heads + (a.count > 1 ? a.x[1].heads : 0);
+    const int end = min(total, (group + 1) * per);
+    const bool plus = e0 < a.pairs, minus = e0 + N > a.pairs && e0 < 2 * a.pairs;
+#pragma unroll 4
+    for (int h = group * per; h < end; ++h) {
+        const int t = h >= a.x[0].heads;
+        const int head = t ? h - a.x[0].heads : h;
+        const uint4* in = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x[t].data) +
+                                                         token * a.x[t].token_stride + head * a.x[t].head_stride);
+        float x[N], y[N], r[N];
+        const uint4 own = in[col];
+        Column<T>::unpack(own, x);
+        if (LAYOUT == UFB_ROTARY_HALF) {
+            uint4 up = make_uint4(0, 0, 0, 0), down = make_uint4(0, 0, 0, 0);
+            const int shift = a.pairs * static_cast<int>(sizeof(T));
+            if (plus) up = window16(in, col * 16 + shift, columns);
+            if (minus) down = window16(in, col * 16 - shift, columns);
+            float u[N], d[N];
+            Column<T>::unpack(up, u);
+            Column<T>::unpack(down, d);
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = e0 + i < a.pairs ? u[i] : (e0 + i < 2 * a.pairs ? d[i] : 0.0f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = (e0 + i) >> 1 < a.pairs ? x[i ^ 1] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) r[i] = x[i] * c[i] + y[i] * s[i];
+        uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out[t].data) + token * a.out[t].token_stride +
+                                             head * a.out[t].head_stride);
+        to[col] = Column<T>::pack(r);
+    }
+}
+
+template <typename T>
+cudaError_t launch(const RotaryArgs& a, int* status, cudaStream_t s) {
+    const int columns = a.head_dim / Column<T>::n;
+    const int heads = a.x[0].heads + (a.count > 1 ? a.x[1].heads : 0);
+    // Several heads to a thread share its table values; with few tokens one head
+    // to a thread spreads the call over more SMs.
+    const long long threads = a.tokens * heads * columns;
+    const int per = threads >= 148ll * 2048 * 4 ? 4 : 1;
+    const int groups = (heads + per - 1) / per;
+    const long long blocks = (a.tokens * groups * columns + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+    if (a.layout == UFB_ROTARY_HALF)
+        rotary_kernel<T, UFB_ROTARY_HALF><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a, columns, groups, per, status);
+    else
+        rotary_kernel<T, UFB_ROTARY_INTERLEAVED><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a, columns, groups, per, status);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t rotary(const RotaryArgs& a, int dtype, int* status, cudaStream_t s) {
+    if (dtype == UFB_F32) return launch<float>(a, status, s);
+    if (dtype == UFB_F16) return launch<__half>(a, status, s);
+    return launch<__nv_bfloat16>(a, status, s);
+}
+
+}  // namespace ufb

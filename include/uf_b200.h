@@ -57,7 +57,8 @@ int ufb_set_conv_narrow(int enable);
 
 /* Synchronise `device` and return then clear its kernel status word:
  * 0 when no kernel reported a pipeline timeout since the last call, else the
- * first recorded code (1..4 = TMA producer / MMA / epilogue / drain wait). */
+ * first recorded code (1..4 = TMA producer / MMA / epilogue / drain wait; the
+ * attention operators below list theirs). */
 int ufb_device_status(int device);
 
 /* ---------------------------------------------------------------------------
@@ -425,6 +426,136 @@ int ufb_stream_decode(ufb_stream_codec* s, const uint8_t* const* data, const siz
 int ufb_conv2d_noalloc(const int16_t* x, int n, int ci, int h, int w, const int16_t* weight, int co, int kh, int kw,
                        const void* bias, int bias_bits, int stride_h, int stride_w, int pad_h, int pad_w, int groups,
                        int16_t* out, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Attention over latent tokens (no counterpart in the reference, whose models
+ * are convolutional): the operators that a context model needs beside the
+ * codec, when the latent tokens of a packet attend to those of earlier
+ * packets.  Rotary positions over several axes, a paged cache of keys and
+ * values held in 8 bits, attention over it, and the cache's pages.
+ *
+ * All pointers are device pointers unless said otherwise; every call is
+ * asynchronous on `stream`.  What only the device can see (a position, slot or
+ * page out of range, too few free pages) is checked by the kernels and recorded
+ * in the status word of ufb_device_status:
+ *   21 a position outside its axis (the token's heads become NaN)
+ *   31 too few free pages, or a stream longer than its table row (extend: no
+ *      stream was changed; fork: the destinations are left empty)
+ *   32 a slot, page or token offset out of range, or a page that is missing
+ *      where tokens are to be stored (what it names is skipped)
+ *   41..44 a bounded wait of the attention kernel gave up
+ * ------------------------------------------------------------------------- */
+
+#define UFB_F32 0
+#define UFB_F16 1
+#define UFB_BF16 2
+
+/* A tensor [tokens, heads, head_dim] whose head_dim elements are contiguous;
+ * strides in elements.  Data and strides are multiples of 16 bytes. */
+typedef struct ufb_heads {
+    void* data;
+    int64_t token_stride, head_stride;
+    int32_t heads;
+} ufb_heads;
+
+#define UFB_ROTARY_MAX_AXES 4
+#define UFB_ROTARY_HALF 0        /* pair j of a head is (x[j], x[j + n]), n = sum of pairs */
+#define UFB_ROTARY_INTERLEAVED 1 /* pair j is (x[2 j], x[2 j + 1]) */
+
+/* cos / sin of every axis, position and pair, written to HOST memory: axis a
+ * holds extents[a] rows of pairs[a] (cos, sin) float pairs, the axes one after
+ * another; pair i of axis a turns by position * bases[a]^(-i / pairs[a]),
+ * computed in 64 bits and rounded once.  Returns the number of floats (table
+ * may be NULL to query it) or a UFB_E* code. */
+int64_t ufb_rotary_table(int axes, const int32_t* pairs, const int32_t* extents, const double* bases, float* table);
+
+/* Rotary positions: every head of count (1..2) tensors x -> out, in one launch.
+ * The head's first sum(pairs) pairs turn by its token's positions
+ * ([tokens, axes] int32), axis after axis; elements past them are copied.
+ * inverse turns back, which is the gradient with respect to x.  Products and
+ * sums in 32 bits.  dtype UFB_F32, UFB_F16 or UFB_BF16; head_dim a multiple of
+ * 16 up to 256.  out must not overlap x. */
+int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t* extents, int layout, int inverse,
+               const int32_t* positions, int64_t tokens, int head_dim, int dtype, int count, const ufb_heads* x,
+               const ufb_heads* out, void* stream);
+
+/* A cache of keys and values for `slots` streams and `layers` layers, in caller-
+ * owned device memory.  A page holds page_tokens tokens of one stream; stream s
+ * keeps its token t on page table[s][t / page_tokens] (-1: no page), the same
+ * page id in every layer.  Key and value of token slot i are
+ * kv[layer][page][side][head][i][:] * scale[layer][page][side][head], side 0 the
+ * key, 1 the value.  refs counts the table entries of each page (0: free).
+ * A page that its stream has not filled is never shared.
+ * page_tokens 16, 32, 64 or 128; head_dim 64 or 128; kv 128-byte aligned. */
+typedef struct ufb_kv_cache {
+    int8_t* kv;       /* [layers][pages][2][heads][page_tokens][head_dim] */
+    float* scale;     /* [layers][pages][2][heads] */
+    int32_t* table;   /* [slots][table_width] */
+    int32_t* lengths; /* [slots] tokens of each stream */
+    int32_t* refs;    /* [pages] */
+    int32_t* work;    /* [ufb_kv_work_ints()] scratch of the page operators */
+    int32_t layers, pages, heads, page_tokens, head_dim, slots, table_width;
+} ufb_kv_cache;
+
+/* int32 entries of ufb_kv_cache.work. */
+int64_t ufb_kv_work_ints(int32_t pages, int32_t slots);
+
+/* Make room: stream slots[i] grows by offsets[i + 1] - offsets[i] tokens
+ * (lengths) and gets the pages for them, lowest free page first, in the order
+ * of the list.  No slot twice. */
+int ufb_kv_extend(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, void* stream);
+
+/* Drop every page of the listed streams; their lengths become 0. */
+int ufb_kv_release(const ufb_kv_cache* c, const int32_t* slots, int n, void* stream);
+
+/* Stream dst[i] becomes a branch of stream src[i] (what it held is released
+ * first): full pages are shared, the tokens of a partly filled last page are
+ * copied, in every layer, to a page of its own (lowest free page first, in the
+ * order of the list).  No dst twice, no dst among src. */
+int ufb_kv_fork(const ufb_kv_cache* c, const int32_t* src, const int32_t* dst, int n, void* stream);
+
+/* Drop the pages of the listed streams that no later query sees through a
+ * window (ufb_kv_attend) of `window` >= 1 keys and `sinks` first tokens. */
+int ufb_kv_trim(const ufb_kv_cache* c, const int32_t* slots, int n, int window, int sinks, void* stream);
+
+/* Move the live pages to the lowest ids: the k-th live page whose id is not
+ * below the number of live pages goes to the k-th free page below it; tables
+ * and refs follow, other pages stay where they are. */
+int ufb_kv_compact(const ufb_kv_cache* c, void* stream);
+
+/* Store new keys and values (dtype UFB_F32, UFB_F16 or UFB_BF16) as the last
+ * offsets[i + 1] - offsets[i] tokens of stream slots[i] (ufb_kv_extend has made
+ * room).  k and v are [tokens, heads, head_dim], stream after stream; max_new is
+ * no less than any stream's count.  For each page, head and side:
+ *   s' = max(s, max |x| * (1 / 127))  (s counts when the page holds earlier tokens)
+ *   earlier q = rint(q * (s / s')),  new q = min(max(rint(x / s'), -127), 127)
+ * in 32 bits.  Values that are not finite stay out of s': infinities are stored
+ * as -127 or 127, NaN as 0. */
+int ufb_kv_append(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
+                  int64_t tokens, int dtype, const ufb_heads* k, const ufb_heads* v, void* stream);
+
+/* The values that n listed pages stand for: out [n][2][heads][page_tokens][head_dim]. */
+int ufb_kv_read(const ufb_kv_cache* c, int layer, const int32_t* pages, int64_t n, int dtype, void* out, void* stream);
+
+/* Attention of the newest tokens over the cache.  Query i of stream slots[b]
+ * (n_b = offsets[b + 1] - offsets[b] queries, L = lengths[slots[b]] keys) stands
+ * at a = L - n_b + i and sees key j when j <= (causal ? a : L - 1), when
+ * window == 0 or j > a - window or j < sinks, and when j's page is present:
+ *   out = sum_j p_j v_j,  p = softmax over the seen keys of scale * q . k_j
+ * Query head h reads key head h / (q heads / cache heads).  A query that sees no
+ * key gives zeros (lse -inf).  q and out [tokens, q heads, head_dim] of dtype
+ * UFB_F16 or UFB_BF16; lse (NULL, or [tokens][q heads] float) receives
+ * ln sum_j exp(scale * q . k_j).  max_new is no less than any stream's count.
+ * Statistics and sums in 32 bits; p and q enter the tensor cores with 11
+ * significant bits (q exactly, see the kernel).
+ * workspace: ufb_kv_attend_workspace() bytes, zero before its first use; calls
+ * that may overlap need one each. */
+int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
+                  int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse, int window,
+                  int sinks, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Workspace of ufb_kv_attend on the current device, in bytes. */
+int64_t ufb_kv_attend_workspace(void);
 
 /* Measurement utility (no reference counterpart): launches `ctas` CTAs that
  * each issue `iters` x 4 dense tcgen05 kind::i8 M=128 N=256 K=32 MMAs from
