@@ -1,11 +1,7 @@
-// Attention over the 8-bit cache (ufb_kv_attend): one warp to a query and head,
-// a running maximum and sum over the keys it sees.
-#include "attention.h"
+// Attention over the 8-bit cache (ufb_kv_attend): the choice of a kernel and its scratch.
+#include "kv_attend.cuh"
 
-#include "capi_util.h"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include <mutex>
 
 namespace ufb {
 
@@ -82,9 +78,44 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-int64_t kv_attend_workspace_bytes(int) { return 256; }
+int64_t kv_attend_workspace_bytes(int sms) {
+    const int ctas = sms < kAttendMaxCtas ? sms : kAttendMaxCtas;
+    const AttendScratch s = scratch_of(nullptr, ctas, kAttendManyRows);
+    return reinterpret_cast<int64_t>(s.sums) + 2ll * ctas * kAttendManyRows * 128 * 4;
+}
+
+bool kv_tensor_map(CUtensorMap& map, const AttendArgs& a, int keys) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode encode = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            encode = reinterpret_cast<Encode>(p);
+    });
+    if (!encode) return false;
+    const cuuint64_t rows = static_cast<cuuint64_t>(a.pages) * 2 * a.heads * a.page_tokens * a.head_dim / 128;
+    if (rows > 0x7fffffffull) return false;
+    const cuuint64_t dims[2] = {128, rows};
+    const cuuint64_t strides[1] = {128};
+    const cuuint32_t box[2] = {128, static_cast<cuuint32_t>((a.page_tokens < keys ? a.page_tokens : keys) * a.head_dim / 128)};
+    const cuuint32_t elem[2] = {1, 1};
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(a.kv), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 cudaError_t kv_attend(const AttendArgs& a, int dtype, cudaStream_t s) {
+    int device = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return e;
+    const long long rows = static_cast<long long>(a.max_new) * a.group;
+    if (rows <= 16) return attend_few(a, dtype, sms, s);
     return dtype == UFB_F16 ? launch<__half>(a, s) : launch<__nv_bfloat16>(a, s);
 }
 
