@@ -13,14 +13,18 @@ import ctypes as C
 
 import torch
 
-from . import UfbError, _check, _stream, library
+from . import UfbError, _check, library
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_QUERY_DTYPES = {torch.float16: 1, torch.bfloat16: 2}
 _LAYOUTS = {"half": 0, "interleaved": 1}
 
 
 class _Heads(C.Structure):
     _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("heads", C.c_int32)]
+
+
+_Pair = _Heads * 2
 
 
 class _Cache(C.Structure):
@@ -59,21 +63,50 @@ def _device(device) -> torch.device:
     return torch.device("cuda", torch.cuda.current_device()) if d.index is None else d
 
 
+# A decoding step makes these calls for every layer and its kernels take a few
+# microseconds, so the wrappers below keep to few and cheap host operations.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(device, fn, *args):
+    """fn(*args, current stream of the device), with that device current."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _check(rc)
+
+
+def _refuse_heads(device, what, dtypes):
+    names = ", ".join(str(d).replace("torch.", "") for d in dtypes)
+    raise UfbError(-1, f"{what}: [tokens, heads, head_dim] tensor of {names} on {device} required")
+
+
 def _head_tensor(t, device, what: str, dtypes=_DTYPES):
-    """[tokens, heads, dim] on the device, rows of 16-byte multiples (copied if not)."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.device == device and t.dtype in dtypes and t.dim() == 3):
-        names = ", ".join(str(d).replace("torch.", "") for d in dtypes)
-        raise UfbError(-1, f"{what}: [tokens, heads, head_dim] tensor of {names} on {device} required")
-    lanes = 16 // t.element_size()
-    tokens, heads, dim = t.shape
+    """[tokens, heads, dim] on the device, rows of 16-byte multiples (copied if
+    not): the tensor, its shape, dtype code and description."""
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        _refuse_heads(device, what, dtypes)
+    shape, code = t.shape, dtypes.get(t.dtype)
+    if code is None or len(shape) != 3:
+        _refuse_heads(device, what, dtypes)
+    tokens, heads, dim = shape
+    ts, hs, es = t.stride()
+    lanes = 4 if code == 0 else 8
     # a stride over one element or none is free: any value does
-    ts = t.stride(0) if tokens > 1 else heads * dim
-    hs = t.stride(1) if heads > 1 else dim
-    if t.stride(2) != 1 or ts % lanes or hs % lanes or t.data_ptr() % 16 or (heads > 1 and hs < dim) or \
-            (tokens > 1 and ts < dim):
-        t = t.contiguous() if not t.is_contiguous() else t.clone()
-        ts, hs = heads * dim, dim
-    return t, _Heads(t.data_ptr(), ts, hs, heads)
+    if tokens <= 1:
+        ts = heads * dim
+    if heads <= 1:
+        hs = dim
+    at = t.data_ptr()
+    if es != 1 or ts % lanes or hs % lanes or at % 16 or (heads > 1 and hs < dim) or (tokens > 1 and ts < dim):
+        t = t.clone(memory_format=torch.contiguous_format)
+        ts, hs, at = heads * dim, dim, t.data_ptr()
+    return t, shape, code, _Heads(at, ts, hs, heads)
 
 
 class Rotary:
@@ -105,6 +138,7 @@ class Rotary:
         host = torch.empty(n, dtype=torch.float32)
         L.ufb_rotary_table(len(pairs), self._pairs, self._extents, b, host.data_ptr())
         self.table = host.to(self.device)
+        self._fn, self._table, self._layout = L.ufb_rotary, self.table.data_ptr(), _LAYOUTS[layout]
 
     def apply(self, positions, q, k=None, inverse=False):
         """Turn q (and k in the same launch) by the tokens' positions
@@ -114,25 +148,27 @@ class Rotary:
         if not (isinstance(positions, torch.Tensor) and positions.device == self.device and
                 positions.dtype == torch.int32 and positions.dim() == 2 and positions.shape[1] == axes):
             raise UfbError(-1, f"positions: int32 tensor [tokens, {axes}] on {self.device} required")
-        positions = positions.contiguous()
-        xs = [q] if k is None else [q, k]
-        ins, outs, keep = [], [], []
-        for x in xs:
-            x, h = _head_tensor(x, self.device, "rotary input")
-            if x.shape[0] != positions.shape[0] or x.shape[2] != xs[0].shape[2] or x.dtype != xs[0].dtype:
-                raise UfbError(-1, "rotary inputs and positions differ in tokens, head_dim or dtype")
-            out = torch.empty(x.shape, dtype=x.dtype, device=self.device)
-            keep.append((x, out))
-            ins.append(h)
-            outs.append(_Heads(out.data_ptr(), x.shape[1] * x.shape[2], x.shape[2], x.shape[1]))
-        if positions.shape[0] and min(x.shape[1] for x in xs) > 0:
-            n = len(xs)
-            with torch.cuda.device(self.device):
-                _check(_lib().ufb_rotary(self.table.data_ptr(), axes, self._pairs, self._extents,
-                                         _LAYOUTS[self.layout], int(bool(inverse)), positions.data_ptr(),
-                                         positions.shape[0], xs[0].shape[2], _DTYPES[xs[0].dtype], n,
-                                         (_Heads * n)(*ins), (_Heads * n)(*outs), _stream(self.table)))
-        return keep[0][1] if k is None else (keep[0][1], keep[1][1])
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        tokens = positions.shape[0]
+        q, qs, code, qh = _head_tensor(q, self.device, "rotary input")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        oh = _Heads(out.data_ptr(), qs[1] * qs[2], qs[2], qs[1])
+        if qs[0] != tokens:
+            raise UfbError(-1, "rotary inputs and positions differ in tokens")
+        if k is None:
+            n, out2, x, y, most = 1, None, C.byref(qh), C.byref(oh), qs[1]
+        else:
+            k, ks, kcode, kh = _head_tensor(k, self.device, "rotary input")
+            if ks[0] != tokens or ks[2] != qs[2] or kcode != code:
+                raise UfbError(-1, "rotary inputs differ in tokens, head_dim or dtype")
+            out2 = torch.empty_like(k, memory_format=torch.contiguous_format)
+            n, most = 2, min(qs[1], ks[1])
+            x, y = _Pair(qh, kh), _Pair(oh, _Heads(out2.data_ptr(), ks[1] * ks[2], ks[2], ks[1]))
+        if tokens and most:
+            _launch(self.device, self._fn, self._table, axes, self._pairs, self._extents, self._layout,
+                    1 if inverse else 0, positions.data_ptr(), tokens, qs[2], code, n, x, y)
+        return out if k is None else (out, out2)
 
 
 class KVPlan:
@@ -157,6 +193,7 @@ class KVPlan:
             offsets.append(offsets[-1] + c)
         ints = torch.tensor(slots + offsets, dtype=torch.int32).to(cache.device)
         self.slots, self.offsets = ints[:self.n], ints[self.n:]
+        self._slots, self._offsets = self.slots.data_ptr(), self.offsets.data_ptr()
 
 
 class KVForkPlan:
@@ -173,6 +210,7 @@ class KVForkPlan:
         self.cache, self.n = cache, len(src)
         ints = torch.tensor(src + dst, dtype=torch.int32).to(cache.device)
         self.src, self.dst = ints[:self.n], ints[self.n:]
+        self._src, self._dst = self.src.data_ptr(), self.dst.data_ptr()
 
 
 class KVCache:
@@ -210,7 +248,8 @@ class KVCache:
         self.table = torch.full((self.slots, self.table_width), -1, dtype=torch.int32, device=d)
         self.lengths = torch.zeros(self.slots, dtype=torch.int32, device=d)
         self.refs = torch.zeros(self.pages, dtype=torch.int32, device=d)
-        n = _lib().ufb_kv_work_ints(self.pages, self.slots)
+        L = self._L = _lib()
+        n = L.ufb_kv_work_ints(self.pages, self.slots)
         if n < 0:
             _check(int(n))
         self._work = torch.zeros(n, dtype=torch.int32, device=d)
@@ -218,6 +257,8 @@ class KVCache:
                                                        self._work)],
                               self.layers, self.pages, self.heads, self.page_tokens, self.head_dim, self.slots,
                               self.table_width)
+        self._ref = C.byref(self._struct)
+        self._default_scale = self.head_dim ** -0.5
         self._workspaces = {}
 
     # -- streams and their pages
@@ -235,46 +276,41 @@ class KVCache:
             raise UfbError(-1, f"a {kind.__name__} of this cache is required")
         return plan
 
-    def _call(self, name, *args):
-        with torch.cuda.device(self.device):
-            _check(getattr(_lib(), name)(C.byref(self._struct), *args, _stream(self.kv)))
-
     def extend(self, plan):
         """Grow the plan's streams by its counts and give them the pages for it."""
         self._own(plan)
-        self._call("ufb_kv_extend", plan.slots.data_ptr(), plan.offsets.data_ptr(), plan.n)
+        _launch(self.device, self._L.ufb_kv_extend, self._ref, plan._slots, plan._offsets, plan.n)
 
     def release(self, plan):
         """Drop the pages of the plan's streams; their lengths become 0."""
         self._own(plan)
-        self._call("ufb_kv_release", plan.slots.data_ptr(), plan.n)
+        _launch(self.device, self._L.ufb_kv_release, self._ref, plan._slots, plan.n)
 
     def trim(self, plan, window, sinks=0):
         """Drop the pages that no later query of the plan's streams sees."""
         self._own(plan)
-        self._call("ufb_kv_trim", plan.slots.data_ptr(), plan.n, int(window), int(sinks))
+        _launch(self.device, self._L.ufb_kv_trim, self._ref, plan._slots, plan.n, int(window), int(sinks))
 
     def fork(self, plan):
         """Make the plan's destinations branches of its sources."""
         self._own(plan, KVForkPlan)
-        self._call("ufb_kv_fork", plan.src.data_ptr(), plan.dst.data_ptr(), plan.n)
+        _launch(self.device, self._L.ufb_kv_fork, self._ref, plan._src, plan._dst, plan.n)
 
     def compact(self):
         """Move the live pages to the lowest ids."""
-        self._call("ufb_kv_compact")
+        _launch(self.device, self._L.ufb_kv_compact, self._ref)
 
     # -- contents
 
     def append(self, layer, plan, k, v):
         """Store k and v [tokens, heads, head_dim] as the newest tokens of the plan's streams."""
         self._own(plan)
-        shape = (plan.tokens, self.heads, self.head_dim)
-        k, kh = _head_tensor(k, self.device, "keys")
-        v, vh = _head_tensor(v, self.device, "values")
-        if k.shape != shape or v.shape != shape or k.dtype != v.dtype:
-            raise UfbError(-1, f"keys and values must be {list(shape)} of one dtype")
-        self._call("ufb_kv_append", int(layer), plan.slots.data_ptr(), plan.offsets.data_ptr(), plan.n, plan.max_new,
-                   plan.tokens, _DTYPES[k.dtype], C.byref(kh), C.byref(vh))
+        k, ks, code, kh = _head_tensor(k, self.device, "keys")
+        v, vs, vcode, vh = _head_tensor(v, self.device, "values")
+        if ks != vs or ks != (plan.tokens, self.heads, self.head_dim) or code != vcode:
+            raise UfbError(-1, f"keys and values must be {[plan.tokens, self.heads, self.head_dim]} of one dtype")
+        _launch(self.device, self._L.ufb_kv_append, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new,
+                plan.tokens, code, C.byref(kh), C.byref(vh))
 
     def read(self, layer, pages, dtype=torch.float32):
         """The values of listed pages (int32 tensor): [n, 2, heads, page_tokens, head_dim]."""
@@ -283,22 +319,25 @@ class KVCache:
             raise UfbError(-1, f"pages: int32 list on {self.device} required")
         if dtype not in _DTYPES:
             raise UfbError(-1, "unsupported dtype")
-        pages = pages.contiguous()
-        out = torch.empty((pages.numel(), 2, self.heads, self.page_tokens, self.head_dim), dtype=dtype,
-                          device=self.device)
-        self._call("ufb_kv_read", int(layer), pages.data_ptr(), pages.numel(), _DTYPES[dtype], out.data_ptr())
+        if not pages.is_contiguous():
+            pages = pages.contiguous()
+        n = pages.shape[0]
+        out = torch.empty((n, 2, self.heads, self.page_tokens, self.head_dim), dtype=dtype, device=self.device)
+        _launch(self.device, self._L.ufb_kv_read, self._ref, layer, pages.data_ptr(), n, _DTYPES[dtype],
+                out.data_ptr())
         return out
 
     def _workspace(self):
         # zeroed once and left zeroed by every call; streams may overlap, so each has its own
-        key = torch.cuda.current_stream(self.device).cuda_stream
+        key = _raw_stream(self.device.index)
         w = self._workspaces.get(key)
         if w is None:
             with torch.cuda.device(self.device):
-                n = _lib().ufb_kv_attend_workspace()
+                n = self._L.ufb_kv_attend_workspace()
             if n < 0:
                 _check(int(n))
-            w = self._workspaces[key] = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            t = torch.zeros(n, dtype=torch.uint8, device=self.device)
+            w = self._workspaces[key] = (t.data_ptr(), n, t)
         return w
 
     def attend(self, layer, plan, q, window=0, sinks=0, causal=True, scale=None, lse=False):
@@ -309,15 +348,15 @@ class KVCache:
         sees nothing gives zeros.  Returns out, or (out, lse [tokens, query
         heads] float32)."""
         self._own(plan)
-        q, qh = _head_tensor(q, self.device, "queries", (torch.float16, torch.bfloat16))
-        if q.shape[0] != plan.tokens or q.shape[2] != self.head_dim or q.shape[1] == 0 or q.shape[1] % self.heads:
+        q, qs, code, qh = _head_tensor(q, self.device, "queries", _QUERY_DTYPES)
+        tokens, heads, dim = qs
+        if tokens != plan.tokens or dim != self.head_dim or heads == 0 or heads % self.heads:
             raise UfbError(-1, f"queries must be [{plan.tokens}, a multiple of {self.heads}, {self.head_dim}]")
-        out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        oh = _Heads(out.data_ptr(), q.shape[1] * q.shape[2], q.shape[2], q.shape[1])
-        l = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if lse else None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        oh = _Heads(out.data_ptr(), heads * dim, dim, heads)
+        l = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if lse else None
         w = self._workspace()
-        self._call("ufb_kv_attend", int(layer), plan.slots.data_ptr(), plan.offsets.data_ptr(), plan.n, plan.max_new,
-                   plan.tokens, _DTYPES[q.dtype], C.byref(qh), C.byref(oh), None if l is None else l.data_ptr(),
-                   int(window), int(sinks), int(bool(causal)),
-                   float(self.head_dim ** -0.5 if scale is None else scale), w.data_ptr(), w.numel())
+        _launch(self.device, self._L.ufb_kv_attend, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new,
+                tokens, code, C.byref(qh), C.byref(oh), None if l is None else l.data_ptr(), window, sinks,
+                1 if causal else 0, self._default_scale if scale is None else scale, w[0], w[1])
         return (out, l) if lse else out

@@ -69,7 +69,7 @@ struct AttendArgs {
     int* status;
     void* workspace;
 };
-cudaError_t kv_attend(const AttendArgs& a, int dtype, cudaStream_t s);
+cudaError_t kv_attend(const AttendArgs& a, int dtype, int sms, cudaStream_t s);
 int64_t kv_attend_workspace_bytes(int sms);
 
 }  // namespace ufb

@@ -46,6 +46,15 @@ bool overlap(const ufb_heads& a, const ufb_heads& b, int64_t tokens, int head_di
     return x < y + span_bytes(b, tokens, head_dim, dtype) && y < x + span_bytes(a, tokens, head_dim, dtype);
 }
 
+// SMs of the current device; 0 with the error recorded.
+int attend_sms() {
+    int device = 0, sms = 0;
+    if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice") ||
+        !cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device attribute"))
+        return 0;
+    return sms;
+}
+
 bool check_cache(const ufb_kv_cache* c) {
     if (!c || !c->kv || !c->scale || !c->table || !c->lengths || !c->refs || !c->work)
         return fail(UFB_EINVAL, "cache tensors must be non-null");
@@ -237,11 +246,8 @@ int ufb_kv_read(const ufb_kv_cache* c, int layer, const int32_t* pages, int64_t 
 
 int64_t ufb_kv_attend_workspace(void) {
     clear_error();
-    int device = 0, sms = 0;
-    if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice") ||
-        !cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device attribute"))
-        return last_code();
-    return kv_attend_workspace_bytes(sms);
+    const int sms = attend_sms();
+    return sms > 0 ? kv_attend_workspace_bytes(sms) : last_code();
 }
 
 int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
@@ -258,8 +264,9 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
         return last_code();
     if (q->heads % c->heads) return err(UFB_EINVAL, "query heads must be a multiple of the cache's heads");
     if (q->heads / c->heads > 128) return err(UFB_ERANGE, "more than 128 query heads to a key head");
-    const int64_t need = ufb_kv_attend_workspace();
-    if (need < 0) return last_code();
+    const int sms = attend_sms();
+    if (sms <= 0) return last_code();
+    const int64_t need = kv_attend_workspace_bytes(sms);
     if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)
         return err(UFB_EINVAL, "attention needs " + std::to_string(need) + " bytes of 256-byte aligned workspace");
     int* status = current_status();
@@ -292,7 +299,7 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
     a.lse = lse;
     a.status = status;
     a.workspace = workspace;
-    return done(kv_attend(a, dtype, static_cast<cudaStream_t>(stream)), "kv attend");
+    return done(kv_attend(a, dtype, sms, static_cast<cudaStream_t>(stream)), "kv attend");
 }
 
 }  // extern "C"

@@ -109,11 +109,7 @@ bool kv_tensor_map(CUtensorMap& map, const AttendArgs& a, int keys) {
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-cudaError_t kv_attend(const AttendArgs& a, int dtype, cudaStream_t s) {
-    int device = 0, sms = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    if (e != cudaSuccess) return e;
+cudaError_t kv_attend(const AttendArgs& a, int dtype, int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(a.max_new) * a.group;
     if (rows <= 16) return attend_few(a, dtype, sms, s);
     return dtype == UFB_F16 ? launch<__half>(a, s) : launch<__nv_bfloat16>(a, s);
