@@ -4,8 +4,8 @@
 //   S = Q K^T,  P = 2^(S f + log2 vs - M),  O = P V,  l = sum P / vs
 //
 // with f the page's key scale times the softmax scale times log2 e and vs its
-// value scale.  Folding log2 vs into the running maximum M keeps P at most 1
-// whatever the pages' scales are, so it can be rounded to float16 for the second
+// value scale.  Folding log2 vs into the running maximum M bounds P whatever the
+// pages' scales are, so it can be rounded to float16 for the second
 // product; l divides it out again, in 32 bits.  out = O / l.
 //
 // Bound by the bytes of the cache.  Work is divided by tiles of 64 keys
@@ -37,6 +37,9 @@ constexpr int kWarps = 8;             // consumer warps
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kStages = 8;
 constexpr int kGroups = kKeys / kGroupKeys;
+// P is taken times 2^kShift: at most 2^15, inside float16, and weights down to
+// 2^-29 of the largest keep all 11 bits.
+constexpr float kShift = 15.0f;
 constexpr int kCodeFull = 41, kCodeEmpty = 42, kCodeDrain = 43;
 
 struct PageScales {
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[h][e] = hidden[h][e] ? 0.0f : ex2(s[h][e] - m[e >> 1]);
+                    s[h][e] = hidden[h][e] ? 0.0f : ex2(s[h][e] - (m[e >> 1] - kShift));
                     if (!hidden[h][e]) sum[e >> 1] += s[h][e];
                 }
             if (sum[0] != 0.0f) l[0] = fmaf(sum[0], sc.inv_value, l[0]);
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
             *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
             if (a.lse && d == 0)
                 a.lse[(p.t.token0 + token) * (a.heads * a.group) + head] =
-                    weight == 0.0f ? -INFINITY : (top + log2f(weight)) * 0.6931471805599453f;
+                    weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
         };
         for (int e = threadIdx.x; e < p.t.rows * (D / 4); e += kWarps * 32) {
             const int row = e / (D / 4), d = e % (D / 4) * 4;

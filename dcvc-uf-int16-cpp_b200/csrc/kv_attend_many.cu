@@ -1,0 +1,535 @@
+// Attention over the 8-bit cache for many rows (more new tokens x query heads of a
+// key head than kv_attend_few.cu takes): frames, pieces of streams.
+//
+//   S = Q K^T,  P = 2^(S f + log2 vs - M),  O = P V,  l = sum P / vs,  out = O / l
+//
+// as there, in tiles of 256 rows x 128 keys on the fifth-generation tensor cores:
+// the rows of all query heads of a key head lie in one tile, so the integers of a
+// key tile are expanded to float16 once for 256 rows.
+//
+// One CTA an SM, four roles:
+//   converter (4 warps)  integers from global memory through registers to float16
+//                        in shared memory, keys and values double buffered, with
+//                        128-byte swizzle; the page scales of each 16 keys
+//   MMA (1 thread)       S_t = Q_t K^T and O_t += P_t V for the two halves t of
+//                        128 rows, in the order O_0 S_0 O_1 S_1, so that one half
+//                        multiplies while the other is in its softmax
+//   softmax (2 x 4 warps) a thread owns a row: S from tensor memory, P back to it
+//                        in float16 over S, where it is the A operand of P V
+// Tensor memory: S_0, S_1 (128 columns each), O_0, O_1.
+//
+// The exponentials bound it at head_dim 128: 16 an SM and cycle make 2048 cycles a
+// tile, as many as its products take.  A running maximum that grows little is
+// kept, so O is rescaled rarely and by the softmax threads themselves.
+//
+// The key tiles of all items are divided equally over the CTAs (kv_attend.cuh);
+// rows shared by CTAs are joined by a second launch.
+#include "kv_attend.cuh"
+#include "umma.cuh"
+
+#include <mutex>
+
+namespace ufb {
+
+namespace {
+
+constexpr int kRows = kAttendManyRows;
+constexpr int kHalf = 128;
+constexpr int kKeys = 128;
+constexpr int kGroups = kKeys / kGroupKeys;
+constexpr int kThreads = 512;         // softmax 0-7, converter 8-11, MMA 12; 13-15 idle
+constexpr int kScaleRing = 4;
+constexpr int kCode = 44;
+// A running maximum stays while it grows by less than 2^kSlack, and P is taken
+// times 2^kShift: it reaches 2^15 at most, inside float16, and weights down to
+// 2^-27 of the largest keep all 11 bits.
+constexpr float kSlack = 2.0f, kShift = 13.0f;
+
+struct alignas(16) GroupScales {
+    float key, log2_value, inv_value, pad;
+};
+
+template <int D>
+struct Smem {
+    alignas(1024) uint8_t q[2][kHalf * D * 2];     // [64 dims][row][128 bytes]
+    alignas(1024) uint8_t k[2][kKeys * D * 2];
+    alignas(1024) uint8_t v[2][kKeys * D * 2];
+    GroupScales scales[kScaleRing][kGroups];
+    alignas(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    ShareSmem share;
+    uint32_t tmem;
+    int dead;
+};
+
+template <int D>
+struct Tmem {
+    __device__ static constexpr uint32_t s(int t) { return t * 128; }
+    __device__ static constexpr uint32_t o(int t) { return 256 + t * D; }
+};
+
+// Address of row `row`, 16-byte chunk `chunk` (8 float16) of a [D / 64][128][128 bytes] tile.
+__device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
+    return (chunk >> 3) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, int row_tiles, int min_share) {
+    extern __shared__ uint8_t raw[];
+    Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.k_full[i], 128);
+            mbar_init(&sm.v_full[i], 128);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_empty[i], 1);
+            mbar_init(&sm.q_full[i], 128);
+            mbar_init(&sm.p_full[i], 128);
+            mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.o_full[i], 1);
+        }
+        mbar_init(&sm.drained, 1);
+        fence_mbar_init();
+        sm.dead = 0;
+    }
+    if (warp == 12) {
+        tmem_alloc(&sm.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    const Share share = locate_share<kKeys, kRows, kThreads>(a, row_tiles, min_share, sm.share);
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    Walker<kKeys, kRows> walk(a, share, row_tiles);
+    volatile int* dead = &sm.dead;
+    // after a wait gave up nobody waits any more: the loops run out on what is there
+    auto wait = [&](uint64_t* bar, int phase) {
+        if (!*dead && !mbar_wait(bar, phase & 1, a.status, kCode)) *dead = 1;
+    };
+    const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
+
+    if (warp < 8) {
+        // ---- softmax: half t, row of the half = thread
+        const int t = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + Tmem<D>::s(t), to = tmem + lanes + Tmem<D>::o(t);
+        int tiles = 0, s_n = 0, o_n = 0;   // key tiles of this CTA so far; phases of this half
+        Piece p;
+        if (t == 0 && row == 0) scratch.items[blockIdx.x * 8] = 0;
+        while (walk.next(a, p)) {
+            if (t * kHalf >= p.t.rows) {
+                tiles += p.end - p.first;
+                continue;
+            }
+            const int r = t * kHalf + row;
+            const bool real = r < p.t.rows;
+            const int in_stream = p.t.row0 + (real ? r : 0);
+            const int token = in_stream / a.group, head = p.head * a.group + in_stream - token * a.group;
+            const int pos = p.t.length - p.t.n_new + token;
+            float unit;
+            {
+                // the row to [1/2, 1) and float16; the softmax scale's sign goes with it
+                const T* src = static_cast<const T*>(a.q.data) + (p.t.token0 + token) * a.q.token_stride +
+                               head * a.q.head_stride;
+                float top = 0.0f;
+                uint4 w[D / 8];
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    w[i] = make_uint4(0, 0, 0, 0);
+                    if (real) w[i] = reinterpret_cast<const uint4*>(src)[i];
+                }
+                float odd = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = unpack2(x[j], T());
+                        top = max3(top, fabsf(f.x), fabsf(f.y));
+                        odd += (f.x - f.x) + (f.y - f.y);  // NaN for what is not finite
+                    }
+                }
+                const float u = row_unit(odd == odd ? top : odd);
+                unit = unit_inverse(u) * fabsf(a.scale_log2);
+                const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                    uint32_t y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = unpack2(x[j], T());
+                        y[j] = pack2(f.x * mul, f.y * mul, __half());
+                    }
+                    *reinterpret_cast<uint4*>(sm.q[t] + tile_at(row, i)) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&sm.q_full[t]);
+            }
+            float m = -INFINITY, l = 0.0f;
+            const int first_pos = p.t.length - p.t.n_new + (p.t.row0 + t * kHalf) / a.group;
+            const int last_pos = p.t.length - p.t.n_new + (p.t.row0 + min(p.t.rows, (t + 1) * kHalf) - 1) / a.group;
+            for (int tile = p.first; tile < p.end; ++tile, ++tiles) {
+                wait(&sm.s_full[t], s_n++);
+                __syncwarp();
+                tc_fence_after();
+                const GroupScales* sc = sm.scales[tiles % kScaleRing];
+                const int key0 = p.t.keys.tile(tile) * kKeys;
+                const bool clear = (!a.causal || key0 + kKeys - 1 <= first_pos) && key0 + kKeys <= p.t.length &&
+                                   (!a.window || last_pos - key0 < a.window || key0 + kKeys <= a.sinks);
+                // columns [low_col, high_col] and [0, sink_col) are seen by this row
+                const int high_col = min(p.t.length - 1, a.causal ? pos : p.t.length - 1) - key0;
+                const int low_col = a.window ? max(pos - a.window + 1, 0) - key0 : 0;
+                const int sink_col = a.window ? a.sinks - key0 : 0;
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[32];
+                    tmem_ld32(ts + c * 32, s);
+                    tmem_wait_ld();
+                    if (!clear) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int col = c * 32 + j;
+                            if (!(col <= high_col && (col >= low_col || col < sink_col))) s[j] = 0xff800000u;
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        float x = __uint_as_float(s[g * 16]);
+#pragma unroll
+                        for (int j = 1; j < 15; j += 2)
+                            x = max3(x, __uint_as_float(s[g * 16 + j]), __uint_as_float(s[g * 16 + j + 1]));
+                        x = fmaxf(x, __uint_as_float(s[g * 16 + 15]));
+                        const GroupScales gs = sc[c * 2 + g];
+                        const float y = fmaf(x, unit * gs.key, gs.log2_value);
+                        top = fmaxf(top, x == -INFINITY ? -INFINITY : y);
+                    }
+                }
+                // the maximum stays while it is within 2^kSlack
+                const bool grow = top > m + kSlack && m != -INFINITY;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float keep = grow ? ex2(m - top) : 1.0f;
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16(to + c * 16, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                        tmem_st16(to + c * 16, o);
+                    }
+                    l *= keep;
+                }
+                if (grow || m == -INFINITY) m = top;
+                const float base = m == -INFINITY ? 0.0f : m - kShift;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t s[32];
+                    tmem_ld32(ts + c * 32, s);
+                    tmem_wait_ld();
+                    uint32_t w[16];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const GroupScales gs = sc[c * 2 + g];
+                        const float f = unit * gs.key, add = gs.log2_value - base;
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            float x = fmaf(__uint_as_float(s[g * 16 + j]), f, add);
+                            float y = fmaf(__uint_as_float(s[g * 16 + j + 1]), f, add);
+                            if (!clear) {
+                                const int col = c * 32 + g * 16 + j;
+                                if (!(col <= high_col && (col >= low_col || col < sink_col))) x = -INFINITY;
+                                if (!(col + 1 <= high_col && (col + 1 >= low_col || col + 1 < sink_col))) y = -INFINITY;
+                            }
+                            x = ex2(x);
+                            y = ex2(y);
+                            sum += x + y;
+                            w[g * 8 + j / 2] = pack2(x, y, __half());
+                        }
+                        if (sum != 0.0f) l = fmaf(sum, gs.inv_value, l);
+                    }
+                    tmem_st16(ts + c * 16, w);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sm.p_full[t]);
+            }
+            wait(&sm.o_full[t], o_n++);
+            __syncwarp();
+            tc_fence_after();
+            const bool whole = p.whole();
+            const int part = 2 * blockIdx.x + (p.first > 0 ? 0 : 1);
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            T* out = static_cast<T*>(a.out.data) + (p.t.token0 + token) * a.out.token_stride + head * a.out.head_stride;
+            float* sums = scratch.sums + (static_cast<long long>(part) * kRows + r) * D;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(to + c * 32, o);
+                tmem_wait_ld();
+                if (real && whole) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float x = __uint_as_float(o[j + 2 * i]) * inv, y = __uint_as_float(o[j + 2 * i + 1]) * inv;
+                            w[i] = pack2(x, y, T());
+                        }
+                        reinterpret_cast<uint4*>(out)[c * 4 + j / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else if (real) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        __stcg(reinterpret_cast<uint4*>(sums + c * 32 + j), make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+                }
+                __syncwarp();
+            }
+            if (real && whole && a.lse)
+                a.lse[(p.t.token0 + token) * (a.heads * a.group) + head] =
+                    l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * 0.6931471805599453f;
+            if (real && !whole) {
+                __stcg(scratch.stats + (part * 2) * kRows + r, m);
+                __stcg(scratch.stats + (part * 2 + 1) * kRows + r, l);
+            }
+            if (!whole && p.first == 0 && t == 0 && row == 0) {
+                int32_t* item = scratch.items + blockIdx.x * 8;
+                item[1] = static_cast<int>(p.t.token0);
+                item[2] = p.t.row0;
+                item[3] = p.t.rows;
+                item[4] = p.head;
+                item[0] = static_cast<int>((p.item_start + p.t.keys.nt - 1) / share.per) - blockIdx.x + 1;
+            }
+            tc_fence_before();
+        }
+    } else if (warp < 12) {
+        // ---- converter
+        constexpr int kLoads = D / 16;   // 16-byte loads of a thread for a tile's keys or values
+        const int w = warp - 8;
+        const int chunk = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;
+        const int sub = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) & 1) * 2 : lane >> 2;
+        constexpr int kStep = D == 128 ? 4 : 8;   // rows of one load of a warp
+        struct Next {
+            int page[2], row[2], head, keys;      // of this warp's two groups of 16 keys; keys 0: no tile
+        };
+        Piece p;
+        bool have = walk.next(a, p);
+        int at = have ? p.first : 0;
+        auto fetch = [&](Next& n) {
+            n.keys = have;
+            n.page[0] = n.page[1] = -1;
+            if (!have) return;
+            n.head = p.head;
+            const int key0 = p.t.keys.tile(at) * kKeys + w * 32;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int key = key0 + g * kGroupKeys, entry = key >> a.page_shift;
+                n.row[g] = key & (a.page_tokens - 1);
+                if (p.t.keys.touches(key) && entry < a.table_width)
+                    n.page[g] = a.table[static_cast<long long>(p.t.slot) * a.table_width + entry];
+            }
+            if (++at == p.end) {
+                have = walk.next(a, p);
+                at = have ? p.first : 0;
+            }
+        };
+        uint4 buf[2][kLoads];
+        float scale[2];   // lanes 0 and 1: key and value scale of the warp's group `lane`
+        auto load = [&](const Next& n, int side) {
+            const int8_t* from[2];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const bool there = n.keys && n.page[g] >= 0 && n.page[g] < a.pages;
+                const long long tile = (static_cast<long long>(n.page[g]) * 2 + side) * a.heads + n.head;
+                from[g] = there ? a.kv + (tile * a.page_tokens + n.row[g]) * D + chunk * 16 : nullptr;
+            }
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = i * kStep + sub;
+                buf[side][i] = make_uint4(0, 0, 0, 0);
+                const int8_t* src = from[(i * kStep) >> 4];  // sub < kStep, a divisor of 16
+                if (src) buf[side][i] = __ldg(reinterpret_cast<const uint4*>(src + (row & 15) * D));
+            }
+        };
+        auto load_scales = [&](const Next& n) {
+            scale[0] = 0.0f, scale[1] = -1.0f;
+            const int page = lane == 0 ? n.page[0] : n.page[1];
+            if (lane < 2 && n.keys && page >= 0 && page < a.pages) {
+                const float* s = a.scale + static_cast<long long>(page) * 2 * a.heads + n.head;
+                scale[0] = s[0];
+                scale[1] = s[a.heads];
+                if (scale[1] < kTinyScale) scale[1] = kTinyScale;
+            }
+        };
+        auto store = [&](int side, uint8_t* to) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int row = w * 32 + i * kStep + sub;
+                const uint32_t x[4] = {buf[side][i].x, buf[side][i].y, buf[side][i].z, buf[side][i].w};
+                uint32_t y[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) int8x4_to_half(x[j], y[2 * j], y[2 * j + 1]);
+                *reinterpret_cast<uint4*>(to + tile_at(row, chunk * 2)) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(to + tile_at(row, chunk * 2 + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+        };
+        Next now, next;
+        fetch(now);
+        load(now, 0);
+        load(now, 1);
+        load_scales(now);
+        fetch(next);
+        for (int n = 0; now.keys; ++n) {
+            const int b = n & 1, phase = (n >> 1) - 1;
+            if (n >= 2) wait(&sm.k_empty[b], phase);
+            store(0, sm.k[b]);
+            if (lane < 2) {
+                GroupScales g;
+                g.key = scale[0];
+                g.log2_value = scale[1] == -1.0f ? -INFINITY : log2f(scale[1]);
+                g.inv_value = scale[1] == -1.0f ? 0.0f : 1.0f / scale[1];
+                g.pad = 0.0f;
+                sm.scales[n % kScaleRing][w * 2 + lane] = g;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&sm.k_full[b]);
+            load(next, 0);
+            load_scales(next);
+            if (n >= 2) wait(&sm.v_empty[b], phase);
+            store(1, sm.v[b]);
+            fence_proxy_async_smem();
+            mbar_arrive(&sm.v_full[b]);
+            load(next, 1);
+            now = next;
+            fetch(next);
+        }
+    } else if (warp == 12) {
+        // ---- MMA: one thread
+        if (lane == 0) {
+            constexpr uint32_t qk = f16_idesc(128, kKeys, false), pv = f16_idesc(128, D, true);
+            uint32_t q_addr[2], k_addr[2], v_addr[2];
+            for (int i = 0; i < 2; ++i) {
+                q_addr[i] = smem_u32(sm.q[i]);
+                k_addr[i] = smem_u32(sm.k[i]);
+                v_addr[i] = smem_u32(sm.v[i]);
+            }
+            int n = 0;                    // key tiles so far
+            int q_n[2] = {0, 0}, p_n[2] = {0, 0};
+            auto scores = [&](int t, int b) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                    mma_f16(tmem + Tmem<D>::s(t), sw128_desc(q_addr[t] + off), sw128_desc(k_addr[b] + off), qk, k > 0);
+                }
+                mma_commit(&sm.s_full[t]);
+            };
+            Piece p;
+            while (walk.next(a, p)) {
+                const int halves = p.t.rows > kHalf ? 2 : 1;
+                const int count = p.end - p.first;
+                wait(&sm.k_full[n & 1], n >> 1);
+                for (int t = 0; t < halves; ++t) wait(&sm.q_full[t], q_n[t]++);
+                tc_fence_after();
+                for (int t = 0; t < halves; ++t) scores(t, n & 1);
+                mma_commit(&sm.k_empty[n & 1]);
+                for (int i = 0; i < count; ++i, ++n) {
+                    const int b = n & 1, c = (n + 1) & 1;
+                    wait(&sm.v_full[b], n >> 1);
+                    if (i + 1 < count) wait(&sm.k_full[c], (n + 1) >> 1);
+                    for (int t = 0; t < halves; ++t) {
+                        wait(&sm.p_full[t], p_n[t]++);
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k)
+                            mma_f16_ts(tmem + Tmem<D>::o(t), tmem + Tmem<D>::s(t) + k * 8,
+                                       sw128_n_major_desc(v_addr[b] + k * 16 * 128, 128 * 128), pv, i > 0 || k > 0);
+                        if (i + 1 < count) scores(t, c);
+                        else mma_commit(&sm.o_full[t]);
+                    }
+                    mma_commit(&sm.v_empty[b]);
+                    if (i + 1 < count) mma_commit(&sm.k_empty[c]);
+                }
+            }
+            // nothing may be in flight when tensor memory is given back
+            mma_commit(&sm.drained);
+            mbar_wait(&sm.drained, 0, a.status, kCode);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Rows that several CTAs share: the item that CTA x's share ends in, 16 rows a block.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_kernel(const AttendArgs a, int ctas) {
+    const AttendScratch scratch = scratch_of(a.workspace, ctas, kRows);
+    const int c0 = blockIdx.x;
+    const int32_t* item = scratch.items + c0 * 8;
+    const int parts = item[0];
+    if (parts == 0) return;
+    const int rows = min(item[3] - static_cast<int>(blockIdx.y) * 16, 16);
+    for (int e = threadIdx.x; e < rows * (D / 4); e += 128) {
+        const int row = blockIdx.y * 16 + e / (D / 4), d = e % (D / 4) * 4;
+        float top = -INFINITY;
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) top = fmaxf(top, scratch.stats[(2 * (c0 + i) + (i == 0)) * 2 * kRows + row]);
+        float weight = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) {
+            const int from = 2 * (c0 + i) + (i == 0);
+            const float m = scratch.stats[from * 2 * kRows + row], l = scratch.stats[(from * 2 + 1) * kRows + row];
+            const float4 x = *reinterpret_cast<const float4*>(scratch.sums + (static_cast<long long>(from) * kRows + row) * D + d);
+            const float mul = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2(m - top);
+            weight += l * mul;
+            v.x += x.x * mul, v.y += x.y * mul, v.z += x.z * mul, v.w += x.w * mul;
+        }
+        const int in_stream = item[2] + row, token = in_stream / a.group;
+        const int head = item[4] * a.group + in_stream - token * a.group;
+        const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+        T* to = static_cast<T*>(a.out.data) + (item[1] + static_cast<long long>(token)) * a.out.token_stride +
+                head * a.out.head_stride + d;
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
+        if (a.lse && d == 0)
+            a.lse[(item[1] + static_cast<long long>(token)) * (a.heads * a.group) + head] =
+                weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
+    }
+}
+
+template <typename T, int D>
+cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
+    auto kernel = many_kernel<T, D>;
+    const int smem = sizeof(Smem<D>) + 1024;
+    static std::once_flag once;
+    static cudaError_t attr = cudaSuccess;
+    std::call_once(once, [&] { attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    if (attr != cudaSuccess) return attr;
+    const long long row_tiles = (static_cast<long long>(a.max_new) * a.group + kRows - 1) / kRows;
+    if (row_tiles * a.n > 0x3fffffff) return cudaErrorInvalidValue;
+    const int ctas = sms < kAttendMaxCtas ? sms : kAttendMaxCtas;
+    many_kernel<T, D><<<ctas, kThreads, smem, s>>>(a, static_cast<int>(row_tiles), 1);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    join_kernel<T, D><<<dim3(ctas, kRows / 16), 128, 0, s>>>(a, ctas);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t attend_many(const AttendArgs& a, int dtype, int sms, cudaStream_t s) {
+    if (a.head_dim == 64)
+        return dtype == UFB_F16 ? launch<__half, 64>(a, sms, s) : launch<__nv_bfloat16, 64>(a, sms, s);
+    return dtype == UFB_F16 ? launch<__half, 128>(a, sms, s) : launch<__nv_bfloat16, 128>(a, sms, s);
+}
+
+}  // namespace ufb

@@ -546,8 +546,10 @@ int ufb_kv_read(const ufb_kv_cache* c, int layer, const int32_t* pages, int64_t 
  * key gives zeros (lse -inf).  q and out [tokens, q heads, head_dim] of dtype
  * UFB_F16 or UFB_BF16; lse (NULL, or [tokens][q heads] float) receives
  * ln sum_j exp(scale * q . k_j).  max_new is no less than any stream's count.
- * Statistics and sums in 32 bits; p and q enter the tensor cores with 11
- * significant bits (q exactly, see the kernel).
+ * Statistics and sums in 32 bits.  q and p enter the tensor cores as float16: q
+ * after a power of two for each query and head, so that no value of its type is
+ * out of range; p with 11 significant bits down to 2^-27 of the largest p times
+ * value scale of its row, and in steps of 2^-37 of it below.  Scales are not negative.
  * workspace: ufb_kv_attend_workspace() bytes, zero before its first use; calls
  * that may overlap need one each. */
 int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,

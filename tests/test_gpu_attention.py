@@ -181,6 +181,7 @@ def attend_ref(cache, layer, slots, counts, q, window, sinks, causal, scale):
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device=q.device)
     tol, tol_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    ids = {s: cache.table[s, :-(-int(cache.lengths[s]) // cache.page_tokens)].long().clamp(min=0) for s in slots}
     t = 0
     for slot, n in zip(slots, counts):
         kv, ok = contents(cache, layer, slot)
@@ -206,7 +207,10 @@ def attend_ref(cache, layer, slots, counts, q, window, sinks, causal, scale):
             rows = torch.nonzero(some)[:, 0] + t
             out[rows, h] = p @ v
             lse[rows, h] = l
-            tol[rows, h] = (p @ v.abs()) * (2.0 ** -11 + 2 * err[:, None])
+            unit = cache.scale[layer, ids[slot], 1, h // group].double().repeat_interleave(cache.page_tokens)[:length]
+            steps = torch.where(unit[:, None] > 0, v.abs() / unit[:, None], 0)
+            small = 2.0 ** -38 * (p * unit).amax(1)[:, None] * (seen[some].double() @ steps)
+            tol[rows, h] = (p @ v.abs()) * (2.0 ** -11 + 2 * err[:, None]) + small
             tol_lse[rows, h] = err + 2.0 ** -20 * l.abs()
         t += n
     return out, lse, tol, tol_lse
