@@ -28,6 +28,7 @@
 #include "umma.cuh"
 
 #include <mutex>
+#include <type_traits>
 
 namespace ufb {
 
@@ -56,7 +57,7 @@ struct Smem {
     alignas(1024) uint8_t v[2][kKeys * D * 2];
     GroupScales scales[kScaleRing][kGroups];
     alignas(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drained;
+    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], drained;
     ShareSmem share;
     uint32_t tmem;
     int dead;
@@ -73,7 +74,26 @@ __device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
     return (chunk >> 3) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
+// The lowest n bits (none below 0, all from 32 on).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
+
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// Two 32-bit multiply-adds (x, y) = (x, y) f + add, two additions (a, b) += (x, y).
+__device__ __forceinline__ void fma2(float& x, float& y, float f, float add) {
+    asm("{\n\t.reg .b64 v, m, c;\n\t"
+        "mov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
+        "fma.rn.f32x2 v, v, m, c;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(f), "f"(add));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 v, w;\n\t"
+        "mov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\t"
+        "add.rn.f32x2 v, v, w;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(x), "f"(y));
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, int row_tiles, int min_share) {
@@ -87,7 +107,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
             mbar_init(&sm.q_full[i], 128);
-            mbar_init(&sm.p_full[i], 128);
+            mbar_init(&sm.p_full[i][0], 128);
+            mbar_init(&sm.p_full[i][1], 128);
             mbar_init(&sm.s_full[i], 1);
             mbar_init(&sm.o_full[i], 1);
         }
@@ -111,7 +132,9 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
     };
     const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
 
+    // the registers of 512 threads at 128: 2 x 176 + 104 + 56 = 4 x 128
     if (warp < 8) {
+        regs_inc<176>();
         // ---- softmax: half t, row of the half = thread
         const int t = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -180,35 +203,44 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 const int key0 = p.t.keys.tile(tile) * kKeys;
                 const bool clear = (!a.causal || key0 + kKeys - 1 <= first_pos) && key0 + kKeys <= p.t.length &&
                                    (!a.window || last_pos - key0 < a.window || key0 + kKeys <= a.sinks);
-                // columns [low_col, high_col] and [0, sink_col) are seen by this row
-                const int high_col = min(p.t.length - 1, a.causal ? pos : p.t.length - 1) - key0;
-                const int low_col = a.window ? max(pos - a.window + 1, 0) - key0 : 0;
-                const int sink_col = a.window ? a.sinks - key0 : 0;
-                float top = -INFINITY;
+                // columns of this row's keys, a bit each
+                uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
+                if (!clear) {
+                    const int high = min(p.t.length - 1, a.causal ? pos : p.t.length - 1) - key0;
+                    const int low = a.window ? max(pos - a.window + 1, 0) - key0 : 0;
+                    const int sink = a.window ? a.sinks - key0 : 0;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t s[32];
-                    tmem_ld32(ts + c * 32, s);
-                    tmem_wait_ld();
-                    if (!clear) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int col = c * 32 + j;
-                            if (!(col <= high_col && (col >= low_col || col < sink_col))) s[j] = 0xff800000u;
-                        }
-                    }
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        float x = __uint_as_float(s[g * 16]);
-#pragma unroll
-                        for (int j = 1; j < 15; j += 2)
-                            x = max3(x, __uint_as_float(s[g * 16 + j]), __uint_as_float(s[g * 16 + j + 1]));
-                        x = fmaxf(x, __uint_as_float(s[g * 16 + 15]));
-                        const GroupScales gs = sc[c * 2 + g];
-                        const float y = fmaf(x, unit * gs.key, gs.log2_value);
-                        top = fmaxf(top, x == -INFINITY ? -INFINITY : y);
-                    }
+                    for (int c = 0; c < 4; ++c)
+                        seen[c] = bits_below(high + 1 - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
                 }
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s[c]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_tie32(s[c]);
+                float top = -INFINITY;
+                auto maximum = [&](auto masked) {
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        float x[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            x[j] = __uint_as_float(s[g / 2][(g % 2) * 16 + j]);
+                            if (decltype(masked)::value && !(seen[g / 2] & (1u << ((g % 2) * 16 + j)))) x[j] = -INFINITY;
+                        }
+                        float y = max3(x[0], x[1], x[2]), z = max3(x[3], x[4], x[5]);
+                        y = max3(y, x[6], x[7]), z = max3(z, x[8], x[9]);
+                        y = max3(y, x[10], x[11]), z = max3(z, x[12], x[13]);
+                        y = max3(y, x[14], x[15]);
+                        y = fmaxf(y, z);
+                        const float v = fmaf(y, unit * sc[g].key, sc[g].log2_value);
+                        // -infinity: nothing of the group is seen
+                        top = fmaxf(top, decltype(masked)::value && y == -INFINITY ? y : v);
+                    }
+                };
+                if (clear) maximum(std::false_type());
+                else maximum(std::true_type());
                 // the maximum stays while it is within 2^kSlack
                 const bool grow = top > m + kSlack && m != -INFINITY;
                 if (__any_sync(0xffffffffu, grow)) {
@@ -217,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                     for (int c = 0; c < D / 16; ++c) {
                         uint32_t o[16];
                         tmem_ld16(to + c * 16, o);
-                        tmem_wait_ld();
+                        tmem_wait_ld_regs(o);
 #pragma unroll
                         for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
                         tmem_st16(to + c * 16, o);
@@ -226,38 +258,42 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 }
                 if (grow || m == -INFINITY) m = top;
                 const float base = m == -INFINITY ? 0.0f : m - kShift;
+                auto weights = [&](auto masked) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t s[32];
-                    tmem_ld32(ts + c * 32, s);
-                    tmem_wait_ld();
-                    uint32_t w[16];
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[16];
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const GroupScales gs = sc[c * 2 + g];
-                        const float f = unit * gs.key, add = gs.log2_value - base;
-                        float sum = 0.0f;
+                        for (int h = 0; h < 2; ++h) {
+                            const GroupScales gs = sc[c * 2 + h];
+                            const float f = unit * gs.key, add = gs.log2_value - base;
+                            float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            float x = fmaf(__uint_as_float(s[g * 16 + j]), f, add);
-                            float y = fmaf(__uint_as_float(s[g * 16 + j + 1]), f, add);
-                            if (!clear) {
-                                const int col = c * 32 + g * 16 + j;
-                                if (!(col <= high_col && (col >= low_col || col < sink_col))) x = -INFINITY;
-                                if (!(col + 1 <= high_col && (col + 1 >= low_col || col + 1 < sink_col))) y = -INFINITY;
+                            for (int j = 0; j < 16; j += 2) {
+                                float x = __uint_as_float(s[c][h * 16 + j]), y = __uint_as_float(s[c][h * 16 + j + 1]);
+                                fma2(x, y, f, add);
+                                if (decltype(masked)::value) {
+                                    if (!(seen[c] & (1u << (h * 16 + j)))) x = -INFINITY;
+                                    if (!(seen[c] & (1u << (h * 16 + j + 1)))) y = -INFINITY;
+                                }
+                                x = ex2(x);
+                                y = ex2(y);
+                                add2(sum[0], sum[1], x, y);
+                                w[h * 8 + j / 2] = pack2(x, y, __half());
                             }
-                            x = ex2(x);
-                            y = ex2(y);
-                            sum += x + y;
-                            w[g * 8 + j / 2] = pack2(x, y, __half());
+                            sum[0] += sum[1];
+                            if (sum[0] != 0.0f) l = fmaf(sum[0], gs.inv_value, l);
                         }
-                        if (sum != 0.0f) l = fmaf(sum, gs.inv_value, l);
+                        tmem_st16(ts + c * 16, w);
+                        if (c & 1) {
+                            // P V starts on the first 64 keys while the others are in the works
+                            tmem_wait_st();
+                            tc_fence_before();
+                            mbar_arrive(&sm.p_full[t][c >> 1]);
+                        }
                     }
-                    tmem_st16(ts + c * 16, w);
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&sm.p_full[t]);
+                };
+                if (clear) weights(std::false_type());
+                else weights(std::true_type());
             }
             wait(&sm.o_full[t], o_n++);
             __syncwarp();
@@ -308,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             tc_fence_before();
         }
     } else if (warp < 12) {
+        regs_dec<104>();
         // ---- converter
         constexpr int kLoads = D / 16;   // 16-byte loads of a thread for a tile's keys or values
         const int w = warp - 8;
@@ -341,19 +378,26 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
         uint4 buf[2][kLoads];
         float scale[2];   // lanes 0 and 1: key and value scale of the warp's group `lane`
         auto load = [&](const Next& n, int side) {
+            if (!n.keys) return;
             const int8_t* from[2];
+            bool there[2];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const bool there = n.keys && n.page[g] >= 0 && n.page[g] < a.pages;
+                there[g] = n.page[g] >= 0 && n.page[g] < a.pages;
                 const long long tile = (static_cast<long long>(n.page[g]) * 2 + side) * a.heads + n.head;
-                from[g] = there ? a.kv + (tile * a.page_tokens + n.row[g]) * D + chunk * 16 : nullptr;
+                from[g] = a.kv + ((tile << a.page_shift) + n.row[g] + sub) * D + chunk * 16;
             }
+            if (there[0] && there[1]) {
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int row = i * kStep + sub;
-                buf[side][i] = make_uint4(0, 0, 0, 0);
-                const int8_t* src = from[(i * kStep) >> 4];  // sub < kStep, a divisor of 16
-                if (src) buf[side][i] = __ldg(reinterpret_cast<const uint4*>(src + (row & 15) * D));
+                for (int i = 0; i < kLoads; ++i)  // sub < kStep, a divisor of 16
+                    buf[side][i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    buf[side][i] = make_uint4(0, 0, 0, 0);
+                    if (there[(i * kStep) >> 4])
+                        buf[side][i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
+                }
             }
         };
         auto load_scales = [&](const Next& n) {
@@ -408,56 +452,77 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             now = next;
             fetch(next);
         }
-    } else if (warp == 12) {
-        // ---- MMA: one thread
-        if (lane == 0) {
+    } else {
+        regs_dec<56>();
+        // ---- MMA: the warp waits together, one lane issues
+        if (warp == 12) {
             constexpr uint32_t qk = f16_idesc(128, kKeys, false), pv = f16_idesc(128, D, true);
-            uint32_t q_addr[2], k_addr[2], v_addr[2];
-            for (int i = 0; i < 2; ++i) {
-                q_addr[i] = smem_u32(sm.q[i]);
-                k_addr[i] = smem_u32(sm.k[i]);
-                v_addr[i] = smem_u32(sm.v[i]);
-            }
+            constexpr uint64_t kTile = (kKeys * D * 2) >> 4;   // descriptor step between the two buffers
+            const uint64_t q_desc = sw128_desc(smem_u32(sm.q[0])), k_desc = sw128_desc(smem_u32(sm.k[0]));
+            const uint64_t v_desc = sw128_n_major_desc(smem_u32(sm.v[0]), 128 * 128);
             int n = 0;                    // key tiles so far
             int q_n[2] = {0, 0}, p_n[2] = {0, 0};
             auto scores = [&](int t, int b) {
+                const uint64_t qd = q_desc + t * kTile, kd = k_desc + b * kTile;
+                if (lane == 0) {
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k >> 2) * (128 * 128) + (k & 3) * 32;
-                    mma_f16(tmem + Tmem<D>::s(t), sw128_desc(q_addr[t] + off), sw128_desc(k_addr[b] + off), qk, k > 0);
+                    for (int k = 0; k < D / 16; ++k) {
+                        const int off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                        mma_f16(tmem + Tmem<D>::s(t), qd + off, kd + off, qk, k > 0);
+                    }
+                    mma_commit(&sm.s_full[t]);
                 }
-                mma_commit(&sm.s_full[t]);
+                __syncwarp();
             };
             Piece p;
             while (walk.next(a, p)) {
                 const int halves = p.t.rows > kHalf ? 2 : 1;
                 const int count = p.end - p.first;
                 wait(&sm.k_full[n & 1], n >> 1);
-                for (int t = 0; t < halves; ++t) wait(&sm.q_full[t], q_n[t]++);
-                tc_fence_after();
-                for (int t = 0; t < halves; ++t) scores(t, n & 1);
-                mma_commit(&sm.k_empty[n & 1]);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (t >= halves) break;
+                    wait(&sm.q_full[t], q_n[t]++);
+                    tc_fence_after();
+                    scores(t, n & 1);
+                }
+                if (lane == 0) mma_commit(&sm.k_empty[n & 1]);
                 for (int i = 0; i < count; ++i, ++n) {
                     const int b = n & 1, c = (n + 1) & 1;
                     wait(&sm.v_full[b], n >> 1);
                     if (i + 1 < count) wait(&sm.k_full[c], (n + 1) >> 1);
-                    for (int t = 0; t < halves; ++t) {
-                        wait(&sm.p_full[t], p_n[t]++);
-                        tc_fence_after();
 #pragma unroll
-                        for (int k = 0; k < kKeys / 16; ++k)
-                            mma_f16_ts(tmem + Tmem<D>::o(t), tmem + Tmem<D>::s(t) + k * 8,
-                                       sw128_n_major_desc(v_addr[b] + k * 16 * 128, 128 * 128), pv, i > 0 || k > 0);
+                    for (int t = 0; t < 2; ++t) {
+                        if (t >= halves) break;
+                        const uint64_t vd = v_desc + b * kTile;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            wait(&sm.p_full[t][h], p_n[t]);
+                            tc_fence_after();
+                            if (lane == 0) {
+#pragma unroll
+                                for (int k = h * 4; k < h * 4 + 4; ++k)
+                                    mma_f16_ts(tmem + Tmem<D>::o(t), tmem + Tmem<D>::s(t) + k * 8,
+                                               vd + k * (16 * 128 >> 4), pv, i > 0 || k > 0);
+                            }
+                            __syncwarp();
+                        }
+                        ++p_n[t];
                         if (i + 1 < count) scores(t, c);
-                        else mma_commit(&sm.o_full[t]);
+                        else if (lane == 0) mma_commit(&sm.o_full[t]);
                     }
-                    mma_commit(&sm.v_empty[b]);
-                    if (i + 1 < count) mma_commit(&sm.k_empty[c]);
+                    if (lane == 0) {
+                        mma_commit(&sm.v_empty[b]);
+                        if (i + 1 < count) mma_commit(&sm.k_empty[c]);
+                    }
+                    __syncwarp();
                 }
             }
             // nothing may be in flight when tensor memory is given back
-            mma_commit(&sm.drained);
-            mbar_wait(&sm.drained, 0, a.status, kCode);
+            if (lane == 0) {
+                mma_commit(&sm.drained);
+                mbar_wait(&sm.drained, 0, a.status, kCode);
+            }
         }
         __syncwarp();
     }
