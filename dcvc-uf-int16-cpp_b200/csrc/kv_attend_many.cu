@@ -8,10 +8,10 @@
 // key tile are expanded to float16 once for 256 rows.
 //
 // One CTA an SM, four roles:
-//   converter (4 warps)  integers from global memory through registers to float16
+//   converter (8 warps)  integers from global memory through registers to float16
 //                        in shared memory, keys and values double buffered, with
 //                        128-byte swizzle; the page scales of each 16 keys
-//   MMA (1 thread)       S_t = Q_t K^T and O_t += P_t V for the two halves t of
+//   MMA (1 warp)         S_t = Q_t K^T and O_t += P_t V for the two halves t of
 //                        128 rows, in the order O_0 S_0 O_1 S_1, so that one half
 //                        multiplies while the other is in its softmax
 //   softmax (2 x 4 warps) a thread owns a row: S from tensor memory, P back to it
@@ -38,7 +38,8 @@ constexpr int kRows = kAttendManyRows;
 constexpr int kHalf = 128;
 constexpr int kKeys = 128;
 constexpr int kGroups = kKeys / kGroupKeys;
-constexpr int kThreads = 512;         // softmax 0-7, converter 8-11, MMA 12; 13-15 idle
+constexpr int kMmaWarp = 16;
+constexpr int kThreads = 544;         // warps: softmax 0-7, converter 8-15, MMA 16
 constexpr int kScaleRing = 4;
 constexpr int kCode = 44;
 // A running maximum stays while it grows by less than 2^kSlack, and P is taken
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
         fence_mbar_init();
         sm.dead = 0;
     }
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         tmem_alloc(&sm.tmem, 512);
         tmem_relinquish();
     }
@@ -132,9 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
     };
     const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
 
-    // the registers of 512 threads at 128: 2 x 176 + 104 + 56 = 4 x 128
     if (warp < 8) {
-        regs_inc<176>();
         // ---- softmax: half t, row of the half = thread
         const int t = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -203,40 +202,43 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 const int key0 = p.t.keys.tile(tile) * kKeys;
                 const bool clear = (!a.causal || key0 + kKeys - 1 <= first_pos) && key0 + kKeys <= p.t.length &&
                                    (!a.window || last_pos - key0 < a.window || key0 + kKeys <= a.sinks);
-                // columns of this row's keys, a bit each
-                uint32_t seen[4] = {~0u, ~0u, ~0u, ~0u};
-                if (!clear) {
-                    const int high = min(p.t.length - 1, a.causal ? pos : p.t.length - 1) - key0;
-                    const int low = a.window ? max(pos - a.window + 1, 0) - key0 : 0;
-                    const int sink = a.window ? a.sinks - key0 : 0;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        seen[c] = bits_below(high + 1 - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
-                }
-                uint32_t s[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, s[c]);
-                tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_tie32(s[c]);
+                // columns [0, high) that are from low on or below sink are seen by this row
+                const int high = min(p.t.length, a.causal ? pos + 1 : p.t.length) - key0;
+                const int low = a.window ? max(pos - a.window + 1, 0) - key0 : 0;
+                const int sink = a.window ? a.sinks - key0 : 0;
+                auto seen = [&](int c) {   // of 32 columns, a bit each
+                    return bits_below(high - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
+                };
+                // The loops run over 32 columns and are not unrolled: three roles share
+                // each scheduler's instruction cache.
                 float top = -INFINITY;
                 auto maximum = [&](auto masked) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t s[32];
+                        tmem_ld32(ts + c * 32, s);
+                        tmem_wait_ld();
+                        tmem_tie32(s);
+                        if (decltype(masked)::value) {
+                            const uint32_t bits = seen(c);
 #pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        float x[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            x[j] = __uint_as_float(s[g / 2][(g % 2) * 16 + j]);
-                            if (decltype(masked)::value && !(seen[g / 2] & (1u << ((g % 2) * 16 + j)))) x[j] = -INFINITY;
+                            for (int j = 0; j < 32; ++j)
+                                if (!(bits & (1u << j))) s[j] = 0xff800000u;
                         }
-                        float y = max3(x[0], x[1], x[2]), z = max3(x[3], x[4], x[5]);
-                        y = max3(y, x[6], x[7]), z = max3(z, x[8], x[9]);
-                        y = max3(y, x[10], x[11]), z = max3(z, x[12], x[13]);
-                        y = max3(y, x[14], x[15]);
-                        y = fmaxf(y, z);
-                        const float v = fmaf(y, unit * sc[g].key, sc[g].log2_value);
-                        // -infinity: nothing of the group is seen
-                        top = fmaxf(top, decltype(masked)::value && y == -INFINITY ? y : v);
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const uint32_t* x = s + g * 16;
+                            auto f = [&](int j) { return __uint_as_float(x[j]); };
+                            float y = max3(f(0), f(1), f(2)), z = max3(f(3), f(4), f(5));
+                            y = max3(y, f(6), f(7)), z = max3(z, f(8), f(9));
+                            y = max3(y, f(10), f(11)), z = max3(z, f(12), f(13));
+                            y = max3(y, f(14), f(15));
+                            y = fmaxf(y, z);
+                            const GroupScales gs = sc[c * 2 + g];
+                            const float v = fmaf(y, unit * gs.key, gs.log2_value);
+                            // -infinity: nothing of the group is seen
+                            top = fmaxf(top, decltype(masked)::value && y == -INFINITY ? y : v);
+                        }
                     }
                 };
                 if (clear) maximum(std::false_type());
@@ -259,9 +261,13 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 if (grow || m == -INFINITY) m = top;
                 const float base = m == -INFINITY ? 0.0f : m - kShift;
                 auto weights = [&](auto masked) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t w[16];
+                        uint32_t s[32], w[16];
+                        tmem_ld32(ts + c * 32, s);
+                        const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
+                        tmem_wait_ld();
+                        tmem_tie32(s);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const GroupScales gs = sc[c * 2 + h];
@@ -269,11 +275,11 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                             for (int j = 0; j < 16; j += 2) {
-                                float x = __uint_as_float(s[c][h * 16 + j]), y = __uint_as_float(s[c][h * 16 + j + 1]);
+                                float x = __uint_as_float(s[h * 16 + j]), y = __uint_as_float(s[h * 16 + j + 1]);
                                 fma2(x, y, f, add);
                                 if (decltype(masked)::value) {
-                                    if (!(seen[c] & (1u << (h * 16 + j)))) x = -INFINITY;
-                                    if (!(seen[c] & (1u << (h * 16 + j + 1)))) y = -INFINITY;
+                                    if (!(bits & (1u << (h * 16 + j)))) x = -INFINITY;
+                                    if (!(bits & (1u << (h * 16 + j + 1)))) y = -INFINITY;
                                 }
                                 x = ex2(x);
                                 y = ex2(y);
@@ -343,22 +349,32 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             }
             tc_fence_before();
         }
-    } else if (warp < 12) {
-        regs_dec<104>();
-        // ---- converter
-        constexpr int kLoads = D / 16;   // 16-byte loads of a thread for a tile's keys or values
-        const int w = warp - 8;
+    } else if (warp < kMmaWarp) {
+        // ---- converter: warps 8-11 the keys and the scales, 12-15 the values, 32 keys each
+        constexpr int kLoads = D / 16;   // 16-byte loads of a thread for a tile
+        const int side = (warp - 8) >> 2, w = warp & 3;
         const int chunk = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;
         const int sub = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) & 1) * 2 : lane >> 2;
         constexpr int kStep = D == 128 ? 4 : 8;   // rows of one load of a warp
+        uint64_t* full = side ? sm.v_full : sm.k_full;
+        uint64_t* empty = side ? sm.v_empty : sm.k_empty;
+        uint8_t* tiles = side ? sm.v[0] : sm.k[0];
+        // this thread's two 16-byte pieces of its first row; row & 7 repeats every kStep * 2 rows
+        uint32_t at0[2], at1[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            at0[i] = tile_at(w * 32 + i * kStep + sub, chunk * 2);
+            at1[i] = tile_at(w * 32 + i * kStep + sub, chunk * 2 + 1);
+        }
         struct Next {
-            int page[2], row[2], head, keys;      // of this warp's two groups of 16 keys; keys 0: no tile
+            int page[2], row[2], head;   // of this warp's two groups of 16 keys
+            bool tile;                   // false: no further tile
         };
         Piece p;
         bool have = walk.next(a, p);
         int at = have ? p.first : 0;
         auto fetch = [&](Next& n) {
-            n.keys = have;
+            n.tile = have;
             n.page[0] = n.page[1] = -1;
             if (!have) return;
             n.head = p.head;
@@ -375,10 +391,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 at = have ? p.first : 0;
             }
         };
-        uint4 buf[2][kLoads];
-        float scale[2];   // lanes 0 and 1: key and value scale of the warp's group `lane`
-        auto load = [&](const Next& n, int side) {
-            if (!n.keys) return;
+        uint4 buf[kLoads];
+        float key_scale = 0.0f, value_scale = -1.0f;   // of the warp's group `lane` (0, 1); -1: not there
+        auto load = [&](const Next& n) {
+            if (!n.tile) return;
             const int8_t* from[2];
             bool there[2];
 #pragma unroll
@@ -390,72 +406,60 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             if (there[0] && there[1]) {
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i)  // sub < kStep, a divisor of 16
-                    buf[side][i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
+                    buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
             } else {
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) {
-                    buf[side][i] = make_uint4(0, 0, 0, 0);
+                    buf[i] = make_uint4(0, 0, 0, 0);
                     if (there[(i * kStep) >> 4])
-                        buf[side][i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
+                        buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
                 }
             }
-        };
-        auto load_scales = [&](const Next& n) {
-            scale[0] = 0.0f, scale[1] = -1.0f;
-            const int page = lane == 0 ? n.page[0] : n.page[1];
-            if (lane < 2 && n.keys && page >= 0 && page < a.pages) {
-                const float* s = a.scale + static_cast<long long>(page) * 2 * a.heads + n.head;
-                scale[0] = s[0];
-                scale[1] = s[a.heads];
-                if (scale[1] < kTinyScale) scale[1] = kTinyScale;
-            }
-        };
-        auto store = [&](int side, uint8_t* to) {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                const int row = w * 32 + i * kStep + sub;
-                const uint32_t x[4] = {buf[side][i].x, buf[side][i].y, buf[side][i].z, buf[side][i].w};
-                uint32_t y[8];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) int8x4_to_half(x[j], y[2 * j], y[2 * j + 1]);
-                *reinterpret_cast<uint4*>(to + tile_at(row, chunk * 2)) = make_uint4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<uint4*>(to + tile_at(row, chunk * 2 + 1)) = make_uint4(y[4], y[5], y[6], y[7]);
+            if (side == 0 && lane < 2) {
+                key_scale = 0.0f, value_scale = -1.0f;
+                if (there[lane]) {
+                    const float* s = a.scale + static_cast<long long>(n.page[lane]) * 2 * a.heads + n.head;
+                    key_scale = s[0];
+                    value_scale = s[a.heads];
+                    if (value_scale < kTinyScale) value_scale = kTinyScale;
+                }
             }
         };
         Next now, next;
         fetch(now);
-        load(now, 0);
-        load(now, 1);
-        load_scales(now);
+        load(now);
         fetch(next);
-        for (int n = 0; now.keys; ++n) {
-            const int b = n & 1, phase = (n >> 1) - 1;
-            if (n >= 2) wait(&sm.k_empty[b], phase);
-            store(0, sm.k[b]);
-            if (lane < 2) {
+        for (int n = 0; now.tile; ++n) {
+            const int b = n & 1;
+            if (n >= 2) wait(&empty[b], (n >> 1) - 1);
+            uint8_t* to = tiles + b * (kKeys * D * 2);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t x[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
+                uint32_t y[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) int8x4_to_half(x[j], y[2 * j], y[2 * j + 1]);
+                const int step = (i / 2) * 2 * kStep * 128;
+                *reinterpret_cast<uint4*>(to + at0[i & 1] + step) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(to + at1[i & 1] + step) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            if (side == 0 && lane < 2) {
                 GroupScales g;
-                g.key = scale[0];
-                g.log2_value = scale[1] == -1.0f ? -INFINITY : log2f(scale[1]);
-                g.inv_value = scale[1] == -1.0f ? 0.0f : 1.0f / scale[1];
+                g.key = key_scale;
+                g.log2_value = value_scale == -1.0f ? -INFINITY : log2f(value_scale);
+                g.inv_value = value_scale == -1.0f ? 0.0f : 1.0f / value_scale;
                 g.pad = 0.0f;
                 sm.scales[n % kScaleRing][w * 2 + lane] = g;
             }
             fence_proxy_async_smem();
-            mbar_arrive(&sm.k_full[b]);
-            load(next, 0);
-            load_scales(next);
-            if (n >= 2) wait(&sm.v_empty[b], phase);
-            store(1, sm.v[b]);
-            fence_proxy_async_smem();
-            mbar_arrive(&sm.v_full[b]);
-            load(next, 1);
+            mbar_arrive(&full[b]);
+            load(next);
             now = next;
             fetch(next);
         }
     } else {
-        regs_dec<56>();
         // ---- MMA: the warp waits together, one lane issues
-        if (warp == 12) {
+        {
             constexpr uint32_t qk = f16_idesc(128, kKeys, false), pv = f16_idesc(128, D, true);
             constexpr uint64_t kTile = (kKeys * D * 2) >> 4;   // descriptor step between the two buffers
             const uint64_t q_desc = sw128_desc(smem_u32(sm.q[0])), k_desc = sw128_desc(smem_u32(sm.k[0]));
@@ -528,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
