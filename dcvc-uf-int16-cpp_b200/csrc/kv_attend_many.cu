@@ -156,17 +156,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 // the row to [1/2, 1) and float16; the softmax scale's sign goes with it
                 const T* src = static_cast<const T*>(a.q.data) + (p.t.token0 + token) * a.q.token_stride +
                                head * a.q.head_stride;
-                float top = 0.0f;
-                uint4 w[D / 8];
-#pragma unroll
+                const uint4* vec = reinterpret_cast<const uint4*>(src);
+                float top = 0.0f, odd = 0.0f;
+#pragma unroll 4
                 for (int i = 0; i < D / 8; ++i) {
-                    w[i] = make_uint4(0, 0, 0, 0);
-                    if (real) w[i] = reinterpret_cast<const uint4*>(src)[i];
-                }
-                float odd = 0.0f;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                    const uint4 v = real ? vec[i] : make_uint4(0, 0, 0, 0);
+                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float2 f = unpack2(x[j], T());
@@ -177,9 +172,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 const float u = row_unit(odd == odd ? top : odd);
                 unit = unit_inverse(u) * fabsf(a.scale_log2);
                 const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
-#pragma unroll
+#pragma unroll 4
                 for (int i = 0; i < D / 8; ++i) {
-                    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                    const uint4 v = real ? vec[i] : make_uint4(0, 0, 0, 0);
+                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
                     uint32_t y[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -417,8 +413,9 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             }
             if (side == 0 && lane < 2) {
                 key_scale = 0.0f, value_scale = -1.0f;
-                if (there[lane]) {
-                    const float* s = a.scale + static_cast<long long>(n.page[lane]) * 2 * a.heads + n.head;
+                if (lane == 0 ? there[0] : there[1]) {
+                    const int page = lane == 0 ? n.page[0] : n.page[1];
+                    const float* s = a.scale + static_cast<long long>(page) * 2 * a.heads + n.head;
                     key_scale = s[0];
                     value_scale = s[a.heads];
                     if (value_scale < kTinyScale) value_scale = kTinyScale;
