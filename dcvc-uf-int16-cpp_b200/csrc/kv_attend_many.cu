@@ -98,8 +98,9 @@ __device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, int row_tiles, int min_share) {
-    extern __shared__ uint8_t raw[];
-    Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    // aligned by declaration, so that descriptors are constants (checked below)
+    extern __shared__ __align__(1024) uint8_t raw[];
+    Smem<D>& sm = *reinterpret_cast<Smem<D>*>(raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -115,7 +116,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
         }
         mbar_init(&sm.drained, 1);
         fence_mbar_init();
-        sm.dead = 0;
+        sm.dead = (smem_u32(raw) & 1023) != 0;
+        if (sm.dead) atomicCAS(a.status, 0, kCode);
     }
     if (warp == kMmaWarp) {
         tmem_alloc(&sm.tmem, 512);
@@ -124,11 +126,13 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
     tc_fence_before();
     const Share share = locate_share<kKeys, kRows, kThreads>(a, row_tiles, min_share, sm.share);
     tc_fence_after();
-    const uint32_t tmem = sm.tmem;
+    // all 512 columns are this CTA's: its tensor memory begins at 0
+    constexpr uint32_t tmem = 0;
     Walker<kKeys, kRows> walk(a, share, row_tiles);
     volatile int* dead = &sm.dead;
     // after a wait gave up nobody waits any more: the loops run out on what is there
     auto wait = [&](uint64_t* bar, int phase) {
+        if (mbar_try_wait(bar, phase & 1)) return;
         if (!*dead && !mbar_wait(bar, phase & 1, a.status, kCode)) *dead = 1;
     };
     const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
@@ -463,17 +467,15 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             const uint64_t v_desc = sw128_n_major_desc(smem_u32(sm.v[0]), 128 * 128);
             int n = 0;                    // key tiles so far
             int q_n[2] = {0, 0}, p_n[2] = {0, 0};
+            const uint32_t issue = lane == 0;
             auto scores = [&](int t, int b) {
                 const uint64_t qd = q_desc + t * kTile, kd = k_desc + b * kTile;
-                if (lane == 0) {
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const int off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-                        mma_f16(tmem + Tmem<D>::s(t), qd + off, kd + off, qk, k > 0);
-                    }
-                    mma_commit(&sm.s_full[t]);
+                for (int k = 0; k < D / 16; ++k) {
+                    const int off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                    mma_f16(tmem + Tmem<D>::s(t), qd + off, kd + off, qk, k > 0, issue);
                 }
-                __syncwarp();
+                mma_commit_if(&sm.s_full[t], issue);
             };
             Piece p;
             while (walk.next(a, p)) {
@@ -482,41 +484,39 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 wait(&sm.k_full[n & 1], n >> 1);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    if (t >= halves) break;
+                    if (t >= halves) continue;
                     wait(&sm.q_full[t], q_n[t]++);
+                    __syncwarp();
                     tc_fence_after();
                     scores(t, n & 1);
                 }
-                if (lane == 0) mma_commit(&sm.k_empty[n & 1]);
+                mma_commit_if(&sm.k_empty[n & 1], issue);
+#pragma unroll 1
                 for (int i = 0; i < count; ++i, ++n) {
                     const int b = n & 1, c = (n + 1) & 1;
+                    const bool more = i + 1 < count;
                     wait(&sm.v_full[b], n >> 1);
-                    if (i + 1 < count) wait(&sm.k_full[c], (n + 1) >> 1);
+                    if (more) wait(&sm.k_full[c], (n + 1) >> 1);
+                    const uint64_t vd = v_desc + b * kTile;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        if (t >= halves) break;
-                        const uint64_t vd = v_desc + b * kTile;
+                        if (t >= halves) continue;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             wait(&sm.p_full[t][h], p_n[t]);
-                            tc_fence_after();
-                            if (lane == 0) {
-#pragma unroll
-                                for (int k = h * 4; k < h * 4 + 4; ++k)
-                                    mma_f16_ts(tmem + Tmem<D>::o(t), tmem + Tmem<D>::s(t) + k * 8,
-                                               vd + k * (16 * 128 >> 4), pv, i > 0 || k > 0);
-                            }
                             __syncwarp();
+                            tc_fence_after();
+#pragma unroll
+                            for (int k = h * 4; k < h * 4 + 4; ++k)
+                                mma_f16_ts(tmem + Tmem<D>::o(t), tmem + Tmem<D>::s(t) + k * 8, vd + k * (16 * 128 >> 4),
+                                           pv, i > 0 || k > 0, issue);
                         }
                         ++p_n[t];
-                        if (i + 1 < count) scores(t, c);
-                        else if (lane == 0) mma_commit(&sm.o_full[t]);
+                        if (more) scores(t, c);
+                        else mma_commit_if(&sm.o_full[t], issue);
                     }
-                    if (lane == 0) {
-                        mma_commit(&sm.v_empty[b]);
-                        if (i + 1 < count) mma_commit(&sm.k_empty[c]);
-                    }
-                    __syncwarp();
+                    mma_commit_if(&sm.v_empty[b], issue);
+                    if (more) mma_commit_if(&sm.k_empty[c], issue);
                 }
             }
             // nothing may be in flight when tensor memory is given back
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
     __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(sm.tmem, 512);
     }
 }
 
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendArgs a, int ctas)
 template <typename T, int D>
 cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     auto kernel = many_kernel<T, D>;
-    const int smem = sizeof(Smem<D>) + 1024;
+    const int smem = sizeof(Smem<D>);
     static std::once_flag once;
     static cudaError_t attr = cudaSuccess;
     std::call_once(once, [&] { attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
