@@ -135,7 +135,9 @@ int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t
         a.extent[i] = extents[i];
         a.first[i + 1] = a.first[i] + pairs[i];
         if (a.first[i + 1] > head_dim / 2) return err(UFB_EINVAL, "more rotary pairs than the head holds");
-        if (i + 1 < axes) a.base[i + 1] = a.base[i] + static_cast<long long>(pairs[i]) * extents[i];
+        if (i + 1 < UFB_ROTARY_MAX_AXES) a.base[i + 1] = a.base[i] + static_cast<long long>(pairs[i]) * extents[i];
+        if (a.base[i] + static_cast<long long>(pairs[i]) * extents[i] > INT32_MAX)
+            return err(UFB_ERANGE, "rotary table exceeds indexing bounds");
     }
     a.pairs = a.first[axes];
     if (tokens == 0) return UFB_OK;

@@ -107,40 +107,45 @@ __device__ __forceinline__ uint4 window16(const uint4* row, int at, int columns)
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Thread = (token, group of `per` heads, column).
-template <typename T, int LAYOUT>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, int columns, int groups, int per,
-                                                          int* status) {
-    constexpr int N = Column<T>::n;
-    const long long id = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-    const int col = static_cast<int>(id % columns);
-    const long long unit = id / columns;
-    const int group = static_cast<int>(unit % groups);
-    const long long token = unit / groups;
-    if (token >= a.tokens) return;
+enum Mode { kHalfPairs, kHalf, kInterleaved };
 
-    // this column's (cos, +-sin); sin's sign and the partner's side by element
-    float c[N], s[N];
+// Thread = (token, column), for heads [blockIdx.y * per, + per).  Columns of a head:
+// kHalfPairs: n / N columns that hold the first of both members of N pairs (the
+// second ones are n elements on), then the columns past 2 n; else all D / N.
+template <typename T, Mode MODE>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, int columns, int per, int* status) {
+    constexpr int N = Column<T>::n;
+    const unsigned slots = kThreads / columns;    // tokens of a block
+    const unsigned slot = threadIdx.x / columns;
+    const long long token = static_cast<long long>(blockIdx.x) * slots + slot;
+    if (slot >= slots || token >= a.tokens) return;
+    const int index = threadIdx.x - slot * columns;
+    const int paired = a.pairs / N;
+    const int col = MODE == kHalfPairs && index >= paired ? index + paired : index;
     const int e0 = col * N;
+
+    // this column's (cos, sin): out = x c + partner s, s with the member's and the direction's sign
+    float c[N], s[N];
     bool bad = false;
-    long long row[UFB_ROTARY_MAX_AXES];
+    int row[UFB_ROTARY_MAX_AXES];
 #pragma unroll
     for (int ax = 0; ax < UFB_ROTARY_MAX_AXES; ++ax) {
         row[ax] = 0;
         if (ax < a.axes) {
             const int p = a.positions[token * a.axes + ax];
             bad |= p < 0 || p >= a.extent[ax];
-            row[ax] = a.base[ax] + static_cast<long long>(bad ? 0 : p) * (a.first[ax + 1] - a.first[ax]) - a.first[ax];
+            // a table holds less than 2^31 entries
+            row[ax] = static_cast<int>(a.base[ax]) + (bad ? 0 : p) * (a.first[ax + 1] - a.first[ax]) - a.first[ax];
         }
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const int e = e0 + i;
-        const int pair = LAYOUT == UFB_ROTARY_HALF ? (e < a.pairs ? e : e - a.pairs) : e >> 1;
-        const bool second = LAYOUT == UFB_ROTARY_HALF ? e >= a.pairs : (e & 1);
+        const int pair = MODE == kInterleaved ? e >> 1 : (e < a.pairs ? e : e - a.pairs);
+        const bool second = MODE == kInterleaved ? (e & 1) : e >= a.pairs;
         c[i] = 1.0f, s[i] = -0.0f;  // x * 1 + 0 * -0 is x, zeros of both signs included
         if (pair < a.pairs) {
-            long long r = row[0];
+            int r = row[0];
 #pragma unroll
             for (int ax = 1; ax < UFB_ROTARY_MAX_AXES; ++ax)
                 if (ax < a.axes && pair >= a.first[ax]) r = row[ax];
@@ -150,66 +155,95 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, in
         }
         if (bad) c[i] = s[i] = __int_as_float(0x7fffffff);
     }
-    if (bad && col == 0 && group == 0) atomicCAS(status, 0, kStatusPosition);
+    if (bad && index == 0 && blockIdx.y == 0) atomicCAS(status, 0, kStatusPosition);
 
-    const int total = a.x[0].heads + (a.count > 1 ? a.x[1].heads : 0);
-    const int end = min(total, (group + 1) * per);
+    const int vecs = a.head_dim / N;
+    const int shift = a.pairs * static_cast<int>(sizeof(T));
+    const bool tail = MODE == kHalfPairs && index >= paired;
     const bool plus = e0 < a.pairs, minus = e0 + N > a.pairs && e0 < 2 * a.pairs;
+    const int total = a.x[0].heads + (a.count > 1 ? a.x[1].heads : 0);
+    const int begin = blockIdx.y * per, end = min(total, begin + per);
+    // all heads of one tensor, four at a time in flight
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int h0 = t ? max(begin - a.x[0].heads, 0) : begin;
+        const int h1 = t ? end - a.x[0].heads : min(end, a.x[0].heads);
+        const T* in = static_cast<const T*>(a.x[t].data) + token * a.x[t].token_stride + h0 * a.x[t].head_stride;
+        T* out = static_cast<T*>(a.out[t].data) + token * a.out[t].token_stride + h0 * a.out[t].head_stride;
 #pragma unroll 4
-    for (int h = group * per; h < end; ++h) {
-        const int t = h >= a.x[0].heads;
-        const int head = t ? h - a.x[0].heads : h;
-        const uint4* in = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x[t].data) +
-                                                         token * a.x[t].token_stride + head * a.x[t].head_stride);
-        float x[N], y[N], r[N];
-        const uint4 own = in[col];
-        Column<T>::unpack(own, x);
-        if (LAYOUT == UFB_ROTARY_HALF) {
-            uint4 up = make_uint4(0, 0, 0, 0), down = make_uint4(0, 0, 0, 0);
-            const int shift = a.pairs * static_cast<int>(sizeof(T));
-            if (plus) up = window16(in, col * 16 + shift, columns);
-            if (minus) down = window16(in, col * 16 - shift, columns);
-            float u[N], d[N];
-            Column<T>::unpack(up, u);
-            Column<T>::unpack(down, d);
+        for (int h = h0; h < h1; ++h, in += a.x[t].head_stride, out += a.out[t].head_stride) {
+            const uint4* from = reinterpret_cast<const uint4*>(in);
+            uint4* to = reinterpret_cast<uint4*>(out);
+            float x[N], y[N], r[N];
+            const uint4 own = __ldcs(from + col);
+            Column<T>::unpack(own, x);
+            if (MODE == kHalfPairs) {
+                if (tail) {
+                    __stcs(to + col, bad ? make_uint4(~0u, ~0u, ~0u, ~0u) : own);
+                } else {
+                    Column<T>::unpack(__ldcs(from + col + paired), y);
+                    float q[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) y[i] = e0 + i < a.pairs ? u[i] : (e0 + i < 2 * a.pairs ? d[i] : 0.0f);
-        } else {
+                    for (int i = 0; i < N; ++i) {
+                        r[i] = x[i] * c[i] + y[i] * s[i];
+                        q[i] = y[i] * c[i] - x[i] * s[i];
+                    }
+                    __stcs(to + col, Column<T>::pack(r));
+                    __stcs(to + col + paired, Column<T>::pack(q));
+                }
+                continue;
+            }
+            if (MODE == kHalf) {
+                uint4 up = make_uint4(0, 0, 0, 0), down = make_uint4(0, 0, 0, 0);
+                if (plus) up = window16(from, col * 16 + shift, vecs);
+                if (minus) down = window16(from, col * 16 - shift, vecs);
+                float u[N], d[N];
+                Column<T>::unpack(up, u);
+                Column<T>::unpack(down, d);
 #pragma unroll
-            for (int i = 0; i < N; ++i) y[i] = (e0 + i) >> 1 < a.pairs ? x[i ^ 1] : 0.0f;
+                for (int i = 0; i < N; ++i) y[i] = e0 + i < a.pairs ? u[i] : (e0 + i < 2 * a.pairs ? d[i] : 0.0f);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) y[i] = (e0 + i) >> 1 < a.pairs ? x[i ^ 1] : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = x[i] * c[i] + y[i] * s[i];
+            __stcs(to + col, Column<T>::pack(r));
         }
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = x[i] * c[i] + y[i] * s[i];
-        uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(a.out[t].data) + token * a.out[t].token_stride +
-                                             head * a.out[t].head_stride);
-        to[col] = Column<T>::pack(r);
     }
 }
 
-template <typename T>
-cudaError_t launch(const RotaryArgs& a, int* status, cudaStream_t s) {
-    const int columns = a.head_dim / Column<T>::n;
+template <typename T, Mode MODE>
+cudaError_t launch(const RotaryArgs& a, int columns, int* status, cudaStream_t s) {
     const int heads = a.x[0].heads + (a.count > 1 ? a.x[1].heads : 0);
-    // Several heads to a thread share its table values; with few tokens one head
-    // to a thread spreads the call over more SMs.
-    const long long threads = a.tokens * heads * columns;
-    const int per = threads >= 148ll * 2048 * 4 ? 4 : 1;
-    const int groups = (heads + per - 1) / per;
-    const long long blocks = (a.tokens * groups * columns + kThreads - 1) / kThreads;
+    const unsigned slots = kThreads / columns;
+    const long long blocks = (a.tokens + slots - 1) / slots;
     if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-    if (a.layout == UFB_ROTARY_HALF)
-        rotary_kernel<T, UFB_ROTARY_HALF><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a, columns, groups, per, status);
-    else
-        rotary_kernel<T, UFB_ROTARY_INTERLEAVED><<<static_cast<unsigned>(blocks), kThreads, 0, s>>>(a, columns, groups, per, status);
+    // All heads to a thread share its table values; while that leaves SMs without
+    // two blocks, the heads are spread over more blocks.
+    long long groups = (2 * 148 + blocks - 1) / blocks;
+    if (groups > heads) groups = heads;
+    const int per = static_cast<int>((heads + groups - 1) / groups);
+    rotary_kernel<T, MODE><<<dim3(static_cast<unsigned>(blocks), (heads + per - 1) / per), kThreads, 0, s>>>(a, columns, per, status);
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t dispatch(const RotaryArgs& a, int* status, cudaStream_t s) {
+    constexpr int N = Column<T>::n;
+    const int vecs = a.head_dim / N;
+    if (a.layout == UFB_ROTARY_INTERLEAVED) return launch<T, kInterleaved>(a, vecs, status, s);
+    // pair counts that are whole columns: a thread reads and writes both members
+    if (a.pairs % N == 0) return launch<T, kHalfPairs>(a, vecs - a.pairs / N, status, s);
+    return launch<T, kHalf>(a, vecs, status, s);
 }
 
 }  // namespace
 
 cudaError_t rotary(const RotaryArgs& a, int dtype, int* status, cudaStream_t s) {
-    if (dtype == UFB_F32) return launch<float>(a, status, s);
-    if (dtype == UFB_F16) return launch<__half>(a, status, s);
-    return launch<__nv_bfloat16>(a, status, s);
+    if (dtype == UFB_F32) return dispatch<float>(a, status, s);
+    if (dtype == UFB_F16) return dispatch<__half>(a, status, s);
+    return dispatch<__nv_bfloat16>(a, status, s);
 }
 
 }  // namespace ufb
