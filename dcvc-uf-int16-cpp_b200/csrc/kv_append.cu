@@ -8,8 +8,9 @@
 // steps (a page and head hold at most 16384 of them, 64 a thread), so HBM sees
 // each input once and each byte of the cache at most once: the call is bound by
 // those bytes, or by its latency when every stream brings one token.
-// Every step is one IEEE operation in 32 bits (1 / 127 a constant, x / s' a division):
-// the integers do not depend on the order of work.
+// Every step is one IEEE operation in 32 bits (1 / 127 a constant, x / s' a
+// division, done as a product wherever that cannot change the integer): the
+// integers do not depend on the order of work.
 #include "attention.h"
 
 #include "capi_util.h"
@@ -52,20 +53,37 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
     }
 }
 
-__device__ __forceinline__ int8_t quantise(float x, float scale) {
+// rint(x / scale), saturated; any float values.
+__device__ __forceinline__ uint32_t quantise(float x, float scale) {
     if (scale == 0.0f) return 0;
     const float v = x / scale;
-    return v == v ? static_cast<int8_t>(__float2int_rn(fminf(fmaxf(v, -127.0f), 127.0f))) : 0;
+    return v == v ? static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(v, -127.0f), 127.0f))) & 0xff : 0;
 }
 
-// grid (touched pages of a stream, streams, heads * 2)
-template <typename T>
+// The same for finite x with |x / scale| <= 127.5 and a scale above 2^-100, inv =
+// 1 / scale: x inv is within 127 * 3 * 2^-24 < 2^-15 of the quotient, so its
+// nearest integer is the quotient's unless a tie is that close; those few are
+// divided.  Adding 1.5 * 2^23 rounds to the nearest integer and leaves it in the
+// low byte.
+__device__ __forceinline__ uint32_t quantise_near(float x, float scale, float inv) {
+    const float v = x * inv, t = v + 12582912.0f;
+    uint32_t q = __float_as_uint(t);
+    if (fabsf(v - (t - 12582912.0f)) > 0.5f - 3.0517578125e-5f) q = __float_as_uint(x / scale + 12582912.0f);
+    return q & 0xff;
+}
+
+// A CTA to a (touched page of a stream, head, side): blockIdx.x = page * 2 heads +
+// 2 head + side, so that neighbours read the same tokens; blockIdx.y = stream.
+// G 8-element groups a thread hold a page's new values.
+template <typename T, int D, int G>
 __global__ void __launch_bounds__(kThreads) append_kernel(const ufb_kv_cache c, int layer, const KvBatch b,
                                                           const ufb_heads k, const ufb_heads v, int* status) {
-    constexpr int kMax = 16384 / 8 / kThreads;  // 8-element groups a thread may hold
     __shared__ float top_warp[kThreads / 32];
+    constexpr int per = D / 8;
     const int stream = blockIdx.y;
-    const int head = blockIdx.z >> 1, side = blockIdx.z & 1;
+    const int sides = 2 * c.heads;
+    const int at_page = blockIdx.x / sides, part = blockIdx.x - at_page * sides;
+    const int head = part >> 1, side = part & 1;
     const int slot = b.slots[stream];
     const long long t0 = b.offsets[stream];
     const long long count = b.offsets[stream + 1] - t0;
@@ -75,13 +93,13 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const ufb_kv_cache c, 
         if (first_thread) atomicCAS(status, 0, kStatusIndex);
         return;
     }
-    const int P = c.page_tokens, D = c.head_dim;
+    const int P = c.page_tokens;
     const long long length = c.lengths[slot], start = length - count;
     if (start < 0) {
         if (first_thread) atomicCAS(status, 0, kStatusIndex);
         return;
     }
-    const long long entry = start / P + blockIdx.x;
+    const long long entry = start / P + at_page;
     if (entry * P >= length) return;
     const int page = entry < c.table_width ? c.table[static_cast<long long>(slot) * c.table_width + entry] : -1;
     if (page < 0 || page >= c.pages) {
@@ -92,46 +110,55 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const ufb_kv_cache c, 
     const int hi = static_cast<int>(min(length - entry * P, static_cast<long long>(P)));
     const long long tile = ((static_cast<long long>(layer) * c.pages + page) * 2 + side) * c.heads + head;
     int8_t* q = c.kv + tile * P * D;
+    const float before = lo > 0 ? c.scale[tile] : 0.0f;
 
     const ufb_heads& x = side ? v : k;
     const T* in = static_cast<const T*>(x.data) + (t0 + entry * P + lo - start) * x.token_stride + head * x.head_stride;
-    const int per = D / 8, groups = (hi - lo) * per;
-    float f[kMax][8];
+    const int groups = (hi - lo) * per;
+    float f[G][8];
     float top = 0.0f;
+    bool odd = false;
 #pragma unroll
-    for (int i = 0; i < kMax; ++i) {
+    for (int i = 0; i < G; ++i) {
         const int g = threadIdx.x + i * kThreads;
         if (g < groups) load8<T>(in + (g / per) * x.token_stride + (g % per) * 8, f[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kMax; ++i) {
-        const int g = threadIdx.x + i * kThreads;
-        if (g < groups) {
+    for (int i = 0; i < G; ++i) {
+        if (threadIdx.x + i * kThreads < groups) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float m = fabsf(f[i][j]);
-                if (m < __int_as_float(0x7f800000)) top = fmaxf(top, m);
+                const bool finite = m < __int_as_float(0x7f800000);
+                odd |= !finite;
+                top = fmaxf(top, finite ? m : 0.0f);
             }
         }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if ((threadIdx.x & 31) == 0) top_warp[threadIdx.x >> 5] = top;
-    const float before = lo > 0 ? c.scale[tile] : 0.0f;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) top = fmaxf(top, top_warp[i]);
     const float scale = fmaxf(before, top * (1.0f / 127.0f));
+    const bool near = scale > 7.888609052210118e-31f && !odd;  // 2^-100
+    const float inv = 1.0f / scale;
 
 #pragma unroll
-    for (int i = 0; i < kMax; ++i) {
+    for (int i = 0; i < G; ++i) {
         const int g = threadIdx.x + i * kThreads;
         if (g < groups) {
-            char4 w[2];
-            int8_t* o = reinterpret_cast<int8_t*>(w);
+            uint32_t w[2];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = quantise(f[i][j], scale);
-            *reinterpret_cast<uint2*>(q + static_cast<long long>(lo) * D + g * 8) = *reinterpret_cast<uint2*>(w);
+            for (int h = 0; h < 2; ++h) {
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    o[j] = near ? quantise_near(f[i][4 * h + j], scale, inv) : quantise(f[i][4 * h + j], scale);
+                w[h] = __byte_perm(__byte_perm(o[0], o[1], 0x0040), __byte_perm(o[2], o[3], 0x0040), 0x5410);
+            }
+            *reinterpret_cast<uint2*>(q + lo * D + g * 8) = make_uint2(w[0], w[1]);
         }
     }
     if (scale != before || lo == 0) {
@@ -191,13 +218,28 @@ __global__ void __launch_bounds__(kThreads) read_kernel(const ufb_kv_cache c, in
     }
 }
 
-template <typename T>
+template <typename T, int D>
 cudaError_t append(const ufb_kv_cache& c, int layer, const KvBatch& b, const ufb_heads& k, const ufb_heads& v,
                    int* status, cudaStream_t s) {
     // max_new tokens reach at most this many pages, wherever the first one falls
-    const unsigned touched = static_cast<unsigned>((static_cast<long long>(b.max_new) + c.page_tokens - 2) / c.page_tokens + 1);
-    append_kernel<T><<<dim3(touched, b.n, 2 * c.heads), kThreads, 0, s>>>(c, layer, b, k, v, status);
+    const long long touched = (static_cast<long long>(b.max_new) + c.page_tokens - 2) / c.page_tokens + 1;
+    const long long blocks = touched * 2 * c.heads;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+    const dim3 grid(static_cast<unsigned>(blocks), b.n);
+    // as many registers as a page's new values (or, with few, the call's) need
+    const int tokens = b.max_new < c.page_tokens ? b.max_new : c.page_tokens;
+    const int groups = (tokens * (D / 8) + kThreads - 1) / kThreads;
+    if (groups <= 1) append_kernel<T, D, 1><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, status);
+    else if (groups <= 2) append_kernel<T, D, 2><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, status);
+    else if (groups <= 4) append_kernel<T, D, 4><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, status);
+    else append_kernel<T, D, 8><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, status);
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t append_dim(const ufb_kv_cache& c, int layer, const KvBatch& b, const ufb_heads& k, const ufb_heads& v,
+                       int* status, cudaStream_t s) {
+    return c.head_dim == 64 ? append<T, 64>(c, layer, b, k, v, status, s) : append<T, 128>(c, layer, b, k, v, status, s);
 }
 
 template <typename T>
@@ -213,9 +255,9 @@ cudaError_t read(const ufb_kv_cache& c, int layer, const int32_t* pages, long lo
 
 cudaError_t kv_append(const ufb_kv_cache& c, int layer, const KvBatch& b, int dtype, const ufb_heads& k,
                       const ufb_heads& v, int* status, cudaStream_t s) {
-    if (dtype == UFB_F32) return append<float>(c, layer, b, k, v, status, s);
-    if (dtype == UFB_F16) return append<__half>(c, layer, b, k, v, status, s);
-    return append<__nv_bfloat16>(c, layer, b, k, v, status, s);
+    if (dtype == UFB_F32) return append_dim<float>(c, layer, b, k, v, status, s);
+    if (dtype == UFB_F16) return append_dim<__half>(c, layer, b, k, v, status, s);
+    return append_dim<__nv_bfloat16>(c, layer, b, k, v, status, s);
 }
 
 cudaError_t kv_read(const ufb_kv_cache& c, int layer, const int32_t* pages, long long n, int dtype, void* out,
