@@ -1,13 +1,13 @@
 // New keys and values into the 8-bit cache (ufb_kv_append) and the values that
 // pages stand for (ufb_kv_read).
 //
-// One scale serves a page, head and side, so a CTA takes one (page, head, side)
-// that a stream's new tokens reach: it finds max |x| over the new tokens of the
-// page, s' = max(s, max * (1 / 127)), requantises the earlier tokens only when s' grew,
-// and writes the new integers.  The new values stay in registers between the two
-// steps (a page and head hold at most 16384 of them, 64 a thread), so HBM sees
-// each input once and each byte of the cache at most once: the call is bound by
-// those bytes, or by its latency when every stream brings one token.
+// One scale serves a page, head and side, so a team of threads takes one (page,
+// head, side) that a stream's new tokens reach: it finds max |x| over the new
+// tokens of the page, s' = max(s, max * (1 / 127)), requantises the earlier tokens
+// only when s' grew, and writes the new integers.  The new values stay in
+// registers between the two steps, so HBM sees each input once and each byte of
+// the cache at most once: the call is bound by those bytes, or by its latency
+// when every stream brings one token.
 // Every step is one IEEE operation in 32 bits (1 / 127 a constant, x / s' a
 // division, done as a product wherever that cannot change the integer): the
 // integers do not depend on the order of work.
@@ -24,28 +24,42 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Eight elements as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]);
-
+struct Raw {
+    uint4 v;
+};
 template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&f)[8]) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+struct Raw<float> {
+    uint4 v, w;
+};
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load8(const T* p) {
+    Raw<T> r;
+    r.v = *reinterpret_cast<const uint4*>(p);
+    return r;
 }
 template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float (&f)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ Raw<float> load8<float>(const float* p) {
+    return {reinterpret_cast<const uint4*>(p)[0], reinterpret_cast<const uint4*>(p)[1]};
+}
+
+__device__ __forceinline__ void unpack8(const Raw<float>& r, float (&f)[8]) {
+    f[0] = __uint_as_float(r.v.x), f[1] = __uint_as_float(r.v.y), f[2] = __uint_as_float(r.v.z);
+    f[3] = __uint_as_float(r.v.w), f[4] = __uint_as_float(r.w.x), f[5] = __uint_as_float(r.w.y);
+    f[6] = __uint_as_float(r.w.z), f[7] = __uint_as_float(r.w.w);
+}
+__device__ __forceinline__ void unpack8(const Raw<__half>& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
         f[2 * i] = t.x, f[2 * i + 1] = t.y;
     }
 }
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&f)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ void unpack8(const Raw<__nv_bfloat16>& r, float (&f)[8]) {
+    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         f[2 * i] = __uint_as_float(w[i] << 16);
@@ -53,124 +67,200 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
     }
 }
 
-// rint(x / scale), saturated; any float values.
-__device__ __forceinline__ uint32_t quantise(float x, float scale) {
-    if (scale == 0.0f) return 0;
-    const float v = x / scale;
-    return v == v ? static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(v, -127.0f), 127.0f))) & 0xff : 0;
+// The largest magnitude so far, NaN when any value was: of 32-bit values, or of
+// both halves of 16-bit pairs.
+__device__ __forceinline__ void top_of(uint32_t& top, const Raw<float>& r) {
+    const uint32_t w[8] = {r.v.x, r.v.y, r.v.z, r.v.w, r.w.x, r.w.y, r.w.z, r.w.w};
+    // magnitudes order like their bits without the sign, infinities and NaN last
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, w[i] & 0x7fffffffu);
+}
+__device__ __forceinline__ void top_of(uint32_t& top, const Raw<__half>& r) {
+    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&top), __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+        top = *reinterpret_cast<const uint32_t*>(&m);
+    }
+}
+__device__ __forceinline__ void top_of(uint32_t& top, const Raw<__nv_bfloat16>& r) {
+    const uint32_t w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&top),
+                                             __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[i])));
+        top = *reinterpret_cast<const uint32_t*>(&m);
+    }
+}
+template <typename T>
+__device__ __forceinline__ float top_value(uint32_t top);
+template <>
+__device__ __forceinline__ float top_value<float>(uint32_t top) { return __uint_as_float(top); }
+template <>
+__device__ __forceinline__ float top_value<__half>(uint32_t top) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(max(top & 0xffff, top >> 16))));
+}
+template <>
+__device__ __forceinline__ float top_value<__nv_bfloat16>(uint32_t top) {
+    return __uint_as_float(max(top & 0xffff, top >> 16) << 16);
 }
 
-// The same for finite x with |x / scale| <= 127.5 and a scale above 2^-100, inv =
-// 1 / scale: x inv is within 127 * 3 * 2^-24 < 2^-15 of the quotient, so its
-// nearest integer is the quotient's unless a tie is that close; those few are
-// divided.  Adding 1.5 * 2^23 rounds to the nearest integer and leaves it in the
-// low byte.
-__device__ __forceinline__ uint32_t quantise_near(float x, float scale, float inv) {
-    const float v = x * inv, t = v + 12582912.0f;
-    uint32_t q = __float_as_uint(t);
-    if (fabsf(v - (t - 12582912.0f)) > 0.5f - 3.0517578125e-5f) q = __float_as_uint(x / scale + 12582912.0f);
-    return q & 0xff;
+// rint(x / scale) of eight values, saturated, one IEEE operation after another;
+// any float values.
+__device__ __noinline__ uint2 quantise_exact(float4 a, float4 b, float scale) {
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t w[2] = {0, 0};
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+        const float v = scale == 0.0f ? 0.0f : x[j] / scale;
+        const int q = v == v ? __float2int_rn(fminf(fmaxf(v, -127.0f), 127.0f)) : 0;
+        w[j >> 2] |= (static_cast<uint32_t>(q) & 0xff) << (8 * (j & 3));
+    }
+    return make_uint2(w[0], w[1]);
 }
 
-// A CTA to a (touched page of a stream, head, side): blockIdx.x = page * 2 heads +
-// 2 head + side, so that neighbours read the same tokens; blockIdx.y = stream.
-// G 8-element groups a thread hold a page's new values.
+// The same by products with inv = 1 / scale, for finite x with |x / scale| <=
+// 127.5 and a scale above 2^-100: x inv is within 127 * 3 * 2^-24 < 2^-15 of the
+// quotient, so its nearest integer is the quotient's unless a tie is that close.
+// false: one is, and goes to quantise_ties.  Adding 1.5 * 2^23 rounds to the
+// nearest integer and leaves it in the low byte.
+constexpr float kRound = 12582912.0f, kNoTie = 0.5f - 3.0517578125e-5f;
+__device__ __forceinline__ bool quantise_near(const float (&x)[8], float inv, uint2& out) {
+    uint32_t q[8];
+    float far = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float v = x[j] * inv, t = v + kRound;
+        far = fmaxf(far, fabsf(v - (t - kRound)));
+        q[j] = __float_as_uint(t);
+    }
+    out.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    out.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+    return far <= kNoTie;
+}
+
+// quantise_near's integers, those of them at a tie by division (16-bit inputs meet
+// ties often: half the largest value is one).
+__device__ __noinline__ uint2 quantise_ties(float4 a, float4 b, float scale, float inv) {
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float v = x[j] * inv;
+        float t = v + kRound;
+        if (fabsf(v - (t - kRound)) > kNoTie) t = x[j] / scale + kRound;
+        w[j >> 2] |= (__float_as_uint(t) & 0xff) << (8 * (j & 3));
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// `team` threads (a power of two, 32 to 256) to a tile (touched page of a stream,
+// head, side); tile = page * 2 heads + 2 head + side, so that neighbours read the
+// same tokens; blockIdx.y = stream.  G 8-element groups a thread hold a tile's new
+// values: what a thread does once for its tile costs as much as about 20 elements.
 template <typename T, int D, int G>
 __global__ void __launch_bounds__(kThreads) append_kernel(const ufb_kv_cache c, int layer, const KvBatch b,
-                                                          const ufb_heads k, const ufb_heads v, int* status) {
+                                                          const ufb_heads k, const ufb_heads v, int tiles, int team,
+                                                          int* status) {
     __shared__ float top_warp[kThreads / 32];
     constexpr int per = D / 8;
     const int stream = blockIdx.y;
     const int sides = 2 * c.heads;
-    const int at_page = blockIdx.x / sides, part = blockIdx.x - at_page * sides;
+    const int tile_index = (blockIdx.x * kThreads + threadIdx.x) / team, lane = threadIdx.x & (team - 1);
+    const int at_page = tile_index / sides, part = tile_index - at_page * sides;
     const int head = part >> 1, side = part & 1;
     const int slot = b.slots[stream];
-    const long long t0 = b.offsets[stream];
-    const long long count = b.offsets[stream + 1] - t0;
+    const int t0 = b.offsets[stream], count = b.offsets[stream + 1] - t0;
     if (count <= 0) return;
-    const bool first_thread = threadIdx.x == 0;
-    if (slot < 0 || slot >= c.slots || t0 < 0 || t0 + count > b.tokens || count > b.max_new) {
-        if (first_thread) atomicCAS(status, 0, kStatusIndex);
-        return;
+    const int P = c.page_tokens, shift = 31 - __clz(P);  // a power of two
+    int page = -1, lo = 0, hi = 0;
+    long long first = 0;   // the tile's first new token
+    if (slot < 0 || slot >= c.slots || t0 < 0 || t0 + static_cast<long long>(count) > b.tokens || count > b.max_new ||
+        c.lengths[slot] < count) {
+        if (threadIdx.x == 0) atomicCAS(status, 0, kStatusIndex);
+    } else if (tile_index < tiles) {
+        const int length = c.lengths[slot], start = length - count;
+        const int entry = (start >> shift) + at_page;
+        const long long begin = static_cast<long long>(entry) << shift;
+        if (begin < length) {
+            page = entry < c.table_width ? c.table[static_cast<long long>(slot) * c.table_width + entry] : -1;
+            if (page < 0 || page >= c.pages) {
+                page = -1;
+                if (lane == 0) atomicCAS(status, 0, kStatusIndex);
+            } else {
+                lo = static_cast<int>(max(start - begin, 0ll));
+                hi = static_cast<int>(min(length - begin, static_cast<long long>(P)));
+                first = t0 + begin + lo - start;
+            }
+        }
     }
-    const int P = c.page_tokens;
-    const long long length = c.lengths[slot], start = length - count;
-    if (start < 0) {
-        if (first_thread) atomicCAS(status, 0, kStatusIndex);
-        return;
-    }
-    const long long entry = start / P + at_page;
-    if (entry * P >= length) return;
-    const int page = entry < c.table_width ? c.table[static_cast<long long>(slot) * c.table_width + entry] : -1;
-    if (page < 0 || page >= c.pages) {
-        if (first_thread) atomicCAS(status, 0, kStatusIndex);
-        return;
-    }
-    const int lo = static_cast<int>(max(start - entry * P, 0ll));
-    const int hi = static_cast<int>(min(length - entry * P, static_cast<long long>(P)));
-    const long long tile = ((static_cast<long long>(layer) * c.pages + page) * 2 + side) * c.heads + head;
+    const long long tile = ((static_cast<long long>(layer) * c.pages + (page < 0 ? 0 : page)) * 2 + side) * c.heads + head;
     int8_t* q = c.kv + tile * P * D;
     const float before = lo > 0 ? c.scale[tile] : 0.0f;
 
     const ufb_heads& x = side ? v : k;
-    const T* in = static_cast<const T*>(x.data) + (t0 + entry * P + lo - start) * x.token_stride + head * x.head_stride;
+    const T* in = static_cast<const T*>(x.data) + first * x.token_stride + head * x.head_stride +
+                  (lane / per) * x.token_stride + (lane % per) * 8;
     const int groups = (hi - lo) * per;
-    float f[G][8];
-    float top = 0.0f;
-    bool odd = false;
+    const long long step = (team / per) * x.token_stride;   // team is a multiple of per
+    Raw<T> raw[G];
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-        const int g = threadIdx.x + i * kThreads;
-        if (g < groups) load8<T>(in + (g / per) * x.token_stride + (g % per) * 8, f[i]);
-    }
+    for (int i = 0; i < G; ++i)
+        if (lane + i * team < groups) raw[i] = load8<T>(in + i * step);
+    uint32_t bits = 0;
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-        if (threadIdx.x + i * kThreads < groups) {
+    for (int i = 0; i < G; ++i)
+        if (lane + i * team < groups) top_of(bits, raw[i]);
+    float top = top_value<T>(bits);
+    const bool odd = !(top < __int_as_float(0x7f800000));
+    if (odd) {
+        // not all finite: the largest of those that are
+        top = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float m = fabsf(f[i][j]);
-                const bool finite = m < __int_as_float(0x7f800000);
-                odd |= !finite;
-                top = fmaxf(top, finite ? m : 0.0f);
-            }
+        for (int i = 0; i < G; ++i) {
+            if (lane + i * team >= groups) continue;
+            float f[8];
+            unpack8(raw[i], f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fabsf(f[j]) < __int_as_float(0x7f800000) ? fmaxf(top, fabsf(f[j])) : top;
         }
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if ((threadIdx.x & 31) == 0) top_warp[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kThreads / 32; ++i) top = fmaxf(top, top_warp[i]);
+    if (team > 32) {
+        if ((threadIdx.x & 31) == 0) top_warp[threadIdx.x >> 5] = top;
+        __syncthreads();
+        const int warp0 = (threadIdx.x & ~(team - 1)) >> 5;
+        for (int i = 0; i < team / 32; ++i) top = fmaxf(top, top_warp[warp0 + i]);
+    }
+    if (page < 0) return;
     const float scale = fmaxf(before, top * (1.0f / 127.0f));
     const bool near = scale > 7.888609052210118e-31f && !odd;  // 2^-100
     const float inv = 1.0f / scale;
 
 #pragma unroll
     for (int i = 0; i < G; ++i) {
-        const int g = threadIdx.x + i * kThreads;
+        const int g = lane + i * team;
         if (g < groups) {
-            uint32_t w[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t o[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    o[j] = near ? quantise_near(f[i][4 * h + j], scale, inv) : quantise(f[i][4 * h + j], scale);
-                w[h] = __byte_perm(__byte_perm(o[0], o[1], 0x0040), __byte_perm(o[2], o[3], 0x0040), 0x5410);
-            }
-            *reinterpret_cast<uint2*>(q + lo * D + g * 8) = make_uint2(w[0], w[1]);
+            float f[8];
+            unpack8(raw[i], f);
+            uint2 w;
+            const float4 a = make_float4(f[0], f[1], f[2], f[3]), z = make_float4(f[4], f[5], f[6], f[7]);
+            if (!near) w = quantise_exact(a, z, scale);
+            else if (!quantise_near(f, inv, w)) w = quantise_ties(a, z, scale, inv);
+            *reinterpret_cast<uint2*>(q + lo * D + g * 8) = w;
         }
     }
     if (scale != before || lo == 0) {
         const float ratio = before / scale;  // used for earlier tokens only: lo > 0, scale > 0
-        for (int i = threadIdx.x; i < lo * D / 16; i += kThreads) {
+        for (int i = lane; i < lo * D / 16; i += team) {
             uint4 w = reinterpret_cast<uint4*>(q)[i];
             int8_t* o = reinterpret_cast<int8_t*>(&w);
-#pragma unroll
+#pragma unroll 4
             for (int j = 0; j < 16; ++j) o[j] = static_cast<int8_t>(__float2int_rn(static_cast<float>(o[j]) * ratio));
             reinterpret_cast<uint4*>(q)[i] = w;
         }
-        if (first_thread) c.scale[tile] = scale;
+        if (lane == 0) c.scale[tile] = scale;
     }
 }
 
@@ -223,16 +313,21 @@ cudaError_t append(const ufb_kv_cache& c, int layer, const KvBatch& b, const ufb
                    int* status, cudaStream_t s) {
     // max_new tokens reach at most this many pages, wherever the first one falls
     const long long touched = (static_cast<long long>(b.max_new) + c.page_tokens - 2) / c.page_tokens + 1;
-    const long long blocks = touched * 2 * c.heads;
-    if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-    const dim3 grid(static_cast<unsigned>(blocks), b.n);
-    // as many registers as a page's new values (or, with few, the call's) need
+    const long long tiles = touched * 2 * c.heads;
+    if (tiles > 0x7fffffffll / 256) return cudaErrorInvalidValue;
+    // 8 groups a thread (a page of 64 tokens x 128: 54 us for 32640 float16 tokens of 8
+    // heads; 4 groups 58, 16 groups 87 us); calls of few tokens need their latency: 1
+    constexpr int kMost = 8;
     const int tokens = b.max_new < c.page_tokens ? b.max_new : c.page_tokens;
-    const int groups = (tokens * (D / 8) + kThreads - 1) / kThreads;
-    if (groups <= 1) append_kernel<T, D, 1><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, status);
-    else if (groups <= 2) append_kernel<T, D, 2><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, status);
-    else if (groups <= 4) append_kernel<T, D, 4><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, status);
-    else append_kernel<T, D, 8><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, status);
+    const int groups = tokens * (D / 8);
+    const int most = groups <= kThreads ? 1 : kMost;
+    int team = 32;
+    while (team * most < groups) team *= 2;
+    const dim3 grid(static_cast<unsigned>((tiles * team + kThreads - 1) / kThreads), b.n);
+    if (most == 1)
+        append_kernel<T, D, 1><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, static_cast<int>(tiles), team, status);
+    else
+        append_kernel<T, D, kMost><<<grid, kThreads, 0, s>>>(c, layer, b, k, v, static_cast<int>(tiles), team, status);
     return cudaGetLastError();
 }
 
