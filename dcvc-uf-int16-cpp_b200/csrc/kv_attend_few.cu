@@ -11,14 +11,18 @@
 // Bound by the bytes of the cache.  Work is divided by tiles of 64 keys
 // (kv_attend.cuh), one CTA to an SM; a producer warp streams the integers by TMA
 // into a ring (8 stages, 128 KB in flight at head_dim 128, against the 35 KB that
-// HBM's latency needs), and two groups of four warps take the stages in turn, 16
-// keys a warp.  With at most 16 rows the products are m16n8k16 tensor
-// instructions on registers: a tile of 128 rows, which tcgen05 needs, would be
-// seven eighths padding and its operands would have to go back through shared
-// memory as float16, while here the integers are expanded in the registers they
-// were loaded to.  Which dims and keys share an instruction is free as long as
-// both operands agree; the order below makes every shared-memory read 16 (or 8)
-// bytes wide and free of bank conflicts under TMA's 128-byte swizzle.
+// HBM's latency needs), and the other warps take 32 keys of a stage each, in turn.
+//
+// The products are m16n8k16 tensor instructions on registers with the rows as the
+// narrow side: S^T = K Q^T and O^T = V^T P^T in tiles of 8 rows.  A tile of 128
+// rows, which tcgen05 needs, would be mostly padding here, and its operands would
+// have to go back through shared memory as float16, while these integers are
+// expanded in the registers they were loaded to.  8 rows (one token of up to 8
+// query heads) leave registers for 15 consumer warps, 16 rows for 7: the
+// expansion is a chain of dependent instructions, and warps are what hides it.
+// Which dims and keys share an instruction is free as long as both operands agree;
+// the order below makes every shared-memory read 16 (or 8) bytes wide and free of
+// bank conflicts under TMA's 128-byte swizzle.
 //
 // Parts of an item that several CTAs share are joined by the CTA that arrives
 // last, in the order of the CTAs, so the sum does not depend on which one it is.
@@ -26,17 +30,18 @@
 #include "umma.cuh"
 
 #include <mutex>
+#include <type_traits>
 
 namespace ufb {
 
 namespace {
 
-constexpr int kRows = 16;
 constexpr int kKeys = 64;             // keys of a stage
-constexpr int kWarps = 8;             // consumer warps
-constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kWarpKeys = 32;         // keys of a consumer warp's step
 constexpr int kStages = 8;
 constexpr int kGroups = kKeys / kGroupKeys;
+// With 8 (NT 1) or 16 (NT 2) rows: consumer warps; the producer makes 16 or 8 of it.
+__host__ __device__ constexpr int consumers(int nt) { return nt == 1 ? 15 : 7; }
 // P is taken times 2^kShift: at most 2^15, inside float16, and weights down to
 // 2^-29 of the largest keep all 11 bits.
 constexpr float kShift = 15.0f;
@@ -47,11 +52,11 @@ struct PageScales {
     float pad;
 };
 
-template <int D>
+template <int D, int NT>
 struct Smem {
-    alignas(1024) uint8_t ring[kStages][2][kKeys * D];   // key, value integers
-    float sums[kWarps][kRows][D];
-    float stats[2][2][kWarps][kRows];                    // by piece parity: maxima, weights
+    alignas(1024) uint8_t ring[kStages][2][kKeys * D];      // key, value integers
+    float sums[consumers(NT)][8 * NT][D];
+    float stats[2][2][consumers(NT)][8 * NT];               // by piece parity: maxima, weights
     PageScales scales[kStages][kGroups];
     alignas(8) uint64_t full[kStages], empty[kStages];
     ShareSmem share;
@@ -60,39 +65,49 @@ struct Smem {
 };
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+// The transpose of an 8 x 8 matrix of float16, a row to four lanes.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+template <int N>
+__device__ __forceinline__ void consumers_sync() {
+    asm volatile("bar.sync 1, %0;" ::"n"(N * 32) : "memory");
+}
 
 // The dims of lane quarter c in k step t, four in a row (also Q's fragments).
 template <int D>
 __device__ __forceinline__ int key_dim(int c, int t) {
     return D == 128 ? (t >> 2) * 64 + c * 16 + (t & 3) * 4 : (t >> 1) * 32 + c * 8 + (t & 1) * 4;
 }
-// The first of the D / 8 dims of output column n (0..7), one a value tile.
+// The first of the D / 8 dims that lane row n (0..7) has of a value row.
 template <int D>
 __device__ __forceinline__ int value_dim(int n) {
     if (D == 128) return (((n & 1) << 2) | (n >> 1)) * 16;
     const int pair = n >> 1;  // 16-byte chunks 0, 2, 1, 3
     return ((((pair & 1) << 1) | (pair >> 1)) * 2 + (n & 1)) * 8;
 }
-// The key (of 8) that column n of a score tile stands for.
+// The key (of 8) that lane row n of a score tile stands for.
 __device__ __forceinline__ int key_of(int n) { return ((n & 1) << 2) | (n >> 1); }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant__ CUtensorMap map, const AttendArgs a,
-                                                          int row_tiles, int min_share) {
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
+    few_kernel(const __grid_constant__ CUtensorMap map, const AttendArgs a, int row_tiles, int min_share) {
+    constexpr int kWarps = consumers(NT), kRows = 8 * NT, kThreads = 32 * (kWarps + 1);
     extern __shared__ uint8_t raw[];
-    Smem<D>& sm = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&sm.full[i], 1);
-            mbar_init(&sm.empty[i], kWarps / 2);
+            mbar_init(&sm.empty[i], kKeys / kWarpKeys);
         }
         fence_mbar_init();
         sm.dead = 0;
@@ -205,26 +220,25 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 
     // ---- consumers
     const int g = lane >> 2, c = lane & 3;
-    const int half = warp >> 2, quarter = warp & 3;
-    constexpr int kSteps = D / 16, kTiles = D / 8;
+    constexpr int kSteps = D / 16, kTiles = D / 16;   // of keys' dims; of output dims
     const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
     int it = 0, parity = 0;
     Piece p;
     while (walk.next(a, p)) {
-        // Q fragments: rows g and g + 8, brought to [1/2, 1) and rounded to float16
-        uint32_t q[kSteps][4];
-        float unit[2];
-        int pos[2];   // where the row stands
+        // Q fragments: row 8 n + g, brought to [1/2, 1) and rounded to float16; then what
+        // the scores of rows 8 n + 2 c and + 1 need
+        uint32_t q[NT][kSteps][2];
+        float unit[NT][2], offset[NT][2];
+        int pos[NT][2];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = g + r * 8;
+        for (int n = 0; n < NT; ++n) {
+            const int row = n * 8 + g;
             const bool real = row < p.t.rows;
             const int in_stream = p.t.row0 + row;
             const int token = real ? in_stream / a.group : 0;
-            pos[r] = p.t.length - p.t.n_new + token;
             const T* src = static_cast<const T*>(a.q.data) + (p.t.token0 + token) * a.q.token_stride +
                            (p.head * a.group + in_stream - token * a.group) * a.q.head_stride;
-            float top = 0.0f;
+            float top = 0.0f, odd = 0.0f;
             uint2 w[kSteps];
 #pragma unroll
             for (int t = 0; t < kSteps; ++t) {
@@ -234,193 +248,254 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
 #pragma unroll
             for (int t = 0; t < kSteps; ++t) {
                 const float2 x = unpack2(w[t].x, T()), y = unpack2(w[t].y, T());
-                const float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y)));
-                // fmaxf drops NaN: x - x is NaN for what is not finite
-                const float odd = (x.x - x.x) + (x.y - x.y) + (y.x - y.x) + (y.y - y.y);
-                top = odd == odd && top == top ? fmaxf(top, m) : __int_as_float(0x7fffffff);
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+                odd += (x.x - x.x) + (x.y - x.y) + (y.x - y.x) + (y.y - y.y);  // NaN for what is not finite
             }
 #pragma unroll
             for (int o = 1; o < 4; o <<= 1) {
-                const float other = __shfl_xor_sync(0xffffffffu, top, o);
-                top = top == top && other == other ? fmaxf(top, other) : __int_as_float(0x7fffffff);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                odd += __shfl_xor_sync(0xffffffffu, odd, o);
             }
-            const float u = row_unit(top);
-            unit[r] = unit_inverse(u) * a.scale_log2;
+            const float u = row_unit(odd == odd ? top : odd);
             const float mul = u == u ? u : 0.0f;
+            float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < kSteps; ++t) {
                 const float2 x = unpack2(w[t].x, T()), y = unpack2(w[t].y, T());
-                q[t][r] = pack2(x.x * mul, x.y * mul, __half());
-                q[t][2 + r] = pack2(y.x * mul, y.y * mul, __half());
+                q[n][t][0] = pack2(x.x * mul, x.y * mul, __half());
+                q[n][t][1] = pack2(y.x * mul, y.y * mul, __half());
+                const float2 x16 = unpack2(q[n][t][0], __half()), y16 = unpack2(q[n][t][1], __half());
+                sum += (x16.x + x16.y) + (y16.x + y16.y);
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const float f = unit_inverse(u) * a.scale_log2;
+            const int at = p.t.length - p.t.n_new + token;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int from = (2 * c + r) * 4;
+                // keys enter as (integer + 128) 2^-24 (below): scale and offset take that back
+                unit[n][r] = __shfl_sync(0xffffffffu, f, from) * 16777216.0f;
+                offset[n][r] = __shfl_sync(0xffffffffu, sum, from) * (-128.0f / 16777216.0f);
+                pos[n][r] = __shfl_sync(0xffffffffu, at, from);
             }
         }
-        float o[kTiles][4];
+        float o[NT][kTiles][4];
+        float m[NT][2], l[NT][2];
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
+            m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
+        }
         const int last_pos = p.t.length - p.t.n_new + (p.t.row0 + p.t.rows - 1) / a.group;
         const int first_pos = p.t.length - p.t.n_new + p.t.row0 / a.group;
 
-        for (int t = p.first; t < p.end; ++t, ++it) {
-            if ((it & 1) != half) continue;
-            const int stage = it % kStages;
+        // steps of 32 keys go round the warps
+        const int steps_before = it * (kKeys / kWarpKeys);
+        const int steps = (p.end - p.first) * (kKeys / kWarpKeys);
+        int step = (warp - steps_before % kWarps + kWarps) % kWarps;
+#pragma unroll 1
+        for (; step < steps; step += kWarps) {
+            const int index = it + step / (kKeys / kWarpKeys), stage = index % kStages;
+            const int part = (step % (kKeys / kWarpKeys)) * kWarpKeys;
             // after a wait gave up the warps go on without waiting: they meet at barriers
-            if (!*dead && !mbar_wait(&sm.full[stage], (it / kStages) & 1, a.status, kCodeFull)) *dead = 1;
-            const PageScales sc = sm.scales[stage][quarter];
-            // S: two tiles of 8 keys
+            if (!mbar_try_wait(&sm.full[stage], (index / kStages) & 1) && !*dead &&
+                !mbar_wait(&sm.full[stage], (index / kStages) & 1, a.status, kCodeFull))
+                *dead = 1;
+            __syncwarp();
+            constexpr int kM = kWarpKeys / 16;    // score tiles of 16 keys
+            const PageScales* sc = &sm.scales[stage][part / kGroupKeys];
             const uint8_t* keys = sm.ring[stage][0];
             const uint8_t* values = sm.ring[stage][1];
-            float s[2][4];
+            float s[kM][NT][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                s[h][0] = s[h][1] = s[h][2] = s[h][3] = 0.0f;
-                const int key = quarter * 16 + h * 8 + key_of(g);
-                uint32_t w[kSteps];
-                if (D == 128) {
+            for (int x = 0; x < kM; ++x)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(keys + key * 128 + (((c + i * 4) ^ (key & 7)) << 4));
-                        w[i * 4] = v.x, w[i * 4 + 1] = v.y, w[i * 4 + 2] = v.z, w[i * 4 + 3] = v.w;
+                for (int n = 0; n < NT; ++n) s[x][n][0] = s[x][n][1] = s[x][n][2] = s[x][n][3] = 0.0f;
+            // S^T, half the dims at a time
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t w[kM][2][kSteps / 2];
+#pragma unroll
+                for (int x = 0; x < kM; ++x)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int key = part + x * 16 + h * 8 + key_of(g);
+                        if (D == 128) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(keys + key * 128 + (((c + i * 4) ^ (key & 7)) << 4));
+                            w[x][h][0] = v.x, w[x][h][1] = v.y;
+                            w[x][h][2 % (kSteps / 2)] = v.z, w[x][h][3 % (kSteps / 2)] = v.w;
+                        } else {
+                            const int row = key >> 1;
+                            const uint2 v = *reinterpret_cast<const uint2*>(
+                                keys + row * 128 + ((((key & 1) * 4 + i * 2 + (c >> 1)) ^ (row & 7)) << 4) + (c & 1) * 8);
+                            w[x][h][0] = v.x, w[x][h][1] = v.y;
+                        }
                     }
-                } else {
-                    const int row = key >> 1, base = (key & 1) * 4;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint2 v = *reinterpret_cast<const uint2*>(
-                            keys + row * 128 + (((base + i * 2 + (c >> 1)) ^ (row & 7)) << 4) + (c & 1) * 8);
-                        w[i * 2] = v.x, w[i * 2 + 1] = v.y;
+                for (int k = 0; k < kSteps / 2; ++k)
+#pragma unroll
+                    for (int x = 0; x < kM; ++x) {
+                        // an integer plus 128 in the low byte is a float16 below the normal ones,
+                        // (integer + 128) 2^-24, exactly
+                        const uint32_t u = w[x][0][k] ^ 0x80808080u, v = w[x][1][k] ^ 0x80808080u;
+                        const uint32_t f[4] = {__byte_perm(u, 0, 0x4140), __byte_perm(v, 0, 0x4140),
+                                               __byte_perm(u, 0, 0x4342), __byte_perm(v, 0, 0x4342)};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            mma16816(s[x][n], f, q[n][i * (kSteps / 2) + k][0], q[n][i * (kSteps / 2) + k][1]);
+                    }
+            }
+            // scores in base 2 with the value scale, the maximum, P
+            const int key0 = p.t.keys.tile(p.first + step / (kKeys / kWarpKeys)) * kKeys + part;
+            const bool clear = (!a.causal || key0 + kWarpKeys - 1 <= first_pos) && key0 + kWarpKeys <= p.t.length &&
+                               (!a.window || last_pos - key0 < a.window || key0 + kWarpKeys <= a.sinks);
+            uint32_t pb[kM][NT][2];
+            auto softmax = [&](auto masked) {
+                constexpr bool kMasked = decltype(masked)::value;
+                uint32_t hidden = 0;   // of this thread's scores, a bit each
+                float top[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    top[n][0] = top[n][1] = -INFINITY;
+#pragma unroll
+                    for (int x = 0; x < kM; ++x) {
+                        const float f[2] = {unit[n][0] * sc[x].key, unit[n][1] * sc[x].key};
+                        const float add[2] = {fmaf(f[0], offset[n][0], sc[x].log2_value), fmaf(f[1], offset[n][1], sc[x].log2_value)};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[x][n][e] = fmaf(s[x][n][e], f[e & 1], add[e & 1]);
+                            if (kMasked) {
+                                const int key = key0 + x * 16 + (e >> 1) * 8 + key_of(g), at = pos[n][e & 1];
+                                const bool seen = key < p.t.length && (!a.causal || key <= at) &&
+                                                  (!a.window || at - key < a.window || key < a.sinks);
+                                if (!seen) s[x][n][e] = -INFINITY, hidden |= 1u << ((x * NT + n) * 4 + e);
+                            }
+                            top[n][e & 1] = fmaxf(top[n][e & 1], s[x][n][e]);
+                        }
+                    }
+                }
+                bool grew = false;
+                float keep[NT][2], base[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float x = top[n][r];
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        const float next = fmaxf(m[n][r], x);
+                        grew |= next > m[n][r];
+                        keep[n][r] = next == -INFINITY ? 1.0f : ex2(m[n][r] - next);
+                        base[n][r] = next == -INFINITY ? 0.0f : next - kShift;
+                        m[n][r] = next;
+                    }
+                if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int j = 0; j < kTiles; ++j) {
+                            o[n][j][0] *= keep[n][0], o[n][j][1] *= keep[n][1];
+                            o[n][j][2] *= keep[n][0], o[n][j][3] *= keep[n][1];
+                        }
+                        l[n][0] *= keep[n][0], l[n][1] *= keep[n][1];
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    uint32_t b0, b1;
-                    int8x4_to_half(w[k], b0, b1);
-                    mma16816(s[h], q[k], b0, b1);
+                for (int x = 0; x < kM; ++x)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            s[x][n][e] = ex2(s[x][n][e] - base[n][e & 1]);
+                            // a hidden weight is 0 also where its row or scale is not finite
+                            if (kMasked && (hidden & (1u << ((x * NT + n) * 4 + e)))) s[x][n][e] = 0.0f;
+                        }
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float sum = s[x][n][r] + s[x][n][2 + r];
+                            if (sum != 0.0f) l[n][r] = fmaf(sum, sc[x].inv_value, l[n][r]);
+                        }
+                        // from (key, two rows) to (two keys, row)
+                        pb[x][n][0] = transpose8(pack2(s[x][n][0], s[x][n][1], __half()));
+                        pb[x][n][1] = transpose8(pack2(s[x][n][2], s[x][n][3], __half()));
+                    }
+            };
+            if (clear) softmax(std::false_type());
+            else softmax(std::true_type());
+            // O^T += V^T P^T, 16 keys at a time
+#pragma unroll
+            for (int x = 0; x < kM; ++x) {
+                uint32_t v[4][D / 32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = part + x * 16 + (i >> 1) * 8 + (i & 1) * 4 + c;
+                    if (D == 128) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(values + key * 128 + (((value_dim<D>(g) >> 4) ^ (key & 7)) << 4));
+                        v[i][0] = y.x, v[i][1] = y.y, v[i][2 % (D / 32)] = y.z, v[i][3 % (D / 32)] = y.w;
+                    } else {
+                        const int row = key >> 1, chunk = (key & 1) * 4 + (value_dim<D>(g) >> 4);
+                        const uint2 y = *reinterpret_cast<const uint2*>(values + row * 128 + ((chunk ^ (row & 7)) << 4) + (g & 1) * 8);
+                        v[i][0] = y.x, v[i][1] = y.y;
+                    }
+                }
+                if (x == kM - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.empty[stage]);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const uint32_t w0 = v[0][i] ^ 0x80808080u, w1 = v[1][i] ^ 0x80808080u;
+                    const uint32_t w2 = v[2][i] ^ 0x80808080u, w3 = v[3][i] ^ 0x80808080u;
+                    // (key, key') pairs of dims 0, 1 and of dims 2, 3 of the word
+                    const uint32_t e[2][2] = {{__byte_perm(w0, w1, 0x5140), __byte_perm(w2, w3, 0x5140)},
+                                              {__byte_perm(w0, w1, 0x7362), __byte_perm(w2, w3, 0x7362)}};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t f[4] = {half2_minus_1152(__byte_perm(e[j][0], 0x64646464u, 0x4140)),
+                                               half2_minus_1152(__byte_perm(e[j][0], 0x64646464u, 0x4342)),
+                                               half2_minus_1152(__byte_perm(e[j][1], 0x64646464u, 0x4140)),
+                                               half2_minus_1152(__byte_perm(e[j][1], 0x64646464u, 0x4342))};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma16816(o[n][i * 2 + j], f, pb[x][n][0], pb[x][n][1]);
+                    }
                 }
             }
-            // scores in base 2, with the value scale
-            const int key0 = p.t.keys.tile(t) * kKeys + quarter * kGroupKeys;
-            const bool clear = (!a.causal || key0 + kGroupKeys - 1 <= first_pos) && key0 + kGroupKeys <= p.t.length &&
-                               (!a.window || last_pos - key0 < a.window || key0 + kGroupKeys <= a.sinks);
-            const float f[2] = {unit[0] * sc.key, unit[1] * sc.key};
+        }
+        it += p.end - p.first;
+
+        // ---- the warps' sums become one
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[h][e] = fmaf(s[h][e], f[e >> 1], sc.log2_value);
-            bool hidden[2][4];
-            if (!clear || sc.log2_value == -INFINITY) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + h * 8 + key_of(2 * c + (e & 1)), at = pos[e >> 1];
-                        const bool seen = key < p.t.length && (!a.causal || key <= at) &&
-                                          (!a.window || at - key < a.window || key < a.sinks);
-                        hidden[h][e] = !seen || sc.log2_value == -INFINITY;
-                        if (hidden[h][e]) s[h][e] = -INFINITY;
-                    }
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) hidden[h][e] = false;
-            }
-            float keep[2];
-            bool grew = false;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                float top = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float next = fmaxf(m[r], top);
-                grew |= next > m[r];
-                keep[r] = next == -INFINITY ? 1.0f : ex2(m[r] - next);
-                m[r] = next;
-            }
-            if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-                for (int j = 0; j < kTiles; ++j) {
-                    o[j][0] *= keep[0], o[j][1] *= keep[0];
-                    o[j][2] *= keep[1], o[j][3] *= keep[1];
-                }
-                l[0] *= keep[0], l[1] *= keep[1];
-            }
-            float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[h][e] = hidden[h][e] ? 0.0f : ex2(s[h][e] - (m[e >> 1] - kShift));
-                    if (!hidden[h][e]) sum[e >> 1] += s[h][e];
-                }
-            if (sum[0] != 0.0f) l[0] = fmaf(sum[0], sc.inv_value, l[0]);
-            if (sum[1] != 0.0f) l[1] = fmaf(sum[1], sc.inv_value, l[1]);
-            // O += P V
-            const uint32_t pa[4] = {pack2(s[0][0], s[0][1], __half()), pack2(s[0][2], s[0][3], __half()),
-                                    pack2(s[1][0], s[1][1], __half()), pack2(s[1][2], s[1][3], __half())};
-            uint32_t v[4][kTiles / 4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = quarter * 16 + (i >> 1) * 8 + (i & 1) * 4 + c;
-                if (D == 128) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(values + key * 128 + (((value_dim<D>(g) >> 4) ^ (key & 7)) << 4));
-                    v[i][0] = x.x, v[i][1] = x.y, v[i][2 % (kTiles / 4)] = x.z, v[i][3 % (kTiles / 4)] = x.w;
-                } else {
-                    const int row = key >> 1, chunk = (key & 1) * 4 + (value_dim<D>(g) >> 4);
-                    const uint2 x = *reinterpret_cast<const uint2*>(values + row * 128 + ((chunk ^ (row & 7)) << 4) + (g & 1) * 8);
-                    v[i][0] = x.x, v[i][1] = x.y;
+                for (int d = 4; d < 32; d <<= 1) l[n][r] += __shfl_xor_sync(0xffffffffu, l[n][r], d);
+                if (g == 0) {
+                    sm.stats[parity][0][warp][n * 8 + 2 * c + r] = m[n][r];
+                    sm.stats[parity][1][warp][n * 8 + 2 * c + r] = l[n][r];
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.empty[stage]);
+        consumers_sync<kWarps>();
 #pragma unroll
-            for (int i = 0; i < kTiles / 4; ++i) {
-                const uint32_t w0 = v[0][i] ^ 0x80808080u, w1 = v[1][i] ^ 0x80808080u;
-                const uint32_t w2 = v[2][i] ^ 0x80808080u, w3 = v[3][i] ^ 0x80808080u;
-                const uint32_t x0 = __byte_perm(w0, w1, 0x5140), y0 = __byte_perm(w0, w1, 0x7362);
-                const uint32_t x1 = __byte_perm(w2, w3, 0x5140), y1 = __byte_perm(w2, w3, 0x7362);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t b0 = half2_minus_1152(__byte_perm(j < 2 ? x0 : y0, 0x64646464u, (j & 1) ? 0x4342 : 0x4140));
-                    const uint32_t b1 = half2_minus_1152(__byte_perm(j < 2 ? x1 : y1, 0x64646464u, (j & 1) ? 0x4342 : 0x4140));
-                    mma16816(o[i * 4 + j], pa, b0, b1);
+            for (int r = 0; r < 2; ++r) {
+                const int row = n * 8 + 2 * c + r;
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.stats[parity][0][w][row]);
+                const float mul = m[n][r] == -INFINITY ? (l[n][r] == 0.0f ? 0.0f : 1.0f) : ex2(m[n][r] - top);
+                if (row < p.t.rows) {
+                    float* to = &sm.sums[warp][row][value_dim<D>(g)];
+#pragma unroll
+                    for (int j = 0; j < kTiles; j += 2)
+                        *reinterpret_cast<float4*>(to + j * 2) = make_float4(o[n][j][r] * mul, o[n][j][2 + r] * mul,
+                                                                             o[n][j + 1][r] * mul, o[n][j + 1][2 + r] * mul);
                 }
             }
-        }
-
-        // ---- the eight warps' sums become one
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (c == 0) {
-                sm.stats[parity][0][warp][g + 8 * r] = m[r];
-                sm.stats[parity][1][warp][g + 8 * r] = l[r];
-            }
-        }
-        consumers_sync();
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = g + 8 * r;
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.stats[parity][0][w][row]);
-            const float mul = m[r] == -INFINITY ? 0.0f : ex2(m[r] - top);
-            if (row < p.t.rows) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    float* to = &sm.sums[warp][row][value_dim<D>(2 * c + n)];
-#pragma unroll
-                    for (int j = 0; j < kTiles; j += 4)
-                        *reinterpret_cast<float4*>(to + j) =
-                            m[r] == -INFINITY && l[r] == 0.0f
-                                ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                : make_float4(o[j][2 * r + n] * mul, o[j + 1][2 * r + n] * mul, o[j + 2][2 * r + n] * mul,
-                                              o[j + 3][2 * r + n] * mul);
-                }
-            }
-        }
-        consumers_sync();
+        consumers_sync<kWarps>();
         const bool whole = p.whole();
         const int part = 2 * blockIdx.x + (p.first > 0 ? 0 : 1);
         auto finish = [&](int row, int d, float4 v, float top, float weight) {
@@ -461,13 +536,13 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
             const int c0 = static_cast<int>(p.item_start / share.per);
             const int c1 = static_cast<int>((p.item_start + p.t.keys.nt - 1) / share.per);
             __threadfence();
-            consumers_sync();
+            consumers_sync<kWarps>();
             if (threadIdx.x == 0) {
                 const int before = atomicAdd(scratch.counters + c0, 1);
                 sm.last = before == c1 - c0;
                 if (sm.last) scratch.counters[c0] = 0;
             }
-            consumers_sync();
+            consumers_sync<kWarps>();
             if (sm.last) {
                 __threadfence();
                 for (int e = threadIdx.x; e < p.t.rows * (D / 4); e += kWarps * 32) {
@@ -496,10 +571,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_kernel(const __grid_constant_
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
-    auto kernel = few_kernel<T, D>;
-    const int smem = sizeof(Smem<D>) + 1024;
+    auto kernel = few_kernel<T, D, NT>;
+    const int smem = sizeof(Smem<D, NT>) + 1024;
     static std::once_flag once;
     static cudaError_t attr = cudaSuccess;
     std::call_once(once, [&] { attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
@@ -507,17 +582,23 @@ cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     CUtensorMap map;
     // boxes of the keys that lie together in a page, 64 at most
     if (!kv_tensor_map(map, a, kKeys)) return cudaErrorInvalidValue;
-    const int row_tiles = static_cast<int>((static_cast<long long>(a.max_new) * a.group + kRows - 1) / kRows);
-    few_kernel<T, D><<<sms < kAttendMaxCtas ? sms : kAttendMaxCtas, kThreads, smem, s>>>(map, a, row_tiles, 1);
+    const int row_tiles = static_cast<int>((static_cast<long long>(a.max_new) * a.group + 8 * NT - 1) / (8 * NT));
+    kernel<<<sms < kAttendMaxCtas ? sms : kAttendMaxCtas, 32 * (consumers(NT) + 1), smem, s>>>(map, a, row_tiles, 1);
     return cudaGetLastError();
+}
+
+template <typename T, int D>
+cudaError_t launch_rows(const AttendArgs& a, int sms, cudaStream_t s) {
+    const long long rows = static_cast<long long>(a.max_new) * a.group;
+    return rows <= 8 ? launch<T, D, 1>(a, sms, s) : launch<T, D, 2>(a, sms, s);
 }
 
 }  // namespace
 
 cudaError_t attend_few(const AttendArgs& a, int dtype, int sms, cudaStream_t s) {
     if (a.head_dim == 64)
-        return dtype == UFB_F16 ? launch<__half, 64>(a, sms, s) : launch<__nv_bfloat16, 64>(a, sms, s);
-    return dtype == UFB_F16 ? launch<__half, 128>(a, sms, s) : launch<__nv_bfloat16, 128>(a, sms, s);
+        return dtype == UFB_F16 ? launch_rows<__half, 64>(a, sms, s) : launch_rows<__nv_bfloat16, 64>(a, sms, s);
+    return dtype == UFB_F16 ? launch_rows<__half, 128>(a, sms, s) : launch_rows<__nv_bfloat16, 128>(a, sms, s);
 }
 
 }  // namespace ufb
