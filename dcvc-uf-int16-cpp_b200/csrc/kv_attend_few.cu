@@ -10,7 +10,7 @@
 //
 // Bound by the bytes of the cache.  Work is divided by tiles of 64 keys
 // (kv_attend.cuh), one CTA to an SM; a producer warp streams the integers by TMA
-// into a ring (8 stages, 128 KB in flight at head_dim 128, against the 35 KB that
+// into a ring (7 stages, 112 KB in flight at head_dim 128, against the 35 KB that
 // HBM's latency needs), and the other warps take 32 keys of a stage each, in turn.
 //
 // The products are m16n8k16 tensor instructions on registers with the rows as the
@@ -18,7 +18,7 @@
 // rows, which tcgen05 needs, would be mostly padding here, and its operands would
 // have to go back through shared memory as float16, while these integers are
 // expanded in the registers they were loaded to.  8 rows (one token of up to 8
-// query heads) leave registers for 15 consumer warps, 16 rows for 7: the
+// query heads) leave registers for 14 consumer warps, 16 rows for 6: the
 // expansion is a chain of dependent instructions, and warps are what hides it.
 // Which dims and keys share an instruction is free as long as both operands agree;
 // the order below makes every shared-memory read 16 (or 8) bytes wide and free of
@@ -38,10 +38,14 @@ namespace {
 
 constexpr int kKeys = 64;             // keys of a stage
 constexpr int kWarpKeys = 32;         // keys of a consumer warp's step
-constexpr int kStages = 8;
+constexpr int kScaleRing = 32;        // stages whose scales are kept
 constexpr int kGroups = kKeys / kGroupKeys;
-// With 8 (NT 1) or 16 (NT 2) rows: consumer warps; the producer makes 16 or 8 of it.
-__host__ __device__ constexpr int consumers(int nt) { return nt == 1 ? 15 : 7; }
+// With 8 (NT 1) or 16 (NT 2) rows: consumer warps, and stages of the ring.  A warp
+// comes back to every (consumers / 2)-th stage, and the ring is a multiple of that:
+// a warp has seen each earlier use of a stage it waits for, which a barrier's parity
+// needs (copies may land out of order).
+__host__ __device__ constexpr int consumers(int nt) { return nt == 1 ? 14 : 6; }
+__host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 7 : 9; }
 // P is taken times 2^kShift: at most 2^15, inside float16, and weights down to
 // 2^-29 of the largest keep all 11 bits.
 constexpr float kShift = 15.0f;
@@ -54,11 +58,11 @@ struct PageScales {
 
 template <int D, int NT>
 struct Smem {
-    alignas(1024) uint8_t ring[kStages][2][kKeys * D];      // key, value integers
+    alignas(1024) uint8_t ring[stages(NT)][2][kKeys * D];      // key, value integers
     float sums[consumers(NT)][8 * NT][D];
     float stats[2][2][consumers(NT)][8 * NT];               // by piece parity: maxima, weights
-    PageScales scales[kStages][kGroups];
-    alignas(8) uint64_t full[kStages], empty[kStages];
+    PageScales scales[kScaleRing][kGroups];
+    alignas(8) uint64_t full[stages(NT)], empty[stages(NT)];
     ShareSmem share;
     int last;
     int dead;
@@ -100,7 +104,8 @@ __device__ __forceinline__ int key_of(int n) { return ((n & 1) << 2) | (n >> 1);
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
     few_kernel(const __grid_constant__ CUtensorMap map, const AttendArgs a, int row_tiles, int min_share) {
-    constexpr int kWarps = consumers(NT), kRows = 8 * NT, kThreads = 32 * (kWarps + 1);
+    constexpr int kWarps = consumers(NT), kRows = 8 * NT, kThreads = 32 * (kWarps + 1), kStages = stages(NT);
+    static_assert(kStages % (kWarps * kWarpKeys / kKeys) == 0, "see consumers");
     extern __shared__ uint8_t raw[];
     Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -117,35 +122,32 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
     volatile int* dead = &sm.dead;
 
     if (warp == kWarps) {
-        // ---- producer: a batch is up to 8 stages of one piece, lane = (stage, group of 16 keys)
+        // ---- producer: a batch is up to 8 stages of one piece, lane = (stage, group of 16
+        // keys).  Pages are looked up two batches ahead, scales one, so no load is waited
+        // for; the four lanes of a stage wait for it and start its copies by themselves.
         if (lane == 0) prefetch_tmap(&map);
+        // no more than the ring: a batch must not wait for its own stages
+        constexpr int kBatch = kStages < 32 / kGroups ? kStages : 32 / kGroups;
+        static_assert(kScaleRing >= kStages + 32 / kGroups, "a batch's scales may not meet those in use");
         struct Batch {
-            int count, page, row, head;  // row: the group's first token slot in its page
+            int count, page, row, head;  // page -1: not there; row: the group's first token slot in it
             float key, value;
         };
         Piece p;
         bool have = walk.next(a, p);
         int at = have ? p.first : 0;
-        auto fetch = [&](Batch& b) {
+        auto look_up = [&](Batch& b) {
             b.count = 0;
-            if (!have) return;
-            b.count = min(32 / kGroups, p.end - at);
             b.page = -1;
+            if (!have) return;
+            b.count = min(kBatch, p.end - at);
             b.head = p.head;
-            const int t = at + lane / kGroups;
             if (lane / kGroups < b.count) {
-                const int key = p.t.keys.tile(t) * kKeys + (lane % kGroups) * kGroupKeys;
+                const int key = p.t.keys.tile(at + lane / kGroups) * kKeys + (lane % kGroups) * kGroupKeys;
                 const int entry = key >> a.page_shift;
-                if (p.t.keys.touches(key) && entry < a.table_width) {
-                    const int page = a.table[static_cast<long long>(p.t.slot) * a.table_width + entry];
-                    if (page >= 0 && page < a.pages) {
-                        b.page = page;
-                        b.row = key & (a.page_tokens - 1);
-                        const float* s = a.scale + static_cast<long long>(page) * 2 * a.heads + p.head;
-                        b.key = s[0];
-                        b.value = s[a.heads];
-                    }
-                }
+                b.row = key & (a.page_tokens - 1);
+                if (p.t.keys.touches(key) && entry < a.table_width)
+                    b.page = a.table[static_cast<long long>(p.t.slot) * a.table_width + entry];
             }
             at += b.count;
             if (at == p.end) {
@@ -153,12 +155,25 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 at = have ? p.first : 0;
             }
         };
-        Batch now, next;
-        fetch(now);
+        auto load_scales = [&](Batch& b) {
+            if (b.page >= a.pages) b.page = -1;
+            if (b.page < 0) return;
+            const float* s = a.scale + static_cast<long long>(b.page) * 2 * a.heads + b.head;
+            b.key = s[0];
+            b.value = s[a.heads];
+        };
+        // one copy brings the 16-key groups that lie together in a page, when any of them is there
+        const int box = min(a.page_tokens, kKeys), per = box / kGroupKeys;
+        const bool lead = lane % kGroups % per == 0;
+        Batch now, next, later;
+        look_up(now);
+        load_scales(now);
+        look_up(next);
         int it = 0;
         bool ok = true;
-        while (now.count && ok) {
-            fetch(next);
+        while (now.count) {
+            load_scales(next);
+            look_up(later);
             PageScales sc;
             sc.key = sc.inv_value = 0.0f;
             sc.log2_value = -INFINITY;
@@ -168,52 +183,52 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 sc.log2_value = log2f(v);
                 sc.inv_value = 1.0f / v;
             }
-            // one copy brings the 16-key groups that lie together in a page
-            const int box = min(a.page_tokens, kKeys);                   // keys of a copy
-            const bool lead = (lane % kGroups) * kGroupKeys % box == 0;  // first group of its copy
-            // a page is loaded when any of its groups is there
-            unsigned there = __ballot_sync(0xffffffffu, now.page >= 0);
-            const int per = box / kGroupKeys;
-            const unsigned mine = (there >> lane) & ((1u << per) - 1);
-            const int from = mine ? __ffs(mine) - 1 : 0;
+            // what lay here belongs to a stage that was read before the last one that was
+            // waited for
+            const int mine = lane / kGroups, stage_it = it + mine;
+            sm.scales[stage_it % kScaleRing][lane % kGroups] = sc;
+            __syncwarp();
+            const unsigned there = __ballot_sync(0xffffffffu, now.page >= 0);
+            const unsigned near = (there >> lane) & ((1u << per) - 1);
+            const int from = near ? __ffs(near) - 1 : 0;
             const int page = __shfl_sync(0xffffffffu, now.page, (lane + from) & 31);
             const int row = __shfl_sync(0xffffffffu, now.row, (lane + from) & 31) - from * kGroupKeys;
-            const bool copy = lead && mine != 0;
+            const bool copy = lead && near != 0;
             const unsigned copies = __ballot_sync(0xffffffffu, copy);
-            for (int s = 0; s < now.count; ++s, ++it) {
-                const int stage = it % kStages;
-                if (it >= kStages) ok = mbar_wait(&sm.empty[stage], (it / kStages - 1) & 1, a.status, kCodeEmpty);
-                ok = __shfl_sync(0xffffffffu, ok, 0) && !*dead;
+            const int bytes = __popc((copies >> (mine * kGroups)) & ((1u << kGroups) - 1)) * 2 * box * D;
+            // the cache as rows of 128 bytes
+            const long long tile = static_cast<long long>(page) * 2 * a.heads + now.head;
+            const int off = (lane % kGroups) * kGroupKeys * D;
+            const int key_row = static_cast<int>((tile * a.page_tokens + row) * D / 128);
+            const int value_row = static_cast<int>(((tile + a.heads) * a.page_tokens + row) * D / 128);
+            const int stage = stage_it % kStages;
+            for (int s = 0; s < now.count; ++s) {
+                if (mine != s) continue;
+                if (stage_it >= kStages) ok = mbar_wait(&sm.empty[stage], (stage_it / kStages - 1) & 1, a.status, kCodeEmpty);
                 if (!ok) break;
-                if (lane / kGroups == s) {
-                    sm.scales[stage][lane % kGroups] = sc;
-                }
-                __syncwarp();
-                const int n = __popc((copies >> (s * kGroups)) & ((1u << kGroups) - 1));
-                if (lane == 0) {
-                    if (n) mbar_arrive_expect_tx(&sm.full[stage], n * 2 * box * D);
+                if (lane % kGroups == 0) {
+                    if (bytes) mbar_arrive_expect_tx(&sm.full[stage], bytes);
                     else mbar_arrive(&sm.full[stage]);
                 }
-                __syncwarp();
-                if (lane / kGroups == s && copy) {
-                    // the cache as rows of 128 bytes
-                    const long long tile = static_cast<long long>(page) * 2 * a.heads + now.head;
-                    const int off = (lane % kGroups) * kGroupKeys * D;
-                    const long long key_row = (tile * a.page_tokens + row) * D / 128;
-                    const long long value_row = ((tile + a.heads) * a.page_tokens + row) * D / 128;
-                    tma_load_2d(&sm.ring[stage][0][off], &map, &sm.full[stage], 0, static_cast<int>(key_row));
-                    tma_load_2d(&sm.ring[stage][1][off], &map, &sm.full[stage], 0, static_cast<int>(value_row));
+                if (copy) {
+                    tma_load_2d(&sm.ring[stage][0][off], &map, &sm.full[stage], 0, key_row);
+                    tma_load_2d(&sm.ring[stage][1][off], &map, &sm.full[stage], 0, value_row);
                 }
-                __syncwarp();
             }
-            now = next;
-        }
-        if (!ok) {
-            *dead = 1;
-            // copies still in flight must land before the CTA's shared memory goes
-            if (lane == 0)
+            __syncwarp();
+            if (__any_sync(0xffffffffu, !ok) || *dead) {
+                // somebody gave up: copies still in flight must land before the CTA's shared
+                // memory goes, those of this batch's filled stages and of the ones before
+                *dead = 1;
+                if (ok && mine < now.count) mbar_wait(&sm.full[stage], (stage_it / kStages) & 1, a.status, kCodeDrain);
+                __syncwarp();
                 for (int i = max(0, it - kStages); i < it; ++i)
                     mbar_wait(&sm.full[i % kStages], (i / kStages) & 1, a.status, kCodeDrain);
+                return;
+            }
+            it += now.count;
+            now = next;
+            next = later;
         }
         return;
     }
@@ -305,7 +320,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 *dead = 1;
             __syncwarp();
             constexpr int kM = kWarpKeys / 16;    // score tiles of 16 keys
-            const PageScales* sc = &sm.scales[stage][part / kGroupKeys];
+            const PageScales* sc = &sm.scales[index % kScaleRing][part / kGroupKeys];
             const uint8_t* keys = sm.ring[stage][0];
             const uint8_t* values = sm.ring[stage][1];
             float s[kM][NT][4];
