@@ -25,13 +25,14 @@ bool kv_tensor_map(CUtensorMap& map, const AttendArgs& a, int keys) {
             encode = reinterpret_cast<Encode>(p);
     });
     if (!encode) return false;
-    const cuuint64_t rows = static_cast<cuuint64_t>(a.pages) * 2 * a.heads * a.page_tokens * a.head_dim / 128;
-    if (rows > 0x7fffffffull) return false;
-    const cuuint64_t dims[2] = {128, rows};
-    const cuuint64_t strides[1] = {128};
-    const cuuint32_t box[2] = {128, static_cast<cuuint32_t>((a.page_tokens < keys ? a.page_tokens : keys) * a.head_dim / 128)};
-    const cuuint32_t elem[2] = {1, 1};
-    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(a.kv), dims, strides, box, elem,
+    // rows of 128 bytes of a page's head, heads, key and value, pages
+    const cuuint64_t rows = static_cast<cuuint64_t>(a.page_tokens) * a.head_dim / 128, heads = a.heads;
+    const cuuint64_t dims[5] = {128, rows, heads, 2, static_cast<cuuint64_t>(a.pages)};
+    const cuuint64_t strides[4] = {128, rows * 128, rows * 128 * heads, rows * 128 * heads * 2};
+    const cuuint32_t box[5] = {128, static_cast<cuuint32_t>((a.page_tokens < keys ? a.page_tokens : keys) * a.head_dim / 128),
+                               1, 2, 1};
+    const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+    return encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<int8_t*>(a.kv), dims, strides, box, elem,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

@@ -279,8 +279,9 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// The layer's integers as rows of 128 bytes, in boxes of the keys (at most
-// `keys`) that lie together in a page, with TMA's 128-byte swizzle.
+// The layer's integers as (128 bytes, rows of a head, heads, key and value, pages),
+// in boxes of the keys (at most `keys`) that lie together in a page and their
+// values, with TMA's 128-byte swizzle.
 bool kv_tensor_map(CUtensorMap& map, const AttendArgs& a, int keys);
 
 cudaError_t attend_few(const AttendArgs& a, int dtype, int sms, cudaStream_t s);

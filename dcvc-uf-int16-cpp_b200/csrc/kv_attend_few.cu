@@ -58,7 +58,7 @@ struct PageScales {
 
 template <int D, int NT>
 struct Smem {
-    alignas(1024) uint8_t ring[stages(NT)][2][kKeys * D];      // key, value integers
+    alignas(1024) uint8_t ring[stages(NT)][2 * kKeys * D];     // copies of key, then value integers
     float sums[consumers(NT)][8 * NT][D];
     float stats[2][2][consumers(NT)][8 * NT];               // by piece parity: maxima, weights
     PageScales scales[kScaleRing][kGroups];
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
             // what lay here belongs to a stage that was read before the last one that was
             // waited for
             const int mine = lane / kGroups, stage_it = it + mine;
-            sm.scales[stage_it % kScaleRing][lane % kGroups] = sc;
+            if (mine < now.count) sm.scales[stage_it % kScaleRing][lane % kGroups] = sc;
             __syncwarp();
             const unsigned there = __ballot_sync(0xffffffffu, now.page >= 0);
             const unsigned near = (there >> lane) & ((1u << per) - 1);
@@ -196,11 +196,8 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
             const bool copy = lead && near != 0;
             const unsigned copies = __ballot_sync(0xffffffffu, copy);
             const int bytes = __popc((copies >> (mine * kGroups)) & ((1u << kGroups) - 1)) * 2 * box * D;
-            // the cache as rows of 128 bytes
-            const long long tile = static_cast<long long>(page) * 2 * a.heads + now.head;
-            const int off = (lane % kGroups) * kGroupKeys * D;
-            const int key_row = static_cast<int>((tile * a.page_tokens + row) * D / 128);
-            const int value_row = static_cast<int>(((tile + a.heads) * a.page_tokens + row) * D / 128);
+            // a copy's place: [copy][key, value][16-key groups of it]
+            const int off = (lane % kGroups) * kGroupKeys * 2 * D, map_row = row * D / 128;
             const int stage = stage_it % kStages;
             for (int s = 0; s < now.count; ++s) {
                 if (mine != s) continue;
@@ -210,10 +207,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                     if (bytes) mbar_arrive_expect_tx(&sm.full[stage], bytes);
                     else mbar_arrive(&sm.full[stage]);
                 }
-                if (copy) {
-                    tma_load_2d(&sm.ring[stage][0][off], &map, &sm.full[stage], 0, key_row);
-                    tma_load_2d(&sm.ring[stage][1][off], &map, &sm.full[stage], 0, value_row);
-                }
+                if (copy) tma_load_5d(&sm.ring[stage][off], &map, &sm.full[stage], 0, map_row, now.head, 0, page);
             }
             __syncwarp();
             if (__any_sync(0xffffffffu, !ok) || *dead) {
@@ -321,8 +315,15 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
             __syncwarp();
             constexpr int kM = kWarpKeys / 16;    // score tiles of 16 keys
             const PageScales* sc = &sm.scales[index % kScaleRing][part / kGroupKeys];
-            const uint8_t* keys = sm.ring[stage][0];
-            const uint8_t* values = sm.ring[stage][1];
+            // where the step's 16-key groups lie, less their offset in the stage
+            const int box = min(a.page_tokens, kKeys);
+            const uint8_t *keys[kM], *values[kM];
+#pragma unroll
+            for (int x = 0; x < kM; ++x) {
+                const int first = part + x * 16, copy = first & ~(box - 1);
+                keys[x] = sm.ring[stage] + (copy * 2 + first - copy) * D;
+                values[x] = keys[x] + box * D;
+            }
             float s[kM][NT][4];
 #pragma unroll
             for (int x = 0; x < kM; ++x)
@@ -336,15 +337,15 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 for (int x = 0; x < kM; ++x)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const int key = part + x * 16 + h * 8 + key_of(g);
+                        const int key = h * 8 + key_of(g);
                         if (D == 128) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(keys + key * 128 + (((c + i * 4) ^ (key & 7)) << 4));
+                            const uint4 v = *reinterpret_cast<const uint4*>(keys[x] + key * 128 + (((c + i * 4) ^ (key & 7)) << 4));
                             w[x][h][0] = v.x, w[x][h][1] = v.y;
                             w[x][h][2 % (kSteps / 2)] = v.z, w[x][h][3 % (kSteps / 2)] = v.w;
                         } else {
                             const int row = key >> 1;
                             const uint2 v = *reinterpret_cast<const uint2*>(
-                                keys + row * 128 + ((((key & 1) * 4 + i * 2 + (c >> 1)) ^ (row & 7)) << 4) + (c & 1) * 8);
+                                keys[x] + row * 128 + ((((key & 1) * 4 + i * 2 + (c >> 1)) ^ (row & 7)) << 4) + (c & 1) * 8);
                             w[x][h][0] = v.x, w[x][h][1] = v.y;
                         }
                     }
@@ -445,13 +446,13 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 uint32_t v[4][D / 32];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = part + x * 16 + (i >> 1) * 8 + (i & 1) * 4 + c;
+                    const int key = (i >> 1) * 8 + (i & 1) * 4 + c;
                     if (D == 128) {
-                        const uint4 y = *reinterpret_cast<const uint4*>(values + key * 128 + (((value_dim<D>(g) >> 4) ^ (key & 7)) << 4));
+                        const uint4 y = *reinterpret_cast<const uint4*>(values[x] + key * 128 + (((value_dim<D>(g) >> 4) ^ (key & 7)) << 4));
                         v[i][0] = y.x, v[i][1] = y.y, v[i][2 % (D / 32)] = y.z, v[i][3 % (D / 32)] = y.w;
                     } else {
                         const int row = key >> 1, chunk = (key & 1) * 4 + (value_dim<D>(g) >> 4);
-                        const uint2 y = *reinterpret_cast<const uint2*>(values + row * 128 + ((chunk ^ (row & 7)) << 4) + (g & 1) * 8);
+                        const uint2 y = *reinterpret_cast<const uint2*>(values[x] + row * 128 + ((chunk ^ (row & 7)) << 4) + (g & 1) * 8);
                         v[i][0] = y.x, v[i][1] = y.y;
                     }
                 }
