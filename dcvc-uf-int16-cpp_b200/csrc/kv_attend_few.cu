@@ -40,6 +40,7 @@ constexpr int kKeys = 64;             // keys of a stage
 constexpr int kWarpKeys = 32;         // keys of a consumer warp's step
 constexpr int kScaleRing = 32;        // stages whose scales are kept
 constexpr int kGroups = kKeys / kGroupKeys;
+constexpr int kMinShare = 7;          // tiles of a CTA's share at least: as many as its warps take at once
 // With 8 (NT 1) or 16 (NT 2) rows: consumer warps, and stages of the ring.  A warp
 // comes back to every (consumers / 2)-th stage, and the ring is a multiple of that:
 // a warp has seen each earlier use of a stage it waits for, which a barrier's parity
@@ -85,6 +86,8 @@ template <int N>
 __device__ __forceinline__ void consumers_sync() {
     asm volatile("bar.sync 1, %0;" ::"n"(N * 32) : "memory");
 }
+
+__device__ __forceinline__ void joiners_sync(int warps) { asm volatile("bar.sync 2, %0;" ::"r"(warps * 32) : "memory"); }
 
 // The dims of lane quarter c in k step t, four in a row (also Q's fragments).
 template <int D>
@@ -524,62 +527,66 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 a.lse[(p.t.token0 + token) * (a.heads * a.group) + head] =
                     weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
         };
-        for (int e = threadIdx.x; e < p.t.rows * (D / 4); e += kWarps * 32) {
-            const int row = e / (D / 4), d = e % (D / 4) * 4;
-            float top = -INFINITY, weight = 0.0f;
+        // as many warps as there is to sum; the others go on to the next piece
+        const int joiners = min(kWarps, (p.t.rows * (D / 4) + 31) / 32);
+        if (warp < joiners) {
+            for (int e = threadIdx.x; e < p.t.rows * (D / 4); e += joiners * 32) {
+                const int row = e / (D / 4), d = e % (D / 4) * 4;
+                float top = -INFINITY, weight = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.stats[parity][0][w][row]);
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm.stats[parity][0][w][row]);
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float mw = sm.stats[parity][0][w][row], lw = sm.stats[parity][1][w][row];
-                if (lw != 0.0f) weight += lw * (mw == -INFINITY ? 1.0f : ex2(mw - top));
-                const float4 x = *reinterpret_cast<const float4*>(&sm.sums[w][row][d]);
-                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-            }
-            if (whole) {
-                finish(row, d, v, top, weight);
-            } else {
-                __stcg(reinterpret_cast<float4*>(scratch.sums + (static_cast<long long>(part) * kRows + row) * D + d), v);
-                if (d == 0) {
-                    __stcg(scratch.stats + (part * 2) * kRows + row, top);
-                    __stcg(scratch.stats + (part * 2 + 1) * kRows + row, weight);
+                for (int w = 0; w < kWarps; ++w) {
+                    const float mw = sm.stats[parity][0][w][row], lw = sm.stats[parity][1][w][row];
+                    if (lw != 0.0f) weight += lw * (mw == -INFINITY ? 1.0f : ex2(mw - top));
+                    const float4 x = *reinterpret_cast<const float4*>(&sm.sums[w][row][d]);
+                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                }
+                if (whole) {
+                    finish(row, d, v, top, weight);
+                } else {
+                    __stcg(reinterpret_cast<float4*>(scratch.sums + (static_cast<long long>(part) * kRows + row) * D + d), v);
+                    if (d == 0) {
+                        __stcg(scratch.stats + (part * 2) * kRows + row, top);
+                        __stcg(scratch.stats + (part * 2 + 1) * kRows + row, weight);
+                    }
                 }
             }
-        }
-        if (!whole) {
-            // CTAs of this item: the one its first tile falls to .. the one its last tile falls to
-            const int c0 = static_cast<int>(p.item_start / share.per);
-            const int c1 = static_cast<int>((p.item_start + p.t.keys.nt - 1) / share.per);
-            __threadfence();
-            consumers_sync<kWarps>();
-            if (threadIdx.x == 0) {
-                const int before = atomicAdd(scratch.counters + c0, 1);
-                sm.last = before == c1 - c0;
-                if (sm.last) scratch.counters[c0] = 0;
-            }
-            consumers_sync<kWarps>();
-            if (sm.last) {
+            if (!whole) {
+                // CTAs of this item: the one its first tile falls to .. the one its last tile falls to
+                const int c0 = static_cast<int>(p.item_start / share.per);
+                const int c1 = static_cast<int>((p.item_start + p.t.keys.nt - 1) / share.per);
                 __threadfence();
-                for (int e = threadIdx.x; e < p.t.rows * (D / 4); e += kWarps * 32) {
-                    const int row = e / (D / 4), d = e % (D / 4) * 4;
-                    float top = -INFINITY, weight = 0.0f;
+                joiners_sync(joiners);
+                if (threadIdx.x == 0) {
+                    const int before = atomicAdd(scratch.counters + c0, 1);
+                    sm.last = before == c1 - c0;
+                    if (sm.last) scratch.counters[c0] = 0;
+                }
+                joiners_sync(joiners);
+                if (sm.last) {
+                    __threadfence();
+                    for (int e = threadIdx.x; e < p.t.rows * (D / 4); e += joiners * 32) {
+                        const int row = e / (D / 4), d = e % (D / 4) * 4;
+                        float top = -INFINITY, weight = 0.0f;
 #pragma unroll 4
-                    for (int i = c0; i <= c1; ++i)
-                        top = fmaxf(top, __ldcg(scratch.stats + (2 * i + (i == c0)) * 2 * kRows + row));
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        for (int i = c0; i <= c1; ++i)
+                            top = fmaxf(top, __ldcg(scratch.stats + (2 * i + (i == c0)) * 2 * kRows + row));
+                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-                    for (int i = c0; i <= c1; ++i) {
-                        const int from = 2 * i + (i == c0);
-                        const float mi = __ldcg(scratch.stats + from * 2 * kRows + row);
-                        const float li = __ldcg(scratch.stats + (from * 2 + 1) * kRows + row);
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(
-                            scratch.sums + (static_cast<long long>(from) * kRows + row) * D + d));
-                        const float mul = mi == -INFINITY ? (li == 0.0f ? 0.0f : 1.0f) : ex2(mi - top);
-                        weight += li * mul;
-                        v.x += x.x * mul, v.y += x.y * mul, v.z += x.z * mul, v.w += x.w * mul;
+                        for (int i = c0; i <= c1; ++i) {
+                            const int from = 2 * i + (i == c0);
+                            const float mi = __ldcg(scratch.stats + from * 2 * kRows + row);
+                            const float li = __ldcg(scratch.stats + (from * 2 + 1) * kRows + row);
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(
+                                scratch.sums + (static_cast<long long>(from) * kRows + row) * D + d));
+                            const float mul = mi == -INFINITY ? (li == 0.0f ? 0.0f : 1.0f) : ex2(mi - top);
+                            weight += li * mul;
+                            v.x += x.x * mul, v.y += x.y * mul, v.z += x.z * mul, v.w += x.w * mul;
+                        }
+                        finish(row, d, v, top, weight);
                     }
-                    finish(row, d, v, top, weight);
                 }
             }
         }
@@ -599,7 +606,7 @@ cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     // boxes of the keys that lie together in a page, 64 at most
     if (!kv_tensor_map(map, a, kKeys)) return cudaErrorInvalidValue;
     const int row_tiles = static_cast<int>((static_cast<long long>(a.max_new) * a.group + 8 * NT - 1) / (8 * NT));
-    kernel<<<sms < kAttendMaxCtas ? sms : kAttendMaxCtas, 32 * (consumers(NT) + 1), smem, s>>>(map, a, row_tiles, 1);
+    kernel<<<sms < kAttendMaxCtas ? sms : kAttendMaxCtas, 32 * (consumers(NT) + 1), smem, s>>>(map, a, row_tiles, kMinShare);
     return cudaGetLastError();
 }
 
