@@ -84,6 +84,11 @@ __device__ __forceinline__ bool row_tile(const AttendArgs& a, int stream, int rt
     return true;
 }
 
+// a / b of values that nearly always fit 32 bits, where a division is much shorter.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((a | b) >> 31) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
 // Where a CTA's share of the sequence begins.
 struct Share {
     long long total;        // tiles of the call
@@ -124,7 +129,7 @@ __device__ __forceinline__ Share locate_share(const AttendArgs& a, int row_tiles
     s.total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) s.total += sm.warp[w];
-    s.per = (s.total + gridDim.x - 1) / gridDim.x;
+    s.per = quotient(s.total + gridDim.x - 1, gridDim.x);
     if (s.per < min_share) s.per = min_share;
     const long long start = s.per * blockIdx.x;
     long long before = 0;
@@ -198,7 +203,7 @@ struct Walker {
             loaded = false;
         }
         p.t = t;
-        p.head = static_cast<int>((pos - pair_start) / t.keys.nt);
+        p.head = static_cast<int>(quotient(pos - pair_start, t.keys.nt));
         p.item_start = pair_start + static_cast<long long>(p.head) * t.keys.nt;
         p.first = static_cast<int>(pos - p.item_start);
         p.end = static_cast<int>(min(static_cast<long long>(t.keys.nt), end - p.item_start));

@@ -9,7 +9,7 @@
 // product; l divides it out again, in 32 bits.  out = O / l.
 //
 // Bound by the bytes of the cache.  Work is divided by tiles of 64 keys
-// (kv_attend.cuh), one CTA to an SM; a producer warp streams the integers by TMA
+// (kv_attend.cuh), one CTA to an SM; two producer warps stream the integers by TMA
 // into a ring (7 stages, 112 KB in flight at head_dim 128, against the 35 KB that
 // HBM's latency needs), and the other warps take 32 keys of a stage each, in turn.
 //
@@ -38,7 +38,7 @@ namespace {
 
 constexpr int kKeys = 64;             // keys of a stage
 constexpr int kWarpKeys = 32;         // keys of a consumer warp's step
-constexpr int kScaleRing = 32;        // stages whose scales are kept
+constexpr int kProducers = 2;         // producer warps; a slot of the ring always has the same one
 constexpr int kGroups = kKeys / kGroupKeys;
 constexpr int kMinShare = 7;          // tiles of a CTA's share at least: as many as its warps take at once
 // With 8 (NT 1) or 16 (NT 2) rows: consumer warps, and stages of the ring.  A warp
@@ -62,7 +62,7 @@ struct Smem {
     alignas(1024) uint8_t ring[stages(NT)][2 * kKeys * D];     // copies of key, then value integers
     float sums[consumers(NT)][8 * NT][D];
     float stats[2][2][consumers(NT)][8 * NT];               // by piece parity: maxima, weights
-    PageScales scales[kScaleRing][kGroups];
+    PageScales scales[stages(NT)][kGroups];
     alignas(8) uint64_t full[stages(NT)], empty[stages(NT)];
     ShareSmem share;
     int last;
@@ -105,13 +105,14 @@ __device__ __forceinline__ int value_dim(int n) {
 __device__ __forceinline__ int key_of(int n) { return ((n & 1) << 2) | (n >> 1); }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
+__global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
     few_kernel(const __grid_constant__ CUtensorMap map, const AttendArgs a, int row_tiles, int min_share) {
-    constexpr int kWarps = consumers(NT), kRows = 8 * NT, kThreads = 32 * (kWarps + 1), kStages = stages(NT);
+    constexpr int kWarps = consumers(NT), kRows = 8 * NT, kThreads = 32 * (kWarps + kProducers), kStages = stages(NT);
     static_assert(kStages % (kWarps * kWarpKeys / kKeys) == 0, "see consumers");
     extern __shared__ uint8_t raw[];
     Smem<D, NT>& sm = *reinterpret_cast<Smem<D, NT>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == kThreads - 1) prefetch_tmap(&map);
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&sm.full[i], 1);
@@ -124,14 +125,13 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
     Walker<kKeys, kRows> walk(a, share, row_tiles);
     volatile int* dead = &sm.dead;
 
-    if (warp == kWarps) {
-        // ---- producer: a batch is up to 8 stages of one piece, lane = (stage, group of 16
+    if (warp >= kWarps) {
+        // ---- producers: a batch is up to 8 stages of one piece, lane = (stage, group of 16
         // keys).  Pages are looked up two batches ahead, scales one, so no load is waited
         // for; the four lanes of a stage wait for it and start its copies by themselves.
-        if (lane == 0) prefetch_tmap(&map);
+        // Both producers look at every batch and fill the slots that are theirs.
         // no more than the ring: a batch must not wait for its own stages
         constexpr int kBatch = kStages < 32 / kGroups ? kStages : 32 / kGroups;
-        static_assert(kScaleRing >= kStages + 32 / kGroups, "a batch's scales may not meet those in use");
         struct Batch {
             int count, page, row, head;  // page -1: not there; row: the group's first token slot in it
             float key, value;
@@ -186,11 +186,8 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 sc.log2_value = log2f(v);
                 sc.inv_value = 1.0f / v;
             }
-            // what lay here belongs to a stage that was read before the last one that was
-            // waited for
-            const int mine = lane / kGroups, stage_it = it + mine;
-            if (mine < now.count) sm.scales[stage_it % kScaleRing][lane % kGroups] = sc;
-            __syncwarp();
+            const int mine = lane / kGroups, stage_it = it + mine, stage = stage_it % kStages;
+            const bool fill = mine < now.count && stage % kProducers == warp - kWarps;
             const unsigned there = __ballot_sync(0xffffffffu, now.page >= 0);
             const unsigned near = (there >> lane) & ((1u << per) - 1);
             const int from = near ? __ffs(near) - 1 : 0;
@@ -201,11 +198,15 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
             const int bytes = __popc((copies >> (mine * kGroups)) & ((1u << kGroups) - 1)) * 2 * box * D;
             // a copy's place: [copy][key, value][16-key groups of it]
             const int off = (lane % kGroups) * kGroupKeys * 2 * D, map_row = row * D / 128;
-            const int stage = stage_it % kStages;
+            const unsigned group = ((1u << kGroups) - 1) << (lane & ~(kGroups - 1));
             for (int s = 0; s < now.count; ++s) {
-                if (mine != s) continue;
+                if (mine != s || !fill) continue;
                 if (stage_it >= kStages) ok = mbar_wait(&sm.empty[stage], (stage_it / kStages - 1) & 1, a.status, kCodeEmpty);
+                // the four agree, or those that go on would miss the others below
+                ok = __shfl_sync(group, ok, lane & ~(kGroups - 1));
                 if (!ok) break;
+                sm.scales[stage][lane % kGroups] = sc;
+                __syncwarp(group);
                 if (lane % kGroups == 0) {
                     if (bytes) mbar_arrive_expect_tx(&sm.full[stage], bytes);
                     else mbar_arrive(&sm.full[stage]);
@@ -217,10 +218,10 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 // somebody gave up: copies still in flight must land before the CTA's shared
                 // memory goes, those of this batch's filled stages and of the ones before
                 *dead = 1;
-                if (ok && mine < now.count) mbar_wait(&sm.full[stage], (stage_it / kStages) & 1, a.status, kCodeDrain);
+                if (ok && fill) mbar_wait(&sm.full[stage], (stage_it / kStages) & 1, a.status, kCodeDrain);
                 __syncwarp();
                 for (int i = max(0, it - kStages); i < it; ++i)
-                    mbar_wait(&sm.full[i % kStages], (i / kStages) & 1, a.status, kCodeDrain);
+                    if (i % kStages % kProducers == warp - kWarps) mbar_wait(&sm.full[i % kStages], (i / kStages) & 1, a.status, kCodeDrain);
                 return;
             }
             it += now.count;
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + 1), 1)
                 *dead = 1;
             __syncwarp();
             constexpr int kM = kWarpKeys / 16;    // score tiles of 16 keys
-            const PageScales* sc = &sm.scales[index % kScaleRing][part / kGroupKeys];
+            const PageScales* sc = &sm.scales[stage][part / kGroupKeys];
             // where the step's 16-key groups lie, less their offset in the stage
             const int box = min(a.page_tokens, kKeys);
             const uint8_t *keys[kM], *values[kM];
@@ -606,7 +607,7 @@ cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     // boxes of the keys that lie together in a page, 64 at most
     if (!kv_tensor_map(map, a, kKeys)) return cudaErrorInvalidValue;
     const int row_tiles = static_cast<int>((static_cast<long long>(a.max_new) * a.group + 8 * NT - 1) / (8 * NT));
-    kernel<<<sms < kAttendMaxCtas ? sms : kAttendMaxCtas, 32 * (consumers(NT) + 1), smem, s>>>(map, a, row_tiles, kMinShare);
+    kernel<<<sms < kAttendMaxCtas ? sms : kAttendMaxCtas, 32 * (consumers(NT) + kProducers), smem, s>>>(map, a, row_tiles, kMinShare);
     return cudaGetLastError();
 }
 
