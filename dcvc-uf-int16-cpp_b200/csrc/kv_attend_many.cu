@@ -38,8 +38,10 @@ constexpr int kRows = kAttendManyRows;
 constexpr int kHalf = 128;
 constexpr int kKeys = 128;
 constexpr int kGroups = kKeys / kGroupKeys;
-constexpr int kMmaWarp = 16;
-constexpr int kThreads = 544;         // warps: softmax 0-7, converter 8-15, MMA 16
+constexpr int kMmaWarp = 16, kWalkWarp = 17;
+constexpr int kThreads = 640;         // warps: softmax 0-7, converter 8-15, MMA 16, walker 17; 18, 19 idle
+constexpr int kPieces = 4;            // pieces announced ahead
+constexpr int kReaders = 17;          // warps that read them
 constexpr int kScaleRing = 4;
 constexpr int kCode = 44;
 // A running maximum stays while it grows by less than 2^kSlack, and P is taken
@@ -51,6 +53,12 @@ struct alignas(16) GroupScales {
     float key, log2_value, inv_value, pad;
 };
 
+// A piece of an item as the walker announces it; rows 0: there is none any more.
+struct Announced {
+    KeyRange keys;
+    int rows, row0, first, end, slot, length, start, token0, head, parts, part;  // start: where token 0 stands
+};
+
 template <int D>
 struct Smem {
     alignas(1024) uint8_t q[2][kHalf * D * 2];     // [64 dims][row][128 bytes]
@@ -59,6 +67,8 @@ struct Smem {
     GroupScales scales[kScaleRing][kGroups];
     alignas(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
     uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], drained;
+    uint64_t piece_full[kPieces], piece_empty[kPieces];
+    Announced pieces[kPieces];
     ShareSmem share;
     uint32_t tmem;
     int dead;
@@ -115,6 +125,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             mbar_init(&sm.o_full[i], 1);
         }
         mbar_init(&sm.drained, 1);
+        for (int i = 0; i < kPieces; ++i) {
+            mbar_init(&sm.piece_full[i], 1);
+            mbar_init(&sm.piece_empty[i], kReaders);
+        }
         fence_mbar_init();
         sm.dead = (smem_u32(raw) & 1023) != 0;
         if (sm.dead) atomicCAS(a.status, 0, kCode);
@@ -128,37 +142,51 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
     tc_fence_after();
     // all 512 columns are this CTA's: its tensor memory begins at 0
     constexpr uint32_t tmem = 0;
-    Walker<kKeys, kRows> walk(a, share, row_tiles);
     volatile int* dead = &sm.dead;
-    // after a wait gave up nobody waits any more: the loops run out on what is there
+    // after a wait gave up nobody waits any more, and no further piece is begun
     auto wait = [&](uint64_t* bar, int phase) {
         if (mbar_try_wait(bar, phase & 1)) return;
         if (!*dead && !mbar_wait(bar, phase & 1, a.status, kCode)) *dead = 1;
     };
-    const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
+    // Pieces one after another; a reader gives each back when it is done with it.
+    auto piece_at = [&](int n) -> const Announced& {
+        wait(&sm.piece_full[n % kPieces], n / kPieces);
+        __syncwarp();
+        return sm.pieces[n % kPieces];
+    };
+    auto piece_done = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.piece_empty[n % kPieces]);
+    };
 
+    // the registers of 640 threads at 96: 2 x 128 + 2 x 72 + 80 = 5 x 96
     if (warp < 8) {
+        regs_inc<128>();
         // ---- softmax: half t, row of the half = thread
         const int t = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + Tmem<D>::s(t), to = tmem + lanes + Tmem<D>::o(t);
         int tiles = 0, s_n = 0, o_n = 0;   // key tiles of this CTA so far; phases of this half
-        Piece p;
+        const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
         if (t == 0 && row == 0) scratch.items[blockIdx.x * 8] = 0;
-        while (walk.next(a, p)) {
-            if (t * kHalf >= p.t.rows) {
+        for (int n = 0;; ++n) {
+            const Announced& p = piece_at(n);
+            if (p.rows == 0 || *dead) break;
+            if (t * kHalf >= p.rows) {
                 tiles += p.end - p.first;
+                piece_done(n);
                 continue;
             }
             const int r = t * kHalf + row;
-            const bool real = r < p.t.rows;
-            const int in_stream = p.t.row0 + (real ? r : 0);
+            const bool real = r < p.rows;
+            const int in_stream = p.row0 + (real ? r : 0);
             const int token = in_stream / a.group, head = p.head * a.group + in_stream - token * a.group;
-            const int pos = p.t.length - p.t.n_new + token;
+            const int pos = p.start + token;
+            const long long out_row = p.token0 + static_cast<long long>(token);
             float unit;
             {
                 // the row to [1/2, 1) and float16; the softmax scale's sign goes with it
-                const T* src = static_cast<const T*>(a.q.data) + (p.t.token0 + token) * a.q.token_stride +
+                const T* src = static_cast<const T*>(a.q.data) + out_row * a.q.token_stride +
                                head * a.q.head_stride;
                 const uint4* vec = reinterpret_cast<const uint4*>(src);
                 float top = 0.0f, odd = 0.0f;
@@ -192,18 +220,19 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 mbar_arrive(&sm.q_full[t]);
             }
             float m = -INFINITY, l = 0.0f;
-            const int first_pos = p.t.length - p.t.n_new + (p.t.row0 + t * kHalf) / a.group;
-            const int last_pos = p.t.length - p.t.n_new + (p.t.row0 + min(p.t.rows, (t + 1) * kHalf) - 1) / a.group;
-            for (int tile = p.first; tile < p.end; ++tile, ++tiles) {
+            const int first_pos = p.start + (p.row0 + t * kHalf) / a.group;
+            const int last_pos = p.start + (p.row0 + min(p.rows, (t + 1) * kHalf) - 1) / a.group;
+            const int length = p.length, end = p.end;
+            for (int tile = p.first; tile < end; ++tile, ++tiles) {
                 wait(&sm.s_full[t], s_n++);
                 __syncwarp();
                 tc_fence_after();
                 const GroupScales* sc = sm.scales[tiles % kScaleRing];
-                const int key0 = p.t.keys.tile(tile) * kKeys;
-                const bool clear = (!a.causal || key0 + kKeys - 1 <= first_pos) && key0 + kKeys <= p.t.length &&
+                const int key0 = p.keys.tile(tile) * kKeys;
+                const bool clear = (!a.causal || key0 + kKeys - 1 <= first_pos) && key0 + kKeys <= length &&
                                    (!a.window || last_pos - key0 < a.window || key0 + kKeys <= a.sinks);
                 // columns [0, high) that are from low on or below sink are seen by this row
-                const int high = min(p.t.length, a.causal ? pos + 1 : p.t.length) - key0;
+                const int high = min(length, a.causal ? pos + 1 : length) - key0;
                 const int low = a.window ? max(pos - a.window + 1, 0) - key0 : 0;
                 const int sink = a.window ? a.sinks - key0 : 0;
                 auto seen = [&](int c) {   // of 32 columns, a bit each
@@ -261,13 +290,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 if (grow || m == -INFINITY) m = top;
                 const float base = m == -INFINITY ? 0.0f : m - kShift;
                 auto weights = [&](auto masked) {
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t s[32], w[16];
-                        tmem_ld32(ts + c * 32, s);
+                    // 32 columns: P, the row's weight
+                    auto chunk = [&](int c, uint32_t (&s)[32]) {
                         const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
-                        tmem_wait_ld();
-                        tmem_tie32(s);
+                        uint32_t w[16];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const GroupScales gs = sc[c * 2 + h];
@@ -290,12 +316,24 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                             if (sum[0] != 0.0f) l = fmaf(sum[0], gs.inv_value, l);
                         }
                         tmem_st16(ts + c * 16, w);
-                        if (c & 1) {
-                            // P V starts on the first 64 keys while the others are in the works
-                            tmem_wait_st();
-                            tc_fence_before();
-                            mbar_arrive(&sm.p_full[t][c >> 1]);
-                        }
+                    };
+                    // the next columns are on their way while these are worked on
+                    uint32_t s0[32], s1[32];
+                    tmem_ld32(ts, s0);
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        tmem_wait_ld();
+                        tmem_tie32(s0);
+                        tmem_ld32(ts + half * 64 + 32, s1);
+                        chunk(half * 2, s0);
+                        tmem_wait_ld();
+                        tmem_tie32(s1);
+                        if (half == 0) tmem_ld32(ts + 64, s0);
+                        chunk(half * 2 + 1, s1);
+                        // P V starts on the first 64 keys while the others are in the works
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(&sm.p_full[t][half]);
                     }
                 };
                 if (clear) weights(std::false_type());
@@ -304,10 +342,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             wait(&sm.o_full[t], o_n++);
             __syncwarp();
             tc_fence_after();
-            const bool whole = p.whole();
-            const int part = 2 * blockIdx.x + (p.first > 0 ? 0 : 1);
+            const bool whole = p.part < 0;
+            const int part = 2 * blockIdx.x + p.part;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            T* out = static_cast<T*>(a.out.data) + (p.t.token0 + token) * a.out.token_stride + head * a.out.head_stride;
+            T* out = static_cast<T*>(a.out.data) + out_row * a.out.token_stride + head * a.out.head_stride;
             float* sums = scratch.sums + (static_cast<long long>(part) * kRows + r) * D;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -333,23 +371,25 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 __syncwarp();
             }
             if (real && whole && a.lse)
-                a.lse[(p.t.token0 + token) * (a.heads * a.group) + head] =
+                a.lse[out_row * (a.heads * a.group) + head] =
                     l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * 0.6931471805599453f;
             if (real && !whole) {
                 __stcg(scratch.stats + (part * 2) * kRows + r, m);
                 __stcg(scratch.stats + (part * 2 + 1) * kRows + r, l);
             }
-            if (!whole && p.first == 0 && t == 0 && row == 0) {
+            if (p.parts && t == 0 && row == 0) {
                 int32_t* item = scratch.items + blockIdx.x * 8;
-                item[1] = static_cast<int>(p.t.token0);
-                item[2] = p.t.row0;
-                item[3] = p.t.rows;
+                item[1] = p.token0;
+                item[2] = p.row0;
+                item[3] = p.rows;
                 item[4] = p.head;
-                item[0] = static_cast<int>((p.item_start + p.t.keys.nt - 1) / share.per) - blockIdx.x + 1;
+                item[0] = p.parts;
             }
+            piece_done(n);
             tc_fence_before();
         }
     } else if (warp < kMmaWarp) {
+        regs_dec<72>();
         // ---- converter: warps 8-11 the keys and the scales, 12-15 the values, 32 keys each
         constexpr int kLoads = D / 16;   // 16-byte loads of a thread for a tile
         const int side = (warp - 8) >> 2, w = warp & 3;
@@ -370,25 +410,29 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             int page[2], row[2], head;   // of this warp's two groups of 16 keys
             bool tile;                   // false: no further tile
         };
-        Piece p;
-        bool have = walk.next(a, p);
-        int at = have ? p.first : 0;
+        int piece = 0, at = -1;   // the piece being looked up and its next tile; -1: not begun
+        bool have = true;
         auto fetch = [&](Next& n) {
-            n.tile = have;
+            n.tile = false;
             n.page[0] = n.page[1] = -1;
             if (!have) return;
+            const Announced& p = piece_at(piece);
+            have = p.rows > 0 && !*dead;
+            if (!have) return;
+            if (at < 0) at = p.first;
+            n.tile = true;
             n.head = p.head;
-            const int key0 = p.t.keys.tile(at) * kKeys + w * 32;
+            const int key0 = p.keys.tile(at) * kKeys + w * 32;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const int key = key0 + g * kGroupKeys, entry = key >> a.page_shift;
                 n.row[g] = key & (a.page_tokens - 1);
-                if (p.t.keys.touches(key) && entry < a.table_width)
-                    n.page[g] = a.table[static_cast<long long>(p.t.slot) * a.table_width + entry];
+                if (p.keys.touches(key) && entry < a.table_width)
+                    n.page[g] = a.table[static_cast<long long>(p.slot) * a.table_width + entry];
             }
             if (++at == p.end) {
-                have = walk.next(a, p);
-                at = have ? p.first : 0;
+                piece_done(piece++);
+                at = -1;
             }
         };
         uint4 buf[kLoads];
@@ -459,8 +503,42 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             fetch(next);
         }
     } else {
+        regs_dec<80>();
+        if (warp == kWalkWarp) {
+            // ---- walker: announces this CTA's pieces
+            Walker<kKeys, kRows> walk(a, share, row_tiles);
+            Piece p;
+            bool more = true;
+            for (int n = 0; more; ++n) {
+                more = walk.next(a, p) && !*dead;
+                if (n >= kPieces) wait(&sm.piece_empty[n % kPieces], n / kPieces - 1);
+                if (lane == 0) {
+                    Announced& o = sm.pieces[n % kPieces];
+                    o.rows = more ? p.t.rows : 0;
+                    if (more) {
+                        o.keys = p.t.keys;
+                        o.row0 = p.t.row0;
+                        o.first = p.first;
+                        o.end = p.end;
+                        o.slot = p.t.slot;
+                        o.length = p.t.length;
+                        o.start = p.t.length - p.t.n_new;
+                        o.token0 = static_cast<int>(p.t.token0);
+                        o.head = p.head;
+                        // the part of a shared item: 0 where an earlier CTA began it, 1 where this
+                        // one does, which then tells how many parts there are
+                        o.part = p.whole() ? -1 : (p.first > 0 ? 0 : 1);
+                        o.parts = o.part == 1 ? static_cast<int>(quotient(p.item_start + p.t.keys.nt - 1, share.per)) -
+                                                    static_cast<int>(blockIdx.x) + 1
+                                              : 0;
+                    }
+                    mbar_arrive(&sm.piece_full[n % kPieces]);
+                }
+                __syncwarp();
+            }
+        }
         // ---- MMA: the warp waits together, one lane issues
-        {
+        if (warp == kMmaWarp) {
             constexpr uint32_t qk = f16_idesc(128, kKeys, false), pv = f16_idesc(128, D, true);
             constexpr uint64_t kTile = (kKeys * D * 2) >> 4;   // descriptor step between the two buffers
             const uint64_t q_desc = sw128_desc(smem_u32(sm.q[0])), k_desc = sw128_desc(smem_u32(sm.k[0]));
@@ -477,10 +555,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 }
                 mma_commit_if(&sm.s_full[t], issue);
             };
-            Piece p;
-            while (walk.next(a, p)) {
-                const int halves = p.t.rows > kHalf ? 2 : 1;
+            for (int piece = 0;; ++piece) {
+                const Announced& p = piece_at(piece);
+                if (p.rows == 0 || *dead) break;
+                const int halves = p.rows > kHalf ? 2 : 1;
                 const int count = p.end - p.first;
+                piece_done(piece);
                 wait(&sm.k_full[n & 1], n >> 1);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
