@@ -10,6 +10,7 @@ by ``device_status``.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -20,11 +21,9 @@ _QUERY_DTYPES = {torch.float16: 1, torch.bfloat16: 2}
 _LAYOUTS = {"half": 0, "interleaved": 1}
 
 
-class _Heads(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("heads", C.c_int32)]
-
-
-_Pair = _Heads * 2
+# ufb_heads (data, token stride, head stride, heads), one or two of them
+_heads = struct.Struct("@Pqqi4x").pack
+_heads2 = struct.Struct("@Pqqi4xPqqi4x").pack
 
 
 class _Cache(C.Structure):
@@ -37,7 +36,7 @@ def _lib():
     if getattr(L, "_attention_ready", False):
         return L
     vp, ci, i64 = C.c_void_p, C.c_int, C.c_int64
-    cache, heads = C.POINTER(_Cache), C.POINTER(_Heads)
+    cache = heads = vp  # addresses; ufb_heads as packed bytes
     L.ufb_rotary_table.restype = i64
     L.ufb_rotary_table.argtypes = [ci, vp, vp, vp, vp]
     L.ufb_rotary.argtypes = [vp, ci, vp, vp, ci, ci, vp, i64, ci, ci, ci, heads, heads, vp]
@@ -88,7 +87,7 @@ def _refuse_heads(device, what, dtypes):
 
 def _head_tensor(t, device, what: str, dtypes=_DTYPES):
     """[tokens, heads, dim] on the device, rows of 16-byte multiples (copied if
-    not): the tensor, its shape, dtype code and description."""
+    not): the tensor, its sizes, dtype code, address and strides."""
     if not isinstance(t, torch.Tensor) or t.device != device:
         _refuse_heads(device, what, dtypes)
     shape, code = t.shape, dtypes.get(t.dtype)
@@ -106,7 +105,7 @@ def _head_tensor(t, device, what: str, dtypes=_DTYPES):
     if es != 1 or ts % lanes or hs % lanes or at % 16 or (heads > 1 and hs < dim) or (tokens > 1 and ts < dim):
         t = t.clone(memory_format=torch.contiguous_format)
         ts, hs, at = heads * dim, dim, t.data_ptr()
-    return t, shape, code, _Heads(at, ts, hs, heads)
+    return t, tokens, heads, dim, code, at, ts, hs
 
 
 class Rotary:
@@ -139,35 +138,37 @@ class Rotary:
         L.ufb_rotary_table(len(pairs), self._pairs, self._extents, b, host.data_ptr())
         self.table = host.to(self.device)
         self._fn, self._table, self._layout = L.ufb_rotary, self.table.data_ptr(), _LAYOUTS[layout]
+        self._axes, self._pairs_at, self._extents_at = len(pairs), C.addressof(self._pairs), C.addressof(self._extents)
 
     def apply(self, positions, q, k=None, inverse=False):
         """Turn q (and k in the same launch) by the tokens' positions
         ([tokens, axes] int32); inverse turns back, which is the gradient with
         respect to the input.  Returns new tensors: q, or (q, k)."""
-        axes = len(self.pairs)
         if not (isinstance(positions, torch.Tensor) and positions.device == self.device and
-                positions.dtype == torch.int32 and positions.dim() == 2 and positions.shape[1] == axes):
-            raise UfbError(-1, f"positions: int32 tensor [tokens, {axes}] on {self.device} required")
+                positions.dtype == torch.int32 and positions.dim() == 2 and positions.shape[1] == self._axes):
+            raise UfbError(-1, f"positions: int32 tensor [tokens, {self._axes}] on {self.device} required")
         if not positions.is_contiguous():
             positions = positions.contiguous()
         tokens = positions.shape[0]
-        q, qs, code, qh = _head_tensor(q, self.device, "rotary input")
+        device = self.device
+        q, qt, qn, dim, code, qa, qts, qhs = _head_tensor(q, device, "rotary input")
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        oh = _Heads(out.data_ptr(), qs[1] * qs[2], qs[2], qs[1])
-        if qs[0] != tokens:
+        if qt != tokens:
             raise UfbError(-1, "rotary inputs and positions differ in tokens")
         if k is None:
-            n, out2, x, y, most = 1, None, C.byref(qh), C.byref(oh), qs[1]
+            n, most = 1, qn
+            x, y = _heads(qa, qts, qhs, qn), _heads(out.data_ptr(), qn * dim, dim, qn)
         else:
-            k, ks, kcode, kh = _head_tensor(k, self.device, "rotary input")
-            if ks[0] != tokens or ks[2] != qs[2] or kcode != code:
+            k, kt, kn, kdim, kcode, ka, kts, khs = _head_tensor(k, device, "rotary input")
+            if kt != tokens or kdim != dim or kcode != code:
                 raise UfbError(-1, "rotary inputs differ in tokens, head_dim or dtype")
             out2 = torch.empty_like(k, memory_format=torch.contiguous_format)
-            n, most = 2, min(qs[1], ks[1])
-            x, y = _Pair(qh, kh), _Pair(oh, _Heads(out2.data_ptr(), ks[1] * ks[2], ks[2], ks[1]))
+            n, most = 2, min(qn, kn)
+            x = _heads2(qa, qts, qhs, qn, ka, kts, khs, kn)
+            y = _heads2(out.data_ptr(), qn * dim, dim, qn, out2.data_ptr(), kn * dim, dim, kn)
         if tokens and most:
-            _launch(self.device, self._fn, self._table, axes, self._pairs, self._extents, self._layout,
-                    1 if inverse else 0, positions.data_ptr(), tokens, qs[2], code, n, x, y)
+            _launch(device, self._fn, self._table, self._axes, self._pairs_at, self._extents_at, self._layout,
+                    1 if inverse else 0, positions.data_ptr(), tokens, dim, code, n, x, y)
         return out if k is None else (out, out2)
 
 
@@ -257,8 +258,9 @@ class KVCache:
                                                        self._work)],
                               self.layers, self.pages, self.heads, self.page_tokens, self.head_dim, self.slots,
                               self.table_width)
-        self._ref = C.byref(self._struct)
+        self._ref = C.addressof(self._struct)
         self._default_scale = self.head_dim ** -0.5
+        self._append, self._attend = L.ufb_kv_append, L.ufb_kv_attend
         self._workspaces = {}
 
     # -- streams and their pages
@@ -305,12 +307,13 @@ class KVCache:
     def append(self, layer, plan, k, v):
         """Store k and v [tokens, heads, head_dim] as the newest tokens of the plan's streams."""
         self._own(plan)
-        k, ks, code, kh = _head_tensor(k, self.device, "keys")
-        v, vs, vcode, vh = _head_tensor(v, self.device, "values")
-        if ks != vs or ks != (plan.tokens, self.heads, self.head_dim) or code != vcode:
+        device = self.device
+        k, kt, kn, kd, code, ka, kts, khs = _head_tensor(k, device, "keys")
+        v, vt, vn, vd, vcode, va, vts, vhs = _head_tensor(v, device, "values")
+        if not (kt == vt == plan.tokens and kn == vn == self.heads and kd == vd == self.head_dim and code == vcode):
             raise UfbError(-1, f"keys and values must be {[plan.tokens, self.heads, self.head_dim]} of one dtype")
-        _launch(self.device, self._L.ufb_kv_append, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new,
-                plan.tokens, code, C.byref(kh), C.byref(vh))
+        _launch(device, self._append, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new, kt, code,
+                _heads(ka, kts, khs, kn), _heads(va, vts, vhs, vn))
 
     def read(self, layer, pages, dtype=torch.float32):
         """The values of listed pages (int32 tensor): [n, 2, heads, page_tokens, head_dim]."""
@@ -348,15 +351,15 @@ class KVCache:
         sees nothing gives zeros.  Returns out, or (out, lse [tokens, query
         heads] float32)."""
         self._own(plan)
-        q, qs, code, qh = _head_tensor(q, self.device, "queries", _QUERY_DTYPES)
-        tokens, heads, dim = qs
+        device = self.device
+        q, tokens, heads, dim, code, qa, qts, qhs = _head_tensor(q, device, "queries", _QUERY_DTYPES)
         if tokens != plan.tokens or dim != self.head_dim or heads == 0 or heads % self.heads:
             raise UfbError(-1, f"queries must be [{plan.tokens}, a multiple of {self.heads}, {self.head_dim}]")
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        oh = _Heads(out.data_ptr(), heads * dim, dim, heads)
-        l = torch.empty((tokens, heads), dtype=torch.float32, device=self.device) if lse else None
+        l = torch.empty((tokens, heads), dtype=torch.float32, device=device) if lse else None
         w = self._workspace()
-        _launch(self.device, self._L.ufb_kv_attend, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new,
-                tokens, code, C.byref(qh), C.byref(oh), None if l is None else l.data_ptr(), window, sinks,
-                1 if causal else 0, self._default_scale if scale is None else scale, w[0], w[1])
+        _launch(device, self._attend, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new, tokens, code,
+                _heads(qa, qts, qhs, heads), _heads(out.data_ptr(), heads * dim, dim, heads),
+                None if l is None else l.data_ptr(), window, sinks, 1 if causal else 0,
+                self._default_scale if scale is None else scale, w[0], w[1])
         return (out, l) if lse else out

@@ -5,6 +5,7 @@
 #include "attention.h"
 #include "capi_util.h"
 
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -48,10 +49,14 @@ bool overlap(const ufb_heads& a, const ufb_heads& b, int64_t tokens, int head_di
 
 // SMs of the current device; 0 with the error recorded.
 int attend_sms() {
-    int device = 0, sms = 0;
-    if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice") ||
-        !cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device attribute"))
-        return 0;
+    static std::atomic<int> known[64];
+    int device = 0;
+    if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice")) return 0;
+    int sms = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+    if (sms == 0) {
+        if (!cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device attribute")) return 0;
+        if (device < 64) known[device].store(sms, std::memory_order_relaxed);
+    }
     return sms;
 }
 

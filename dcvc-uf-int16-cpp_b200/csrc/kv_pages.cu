@@ -258,17 +258,15 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const ufb_kv_cache c)
     for (int base = 0; base < c.pages; base += kThreads) {
         const int p = base + threadIdx.x;
         const bool used = p < c.pages && c.refs[p] > 0;
-        const bool hole = p < live && !used, mover = p >= live && used;
-        const int at_hole = block_scan(hole, warp_sum, total) + holes;
-        holes += total;
-        const int at_mover = block_scan(mover, warp_sum, total) + movers;
-        movers += total;
-        if (hole) w.found[at_hole] = p;
-        if (mover) w.source[at_mover] = p;
+        const bool hole = p < c.pages && p < live && !used, mover = p >= live && used;
+        // a page is one or the other: both counts in one sum of at most 1024 each
+        const int at = block_scan(hole + (mover << 16), warp_sum, total);
+        if (hole) w.found[holes + (at & 0xffff)] = p;
+        if (mover) w.source[movers + (at >> 16)] = p;
+        if (p < c.pages) w.rest[p] = p;   // the page's new id, for the tables
+        holes += total & 0xffff;
+        movers += total >> 16;
     }
-    __syncthreads();
-    // rest[page] = the page's new id, for the table pass
-    for (int p = threadIdx.x; p < c.pages; p += kThreads) w.rest[p] = p;
     __syncthreads();
     for (int i = threadIdx.x; i < movers; i += kThreads) {
         const int from = w.source[i], to = w.found[i];
@@ -279,27 +277,32 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const ufb_kv_cache c)
     if (threadIdx.x == 0) *w.moves = movers;
 }
 
-__global__ void __launch_bounds__(256) remap_kernel(const ufb_kv_cache c) {
-    const Work w = work_of(c);
-    const long long entries = static_cast<long long>(c.slots) * c.table_width;
-    for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < entries; i += gridDim.x * 256ll) {
-        const int page = c.table[i];
-        if (page >= 0 && page < c.pages) {
-            const int to = w.rest[page];
-            if (to != page) c.table[i] = to;
-        }
-    }
-}
+// Waits for the kernel before this one (launched with programmatic serialization:
+// this one's blocks start while that one runs).
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Moves of the list: grid (moves upper bound or less, layers * 2 sides).  A CTA
-// copies the valid tokens of every head of one side; PARTIAL: rest[move] tokens
-// of each head, else whole pages.
+// copies the tokens of every head of one side.  PARTIAL: rest[move] tokens of each
+// head.  Else whole pages, and one more row of blocks (y = layers * 2) takes the
+// moved pages' new ids (rest[page]) into the tables.
 template <bool PARTIAL>
 __global__ void __launch_bounds__(256) move_kernel(const ufb_kv_cache c) {
     const Work w = work_of(c);
-    const int moves = *w.moves;
     const int side = blockIdx.y & 1, layer = blockIdx.y >> 1;
     const int head_vecs = c.page_tokens * c.head_dim / 16;
+    wait_for_previous();
+    const int moves = *w.moves;
+    if (!PARTIAL && layer == c.layers) {
+        const long long entries = static_cast<long long>(c.slots) * c.table_width;
+        for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; moves && i < entries; i += gridDim.x * 256ll) {
+            const int page = c.table[i];
+            if (page >= 0 && page < c.pages) {
+                const int to = w.rest[page];
+                if (to != page) c.table[i] = to;
+            }
+        }
+        return;
+    }
     for (int m = blockIdx.x; m < moves; m += gridDim.x) {
         const long long from = ((static_cast<long long>(layer) * c.pages + w.source[m]) * 2 + side) * c.heads;
         const long long to = ((static_cast<long long>(layer) * c.pages + w.found[m]) * 2 + side) * c.heads;
@@ -310,16 +313,17 @@ __global__ void __launch_bounds__(256) move_kernel(const ufb_kv_cache c) {
         constexpr int kBatch = 8;
         for (int base = threadIdx.x; base < total; base += 256 * kBatch) {
             uint4 v[kBatch];
+            int at[kBatch];
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
                 const int i = base + j * 256;
-                if (i < total) v[j] = __ldcs(in + (PARTIAL ? (i / vecs) * head_vecs + i % vecs : i));
+                const int head = PARTIAL ? i / vecs : 0;
+                at[j] = PARTIAL ? head * head_vecs + i - head * vecs : i;
+                if (i < total) v[j] = __ldcs(in + at[j]);
             }
 #pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const int i = base + j * 256;
-                if (i < total) out[PARTIAL ? (i / vecs) * head_vecs + i % vecs : i] = v[j];
-            }
+            for (int j = 0; j < kBatch; ++j)
+                if (base + j * 256 < total) out[at[j]] = v[j];
         }
         for (int h = threadIdx.x; h < c.heads; h += 256) c.scale[to + h] = c.scale[from + h];
     }
@@ -327,9 +331,17 @@ __global__ void __launch_bounds__(256) move_kernel(const ufb_kv_cache c) {
 
 template <bool PARTIAL>
 cudaError_t move(const ufb_kv_cache& c, int most, cudaStream_t s) {
-    // gridDim.y is bounded by 65535: kv_pages callers check layers
-    move_kernel<PARTIAL><<<dim3(most < 1024 ? most : 1024, c.layers * 2), 256, 0, s>>>(c);
-    return cudaGetLastError();
+    // layers are checked: gridDim.y stays below 65536
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(most < 1024 ? most : 1024, c.layers * 2 + (PARTIAL ? 0 : 1));
+    config.blockDim = dim3(256);
+    config.stream = s;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, move_kernel<PARTIAL>, c);
 }
 
 }  // namespace
@@ -360,12 +372,7 @@ cudaError_t kv_fork(const ufb_kv_cache& c, const int32_t* src, const int32_t* ds
 
 cudaError_t kv_compact(const ufb_kv_cache& c, int*, cudaStream_t s) {
     compact_kernel<<<1, kThreads, 0, s>>>(c);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    const long long entries = static_cast<long long>(c.slots) * c.table_width;
-    const long long blocks = (entries + 255) / 256;
-    remap_kernel<<<static_cast<unsigned>(blocks < 1184 ? blocks : 1184), 256, 0, s>>>(c);
-    e = cudaGetLastError();
+    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? move<false>(c, c.pages, s) : e;
 }
 

@@ -16,6 +16,11 @@ def att(ufb):
     return sys.modules[ufb.__name__ + ".attention"]
 
 
+class Heads(C.Structure):
+    """ufb_heads as include/uf_b200.h has it."""
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("heads", C.c_int32)]
+
+
 def _cache(att, **over):
     a = 1 << 20  # a fake device address; no check reads through it
     f = dict(kv=a, scale=a, table=a, lengths=a, refs=a, work=a, layers=2, pages=8, heads=2, page_tokens=64,
@@ -25,7 +30,14 @@ def _cache(att, **over):
 
 
 def _heads(att, data=1 << 24, token=512, head=128, heads=2):
-    return att._Heads(data, token, head, heads)
+    return Heads(data, token, head, heads)
+
+
+def test_packed_heads_match_the_struct(att):
+    """The Python view packs ufb_heads by itself."""
+    h = Heads(1 << 40, 1 << 35, -7, 12)
+    assert att._heads(1 << 40, 1 << 35, -7, 12) == bytes(h) and C.sizeof(Heads) == 32
+    assert att._heads2(1, 2, 3, 4, 5, 6, 7, 8) == bytes(Heads(1, 2, 3, 4)) + bytes(Heads(5, 6, 7, 8))
 
 
 def test_rotary_table(att):
@@ -56,15 +68,15 @@ def test_rotary_refusals(att):
     L = att._lib()
     pairs, extents = (C.c_int32 * 2)(16, 16), (C.c_int32 * 2)(8, 8)
     base = dict(table=4096, axes=2, pairs=pairs, extents=extents, layout=0, inverse=0, positions=4096, tokens=3,
-                head_dim=64, dtype=1, count=1, x=(att._Heads * 1)(_heads(att, 1 << 24, 256, 64, 4)),
-                out=(att._Heads * 1)(_heads(att, 1 << 25, 256, 64, 4)))
+                head_dim=64, dtype=1, count=1, x=(Heads * 1)(_heads(att, 1 << 24, 256, 64, 4)),
+                out=(Heads * 1)(_heads(att, 1 << 25, 256, 64, 4)))
 
     def call(**over):
         f = {**base, **over}
         return L.ufb_rotary(*[f[k] for k in ("table", "axes", "pairs", "extents", "layout", "inverse", "positions",
                                              "tokens", "head_dim", "dtype", "count", "x", "out")], None)
 
-    one = lambda *a: (att._Heads * 1)(_heads(att, *a))
+    one = lambda *a: (Heads * 1)(_heads(att, *a))
     for over in (dict(axes=0), dict(axes=5), dict(pairs=None), dict(dtype=3), dict(layout=2), dict(head_dim=40),
                  dict(head_dim=272), dict(head_dim=48), dict(count=0), dict(count=3), dict(table=None),
                  dict(positions=None), dict(x=None), dict(x=one(None, 256, 64, 4)), dict(x=one(1 << 24, 256, 64, 0)),
