@@ -238,26 +238,20 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 auto seen = [&](int c) {   // of 32 columns, a bit each
                     return bits_below(high - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
                 };
-                // The loops run over 32 columns and are not unrolled: three roles share
-                // each scheduler's instruction cache.
+                // 64 columns at a time, the later ones first: the others stay for their
+                // weights.  Loops are not unrolled: three roles share each scheduler's
+                // instruction cache.
+                uint32_t s0[32], s1[32];
                 float top = -INFINITY;
                 auto maximum = [&](auto masked) {
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t s[32];
-                        tmem_ld32(ts + c * 32, s);
-                        tmem_wait_ld();
-                        tmem_tie32(s);
-                        if (decltype(masked)::value) {
-                            const uint32_t bits = seen(c);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!(bits & (1u << j))) s[j] = 0xff800000u;
-                        }
+                    auto chunk = [&](int c, const uint32_t (&s)[32]) {
+                        const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            const uint32_t* x = s + g * 16;
-                            auto f = [&](int j) { return __uint_as_float(x[j]); };
+                            auto f = [&](int j) {
+                                return decltype(masked)::value && !(bits & (1u << (g * 16 + j))) ? -INFINITY
+                                                                                              : __uint_as_float(s[g * 16 + j]);
+                            };
                             float y = max3(f(0), f(1), f(2)), z = max3(f(3), f(4), f(5));
                             y = max3(y, f(6), f(7)), z = max3(z, f(8), f(9));
                             y = max3(y, f(10), f(11)), z = max3(z, f(12), f(13));
@@ -268,6 +262,16 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                             // -infinity: nothing of the group is seen
                             top = fmaxf(top, decltype(masked)::value && y == -INFINITY ? y : v);
                         }
+                    };
+#pragma unroll 1
+                    for (int c = 2; c >= 0; c -= 2) {
+                        tmem_ld32(ts + c * 32, s0);
+                        tmem_ld32(ts + c * 32 + 32, s1);
+                        tmem_wait_ld();
+                        tmem_tie32(s0);
+                        tmem_tie32(s1);
+                        chunk(c, s0);
+                        chunk(c + 1, s1);
                     }
                 };
                 if (clear) maximum(std::false_type());
@@ -318,18 +322,15 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                         tmem_st16(ts + c * 16, w);
                     };
                     // the next columns are on their way while these are worked on
-                    uint32_t s0[32], s1[32];
-                    tmem_ld32(ts, s0);
 #pragma unroll 1
                     for (int half = 0; half < 2; ++half) {
                         tmem_wait_ld();
                         tmem_tie32(s0);
-                        tmem_ld32(ts + half * 64 + 32, s1);
-                        chunk(half * 2, s0);
-                        tmem_wait_ld();
                         tmem_tie32(s1);
+                        chunk(half * 2, s0);
                         if (half == 0) tmem_ld32(ts + 64, s0);
                         chunk(half * 2 + 1, s1);
+                        if (half == 0) tmem_ld32(ts + 96, s1);
                         // P V starts on the first 64 keys while the others are in the works
                         tmem_wait_st();
                         tc_fence_before();
