@@ -53,7 +53,7 @@ constexpr float kShift = 15.0f;
 constexpr int kCodeFull = 41, kCodeEmpty = 42, kCodeDrain = 43;
 
 struct PageScales {
-    float key, log2_value, inv_value;  // log2_value -inf: the 16 keys are not there
+    float key, log2_value, inv_value;  // key times 2^24; log2_value -inf: the 16 keys are not there
     float pad;
 };
 
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
             sc.log2_value = -INFINITY;
             if (now.page >= 0) {
                 const float v = now.value < kTinyScale ? kTinyScale : now.value;
-                sc.key = now.key;
+                sc.key = now.key * kKeyUnit;
                 sc.log2_value = log2f(v);
                 sc.inv_value = 1.0f / v;
             }
@@ -287,9 +287,8 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int from = (2 * c + r) * 4;
-                // keys enter as (integer + 128) 2^-24 (below): scale and offset take that back
-                unit[n][r] = __shfl_sync(0xffffffffu, f, from) * 16777216.0f;
-                offset[n][r] = __shfl_sync(0xffffffffu, sum, from) * (-128.0f / 16777216.0f);
+                unit[n][r] = __shfl_sync(0xffffffffu, f, from);
+                offset[n][r] = __shfl_sync(0xffffffffu, sum, from) * kKeyOffset;
                 pos[n][r] = __shfl_sync(0xffffffffu, at, from);
             }
         }
@@ -357,11 +356,9 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
                 for (int k = 0; k < kSteps / 2; ++k)
 #pragma unroll
                     for (int x = 0; x < kM; ++x) {
-                        // an integer plus 128 in the low byte is a float16 below the normal ones,
-                        // (integer + 128) 2^-24, exactly
-                        const uint32_t u = w[x][0][k] ^ 0x80808080u, v = w[x][1][k] ^ 0x80808080u;
-                        const uint32_t f[4] = {__byte_perm(u, 0, 0x4140), __byte_perm(v, 0, 0x4140),
-                                               __byte_perm(u, 0, 0x4342), __byte_perm(v, 0, 0x4342)};
+                        uint32_t f[4];
+                        keyx4_to_half(w[x][0][k], f[0], f[2]);
+                        keyx4_to_half(w[x][1][k], f[1], f[3]);
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
                             mma16816(s[x][n], f, q[n][i * (kSteps / 2) + k][0], q[n][i * (kSteps / 2) + k][1]);
