@@ -627,41 +627,63 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
     }
 }
 
-// Rows that several CTAs share: the item that CTA x's share ends in, 16 rows a block.
+// Rows that several CTAs share: the item that CTA x's share ends in, a block's rows
+// from kJoinRows * y on.  The parts' maxima and weights come first, once a row, by a
+// warp; then a thread adds the parts of four columns, in the order of the CTAs.
+constexpr int kJoinThreads = 256;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) join_kernel(const AttendArgs a, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendArgs a, int ctas) {
+    constexpr int kJoinRows = kJoinThreads / (D / 4);
+    __shared__ float share[kAttendMaxCtas][kJoinRows];   // of a part in a row's sum
+    __shared__ float tops[kJoinRows], weights[kJoinRows];
     const AttendScratch scratch = scratch_of(a.workspace, ctas, kRows);
-    const int c0 = blockIdx.x;
+    const int c0 = blockIdx.x, first = blockIdx.y * kJoinRows;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int32_t* item = scratch.items + c0 * 8;
-    const int parts = item[0];
-    if (parts == 0) return;
-    const int rows = min(item[3] - static_cast<int>(blockIdx.y) * 16, 16);
-    for (int e = threadIdx.x; e < rows * (D / 4); e += 128) {
-        const int row = blockIdx.y * 16 + e / (D / 4), d = e % (D / 4) * 4;
+    const int parts = item[0], rows = min(item[3] - first, kJoinRows);
+    if (parts == 0 || rows <= 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < rows; r += kJoinThreads / 32) {
         float top = -INFINITY;
-#pragma unroll 4
-        for (int i = 0; i < parts; ++i) top = fmaxf(top, scratch.stats[(2 * (c0 + i) + (i == 0)) * 2 * kRows + row]);
+        for (int i = lane; i < parts; i += 32)
+            top = fmaxf(top, scratch.stats[(2 * (c0 + i) + (i == 0)) * 2 * kRows + first + r]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         float weight = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int i = 0; i < parts; ++i) {
+        for (int i = lane; i < parts; i += 32) {
             const int from = 2 * (c0 + i) + (i == 0);
-            const float m = scratch.stats[from * 2 * kRows + row], l = scratch.stats[(from * 2 + 1) * kRows + row];
-            const float4 x = *reinterpret_cast<const float4*>(scratch.sums + (static_cast<long long>(from) * kRows + row) * D + d);
+            const float m = scratch.stats[from * 2 * kRows + first + r], l = scratch.stats[(from * 2 + 1) * kRows + first + r];
             const float mul = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2(m - top);
+            share[i][r] = mul;
             weight += l * mul;
-            v.x += x.x * mul, v.y += x.y * mul, v.z += x.z * mul, v.w += x.w * mul;
         }
-        const int in_stream = item[2] + row, token = in_stream / a.group;
-        const int head = item[4] * a.group + in_stream - token * a.group;
-        const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
-        T* to = static_cast<T*>(a.out.data) + (item[1] + static_cast<long long>(token)) * a.out.token_stride +
-                head * a.out.head_stride + d;
-        *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
-        if (a.lse && d == 0)
-            a.lse[(item[1] + static_cast<long long>(token)) * (a.heads * a.group) + head] =
-                weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) weight += __shfl_xor_sync(0xffffffffu, weight, o);
+        if (lane == 0) tops[r] = top, weights[r] = weight;
     }
+    __syncthreads();
+    const int r = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    if (r >= rows) return;
+    const int row = first + r;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) {
+        const int from = 2 * (c0 + i) + (i == 0);
+        const float4 x = *reinterpret_cast<const float4*>(scratch.sums + (static_cast<long long>(from) * kRows + row) * D + d);
+        const float mul = share[i][r];
+        v.x += x.x * mul, v.y += x.y * mul, v.z += x.z * mul, v.w += x.w * mul;
+    }
+    const int in_stream = item[2] + row, token = in_stream / a.group;
+    const int head = item[4] * a.group + in_stream - token * a.group;
+    const float top = tops[r], weight = weights[r];
+    const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+    const long long out_row = item[1] + static_cast<long long>(token);
+    T* to = static_cast<T*>(a.out.data) + out_row * a.out.token_stride + head * a.out.head_stride + d;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
+    if (a.lse && d == 0)
+        a.lse[out_row * (a.heads * a.group) + head] =
+            weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
 }
 
 template <typename T, int D>
@@ -678,8 +700,17 @@ cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     many_kernel<T, D><<<ctas, kThreads, smem, s>>>(a, static_cast<int>(row_tiles), 1);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    join_kernel<T, D><<<dim3(ctas, kRows / 16), 128, 0, s>>>(a, ctas);
-    return cudaGetLastError();
+    // its blocks start while the last CTAs still work, and wait for them
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(ctas, kRows * (D / 4) / kJoinThreads);
+    config.blockDim = dim3(kJoinThreads);
+    config.stream = s;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, join_kernel<T, D>, a, ctas);
 }
 
 }  // namespace
