@@ -80,6 +80,12 @@ def _launch(device, fn, *args):
         _check(rc)
 
 
+def _check_ints(layer, window=0, sinks=0):
+    # ctypes would cut larger numbers to 32 bits
+    if layer >> 31 or window >> 31 or sinks >> 31:
+        raise UfbError(-1, "layer, window and sinks must be 32-bit numbers that are not negative")
+
+
 def _refuse_heads(device, what, dtypes):
     names = ", ".join(str(d).replace("torch.", "") for d in dtypes)
     raise UfbError(-1, f"{what}: [tokens, heads, head_dim] tensor of {names} on {device} required")
@@ -291,6 +297,7 @@ class KVCache:
     def trim(self, plan, window, sinks=0):
         """Drop the pages that no later query of the plan's streams sees."""
         self._own(plan)
+        _check_ints(0, window, sinks)
         _launch(self.device, self._L.ufb_kv_trim, self._ref, plan._slots, plan.n, int(window), int(sinks))
 
     def fork(self, plan):
@@ -307,6 +314,7 @@ class KVCache:
     def append(self, layer, plan, k, v):
         """Store k and v [tokens, heads, head_dim] as the newest tokens of the plan's streams."""
         self._own(plan)
+        _check_ints(layer)
         device = self.device
         k, kt, kn, kd, code, ka, kts, khs = _head_tensor(k, device, "keys")
         v, vt, vn, vd, vcode, va, vts, vhs = _head_tensor(v, device, "values")
@@ -322,6 +330,7 @@ class KVCache:
             raise UfbError(-1, f"pages: int32 list on {self.device} required")
         if dtype not in _DTYPES:
             raise UfbError(-1, "unsupported dtype")
+        _check_ints(layer)
         if not pages.is_contiguous():
             pages = pages.contiguous()
         n = pages.shape[0]
@@ -349,8 +358,10 @@ class KVCache:
         j when j <= a (all keys when not causal) and, with a window, j > a -
         window or j < sinks.  scale defaults to head_dim ** -0.5.  A query that
         sees nothing gives zeros.  Returns out, or (out, lse [tokens, query
-        heads] float32)."""
+        heads] float32).  Every CUDA stream has its own scratch; a call captured
+        in a graph keeps that of the stream it was captured on."""
         self._own(plan)
+        _check_ints(layer, window, sinks)
         device = self.device
         q, tokens, heads, dim, code, qa, qts, qhs = _head_tensor(q, device, "queries", _QUERY_DTYPES)
         if tokens != plan.tokens or dim != self.head_dim or heads == 0 or heads % self.heads:

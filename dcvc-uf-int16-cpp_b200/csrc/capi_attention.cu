@@ -15,6 +15,8 @@ using namespace ufb;
 
 namespace {
 
+constexpr int kMostKeys = 1 << 30;  // of a stream
+
 int element_size(int dtype) { return dtype == UFB_F32 ? 4 : 2; }
 
 int* current_status() {
@@ -69,7 +71,9 @@ bool check_cache(const ufb_kv_cache* c) {
         return fail(UFB_EINVAL, "page_tokens must be 16, 32, 64 or 128");
     if (c->head_dim != 64 && c->head_dim != 128) return fail(UFB_EINVAL, "head_dim must be 64 or 128");
     if (reinterpret_cast<uintptr_t>(c->kv) % 128) return fail(UFB_EINVAL, "cache kv must be 128-byte aligned");
-    if (c->layers > 32767 || c->heads > 32767) return fail(UFB_ERANGE, "cache exceeds grid bounds");
+    if (c->layers > 32766 || c->heads > 32767) return fail(UFB_ERANGE, "cache exceeds grid bounds");
+    if (static_cast<int64_t>(c->table_width) * c->page_tokens > kMostKeys)
+        return fail(UFB_ERANGE, "a stream may hold 2^30 tokens at most");
     return true;
 }
 
@@ -297,7 +301,7 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
     a.head_dim = c->head_dim;
     a.slots_total = c->slots;
     a.table_width = c->table_width;
-    a.window = window;
+    a.window = window < kMostKeys ? window : kMostKeys;  // positions less the window stay in 32 bits
     a.sinks = sinks;
     a.causal = causal != 0;
     a.scale_log2 = scale * 1.4426950408889634f;

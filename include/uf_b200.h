@@ -486,7 +486,8 @@ int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t
  * kv[layer][page][side][head][i][:] * scale[layer][page][side][head], side 0 the
  * key, 1 the value.  refs counts the table entries of each page (0: free).
  * A page that its stream has not filled is never shared.
- * page_tokens 16, 32, 64 or 128; head_dim 64 or 128; kv 128-byte aligned. */
+ * page_tokens 16, 32, 64 or 128; head_dim 64 or 128; kv 128-byte aligned;
+ * table_width * page_tokens at most 2^30. */
 typedef struct ufb_kv_cache {
     int8_t* kv;       /* [layers][pages][2][heads][page_tokens][head_dim] */
     float* scale;     /* [layers][pages][2][heads] */
@@ -550,8 +551,8 @@ int ufb_kv_read(const ufb_kv_cache* c, int layer, const int32_t* pages, int64_t 
  * after a power of two for each query and head, so that no value of its type is
  * out of range; p with 11 significant bits down to 2^-27 of the largest p times
  * value scale of its row, and in steps of 2^-37 of it below.  Scales are not negative.
- * workspace: ufb_kv_attend_workspace() bytes, zero before its first use; calls
- * that may overlap need one each. */
+ * workspace: ufb_kv_attend_workspace() bytes, zero before its first use (and
+ * again after a status of 41..44); calls that may overlap need one each. */
 int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
                   int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse, int window,
                   int sinks, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream);

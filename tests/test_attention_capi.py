@@ -106,6 +106,8 @@ def test_cache_refusals(att):
         assert L.ufb_kv_append(c, 0, 4096, 4096, 1, 1, 1, 1, h, h, None) == EINVAL
         assert L.ufb_kv_read(c, 0, 4096, 1, 0, 4096, None) == EINVAL
         assert L.ufb_kv_attend(c, 0, 4096, 4096, 1, 1, 1, 1, h, h, None, 0, 0, 1, 1.0, 4096, 1 << 30, None) == EINVAL
+    for over in (dict(table_width=1 << 25), dict(layers=32767), dict(heads=40000)):
+        assert L.ufb_kv_compact(C.byref(_cache(att, **over)), None) == ERANGE, over
     c = C.byref(_cache(att))
     for n in (-1, 5):
         assert L.ufb_kv_release(c, 4096, n, None) == EINVAL

@@ -406,6 +406,25 @@ def test_attend_in_a_graph(ufb, dev):
     _clean(ufb)
 
 
+@pytest.mark.parametrize("new", [3, 50])
+def test_attend_windows_at_the_ends_of_the_range(ufb, dev, new):
+    """The largest window is none; queries before the first key keep their place."""
+    cache = make_cache(ufb, dev, [100, 2], 2, 64, 16)
+    plan = cache.plan([0, 1], [new, new])
+    q = randn(dev, (2 * new, 4, 64), 1, torch.bfloat16)
+    for causal in (True, False):
+        want = cache.attend(0, plan, q, causal=causal)
+        for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1), (2 ** 30, 1)):
+            assert torch.equal(cache.attend(0, plan, q, window=window, sinks=sinks, causal=causal), want)
+        check_attend(ufb, cache, [0, 1], [new, new], 4, torch.bfloat16, window=2, sinks=1, causal=causal)
+    for kw in ({"window": 2 ** 31}, {"sinks": 2 ** 32}, {"window": -2 ** 33}):
+        with pytest.raises(ufb.UfbError):
+            cache.attend(0, plan, q, **kw)
+    with pytest.raises(ufb.UfbError):
+        cache.attend(2 ** 32, plan, q)
+    _clean(ufb)
+
+
 def test_attend_refusals(ufb, dev):
     cache = make_cache(ufb, dev, [100, 50], 2, 64, 16)
     plan = cache.plan([0, 1], [2, 1])
