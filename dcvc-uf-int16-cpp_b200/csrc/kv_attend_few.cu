@@ -25,7 +25,8 @@
 // bank conflicts under TMA's 128-byte swizzle.
 //
 // 64 streams x 16000 keys x 4 heads of 128: 188 us, 5.6 TB/s, 0.87 of a plain
-// copy's rate (8 consumer warps with the rows as the wide side: 220 us and more);
+// copy's rate (8 consumer warps with the rows as the wide side: 160 us for 127 on 64
+// ragged streams up to 16320 keys);
 // head_dim 64 at 3.3 TB/s, bound by the expansion; one token over 1760 keys 12 us.
 //
 // Parts of an item that several CTAs share are joined by the CTA that arrives
