@@ -268,6 +268,7 @@ class KVCache:
         self._default_scale = self.head_dim ** -0.5
         self._append, self._attend = L.ufb_kv_append, L.ufb_kv_attend
         self._workspaces = {}
+        self._spare = self._new_workspace()
 
     # -- streams and their pages
 
@@ -301,7 +302,8 @@ class KVCache:
         _launch(self.device, self._L.ufb_kv_trim, self._ref, plan._slots, plan.n, int(window), int(sinks))
 
     def fork(self, plan):
-        """Make the plan's destinations branches of its sources."""
+        """Make the plan's destinations branches of its sources, whose tokens have
+        been appended in every layer: full pages are shared from here on."""
         self._own(plan, KVForkPlan)
         _launch(self.device, self._L.ufb_kv_fork, self._ref, plan._src, plan._dst, plan.n)
 
@@ -339,17 +341,30 @@ class KVCache:
                 out.data_ptr())
         return out
 
+    def _new_workspace(self):
+        with torch.cuda.device(self.device):
+            n = self._L.ufb_kv_attend_workspace()
+        if n < 0:
+            _check(int(n))
+        t = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        return t.data_ptr(), n, t
+
     def _workspace(self):
         # zeroed once and left zeroed by every call; streams may overlap, so each has its own
         key = _raw_stream(self.device.index)
         w = self._workspaces.get(key)
         if w is None:
             with torch.cuda.device(self.device):
-                n = self._L.ufb_kv_attend_workspace()
-            if n < 0:
-                _check(int(n))
-            t = torch.zeros(n, dtype=torch.uint8, device=self.device)
-            w = self._workspaces[key] = (t.data_ptr(), n, t)
+                capturing = torch.cuda.is_current_stream_capturing()
+            if not capturing:
+                w = self._new_workspace()
+            elif self._spare is None:
+                raise UfbError(-1, "this stream has no attention scratch yet: call attend on it once before capturing")
+            else:
+                # zeros made here would be zeroed by this graph's replays only, and
+                # another graph of the stream, or the stream itself, may run first
+                w, self._spare = self._spare, None
+            self._workspaces[key] = w
         return w
 
     def attend(self, layer, plan, q, window=0, sinks=0, causal=True, scale=None, lse=False):
@@ -359,7 +374,8 @@ class KVCache:
         window or j < sinks.  scale defaults to head_dim ** -0.5.  A query that
         sees nothing gives zeros.  Returns out, or (out, lse [tokens, query
         heads] float32).  Every CUDA stream has its own scratch; a call captured
-        in a graph keeps that of the stream it was captured on."""
+        in a graph keeps that of the stream it was captured on.  One stream may
+        capture without an earlier call on it; others call attend once before."""
         self._own(plan)
         _check_ints(layer, window, sinks)
         device = self.device

@@ -512,7 +512,9 @@ int ufb_kv_release(const ufb_kv_cache* c, const int32_t* slots, int n, void* str
 /* Stream dst[i] becomes a branch of stream src[i] (what it held is released
  * first): full pages are shared, the tokens of a partly filled last page are
  * copied, in every layer, to a page of its own (lowest free page first, in the
- * order of the list).  No dst twice, no dst among src. */
+ * order of the list).  No dst twice, no dst among src.  The sources' tokens are
+ * stored in every layer before it: what is appended to a shared page afterwards
+ * shows in all its branches. */
 int ufb_kv_fork(const ufb_kv_cache* c, const int32_t* src, const int32_t* dst, int n, void* stream);
 
 /* Drop the pages of the listed streams that no later query sees through a

@@ -406,6 +406,38 @@ def test_attend_in_a_graph(ufb, dev):
     _clean(ufb)
 
 
+def test_attend_captured_without_an_earlier_call(ufb, dev):
+    """The scratch of a capturing stream is zero before any graph runs, whichever
+    graph runs first; a second capturing stream has to have called before."""
+    cache = make_cache(ufb, dev, [3000, 200], 2, 64, 32, spare=8)
+    side, other = torch.cuda.Stream(dev), torch.cuda.Stream(dev)
+    graphs, outs, qs, plans = [], [], [], []   # a graph reads them at every replay
+    for i, new in enumerate((40, 3)):   # tiles of many rows, of few rows
+        plan = cache.plan([0, 1], [new, new])
+        plans.append(plan)
+        q = randn(dev, (2 * new, 4, 64), i, torch.float16)
+        torch.cuda.synchronize(dev)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(cache.attend(0, plan, q))
+        graphs.append(graph)
+        qs.append((q, new))
+    (scratch,) = [w[2] for w in cache._workspaces.values()]
+    assert not bool(scratch.any())
+    for i in (1, 0, 1):
+        outs[i].fill_(float("nan"))
+        graphs[i].replay()
+        torch.cuda.synchronize(dev)
+        q, new = qs[i]
+        want, _, tol, _ = attend_ref(cache, 0, [0, 1], [new, new], q, 0, 0, True, 64 ** -0.5)
+        assert bool(((outs[i].double() - want).abs() <= tol + ULP[torch.float16] * want.abs() + F16_TINY).all())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(ufb.UfbError, match="before capturing"):
+        with torch.cuda.graph(graph, stream=other):
+            cache.attend(0, plan, q)
+    _clean(ufb)
+
+
 @pytest.mark.parametrize("new", [3, 50])
 def test_attend_windows_at_the_ends_of_the_range(ufb, dev, new):
     """The largest window is none; queries before the first key keep their place."""
