@@ -618,6 +618,13 @@ def bench_626(ufb, syn, mi, mv, dev, stream, peak):
     return out
 
 
+def ref_missing():
+    """Why the reference's library cannot be timed here, or None.  Without it the
+    measurements of this framework stand without that CPU baseline."""
+    path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "oracle", "_ref", "libufref.so")
+    return None if os.path.exists(path) else "oracle/_ref/libufref.so is not built (make -C oracle ref REF_ROOT=<reference>)"
+
+
 def ref_decode_sample(threads):
     """Reference IntegerModel::decompress (oracle/_ref) on a 128x128 sample;
     returns (seconds per P packet, seconds per I packet)."""
@@ -922,6 +929,9 @@ def main():
     if args.impl == "reference":
         if rank != 0:
             return
+        if args.workload != "warp" and ref_missing():
+            print(json.dumps({"impl": "reference", "unavailable": ref_missing()}))
+            return
         kind, cores = "reference", threads
         if args.workload == "conv":
             runs = [ref_conv(threads) for _ in range(max(args.steps, 1))]
@@ -963,12 +973,12 @@ def main():
             res["cpu_baseline"] = {"value": v, "unit": "warps/s", "cores": 1, "kind": "port", "sample": note}
     elif args.workload == "conv":
         res = bench_conv_ours(args, rank, world, local)
-        if rank == 0 and world == 1:
+        if rank == 0 and world == 1 and not ref_missing():
             v, note = ref_conv(1)
             res["cpu_baseline"] = {"value": v, "unit": "MAC/s", "cores": 1, "kind": "reference", "sample": note}
     else:
         res = bench_decode_ours(args, rank, world, local)
-        if rank == 0 and world == 1:
+        if rank == 0 and world == 1 and not ref_missing():
             t_p, t_i = ref_decode_sample(threads)
             res["cpu_baseline"] = {"value": ref_fps_1080(t_p, t_i), "unit": "frames/s", "cores": threads,
                                    "kind": "reference", "sample": ref_decode_note(t_p, t_i)}
