@@ -22,7 +22,7 @@
 // cycle) and 2200 for the products (measured alone), side by side.  A tile takes
 // about 4900: the chain S, softmax, P V, S of a half, whose S and P share columns,
 // and four roles' instructions on the same schedulers.  8160 tokens x 24480 keys,
-// 16 heads: 1.84 ms, 890 TFLOP/s, 0.52 of cuBLAS's rate in bfloat16; the first form
+// 16 heads: 1.85 ms, 885 TFLOP/s, 0.52 of cuBLAS's rate in bfloat16; the first form
 // of this kernel took 3.66 ms.  A running maximum that grows little is kept, so O is
 // rescaled rarely and by the softmax threads themselves.
 //
