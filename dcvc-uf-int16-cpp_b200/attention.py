@@ -235,6 +235,10 @@ class KVCache:
         cache.extend(plan)                    # pages for them, once a step
         cache.append(layer, plan, k, v)       # in every layer
         out = cache.attend(layer, plan, q, window=..., sinks=...)
+
+    When the pages do not suffice, extend changes nothing (status 31), and append
+    and attend leave out the streams that were to grow (status 31 again, zeros for
+    their queries) until an extend of theirs is granted, one of no tokens too.
     """
 
     def __init__(self, layers, pages, heads, head_dim, page_tokens=64, slots=1, table_width=None, device="cuda"):

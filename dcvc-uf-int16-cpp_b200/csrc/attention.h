@@ -30,6 +30,12 @@ struct RotaryArgs {
 };
 cudaError_t rotary(const RotaryArgs& a, int dtype, int* status, cudaStream_t s);
 
+// Marks of streams (one for each slot, behind the page operators' scratch in
+// ufb_kv_cache.work): 1 from an extend that was refused to one that is granted.
+__host__ __device__ inline int32_t* kv_refused(const ufb_kv_cache& c) {
+    return c.work + 16 + 3ll * c.pages + c.slots;
+}
+
 // Streams of one call: new tokens [offsets[i], offsets[i + 1]) belong to slots[i].
 struct KvBatch {
     const int32_t* slots;
@@ -57,6 +63,7 @@ struct AttendArgs {
     const float* scale;
     const int32_t* table;
     const int32_t* lengths;
+    const int32_t* refused;          // kv_refused
     const int32_t* slots;
     const int32_t* offsets;
     long long tokens;

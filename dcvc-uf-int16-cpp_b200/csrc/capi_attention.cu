@@ -178,7 +178,7 @@ int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t
 int64_t ufb_kv_work_ints(int32_t pages, int32_t slots) {
     clear_error();
     if (pages <= 0 || slots <= 0) return err(UFB_EINVAL, "empty cache");
-    return 16 + 3ll * pages + slots;
+    return 16 + 3ll * pages + 2ll * slots;
 }
 
 int ufb_kv_extend(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, void* stream) {
@@ -288,6 +288,7 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
     a.scale = c->scale + layer * page_heads;
     a.table = c->table;
     a.lengths = c->lengths;
+    a.refused = kv_refused(*c);
     a.slots = slots;
     a.offsets = offsets;
     a.tokens = tokens;

@@ -180,6 +180,9 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const ufb_kv_cache c, 
     if (slot < 0 || slot >= c.slots || t0 < 0 || t0 + static_cast<long long>(count) > b.tokens || count > b.max_new ||
         c.lengths[slot] < count) {
         if (threadIdx.x == 0) atomicCAS(status, 0, kStatusIndex);
+    } else if (kv_refused(c)[slot]) {
+        // no room was made for them: the stream's last tokens are stored ones, maybe on shared pages
+        if (threadIdx.x == 0) atomicCAS(status, 0, kStatusPages);
     } else if (tile_index < tiles) {
         const int length = c.lengths[slot], start = length - count;
         const int entry = (start >> shift) + at_page;

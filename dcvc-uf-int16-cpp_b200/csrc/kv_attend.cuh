@@ -80,6 +80,11 @@ __device__ __forceinline__ bool row_tile(const AttendArgs& a, int stream, int rt
     if (!ok && rt == 0) atomicCAS(a.status, 0, kStatusIndex);
     if (t.rows <= 0) return false;
     t.length = max(a.lengths[t.slot], 0);
+    if (a.refused[t.slot]) {
+        // its new tokens were not taken in: no position is theirs, they see no key
+        t.length = 0;
+        if (rt == 0) atomicCAS(a.status, 0, kStatusPages);
+    }
     t.keys = key_range<BK>(a, t.length, t.n_new, t.row0 / a.group, (t.row0 + t.rows - 1) / a.group);
     return true;
 }

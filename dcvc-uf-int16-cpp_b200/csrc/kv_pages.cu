@@ -20,7 +20,7 @@ constexpr int kWarps = kThreads / 32;
 
 // Scratch layout (int32): [0] moves to make, [16, 16 + pages) free pages found,
 // in order; then [pages) moves' sources / [pages) token counts; then one offset
-// per request (slots).
+// per request (slots).  Behind it lie the marks of refused streams (kv_refused).
 struct Work {
     int32_t* moves;
     int32_t* found;
@@ -139,11 +139,18 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ufb_kv_cache c, 
                     c.table[static_cast<long long>(slot) * c.table_width + first + e] = page;
                     c.refs[page] = 1;
                 }
-                if (lane == 0) c.lengths[slot] = have + count;
+                if (lane == 0) {
+                    c.lengths[slot] = have + count;
+                    kv_refused(c)[slot] = 0;
+                }
             }
             return;
         }
     }
+    // the lengths stay, so the last tokens of these streams are no new ones: append and
+    // attend of the step that goes on regardless must not take them for such
+    for (int i = threadIdx.x; i < n; i += kThreads)
+        if (valid_slot(c, slots[i]) && offsets[i + 1] > offsets[i]) kv_refused(c)[slots[i]] = 1;
     if (threadIdx.x == 0) atomicCAS(status, 0, any_index ? kStatusIndex : kStatusPages);
 }
 
@@ -171,7 +178,7 @@ __global__ void __launch_bounds__(128) drop_kernel(const ufb_kv_cache c, const i
     }
     if (window == 0) {
         drop_row(c, slot, 0, c.table_width);
-        if ((threadIdx.x & 31) == 0) c.lengths[slot] = 0;
+        if ((threadIdx.x & 31) == 0) c.lengths[slot] = kv_refused(c)[slot] = 0;
         return;
     }
     // the next query stands at length or later: keys below length - window + 1
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const ufb_kv_cache c, co
     if (found != need) {
         for (int i = warp; i < n; i += kWarps) {
             drop_row(c, dst[i], 0, c.table_width);
-            if (lane == 0) c.lengths[dst[i]] = 0;
+            if (lane == 0) c.lengths[dst[i]] = kv_refused(c)[dst[i]] = 0;
         }
         if (threadIdx.x == 0) atomicCAS(status, 0, kStatusPages);
         return;
@@ -241,6 +248,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const ufb_kv_cache c, co
             w.rest[at] = length % P;
         }
         c.lengths[dst[i]] = length;
+        kv_refused(c)[dst[i]] = kv_refused(c)[src[i]];
     }
     if (threadIdx.x == 0) *w.moves = need;
 }

@@ -440,7 +440,9 @@ int ufb_conv2d_noalloc(const int16_t* x, int n, int ci, int h, int w, const int1
  * in the status word of ufb_device_status:
  *   21 a position outside its axis (the token's heads become NaN)
  *   31 too few free pages, or a stream longer than its table row (extend: no
- *      stream was changed; fork: the destinations are left empty)
+ *      stream was changed; append, attend: the stream's extend was refused, its
+ *      tokens are not stored and its queries see no key; fork: the destinations
+ *      are left empty)
  *   32 a slot, page or token offset out of range, or a page that is missing
  *      where tokens are to be stored (what it names is skipped)
  *   41..44 a bounded wait of the attention kernel gave up
@@ -494,7 +496,8 @@ typedef struct ufb_kv_cache {
     int32_t* table;   /* [slots][table_width] */
     int32_t* lengths; /* [slots] tokens of each stream */
     int32_t* refs;    /* [pages] */
-    int32_t* work;    /* [ufb_kv_work_ints()] scratch of the page operators */
+    int32_t* work;    /* [ufb_kv_work_ints()] scratch of the page operators and marks of the
+                       * streams; zero before the cache's first call, kept between calls */
     int32_t layers, pages, heads, page_tokens, head_dim, slots, table_width;
 } ufb_kv_cache;
 
@@ -503,7 +506,12 @@ int64_t ufb_kv_work_ints(int32_t pages, int32_t slots);
 
 /* Make room: stream slots[i] grows by offsets[i + 1] - offsets[i] tokens
  * (lengths) and gets the pages for them, lowest free page first, in the order
- * of the list.  No slot twice. */
+ * of the list.  No slot twice.  When the pages do not suffice (or an index is out
+ * of range) nothing is changed and the streams that were to grow are marked:
+ * ufb_kv_append and ufb_kv_attend, which may be on the stream behind it already,
+ * leave them out (status 31) until an extend of theirs is granted -- one of no
+ * tokens is, and takes the stored tokens for its last again -- or they are
+ * released.  A fork takes its source's mark along. */
 int ufb_kv_extend(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, void* stream);
 
 /* Drop every page of the listed streams; their lengths become 0. */

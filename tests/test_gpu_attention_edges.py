@@ -1,0 +1,111 @@
+"""GPU: the ends of what the latent-attention operators take -- steps that were
+refused, queries and scores of any size, pages of zeros, graphs on one stream.
+
+Tolerances are those of test_gpu_attention.py, which derives them: a score errs
+by up to 2^-16 sum |q k| scale, so a weight exp(s - s') is known to a factor
+exp(2 err)."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_attention import F16_TINY, ULP, _clean, attend_ref, check_attend, contents, make_cache, randn
+
+pytestmark = pytest.mark.gpu
+
+
+def stored(cache):
+    return cache.kv.clone(), cache.scale.clone(), cache.table.clone(), cache.lengths.clone(), cache.refs.clone()
+
+
+def same(before, cache):
+    return all(torch.equal(a, b) for a, b in zip(before, (cache.kv, cache.scale, cache.table, cache.lengths, cache.refs)))
+
+
+@pytest.mark.parametrize("new", [3, 30])
+def test_append_after_a_refused_extend(ufb, dev, new):
+    """A step that got no pages leaves what is stored alone, and its queries see nothing."""
+    cache = make_cache(ufb, dev, [47, 20], 2, 64, 16, spare=0, slots=3)
+    plan = cache.plan([0], [new])
+    x, q = randn(dev, (new, 2, 64), 1, torch.bfloat16), randn(dev, (new, 4, 64), 2, torch.bfloat16)
+    before = stored(cache)
+    cache.extend(plan)
+    assert ufb.device_status(0) == 31
+    cache.append(0, plan, x, -x)
+    assert ufb.device_status(0) == 31 and same(before, cache)
+    out, lse = cache.attend(0, plan, q, lse=True)
+    assert ufb.device_status(0) == 31 and not bool(out.any()) and bool((lse == -math.inf).all())
+    # another stream goes on as ever
+    check_attend(ufb, cache, [1], [1], 4, torch.bfloat16)
+    # a step that is granted takes it off, one of no tokens too
+    cache.extend(cache.plan([0], [0]))
+    check_attend(ufb, cache, [0], [new], 4, torch.bfloat16)
+    cache.extend(plan)
+    assert ufb.device_status(0) == 31
+    cache.release(cache.plan([1], [0]))
+    cache.extend(plan)
+    cache.append(0, plan, x, -x)
+    check_attend(ufb, cache, [0], [new], 4, torch.bfloat16)
+    assert cache.lengths.tolist() == [47 + new, 0, 0]
+    got, _ = contents(cache, 0, 0)
+    steps = float(cache.scale[0, cache.table[0, 47 // 16:-(-(47 + new) // 16)].long()].max())
+    assert float((got[0, :, 47:] - x.double().permute(1, 0, 2)).abs().max()) <= 0.501 * steps
+    _clean(ufb)
+
+
+def test_append_to_shared_pages_after_a_refused_extend(ufb, dev):
+    """Branches that share a full last page keep it, and each other's tokens, when neither is granted its step;
+    a branch made in between is left out as its source is."""
+    cache = make_cache(ufb, dev, [48], 2, 128, 16, layers=2, spare=0, slots=5)
+    cache.fork(cache.fork_plan([0, 0], [1, 2]))
+    assert cache.refs.max() == 3
+    step = cache.plan([1, 2, 4], [20, 7, 0])
+    x = randn(dev, (27, 2, 128), 1, torch.float16)
+    before = stored(cache)
+    cache.extend(step)
+    for layer in range(2):
+        cache.append(layer, step, x, -x)
+        out = cache.attend(layer, step, randn(dev, (27, 4, 128), 2, torch.float16), causal=False)
+        assert not bool(out.any())
+    assert ufb.device_status(0) == 31 and same(before, cache)
+    cache.fork(cache.fork_plan([1, 0], [3, 4]))
+    before = stored(cache)
+    late = cache.plan([3], [5])
+    cache.append(0, late, x[:5], x[:5])
+    assert ufb.device_status(0) == 31 and same(before, cache)
+    check_attend(ufb, cache, [0, 4], [3, 1], 4, torch.float16)   # these asked for nothing
+    cache.release(late)
+    assert cache.refs.max() == 4
+    # its own pages again: the step is granted
+    cache.release(cache.plan([0, 1, 2, 4], [0] * 4))
+    cache.extend(late)
+    cache.append(0, late, x[:5], x[:5])
+    check_attend(ufb, cache, [3], [5], 4, torch.float16)
+    _clean(ufb)
+
+
+def test_refused_steps_of_a_graph(ufb, dev):
+    """A captured step that runs out of pages stops changing what is stored."""
+    cache = make_cache(ufb, dev, [29, 30], 1, 64, 16, spare=2)
+    plan = cache.plan([0, 1], [9, 4])
+    x, q = randn(dev, (13, 1, 64), 1, torch.float16), randn(dev, (13, 4, 64), 2, torch.float16)
+    side = torch.cuda.Stream(dev)
+    torch.cuda.synchronize(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        cache.extend(plan)
+        cache.append(0, plan, x, x)
+        out = cache.attend(0, plan, q)
+    granted = 0
+    for step in range(4):
+        before = stored(cache)
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        status = ufb.device_status(0)
+        if status:
+            assert status == 31 and same(before, cache) and not bool(out.any())
+        else:
+            granted += 1
+            want, _, tol, _ = attend_ref(cache, 0, [0, 1], [9, 4], q, 0, 0, True, 64 ** -0.5)
+            assert bool(((out.double() - want).abs() <= tol + ULP[torch.float16] * want.abs() + F16_TINY).all())
+    assert granted == 2 and cache.lengths.tolist() == [47, 38]
