@@ -255,20 +255,6 @@ __device__ __forceinline__ void int8x4_to_half(uint32_t w, uint32_t& lo, uint32_
     hi = half2_minus_1152(__byte_perm(w, 0x64646464u, 0x4342));
 }
 
-// Four stored keys as float16 in three operations: an integer plus 128 in the low
-// byte is a float16 below the normal ones, (integer + 128) 2^-24, exactly.  The
-// scores take that back: the page's key scale times 2^24 as factor and -128 2^-24
-// times the row's sum of q beside it, in 32 bits.  (Values are not taken this way:
-// their products are sums over thousands of keys, in which 128 would stand above
-// what is left of values of both signs.)
-constexpr float kKeyUnit = 16777216.0f;              // 2^24
-constexpr float kKeyOffset = -128.0f / 16777216.0f;
-__device__ __forceinline__ void keyx4_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    w ^= 0x80808080u;
-    lo = __byte_perm(w, 0, 0x4140);
-    hi = __byte_perm(w, 0, 0x4342);
-}
-
 // Power of two that brings a row's largest |q| into [1/2, 1): its values then
 // are float16 numbers with their own bits (bfloat16 has fewer), whatever their
 // size; what falls below 2^-25 of the largest is lost.  NaN for a row that is

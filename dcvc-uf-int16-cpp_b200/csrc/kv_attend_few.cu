@@ -58,7 +58,7 @@ constexpr float kShift = 15.0f;
 constexpr int kCodeFull = 41, kCodeEmpty = 42, kCodeDrain = 43;
 
 struct PageScales {
-    float key, log2_value, inv_value;  // key times 2^24; log2_value -inf: the 16 keys are not there
+    float key, log2_value, inv_value;  // log2_value -inf: the 16 keys are not there
     float pad;
 };
 
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
             sc.log2_value = -INFINITY;
             if (now.page >= 0) {
                 const float v = now.value < kTinyScale ? kTinyScale : now.value;
-                sc.key = now.key * kKeyUnit;
+                sc.key = now.key;
                 sc.log2_value = log2f(v);
                 sc.inv_value = 1.0f / v;
             }
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
         // Q fragments: row 8 n + g, brought to [1/2, 1) and rounded to float16; then what
         // the scores of rows 8 n + 2 c and + 1 need
         uint32_t q[NT][kSteps][2];
-        float unit[NT][2], offset[NT][2];
+        float unit[NT][2];
         int pos[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -276,24 +276,18 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
             }
             const float u = row_unit(odd == odd ? top : odd);
             const float mul = u == u ? u : 0.0f;
-            float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < kSteps; ++t) {
                 const float2 x = unpack2(w[t].x, T()), y = unpack2(w[t].y, T());
                 q[n][t][0] = pack2(x.x * mul, x.y * mul, __half());
                 q[n][t][1] = pack2(y.x * mul, y.y * mul, __half());
-                const float2 x16 = unpack2(q[n][t][0], __half()), y16 = unpack2(q[n][t][1], __half());
-                sum += (x16.x + x16.y) + (y16.x + y16.y);
             }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             const float f = unit_inverse(u) * a.scale_log2;
             const int at = p.t.length - p.t.n_new + token;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int from = (2 * c + r) * 4;
                 unit[n][r] = __shfl_sync(0xffffffffu, f, from);
-                offset[n][r] = __shfl_sync(0xffffffffu, sum, from) * kKeyOffset;
                 pos[n][r] = __shfl_sync(0xffffffffu, at, from);
             }
         }
@@ -362,8 +356,8 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
 #pragma unroll
                     for (int x = 0; x < kM; ++x) {
                         uint32_t f[4];
-                        keyx4_to_half(w[x][0][k], f[0], f[2]);
-                        keyx4_to_half(w[x][1][k], f[1], f[3]);
+                        int8x4_to_half(w[x][0][k], f[0], f[2]);
+                        int8x4_to_half(w[x][1][k], f[1], f[3]);
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
                             mma16816(s[x][n], f, q[n][i * (kSteps / 2) + k][0], q[n][i * (kSteps / 2) + k][1]);
@@ -384,10 +378,9 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
 #pragma unroll
                     for (int x = 0; x < kM; ++x) {
                         const float f[2] = {unit[n][0] * sc[x].key, unit[n][1] * sc[x].key};
-                        const float add[2] = {fmaf(f[0], offset[n][0], sc[x].log2_value), fmaf(f[1], offset[n][1], sc[x].log2_value)};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            s[x][n][e] = fmaf(s[x][n][e], f[e & 1], add[e & 1]);
+                            s[x][n][e] = fmaf(s[x][n][e], f[e & 1], sc[x].log2_value);
                             if (kMasked) {
                                 const int key = key0 + x * 16 + (e >> 1) * 8 + key_of(g), at = pos[n][e & 1];
                                 const bool seen = key < p.t.length && (!a.causal || key <= at) &&

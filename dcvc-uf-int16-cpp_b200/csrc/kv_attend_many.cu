@@ -54,7 +54,7 @@ constexpr int kCode = 44;
 constexpr float kSlack = 2.0f, kShift = 13.0f;
 
 struct alignas(16) GroupScales {
-    float key, log2_value, inv_value, pad;   // key times 2^24; log2_value -inf: the 16 keys are not there
+    float key, log2_value, inv_value, pad;   // log2_value -inf: the 16 keys are not there
 };
 
 // A piece of an item as the walker announces it; rows 0: there is none any more.
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             const int token = in_stream / a.group, head = p.head * a.group + in_stream - token * a.group;
             const int pos = p.start + token;
             const long long out_row = p.token0 + static_cast<long long>(token);
-            float unit, offset;
+            float unit;
             {
                 // the row to [1/2, 1) and float16; the softmax scale's sign goes with it
                 const T* src = static_cast<const T*>(a.q.data) + out_row * a.q.token_stride +
@@ -208,7 +208,6 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 const float u = row_unit(odd == odd ? top : odd);
                 unit = unit_inverse(u) * fabsf(a.scale_log2);
                 const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
-                float sum = 0.0f;
 #pragma unroll 4
                 for (int i = 0; i < D / 8; ++i) {
                     const uint4 v = real ? vec[i] : make_uint4(0, 0, 0, 0);
@@ -218,12 +217,9 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                     for (int j = 0; j < 4; ++j) {
                         const float2 f = unpack2(x[j], T());
                         y[j] = pack2(f.x * mul, f.y * mul, __half());
-                        const float2 r = unpack2(y[j], __half());
-                        sum += r.x + r.y;
                     }
                     *reinterpret_cast<uint4*>(sm.q[t] + tile_at(row, i)) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
-                offset = sum * kKeyOffset;
                 fence_proxy_async_smem();
                 mbar_arrive(&sm.q_full[t]);
             }
@@ -256,17 +252,17 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                         const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            auto x = [&](int j) {
+                            auto f = [&](int j) {
                                 return decltype(masked)::value && !(bits & (1u << (g * 16 + j))) ? -INFINITY
                                                                                               : __uint_as_float(s[g * 16 + j]);
                             };
-                            float y = max3(x(0), x(1), x(2)), z = max3(x(3), x(4), x(5));
-                            y = max3(y, x(6), x(7)), z = max3(z, x(8), x(9));
-                            y = max3(y, x(10), x(11)), z = max3(z, x(12), x(13));
-                            y = max3(y, x(14), x(15));
+                            float y = max3(f(0), f(1), f(2)), z = max3(f(3), f(4), f(5));
+                            y = max3(y, f(6), f(7)), z = max3(z, f(8), f(9));
+                            y = max3(y, f(10), f(11)), z = max3(z, f(12), f(13));
+                            y = max3(y, f(14), f(15));
                             y = fmaxf(y, z);
                             const GroupScales gs = sc[c * 2 + g];
-                            const float f = unit * gs.key, v = fmaf(y, f, fmaf(f, offset, gs.log2_value));
+                            const float v = fmaf(y, unit * gs.key, gs.log2_value);
                             // -infinity: nothing of the group is seen
                             top = fmaxf(top, decltype(masked)::value && y == -INFINITY ? y : v);
                         }
@@ -309,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const GroupScales gs = sc[c * 2 + h];
-                            const float f = unit * gs.key, add = fmaf(f, offset, gs.log2_value - base);
+                            const float f = unit * gs.key, add = gs.log2_value - base;
                             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                             for (int j = 0; j < 16; j += 2) {
@@ -487,26 +483,19 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             const int b = n & 1;
             if (n >= 2) wait(&empty[b], (n >> 1) - 1);
             uint8_t* to = tiles + b * (kKeys * D * 2);
-            auto store = [&](auto keys) {
 #pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    const uint32_t x[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
-                    uint32_t y[8];
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t x[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
+                uint32_t y[8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (decltype(keys)::value) keyx4_to_half(x[j], y[2 * j], y[2 * j + 1]);
-                        else int8x4_to_half(x[j], y[2 * j], y[2 * j + 1]);
-                    }
-                    const int step = (i / 2) * 2 * kStep * 128;
-                    *reinterpret_cast<uint4*>(to + at0[i & 1] + step) = make_uint4(y[0], y[1], y[2], y[3]);
-                    *reinterpret_cast<uint4*>(to + at1[i & 1] + step) = make_uint4(y[4], y[5], y[6], y[7]);
-                }
-            };
-            if (side == 0) store(std::true_type());
-            else store(std::false_type());
+                for (int j = 0; j < 4; ++j) int8x4_to_half(x[j], y[2 * j], y[2 * j + 1]);
+                const int step = (i / 2) * 2 * kStep * 128;
+                *reinterpret_cast<uint4*>(to + at0[i & 1] + step) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(to + at1[i & 1] + step) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
             if (side == 0 && lane < 2) {
                 GroupScales g;
-                g.key = key_scale * kKeyUnit;
+                g.key = key_scale;
                 g.log2_value = value_scale == -1.0f ? -INFINITY : log2f(value_scale);
                 g.inv_value = value_scale == -1.0f ? 0.0f : 1.0f / value_scale;
                 g.pad = 0.0f;

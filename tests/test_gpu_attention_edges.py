@@ -109,3 +109,56 @@ def test_refused_steps_of_a_graph(ufb, dev):
             want, _, tol, _ = attend_ref(cache, 0, [0, 1], [9, 4], q, 0, 0, True, 64 ** -0.5)
             assert bool(((out.double() - want).abs() <= tol + ULP[torch.float16] * want.abs() + F16_TINY).all())
     assert granted == 2 and cache.lengths.tolist() == [47, 38]
+
+
+def check_sharp(cache, slots, counts, q, scale):
+    """Rows whose best key leads by more than the scores' error give that key's value."""
+    plan = cache.plan(slots, counts)
+    got, lse = cache.attend(0, plan, q, scale=scale, lse=True)
+    assert bool(torch.isfinite(got).all()) and bool(torch.isfinite(lse).all())
+    group, t, sharp = q.shape[1] // cache.heads, 0, 0
+    for slot, n in zip(slots, counts):
+        kv, _ = contents(cache, 0, slot)
+        length = kv.shape[2]
+        at = length - n + torch.arange(n, device=q.device)[:, None]
+        seen = torch.arange(length, device=q.device) <= at
+        for h in range(q.shape[1]):
+            k, v, x = kv[0, h // group], kv[1, h // group], q[t:t + n, h].double()
+            s = torch.where(seen, (x @ k.T) * scale, -math.inf)
+            err = 2.0 ** -16 * torch.where(seen, (x.abs() @ k.T.abs()) * scale, 0).amax(1)
+            best = s.topk(2, dim=1)
+            # the others together: length exp(2 err - lead), below 2^-30 from here on
+            lead = best.values[:, 0] - best.values[:, 1]
+            clear = lead > 2 * err + math.log(length) + 21
+            assert bool(((lse[t:t + n, h].double() - best.values[:, 0]).abs()[clear]
+                         <= (err + 2.0 ** -20 * best.values[:, 0].abs())[clear]).all())
+            want = v[best.indices[:, 0]]
+            tol = (ULP[q.dtype] + 2.0 ** -11) * want.abs() + 2.0 ** -30 * v.abs().max()
+            assert bool(((got[t:t + n, h].double() - want).abs() <= tol)[clear].all())
+            sharp += int(clear.sum())
+        t += n
+    assert sharp * 2 > q.shape[0] * q.shape[1]  # the leads of so few keys are far above the error
+
+
+@pytest.mark.parametrize("mul", [1e5, 1e25, 1e33, 1e36, 2e37])
+@pytest.mark.parametrize("heads,dim,page", [(2, 64, 16), (1, 128, 64)])
+def test_queries_of_any_size(ufb, dev, heads, dim, page, mul):
+    """bfloat16 queries up to the end of their type, scores inside float32's range: few rows."""
+    cache = make_cache(ufb, dev, [70, 41], heads, dim, page)
+    check_sharp(cache, [0, 1], [3, 1], randn(dev, (4, 3 * heads, dim), 11, torch.bfloat16, mul), dim ** -0.5)
+    _clean(ufb)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_scores_beside_an_outlier(ufb, dev, new):
+    """Integers of size 1 and 2 beside the one that sets the page's scale keep their scores."""
+    cache = make_cache(ufb, dev, [500], 2, 128, 64)
+    cache.kv[:, :, 0] = torch.sign(cache.kv[:, :, 0]) * (1 + cache.kv[:, :, 0] % 2)
+    cache.scale[:, :, 0] = 10.0 / 127
+    q = randn(dev, (new, 6, 128), 4, torch.bfloat16).abs() * 30   # of one sign: sum q is as large as sum |q|
+    plan = cache.plan([0], [new])
+    got, lse = cache.attend(0, plan, q, lse=True)
+    want, wl, tol, tl = attend_ref(cache, 0, [0], [new], q, 0, 0, True, 128 ** -0.5)
+    assert bool(((lse.double() - wl).abs() <= tl).all()), float(((lse.double() - wl).abs() / tl).max())
+    assert bool(((got.double() - want).abs() <= tol + ULP[torch.bfloat16] * want.abs()).all())
+    _clean(ufb)
