@@ -52,6 +52,12 @@ constexpr int kCode = 44;
 // times 2^kShift: it reaches 2^15 at most, inside float16, and weights down to
 // 2^-27 of the largest keep all 11 bits.
 constexpr float kSlack = 2.0f, kShift = 13.0f;
+// Scores less their row's maximum in one multiply-add keep what the maximum lost in
+// rounding: up to 2^-4 from this maximum on, and past float16's range from 2^26 on.
+// Warps with such a row, and those with masked keys, round the score first, as the
+// maximum was.  (Sums with the maximum are
+// rounded so that P stays at or below 2^15 whatever the spacing of the scores is.)
+constexpr float kFar = 1048576.0f;   // 2^20
 
 struct alignas(16) GroupScales {
     float key, log2_value, inv_value, pad;   // log2_value -inf: the 16 keys are not there
@@ -224,6 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 mbar_arrive(&sm.q_full[t]);
             }
             float m = -INFINITY, l = 0.0f;
+            bool far = false;   // a row of the warp has scores beyond kFar
             const int first_pos = p.start + (p.row0 + t * kHalf) / a.group;
             const int last_pos = p.start + (p.row0 + min(p.rows, (t + 1) * kHalf) - 1) / a.group;
             const int length = p.length, end = p.end;
@@ -281,22 +288,25 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 if (clear) maximum(std::false_type());
                 else maximum(std::true_type());
                 // the maximum stays while it is within 2^kSlack
-                const bool grow = top > m + kSlack && m != -INFINITY;
+                const bool grow = top > __fadd_rd(m, kSlack);
                 if (__any_sync(0xffffffffu, grow)) {
-                    const float keep = grow ? ex2(m - top) : 1.0f;
+                    if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
+                        const float keep = grow && m != -INFINITY ? ex2(m - top) : 1.0f;
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t o[16];
-                        tmem_ld16(to + c * 16, o);
-                        tmem_wait_ld_regs(o);
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(to + c * 16, o);
+                            tmem_wait_ld_regs(o);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                        tmem_st16(to + c * 16, o);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                            tmem_st16(to + c * 16, o);
+                        }
+                        l *= keep;
                     }
-                    l *= keep;
+                    if (grow) m = top;
+                    far = __any_sync(0xffffffffu, fabsf(m) >= kFar && m != -INFINITY);
                 }
-                if (grow || m == -INFINITY) m = top;
-                const float base = m == -INFINITY ? 0.0f : m - kShift;
+                const float base = m == -INFINITY ? 0.0f : __fsub_ru(m, kShift);
                 auto weights = [&](auto masked) {
                     // 32 columns: P, the row's weight
                     auto chunk = [&](int c, uint32_t (&s)[32]) {
@@ -305,13 +315,14 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const GroupScales gs = sc[c * 2 + h];
-                            const float f = unit * gs.key, add = gs.log2_value - base;
+                            const float f = unit * gs.key, add = decltype(masked)::value ? gs.log2_value : gs.log2_value - base;
                             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                             for (int j = 0; j < 16; j += 2) {
                                 float x = __uint_as_float(s[h * 16 + j]), y = __uint_as_float(s[h * 16 + j + 1]);
                                 fma2(x, y, f, add);
                                 if (decltype(masked)::value) {
+                                    add2(x, y, -base, -base);
                                     if (!(bits & (1u << (h * 16 + j)))) x = -INFINITY;
                                     if (!(bits & (1u << (h * 16 + j + 1)))) y = -INFINITY;
                                 }
@@ -341,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                         mbar_arrive(&sm.p_full[t][half]);
                     }
                 };
-                if (clear) weights(std::false_type());
+                if (clear && !far) weights(std::false_type());
                 else weights(std::true_type());
             }
             wait(&sm.o_full[t], o_n++);

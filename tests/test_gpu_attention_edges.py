@@ -162,3 +162,12 @@ def test_scores_beside_an_outlier(ufb, dev, new):
     assert bool(((lse.double() - wl).abs() <= tl).all()), float(((lse.double() - wl).abs() / tl).max())
     assert bool(((got.double() - want).abs() <= tol + ULP[torch.bfloat16] * want.abs()).all())
     _clean(ufb)
+
+
+@pytest.mark.parametrize("mul", [1e5, 1e6, 3e6, 1e7, 3e7, 1e8, 3e8, 1e9, 1e15, 1e25, 1e33, 2e37])
+@pytest.mark.parametrize("heads,dim,page", [(2, 64, 16), (1, 128, 64)])
+def test_scores_of_any_size_of_many_rows(ufb, dev, heads, dim, page, mul):
+    """Scores whose spacing in 32 bits passes 1, in tiles of many rows: masked and not."""
+    cache = make_cache(ufb, dev, [70, 600], heads, dim, page)
+    check_sharp(cache, [0, 1], [50, 33], randn(dev, (83, 3 * heads, dim), 12, torch.bfloat16, mul), dim ** -0.5)
+    _clean(ufb)
