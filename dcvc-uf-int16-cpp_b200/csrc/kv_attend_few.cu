@@ -53,7 +53,8 @@ constexpr int kMinShare = 7;          // tiles of a CTA's share at least: as man
 __host__ __device__ constexpr int consumers(int nt) { return nt == 1 ? 14 : 6; }
 __host__ __device__ constexpr int stages(int nt) { return nt == 1 ? 7 : 9; }
 // P is taken times 2^kShift: at most 2^15, inside float16, and weights down to
-// 2^-29 of the largest keep all 11 bits.
+// 2^-29 of the largest keep all 11 bits.  (The maximum less kShift is rounded up, or
+// scores spaced by more than 1, from 2^24 on, would give weights of 2^16.)
 constexpr float kShift = 15.0f;
 constexpr int kCodeFull = 41, kCodeEmpty = 42, kCodeDrain = 43;
 
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
                         const float next = fmaxf(m[n][r], x);
                         grew |= next > m[n][r];
                         keep[n][r] = next == -INFINITY ? 1.0f : ex2(m[n][r] - next);
-                        base[n][r] = next == -INFINITY ? 0.0f : next - kShift;
+                        base[n][r] = next == -INFINITY ? 0.0f : __fsub_ru(next, kShift);
                         m[n][r] = next;
                     }
                 if (__any_sync(0xffffffffu, grew)) {

@@ -171,3 +171,12 @@ def test_scores_of_any_size_of_many_rows(ufb, dev, heads, dim, page, mul):
     cache = make_cache(ufb, dev, [70, 600], heads, dim, page)
     check_sharp(cache, [0, 1], [50, 33], randn(dev, (83, 3 * heads, dim), 12, torch.bfloat16, mul), dim ** -0.5)
     _clean(ufb)
+
+
+@pytest.mark.parametrize("mul", [1e6, 3e6, 1e7, 3e7, 1e8, 3e8])
+@pytest.mark.parametrize("heads,dim,page", [(2, 64, 16), (1, 128, 64)])
+def test_scores_of_any_size_of_few_rows(ufb, dev, heads, dim, page, mul):
+    """The same where the spacing of the scores is about that of the weights' range."""
+    cache = make_cache(ufb, dev, [70, 600], heads, dim, page)
+    check_sharp(cache, [0, 1], [5, 5], randn(dev, (10, 3 * heads, dim), 13, torch.bfloat16, mul), dim ** -0.5)
+    _clean(ufb)
