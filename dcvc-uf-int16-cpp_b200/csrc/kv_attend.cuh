@@ -26,8 +26,9 @@ constexpr int kAttendManyRows = 256;    // rows of the widest tile
 constexpr int kGroupKeys = 16;          // keys that share a page, and so a scale, at every page size
 
 // Value scales below this act as this: such a page's values vanish beside any
-// other, but its keys still carry weight.
-constexpr float kTinyScale = 7.888609052210118e-31f;  // 2^-100
+// other, but its keys still carry weight.  A row's weight, the sum of P / scale with
+// P up to 2^15 over up to 2^30 keys, stays inside 32 bits.
+constexpr float kTinyScale = 8.271806125530277e-25f;  // 2^-80
 
 // Keys [0, sink) and [low, hi) hold every key that a tile of rows sees; in tiles
 // of BK keys: [0, sink_tiles) and from low_tile on, nt in all.

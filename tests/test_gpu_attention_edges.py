@@ -180,3 +180,12 @@ def test_scores_of_any_size_of_few_rows(ufb, dev, heads, dim, page, mul):
     cache = make_cache(ufb, dev, [70, 600], heads, dim, page)
     check_sharp(cache, [0, 1], [5, 5], randn(dev, (10, 3 * heads, dim), 13, torch.bfloat16, mul), dim ** -0.5)
     _clean(ufb)
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_lse_of_a_long_stream_of_zero_values(ufb, dev, new):
+    """The weights of many thousand keys whose values are all zero add up."""
+    cache = make_cache(ufb, dev, [40000 if new == 1 else 300000], 1, 64, 64)
+    cache.kv[:, :, 1] = 0
+    cache.scale[:, :, 1] = 0.0
+    check_attend(ufb, cache, [0], [new], 4, torch.bfloat16, mul=0.1)
