@@ -256,16 +256,17 @@ __device__ __forceinline__ void int8x4_to_half(uint32_t w, uint32_t& lo, uint32_
     hi = half2_minus_1152(__byte_perm(w, 0x64646464u, 0x4342));
 }
 
-// Power of two that brings a row's largest |q| into [1/2, 1): its values then
-// are float16 numbers with their own bits (bfloat16 has fewer), whatever their
-// size; what falls below 2^-25 of the largest is lost.  NaN for a row that is
-// not finite.
+// Power of two that brings a row's largest |q| into [2^15, 2^16), float16's last
+// binade: values of float16 rows stay what they are, down to the smallest beside the
+// largest, and bfloat16 values keep their bits down to 2^-32 of the largest.
+// Products with the integers, 128 of them, stay below 2^30.  NaN for a row that is not
+// finite.
 __device__ __forceinline__ float row_unit(float top) {
     if (!(top < __int_as_float(0x7f800000))) return __int_as_float(0x7fffffff);
     if (top < 1.1754943508222875e-38f) return 8.507059173023462e37f;  // 2^126
     const int e = (__float_as_int(top) >> 23) - 126;                    // top in [2^(e-1), 2^e)
-    // 2^-e, kept inside the normal range
-    return __int_as_float((127 - min(max(e, -126), 126)) << 23);
+    // 2^(16 - e), kept where its inverse is a normal number too
+    return __int_as_float((127 + min(16 - e, 126)) << 23);
 }
 
 // 1 / u of a power of two u (NaN stays NaN).

@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
     int it = 0, parity = 0;
     Piece p;
     while (walk.next(a, p)) {
-        // Q fragments: row 8 n + g, brought to [1/2, 1) and rounded to float16; then what
+        // Q fragments: row 8 n + g, brought to [2^15, 2^16) and rounded to float16; then what
         // the scores of rows 8 n + 2 c and + 1 need
         uint32_t q[NT][kSteps][2];
         float unit[NT][2];

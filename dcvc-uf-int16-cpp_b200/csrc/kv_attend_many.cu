@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             const long long out_row = p.token0 + static_cast<long long>(token);
             float unit;
             {
-                // the row to [1/2, 1) and float16; the softmax scale's sign goes with it
+                // the row to [2^15, 2^16) and float16; the softmax scale's sign goes with it
                 const T* src = static_cast<const T*>(a.q.data) + out_row * a.q.token_stride +
                                head * a.q.head_stride;
                 const uint4* vec = reinterpret_cast<const uint4*>(src);

@@ -559,7 +559,8 @@ int ufb_kv_read(const ufb_kv_cache* c, int layer, const int32_t* pages, int64_t 
  * ln sum_j exp(scale * q . k_j).  max_new is no less than any stream's count.
  * Statistics and sums in 32 bits.  q and p enter the tensor cores as float16: q
  * after a power of two for each query and head, so that no value of its type is
- * out of range while the scores (times log2 e) are inside float's; p with 11
+ * out of range while the scores (times log2 e) are inside float's (float16 queries
+ * exactly, bfloat16 ones down to 2^-32 of the largest of their row); p with 11
  * significant bits down to 2^-27 of the largest p times value scale of its row,
  * and in steps of 2^-37 of it below.  Scales are not negative; value scales below
  * 2^-80 (0 among them) count as 2^-80.

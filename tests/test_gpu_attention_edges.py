@@ -189,3 +189,18 @@ def test_lse_of_a_long_stream_of_zero_values(ufb, dev, new):
     cache.kv[:, :, 1] = 0
     cache.scale[:, :, 1] = 0.0
     check_attend(ufb, cache, [0], [new], 4, torch.bfloat16, mul=0.1)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_queries_with_one_large_value(ufb, dev, new):
+    """Where the keys are zero the query is as large as float16 goes: its other values keep theirs."""
+    cache = make_cache(ufb, dev, [300], 2, 64, 32)
+    cache.kv[:, :, 0, :, :, 5] = 0
+    q = randn(dev, (new, 6, 64), 4, torch.float16, 1e-3)
+    q[..., 5] = 60000.0
+    plan = cache.plan([0], [new])
+    got, lse = cache.attend(0, plan, q, scale=100.0, lse=True)
+    want, wl, tol, tl = attend_ref(cache, 0, [0], [new], q, 0, 0, True, 100.0)
+    assert bool(((lse.double() - wl).abs() <= tl).all()), float(((lse.double() - wl).abs() / tl).max())
+    assert bool(((got.double() - want).abs() <= tol + ULP[torch.float16] * want.abs() + F16_TINY).all())
+    _clean(ufb)
