@@ -19,6 +19,7 @@ from . import UfbError, _check, library
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _QUERY_DTYPES = {torch.float16: 1, torch.bfloat16: 2}
 _LAYOUTS = {"half": 0, "interleaved": 1}
+_ATTEND_ZERO = 1024  # UFB_KV_ATTEND_ZERO
 
 
 # ufb_heads (data, token stride, head stride, heads), one or two of them
@@ -50,6 +51,8 @@ def _lib():
     L.ufb_kv_append.argtypes = [cache, ci, vp, vp, ci, ci, i64, ci, heads, heads, vp]
     L.ufb_kv_read.argtypes = [cache, ci, vp, i64, ci, vp, vp]
     L.ufb_kv_attend_workspace.restype = i64
+    L.ufb_capture_id.restype = i64
+    L.ufb_capture_id.argtypes = [vp]
     L.ufb_kv_attend.argtypes = [cache, ci, vp, vp, ci, ci, i64, ci, heads, heads, vp, ci, ci, ci, C.c_float, vp, i64, vp]
     L._attention_ready = True
     return L
@@ -66,12 +69,14 @@ def _device(device) -> torch.device:
 # microseconds, so the wrappers below keep to few and cheap host operations.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
 def _launch(device, fn, *args):
     """fn(*args, current stream of the device), with that device current."""
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
@@ -271,7 +276,7 @@ class KVCache:
         self._ref = C.addressof(self._struct)
         self._default_scale = self.head_dim ** -0.5
         self._append, self._attend = L.ufb_kv_append, L.ufb_kv_attend
-        self._workspaces = {}
+        self._workspaces, self._captures = {}, {}
         self._spare = self._new_workspace()
 
     # -- streams and their pages
@@ -355,21 +360,39 @@ class KVCache:
 
     def _workspace(self):
         # zeroed once and left zeroed by every call; streams may overlap, so each has its own
-        key = _raw_stream(self.device.index)
+        index = self.device.index
+        key = _raw_stream(index)
+        if _current_device() == index:
+            capturing = _capturing()
+        else:
+            with torch.cuda.device(index):
+                capturing = _capturing()
         w = self._workspaces.get(key)
         if w is None:
-            with torch.cuda.device(self.device):
-                capturing = torch.cuda.is_current_stream_capturing()
             if not capturing:
                 w = self._new_workspace()
             elif self._spare is None:
                 raise UfbError(-1, "this stream has no attention scratch yet: call attend on it once before capturing")
             else:
                 # zeros made here would be zeroed by this graph's replays only, and
-                # another graph of the stream, or the stream itself, may run first
+                # the stream's own calls may come first
                 w, self._spare = self._spare, None
             self._workspaces[key] = w
-        return w
+        return self._captured(key) if capturing else w
+
+    def _captured(self, key):
+        # a graph may be replayed beside its stream's calls and other graphs of it, so
+        # each capture has its own, from the graph's memory and zeroed by its replays;
+        # kept here until the stream's next capture, so that nothing else of the graph gets it
+        capture = self._L.ufb_capture_id(key)
+        if capture < 0:
+            _check(capture)
+        held = self._captures.get(key)
+        if held is None or held[0] != capture:
+            t = torch.empty(self._workspaces[key][1], dtype=torch.uint8, device=self.device)
+            t[:_ATTEND_ZERO].zero_()
+            held = self._captures[key] = (capture, (t.data_ptr(), t.numel(), t))
+        return held[1]
 
     def attend(self, layer, plan, q, window=0, sinks=0, causal=True, scale=None, lse=False):
         """Attention of the plan's newest tokens (q [tokens, query heads, head_dim],
@@ -377,9 +400,10 @@ class KVCache:
         j when j <= a (all keys when not causal) and, with a window, j > a -
         window or j < sinks.  scale defaults to head_dim ** -0.5.  A query that
         sees nothing gives zeros.  Returns out, or (out, lse [tokens, query
-        heads] float32).  Every CUDA stream has its own scratch; a call captured
-        in a graph keeps that of the stream it was captured on.  One stream may
-        capture without an earlier call on it; others call attend once before."""
+        heads] float32).  Every CUDA stream has its own scratch, and so has every
+        capture, in its graph's memory: graphs may be replayed beside each other
+        and beside other calls.  One stream may capture without an earlier call
+        on it; others call attend once before."""
         self._own(plan)
         _check_ints(layer, window, sinks)
         device = self.device

@@ -261,6 +261,15 @@ int64_t ufb_kv_attend_workspace(void) {
     return sms > 0 ? kv_attend_workspace_bytes(sms) : last_code();
 }
 
+int64_t ufb_capture_id(void* stream) {
+    clear_error();
+    cudaStreamCaptureStatus state;
+    unsigned long long id = 0;
+    if (!cuda_ok(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &state, &id), "capture info"))
+        return last_code();
+    return state == cudaStreamCaptureStatusActive ? static_cast<int64_t>(id) : 0;
+}
+
 int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
                   int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse, int window,
                   int sinks, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {

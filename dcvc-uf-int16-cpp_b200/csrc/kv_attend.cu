@@ -6,6 +6,7 @@
 namespace ufb {
 
 int64_t kv_attend_workspace_bytes(int sms) {
+    static_assert(kAttendMaxCtas * sizeof(int32_t) <= UFB_KV_ATTEND_ZERO, "the counters begin the scratch");
     const int ctas = sms < kAttendMaxCtas ? sms : kAttendMaxCtas;
     const AttendScratch s = scratch_of(nullptr, ctas, kAttendManyRows);
     return reinterpret_cast<int64_t>(s.sums) + 2ll * ctas * kAttendManyRows * 128 * 4;

@@ -564,14 +564,20 @@ int ufb_kv_read(const ufb_kv_cache* c, int layer, const int32_t* pages, int64_t 
  * significant bits down to 2^-27 of the largest p times value scale of its row,
  * and in steps of 2^-37 of it below.  Scales are not negative; value scales below
  * 2^-80 (0 among them) count as 2^-80.
- * workspace: ufb_kv_attend_workspace() bytes, zero before its first use (and
- * again after a status of 41..44); calls that may overlap need one each. */
+ * workspace: ufb_kv_attend_workspace() bytes, the first UFB_KV_ATTEND_ZERO of them
+ * zero before its first use (and again after a status of 41..44); calls that may
+ * overlap need one each, replays of graphs that hold them included. */
+#define UFB_KV_ATTEND_ZERO 1024
 int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
                   int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse, int window,
                   int sinks, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Workspace of ufb_kv_attend on the current device, in bytes. */
 int64_t ufb_kv_attend_workspace(void);
+
+/* The graph capture that `stream` is in: a number that no other capture has; 0
+ * outside of one. */
+int64_t ufb_capture_id(void* stream);
 
 /* Measurement utility (no reference counterpart): launches `ctas` CTAs that
  * each issue `iters` x 4 dense tcgen05 kind::i8 M=128 N=256 K=32 MMAs from

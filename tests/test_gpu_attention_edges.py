@@ -204,3 +204,39 @@ def test_queries_with_one_large_value(ufb, dev, new):
     assert bool(((lse.double() - wl).abs() <= tl).all()), float(((lse.double() - wl).abs() / tl).max())
     assert bool(((got.double() - want).abs() <= tol + ULP[torch.float16] * want.abs() + F16_TINY).all())
     _clean(ufb)
+
+
+def test_graphs_of_one_stream(ufb, dev):
+    """Graphs captured on one stream, and its own calls, share no scratch: they may run side by side."""
+    cache = make_cache(ufb, dev, [5000, 4000, 3000], 2, 128, 64)
+    plans = [cache.plan([0], [3]), cache.plan([1], [2]), cache.plan([2], [40])]
+    qs = [randn(dev, (p.tokens, 8, 128), i, torch.float16) for i, p in enumerate(plans)]
+    want = [cache.attend(0, p, q) for p, q in zip(plans, qs)]
+    side, others = torch.cuda.Stream(dev), [torch.cuda.Stream(dev) for _ in range(3)]
+    torch.cuda.synchronize(dev)
+    graphs, outs, places = [], [], set()
+    for p, q in zip(plans, qs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append([cache.attend(0, p, q) for _ in range(3)])
+        graphs.append(graph)
+        (held,) = cache._captures.values()
+        places.add(held[1][0])
+    with torch.cuda.stream(side):
+        assert torch.equal(cache.attend(0, plans[0], qs[0]), want[0])
+    places |= {w[0] for w in cache._workspaces.values()}
+    assert len(places) == 5   # three graphs, the default stream, the side stream
+    for _ in range(10):
+        torch.cuda.synchronize(dev)
+        for o in sum(outs, []):
+            o.fill_(float("nan"))
+        torch.cuda.synchronize(dev)
+        for s, graph in zip(others, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(side):
+            eager = [cache.attend(0, p, q) for p, q in zip(plans, qs)]
+        torch.cuda.synchronize(dev)
+        for w, e, o in zip(want, eager, outs):
+            assert torch.equal(e, w) and all(torch.equal(x, w) for x in o)
+    _clean(ufb)
