@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
         for (; step < steps; step += kWarps) {
             const int index = it + step / (kKeys / kWarpKeys), stage = index % kStages;
             const int part = (step % (kKeys / kWarpKeys)) * kWarpKeys;
-            // after a wait gave up the warps go on without waiting: they meet at barriers
+            // after a wait gave up the warps go on without waiting: they meet at barriers, and
+            // every join still counts all its CTAs, so the counters end at zero
             if (!mbar_try_wait(&sm.full[stage], (index / kStages) & 1) && !*dead &&
                 !mbar_wait(&sm.full[stage], (index / kStages) & 1, a.status, kCodeFull))
                 *dead = 1;

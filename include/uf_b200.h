@@ -565,8 +565,9 @@ int ufb_kv_read(const ufb_kv_cache* c, int layer, const int32_t* pages, int64_t 
  * and in steps of 2^-37 of it below.  Scales are not negative; value scales below
  * 2^-80 (0 among them) count as 2^-80.
  * workspace: ufb_kv_attend_workspace() bytes, the first UFB_KV_ATTEND_ZERO of them
- * zero before its first use (and again after a status of 41..44); calls that may
- * overlap need one each, replays of graphs that hold them included. */
+ * zero before its first use; every call leaves them zero, one whose wait gave up
+ * (41..44) too.  Calls that may overlap need one each, replays of graphs that hold
+ * them included. */
 #define UFB_KV_ATTEND_ZERO 1024
 int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
                   int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse, int window,
