@@ -19,6 +19,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace ufb {
 
 constexpr int kAttendMaxCtas = 160;     // CTAs of a launch at most (scratch is sized by the SMs)
@@ -289,6 +291,21 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
 }
 __device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Lets `kernel` have `bytes` of dynamic shared memory.  That is per function and
+// device: `done` holds a bit for each device where it has been set, so that a call
+// costs no more than asking for the device.
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // The layer's integers as (128 bytes, rows of a head, heads, key and value, pages),

@@ -34,7 +34,6 @@
 #include "kv_attend.cuh"
 #include "umma.cuh"
 
-#include <mutex>
 #include <type_traits>
 
 namespace ufb {
@@ -596,9 +595,8 @@ template <typename T, int D, int NT>
 cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     auto kernel = few_kernel<T, D, NT>;
     const int smem = sizeof(Smem<D, NT>) + 1024;
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
-    std::call_once(once, [&] { attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    static std::atomic<uint64_t> allowed;
+    const cudaError_t attr = allow_smem(kernel, smem, allowed);
     if (attr != cudaSuccess) return attr;
     CUtensorMap map;
     // boxes of the keys that lie together in a page, 64 at most

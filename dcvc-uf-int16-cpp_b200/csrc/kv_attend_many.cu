@@ -31,7 +31,6 @@
 #include "kv_attend.cuh"
 #include "umma.cuh"
 
-#include <mutex>
 #include <type_traits>
 
 namespace ufb {
@@ -694,9 +693,8 @@ template <typename T, int D>
 cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     auto kernel = many_kernel<T, D>;
     const int smem = sizeof(Smem<D>);
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
-    std::call_once(once, [&] { attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    static std::atomic<uint64_t> allowed;
+    const cudaError_t attr = allow_smem(kernel, smem, allowed);
     if (attr != cudaSuccess) return attr;
     const long long row_tiles = (static_cast<long long>(a.max_new) * a.group + kRows - 1) / kRows;
     if (row_tiles * a.n > 0x3fffffff) return cudaErrorInvalidValue;

@@ -240,3 +240,18 @@ def test_graphs_of_one_stream(ufb, dev):
         for w, e, o in zip(want, eager, outs):
             assert torch.equal(e, w) and all(torch.equal(x, w) for x in o)
     _clean(ufb)
+
+
+def test_caches_on_two_devices(ufb, dev):
+    """One process, two GPUs, one of them not the current device: both kernels run on either."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    for device in (dev, torch.device("cuda:1"), dev):
+        cache = make_cache(ufb, device, [300, 70], 2, 64, 16, spare=12)
+        for new in (3, 50):
+            check_attend(ufb, cache, [0, 1], [new, new], 4, torch.float16)
+            plan = cache.plan([0, 1], [new, 1])
+            x = randn(device, (new + 1, 2, 64), 1, torch.float16)
+            cache.extend(plan)
+            cache.append(0, plan, x, x)
+        assert ufb.device_status(device.index) == 0
