@@ -49,6 +49,39 @@ bool overlap(const ufb_heads& a, const ufb_heads& b, int64_t tokens, int head_di
     return x < y + span_bytes(b, tokens, head_dim, dtype) && y < x + span_bytes(a, tokens, head_dim, dtype);
 }
 
+// Rows of two heads `apart` elements from one another: whether token t of one and any
+// token t + dt of the other share elements (dt 0 left out for a head and itself).
+bool rows_meet(int64_t apart, int64_t token_stride, int64_t tokens, int head_dim, bool same) {
+    const int64_t most = tokens - 1, at = token_stride > 0 ? -apart / token_stride : 0;
+    const int64_t near = at < -most ? -most : at > most ? most : at;
+    for (int64_t dt = near - 1; dt <= near + 1; ++dt) {
+        const int64_t x = apart + dt * token_stride;
+        if (dt >= -most && dt <= most && !(same && dt == 0) && x < head_dim && x > -head_dim) return true;
+    }
+    return false;
+}
+
+// A tensor that is written: its rows share no memory.
+bool check_output(const ufb_heads* t, int heads, int64_t tokens, int head_dim, int dtype, const char* what) {
+    if (!check_heads(t, heads, head_dim, dtype, what)) return false;
+    if (t->token_stride >= (t->heads - 1) * t->head_stride + head_dim) return true;
+    for (int h = 0; h < t->heads; ++h)
+        if (rows_meet(h * t->head_stride, t->token_stride, tokens, head_dim, h == 0))
+            return fail(UFB_EINVAL, std::string(what) + " has heads that overlap");
+    return true;
+}
+
+// Two tensors that are written: parts of one buffer with one token stride, or apart.
+bool check_outputs(const ufb_heads& a, const ufb_heads& b, int64_t tokens, int head_dim, int dtype, const char* what) {
+    if (!overlap(a, b, tokens, head_dim, dtype)) return true;
+    const int64_t apart = (static_cast<const char*>(b.data) - static_cast<const char*>(a.data)) / element_size(dtype);
+    bool meet = tokens > 1 && a.token_stride != b.token_stride;
+    for (int h = 0; h < a.heads && !meet; ++h)
+        for (int g = 0; g < b.heads && !meet; ++g)
+            meet = rows_meet(apart + g * b.head_stride - h * a.head_stride, a.token_stride, tokens, head_dim, false);
+    return !meet || fail(UFB_EINVAL, std::string(what) + " overlap");
+}
+
 // SMs of the current device; 0 with the error recorded.
 int attend_sms() {
     static std::atomic<int> known[64];
@@ -153,7 +186,7 @@ int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t
     if (!table || !positions) return err(UFB_EINVAL, "rotary table and positions must be non-null");
     for (int i = 0; i < count; ++i) {
         if (!check_heads(x + i, 0, head_dim, dtype, "rotary input") ||
-            !check_heads(out + i, x[i].heads, head_dim, dtype, "rotary output"))
+            !check_output(out + i, x[i].heads, tokens, head_dim, dtype, "rotary output"))
             return last_code();
         a.x[i] = x[i];
         a.out[i] = out[i];
@@ -162,6 +195,7 @@ int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t
         for (int j = 0; j < count; ++j)
             if (overlap(out[i], x[j], tokens, head_dim, dtype))
                 return err(UFB_EINVAL, "rotary output must not overlap its input");
+    if (count == 2 && !check_outputs(out[0], out[1], tokens, head_dim, dtype, "rotary outputs")) return last_code();
     a.table = reinterpret_cast<const float2*>(table);
     a.positions = positions;
     a.tokens = tokens;
@@ -280,7 +314,7 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
     if (!std::isfinite(scale)) return err(UFB_EINVAL, "softmax scale must be finite");
     if (n == 0 || max_new == 0) return UFB_OK;
     if (!check_heads(q, 0, c->head_dim, dtype, "queries") ||
-        !check_heads(out, q->heads, c->head_dim, dtype, "attention output"))
+        !check_output(out, q->heads, tokens, c->head_dim, dtype, "attention output"))
         return last_code();
     if (q->heads % c->heads) return err(UFB_EINVAL, "query heads must be a multiple of the cache's heads");
     if (q->heads / c->heads > 128) return err(UFB_ERANGE, "more than 128 query heads to a key head");

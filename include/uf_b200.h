@@ -453,7 +453,8 @@ int ufb_conv2d_noalloc(const int16_t* x, int n, int ci, int h, int w, const int1
 #define UFB_BF16 2
 
 /* A tensor [tokens, heads, head_dim] whose head_dim elements are contiguous;
- * strides in elements.  Data and strides are multiples of 16 bytes. */
+ * strides in elements.  Data and strides are multiples of 16 bytes; heads that are
+ * written share no memory. */
 typedef struct ufb_heads {
     void* data;
     int64_t token_stride, head_stride;
@@ -476,7 +477,8 @@ int64_t ufb_rotary_table(int axes, const int32_t* pairs, const int32_t* extents,
  * ([tokens, axes] int32), axis after axis; elements past them are copied.
  * inverse turns back, which is the gradient with respect to x.  Products and
  * sums in 32 bits.  dtype UFB_F32, UFB_F16 or UFB_BF16; head_dim a multiple of
- * 16 up to 256.  out must not overlap x. */
+ * 16 up to 256.  out must not overlap x; two results may be parts of one buffer
+ * when they have one token stride. */
 int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t* extents, int layout, int inverse,
                const int32_t* positions, int64_t tokens, int head_dim, int dtype, int count, const ufb_heads* x,
                const ufb_heads* out, void* stream);

@@ -164,3 +164,29 @@ def test_python_view_needs_cuda(ufb):
             ufb.Rotary(pairs, extents, device="cuda:0")
     with pytest.raises(ufb.UfbError):
         ufb.Rotary((4,), (8,), layout="spiral", device="cuda:0")
+
+
+def test_outputs_that_overlap_themselves(att):
+    """Heads of one result, or of the two of a rotary, that share memory are refused; inputs may repeat."""
+    L = att._lib()
+    pairs, extents = (C.c_int32 * 1)(16), (C.c_int32 * 1)(8)
+
+    def rotary(x, out, tokens=3):
+        n = len(x)
+        return L.ufb_rotary(4096, 1, pairs, extents, 0, 0, 4096, tokens, 64, 1, n, (Heads * n)(*x), (Heads * n)(*out), None)
+
+    def at(place, token, head, heads):
+        return Heads((1 << 24) + place * 2, token, head, heads)
+
+    x, far = at(0, 0, 64, 4), 1 << 20
+    for token, head in ((0, 64), (8, 64), (56, 4096), (192, 64), (64, 64), (128, 96), (104, 160), (200, 64)):
+        assert rotary([x], [at(far, token, head, 4)]) == EINVAL, (token, head)
+        assert b"overlap" in L.ufb_last_error()
+    # the second result begins in the first
+    assert rotary([x, at(0, 0, 64, 2)], [at(far, 256, 64, 4), at(far + 192, 256, 64, 2)]) == EINVAL
+    assert b"overlap" in L.ufb_last_error()
+    c, q = C.byref(_cache(att)), _heads(att, token=512, heads=4)
+    bad = _heads(att, data=1 << 25, token=128, heads=4)
+    assert L.ufb_kv_attend(c, 0, 4096, 4096, 1, 3, 3, 1, C.byref(q), C.byref(bad), None, 0, 0, 1, 1.0, 4096, 1 << 40,
+                           None) == EINVAL
+    assert b"overlap" in L.ufb_last_error()

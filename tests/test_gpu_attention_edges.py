@@ -255,3 +255,25 @@ def test_caches_on_two_devices(ufb, dev):
             cache.extend(plan)
             cache.append(0, plan, x, x)
         assert ufb.device_status(device.index) == 0
+
+
+def test_results_in_strided_places(ufb, dev):
+    """The C entries write results as parts of one buffer, head after head, or between other rows."""
+    import ctypes as C
+    import sys
+    att = sys.modules[ufb.__name__ + ".attention"]
+    stream, t, d = torch.cuda.current_stream(dev).cuda_stream, 5, 64
+    rot = ufb.Rotary((8, 12, 12), (64, 22, 40), (10000.0, 100.0, 100.0), device=dev)
+    pos = torch.randint(0, 22, (t, 3), generator=torch.Generator(device=dev).manual_seed(1), device=dev, dtype=torch.int32)
+    q, k = randn(dev, (t, 4, d), 1, torch.float16), randn(dev, (t, 2, d), 2, torch.float16)
+    want = rot.apply(pos, q, k)
+    x = att._heads2(q.data_ptr(), 4 * d, d, 4, k.data_ptr(), 2 * d, d, 2)
+    # [tokens, 6 heads]; [6 heads, tokens]; heads of two results in turn
+    for layout in ((6 * d, d, 4 * d, d), (d, t * d, 4 * t * d, t * d), (8 * d, 2 * d, d, 2 * d)):
+        ts, hs, second, hs2 = layout
+        out = torch.zeros(64 * t * d, dtype=torch.float16, device=dev)
+        y = att._heads2(out.data_ptr(), ts, hs, 4, out.data_ptr() + 2 * second, ts, hs2, 2)
+        assert rot._fn(rot._table, 3, rot._pairs_at, rot._extents_at, 0, 0, pos.data_ptr(), t, d, 1, 2, x, y, stream) == 0
+        assert torch.equal(torch.as_strided(out, (t, 4, d), (ts, hs, 1)), want[0])
+        assert torch.equal(torch.as_strided(out, (t, 2, d), (ts, hs2, 1), second), want[1])
+    _clean(ufb)
