@@ -119,6 +119,28 @@ def _head_tensor(t, device, what: str, dtypes=_DTYPES):
     return t, tokens, heads, dim, code, at, ts, hs
 
 
+class _Turn(torch.autograd.Function):
+    """Rotary.apply of inputs that require a gradient: theirs is the inverse turn."""
+
+    @staticmethod
+    def forward(ctx, rotary, positions, inverse, q, k):
+        ctx.rotary, ctx.inverse = rotary, inverse
+        ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
+        return rotary._turn(positions, q, k, inverse)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        (positions,) = ctx.saved_tensors
+        wanted = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[3:])]
+        given = [g for g in wanted if g is not None]
+        if not given:
+            return None, None, None, None, None
+        turned = ctx.rotary.apply(positions, *given, inverse=not ctx.inverse)
+        back = iter(turned if len(given) == 2 else (turned,))
+        return (None, None, None, *(None if g is None else next(back) for g in (*wanted, None)[:2]))
+
+
 class Rotary:
     """Rotary positions over several axes, for example (time, height, width).
 
@@ -154,7 +176,13 @@ class Rotary:
     def apply(self, positions, q, k=None, inverse=False):
         """Turn q (and k in the same launch) by the tokens' positions
         ([tokens, axes] int32); inverse turns back, which is the gradient with
-        respect to the input.  Returns new tensors: q, or (q, k)."""
+        respect to the input: results of inputs that require one carry it.
+        Returns new tensors: q, or (q, k)."""
+        if torch.is_grad_enabled() and (getattr(q, "requires_grad", False) or getattr(k, "requires_grad", False)):
+            return _Turn.apply(self, positions, inverse, q, k)
+        return self._turn(positions, q, k, inverse)
+
+    def _turn(self, positions, q, k, inverse):
         if not (isinstance(positions, torch.Tensor) and positions.device == self.device and
                 positions.dtype == torch.int32 and positions.dim() == 2 and positions.shape[1] == self._axes):
             raise UfbError(-1, f"positions: int32 tensor [tokens, {self._axes}] on {self.device} required")
@@ -235,6 +263,7 @@ class KVCache:
     ``table`` [slots, table_width] (-1: no page), ``lengths`` [slots], ``refs``
     [pages] -- and no call waits for it on the host.  Calls on one cache belong
     on one stream at a time (or are ordered by events), like writes to any tensor.
+    They are operators of inference: their results carry no gradient.
 
         plan = cache.plan(slots, counts)      # who brings how many tokens
         cache.extend(plan)                    # pages for them, once a step

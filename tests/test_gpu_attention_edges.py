@@ -277,3 +277,38 @@ def test_results_in_strided_places(ufb, dev):
         assert torch.equal(torch.as_strided(out, (t, 4, d), (ts, hs, 1)), want[0])
         assert torch.equal(torch.as_strided(out, (t, 2, d), (ts, hs2, 1), second), want[1])
     _clean(ufb)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rotary_in_autograd(ufb, dev, layout):
+    """A result of inputs that require a gradient carries it: the inverse turn of its own gradient."""
+    rot = ufb.Rotary((5, 6, 9), (30, 40, 50), (10000.0, 100.0, 100.0), layout, device=dev)
+    pos = torch.randint(0, 30, (6, 3), generator=torch.Generator(device=dev).manual_seed(1), device=dev, dtype=torch.int32)
+    q, k = randn(dev, (6, 4, 48), 2), randn(dev, (6, 2, 48), 3)
+    gq, gk = randn(dev, (6, 4, 48), 4), randn(dev, (6, 2, 48), 5)
+    for inverse in (False, True):
+        plain = rot.apply(pos, q, k, inverse=inverse)
+        a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+        y, z = rot.apply(pos, a, b, inverse=inverse)
+        assert torch.equal(y, plain[0]) and torch.equal(z, plain[1])
+        ((y * gq).sum() + (z * gk).sum()).backward()
+        want = rot.apply(pos, gq, gk, inverse=not inverse)
+        assert torch.equal(a.grad, want[0]) and torch.equal(b.grad, want[1])
+        # one of the two inputs alone, one of the two results alone
+        a.grad = None
+        rot.apply(pos, a, k, inverse=inverse)[0].backward(gq)
+        assert torch.equal(a.grad, want[0])
+        b.grad = None
+        (rot.apply(pos, q, b, inverse=inverse)[1] * gk).sum().backward()
+        assert torch.equal(b.grad, want[1])
+        # an input of two uses of a fused projection: the parts' gradients meet in it
+        qkv = torch.cat([q, k], 1).requires_grad_()
+        y, z = rot.apply(pos, qkv[:, :4], qkv[:, 4:], inverse=inverse)
+        ((y * gq).sum() + (z * gk).sum()).backward()
+        assert torch.equal(qkv.grad, torch.cat(want, 1))
+        x = rot.apply(pos, q.clone().requires_grad_(), inverse=inverse)
+        assert x.requires_grad
+        with torch.no_grad():
+            assert not rot.apply(pos, a, b, inverse=inverse)[0].requires_grad
+    assert not rot.apply(pos, q).requires_grad
+    _clean(ufb)
