@@ -543,7 +543,8 @@ int ufb_kv_compact(const ufb_kv_cache* c, void* stream);
  *   s' = max(s, max |x| * (1 / 127))  (s counts when the page holds earlier tokens)
  *   earlier q = rint(q * (s / s')),  new q = min(max(rint(x / s'), -127), 127)
  * in 32 bits.  Values that are not finite stay out of s': infinities are stored
- * as -127 or 127, NaN as 0. */
+ * as -127 or 127, NaN as 0.  Where s' is 0 (no finite value but zeros, infinities
+ * or not) the new integers are all stored as 0. */
 int ufb_kv_append(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
                   int64_t tokens, int dtype, const ufb_heads* k, const ufb_heads* v, void* stream);
 

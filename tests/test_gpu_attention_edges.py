@@ -312,3 +312,24 @@ def test_rotary_in_autograd(ufb, dev, layout):
             assert not rot.apply(pos, a, b, inverse=inverse)[0].requires_grad
     assert not rot.apply(pos, q).requires_grad
     _clean(ufb)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+def test_append_infinities_alone(ufb, dev, dtype):
+    """Without a finite value other than zero the scale is 0 and every new integer with it;
+    beside one, infinities are the ends of the range."""
+    cache = ufb.KVCache(1, 4, 2, 64, 16, 1, 4, device=dev)
+    cache.kv.fill_(55)
+    plan = cache.plan([0], [5])
+    cache.extend(plan)
+    x = torch.zeros((5, 2, 64), dtype=dtype, device=dev)
+    x[0, 0, :4] = torch.tensor([math.inf, -math.inf, math.nan, 0.0])
+    x[1, 1, :4] = torch.tensor([math.inf, -math.inf, math.nan, 1.0])
+    cache.append(0, plan, x, x)
+    page = int(cache.table[0, 0])
+    kv, scale = cache.kv[0, page], cache.scale[0, page]
+    assert bool((scale[:, 0] == 0).all()) and bool((kv[:, 0, :5] == 0).all())
+    assert bool((scale[:, 1] == torch.tensor(1.0 / 127, dtype=torch.float32)).all())
+    assert kv[0, 1, 1, :5].tolist() == [127, -127, 0, 127, 0] and torch.equal(kv[0, 1], kv[1, 1])
+    assert bool((kv[:, :, 5:] == 55).all())
+    _clean(ufb)
