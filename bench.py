@@ -625,6 +625,15 @@ def ref_missing():
     return None if os.path.exists(path) else "oracle/_ref/libufref.so is not built (make -C oracle ref REF_ROOT=<reference>)"
 
 
+def add_cpu_baseline(res, measure):
+    """The reference's CPU figure beside this framework's, or why there is none."""
+    why = ref_missing()
+    if why:
+        res["cpu_baseline_unavailable"] = why
+    else:
+        res["cpu_baseline"] = measure()
+
+
 def ref_decode_sample(threads):
     """Reference IntegerModel::decompress (oracle/_ref) on a 128x128 sample;
     returns (seconds per P packet, seconds per I packet)."""
@@ -973,15 +982,19 @@ def main():
             res["cpu_baseline"] = {"value": v, "unit": "warps/s", "cores": 1, "kind": "port", "sample": note}
     elif args.workload == "conv":
         res = bench_conv_ours(args, rank, world, local)
-        if rank == 0 and world == 1 and not ref_missing():
-            v, note = ref_conv(1)
-            res["cpu_baseline"] = {"value": v, "unit": "MAC/s", "cores": 1, "kind": "reference", "sample": note}
+        if rank == 0 and world == 1:
+            def conv_baseline():
+                v, note = ref_conv(1)
+                return {"value": v, "unit": "MAC/s", "cores": 1, "kind": "reference", "sample": note}
+            add_cpu_baseline(res, conv_baseline)
     else:
         res = bench_decode_ours(args, rank, world, local)
-        if rank == 0 and world == 1 and not ref_missing():
-            t_p, t_i = ref_decode_sample(threads)
-            res["cpu_baseline"] = {"value": ref_fps_1080(t_p, t_i), "unit": "frames/s", "cores": threads,
-                                   "kind": "reference", "sample": ref_decode_note(t_p, t_i)}
+        if rank == 0 and world == 1:
+            def decode_baseline():
+                t_p, t_i = ref_decode_sample(threads)
+                return {"value": ref_fps_1080(t_p, t_i), "unit": "frames/s", "cores": threads, "kind": "reference",
+                        "sample": ref_decode_note(t_p, t_i)}
+            add_cpu_baseline(res, decode_baseline)
     if rank == 0:
         print(json.dumps(res))
     if world > 1:
