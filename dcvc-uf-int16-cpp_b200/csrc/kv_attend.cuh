@@ -276,8 +276,6 @@ __device__ __forceinline__ float unit_inverse(float u) {
     return u == u ? __int_as_float((254 << 23) - __float_as_int(u)) : u;
 }
 
-__device__ __forceinline__ float wide(__half v) { return __half2float(v); }
-__device__ __forceinline__ float wide(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);

@@ -1,5 +1,5 @@
 // Attention over the 8-bit cache for few rows (new tokens x query heads of a key
-// head <= 16 or so): a decoding step.
+// head, up to 32: one tile of 8, or one or two of 16): a decoding step.
 //
 //   S = Q K^T,  P = 2^(S f + log2 vs - M),  O = P V,  l = sum P / vs
 //

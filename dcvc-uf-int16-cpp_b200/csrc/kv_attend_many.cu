@@ -702,7 +702,8 @@ cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     many_kernel<T, D><<<ctas, kThreads, smem, s>>>(a, static_cast<int>(row_tiles), 1);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    // its blocks start while the last CTAs still work, and wait for them
+    // its blocks may start once the CTAs have exited, before that kernel's end is signalled
+    // (it gives no earlier trigger): they wait for that
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(ctas, kRows * (D / 4) / kJoinThreads);
     config.blockDim = dim3(kJoinThreads);

@@ -285,8 +285,10 @@ __global__ void __launch_bounds__(kThreads) compact_kernel(const ufb_kv_cache c)
     if (threadIdx.x == 0) *w.moves = movers;
 }
 
-// Waits for the kernel before this one (launched with programmatic serialization:
-// this one's blocks start while that one runs).
+// Waits for the kernel before this one.  Launched with programmatic serialization,
+// this one's blocks may start once that one's have exited, without its end being
+// flushed and signalled first: that hides part of a launch's latency, no work (the
+// kernel before gives no earlier trigger).
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Moves of the list: grid (moves upper bound or less, layers * 2 sides).  A CTA

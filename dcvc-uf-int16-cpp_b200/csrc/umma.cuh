@@ -1,4 +1,4 @@
-// sm_100a primitives used by the INT16 convolution kernels: mbarriers with
+// sm_100a primitives used by the INT16 convolution and the attention kernels: mbarriers with
 // bounded waits, TMA tile loads, and the tcgen05 tensor-memory / MMA
 // instructions, written directly as inline PTX.
 #pragma once
