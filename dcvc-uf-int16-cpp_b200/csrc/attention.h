@@ -28,7 +28,7 @@ struct RotaryArgs {
     int count;                       // tensors
     ufb_heads x[2], out[2];
 };
-cudaError_t rotary(const RotaryArgs& a, int dtype, int* status, cudaStream_t s);
+cudaError_t rotary(const RotaryArgs& a, int dtype, int sms, int* status, cudaStream_t s);
 
 // Marks of streams (one for each slot, behind the page operators' scratch in
 // ufb_kv_cache.work): 1 from an extend that was refused to one that is granted.

@@ -83,7 +83,7 @@ bool check_outputs(const ufb_heads& a, const ufb_heads& b, int64_t tokens, int h
 }
 
 // SMs of the current device; 0 with the error recorded.
-int attend_sms() {
+int current_sms() {
     static std::atomic<int> known[64];
     int device = 0;
     if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice")) return 0;
@@ -204,9 +204,11 @@ int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t
     a.layout = layout;
     a.inverse = inverse != 0;
     a.count = count;
+    const int sms = current_sms();
+    if (sms <= 0) return last_code();
     int* status = current_status();
     if (!status) return last_code();
-    return done(rotary(a, dtype, status, static_cast<cudaStream_t>(stream)), "rotary");
+    return done(rotary(a, dtype, sms, status, static_cast<cudaStream_t>(stream)), "rotary");
 }
 
 int64_t ufb_kv_work_ints(int32_t pages, int32_t slots) {
@@ -291,7 +293,7 @@ int ufb_kv_read(const ufb_kv_cache* c, int layer, const int32_t* pages, int64_t 
 
 int64_t ufb_kv_attend_workspace(void) {
     clear_error();
-    const int sms = attend_sms();
+    const int sms = current_sms();
     return sms > 0 ? kv_attend_workspace_bytes(sms) : last_code();
 }
 
@@ -318,7 +320,7 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
         return last_code();
     if (q->heads % c->heads) return err(UFB_EINVAL, "query heads must be a multiple of the cache's heads");
     if (q->heads / c->heads > 128) return err(UFB_ERANGE, "more than 128 query heads to a key head");
-    const int sms = attend_sms();
+    const int sms = current_sms();
     if (sms <= 0) return last_code();
     const int64_t need = kv_attend_workspace_bytes(sms);
     if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)

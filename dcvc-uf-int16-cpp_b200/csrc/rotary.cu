@@ -216,14 +216,14 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a, in
 }
 
 template <typename T, Mode MODE>
-cudaError_t launch(const RotaryArgs& a, int columns, int* status, cudaStream_t s) {
+cudaError_t launch(const RotaryArgs& a, int columns, int sms, int* status, cudaStream_t s) {
     const int heads = a.x[0].heads + (a.count > 1 ? a.x[1].heads : 0);
     const unsigned slots = kThreads / columns;
     const long long blocks = (a.tokens + slots - 1) / slots;
     if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
     // All heads to a thread share its table values; while that leaves SMs without
     // two blocks, the heads are spread over more blocks.
-    long long groups = (2 * 148 + blocks - 1) / blocks;
+    long long groups = (2ll * sms + blocks - 1) / blocks;
     if (groups > heads) groups = heads;
     const int per = static_cast<int>((heads + groups - 1) / groups);
     rotary_kernel<T, MODE><<<dim3(static_cast<unsigned>(blocks), (heads + per - 1) / per), kThreads, 0, s>>>(a, columns, per, status);
@@ -231,21 +231,21 @@ cudaError_t launch(const RotaryArgs& a, int columns, int* status, cudaStream_t s
 }
 
 template <typename T>
-cudaError_t dispatch(const RotaryArgs& a, int* status, cudaStream_t s) {
+cudaError_t dispatch(const RotaryArgs& a, int sms, int* status, cudaStream_t s) {
     constexpr int N = Column<T>::n;
     const int vecs = a.head_dim / N;
-    if (a.layout == UFB_ROTARY_INTERLEAVED) return launch<T, kInterleaved>(a, vecs, status, s);
+    if (a.layout == UFB_ROTARY_INTERLEAVED) return launch<T, kInterleaved>(a, vecs, sms, status, s);
     // pair counts that are whole columns: a thread reads and writes both members
-    if (a.pairs % N == 0) return launch<T, kHalfPairs>(a, vecs - a.pairs / N, status, s);
-    return launch<T, kHalf>(a, vecs, status, s);
+    if (a.pairs % N == 0) return launch<T, kHalfPairs>(a, vecs - a.pairs / N, sms, status, s);
+    return launch<T, kHalf>(a, vecs, sms, status, s);
 }
 
 }  // namespace
 
-cudaError_t rotary(const RotaryArgs& a, int dtype, int* status, cudaStream_t s) {
-    if (dtype == UFB_F32) return dispatch<float>(a, status, s);
-    if (dtype == UFB_F16) return dispatch<__half>(a, status, s);
-    return dispatch<__nv_bfloat16>(a, status, s);
+cudaError_t rotary(const RotaryArgs& a, int dtype, int sms, int* status, cudaStream_t s) {
+    if (dtype == UFB_F32) return dispatch<float>(a, sms, status, s);
+    if (dtype == UFB_F16) return dispatch<__half>(a, sms, status, s);
+    return dispatch<__nv_bfloat16>(a, sms, status, s);
 }
 
 }  // namespace ufb
