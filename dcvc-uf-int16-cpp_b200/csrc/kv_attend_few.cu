@@ -27,7 +27,9 @@
 // 64 streams x 16000 keys x 4 heads of 128: 188 us, 5.6 TB/s, 0.87 of a plain
 // copy's rate (8 consumer warps with the rows as the wide side: 160 us for 127 on 64
 // ragged streams up to 16320 keys);
-// head_dim 64 at 3.3 TB/s, bound by the expansion; one token over 1760 keys 12 us.
+// head_dim 64 at 3.3 TB/s: half the bytes a key, and scores, weights and their exchange
+// cost as much a key (not the expansion: a form with two instructions less for four keys
+// took as long); one token over 1760 keys 12 us.
 //
 // Parts of an item that several CTAs share are joined by the CTA that arrives
 // last, in the order of the CTAs, so the sum does not depend on which one it is.

@@ -21,9 +21,10 @@
 // Its floor at head_dim 128: 2048 cycles a tile for the exponentials (16 an SM and
 // cycle) and 2200 for the products (measured alone), side by side.  A tile takes
 // about 4900: the chain S, softmax, P V, S of a half, whose S and P share columns,
-// and four roles' instructions on the same schedulers.  8160 tokens x 24480 keys,
-// 16 heads: 1.85 ms, 885 TFLOP/s, 0.52 of cuBLAS's rate in bfloat16; the first form
-// of this kernel took 3.66 ms.  A running maximum that grows little is kept, so O is
+// and four roles' instructions on the same schedulers; which of them bounds it is not
+// settled (at head_dim 64 a form without the chain took as long).  8160 tokens x 24480
+// keys, 16 heads: 1.82 - 1.87 ms, 875 - 900 TFLOP/s, 0.52 - 0.53 of cuBLAS's rate in
+// bfloat16; the first form of this kernel took 3.66 ms.  A running maximum that grows little is kept, so O is
 // rescaled rarely and by the softmax threads themselves.
 //
 // The key tiles of all items are divided equally over the CTAs (kv_attend.cuh);

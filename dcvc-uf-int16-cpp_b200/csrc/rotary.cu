@@ -7,14 +7,18 @@
 // kernel no sine.
 //
 // Bound by HBM: every element is read once and written once (130560 tokens x 20
-// heads of 128 in bfloat16: 236 us, 5.7 TB/s, 0.88 of a plain copy's rate).  A
+// heads of 128 in bfloat16: 231 - 236 us, 5.7 TB/s, 0.88 of a plain copy's rate).  A
 // thread owns one 16-byte column of a head (8 or 4 elements), reads that column's
 // (c, s) once and applies them to the heads of the same token, since the table
 // bytes of a column are four times its data in 16 bits (one to four heads a thread:
 // 855 us).  In the half layout the partner column lies n elements away: where n is
 // whole columns a thread reads and writes both members; otherwise the partner is
 // read as the two aligned columns around it and shifted into place, so every access
-// stays 16 bytes wide whatever the pair counts are.
+// stays 16 bytes wide whatever the pair counts are: the same tokens with 61 or 63 pairs
+// take 648 us (0.32: a column and the two around its partner are read, and the members of
+// a pair belong to two threads; which of it bounds has not been measured), in float32 385
+// us for 65280 tokens (0.54; whole columns 216 us, 0.96).  Interleaved: 291 us in bfloat16
+// (0.71), 421 in float32 (0.98).
 #include "attention.h"
 
 #include <cuda_bf16.h>
