@@ -314,34 +314,44 @@ def prepare(case, seed):
 
 # ------------------------------------------------------------- plain forms ----
 
+def _ordered(x):
+    """Integers in the order of the 32-bit floats x, equal zeros among them."""
+    bits = (x + 0.0).view(torch.int32)
+    return torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits).long()
+
+
 def _plain_select(state):
     case, scores, finished = state["case"], state["scores"], state["finished"]
-    count, v = case["count"], case["vocab"]
+    v = case["vocab"]
     b, k = scores.shape
+    x = state["logits"]
+    each, count = min(case["count"], v), min(case["count"], k * v)
+    # the best of each beam: larger logits first, then lower tokens
+    key = (_ordered(x.float()) << 32) + (0xFFFFFFFF - torch.arange(v, device=x.device))
+    token = 0xFFFFFFFF - (key.topk(each, -1).values & 0xFFFFFFFF)
+    del key
     # 64 bits: totals of different beams are next to each other, and their order is the result
-    x = state["logits"].double()
+    x = x.double()
+    logit = x.gather(-1, token)
     top = x.amax(-1, keepdim=True)
     lse = top + (x - top).exp_().sum(-1, keepdim=True).log()
-    x += scores.double()[..., None] - lse
+    total = (scores.double()[..., None] + (logit - lse)).float()
     live = torch.isfinite(top[..., 0]) & (scores > -math.inf)
     if finished is not None:
         live &= ~finished
-    x.masked_fill_(~live[..., None], -math.inf)
+    total.masked_fill_(~live[..., None], -math.inf)
     if finished is not None:
-        x[..., 0] = torch.where(finished, scores.double(), x[..., 0])
-    # one order of values and places: higher totals first, then lower places
-    bits = (x.float() + 0.0).view(torch.int32)
-    del x
-    value = torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits).long().view(b, k * v)
-    place = torch.arange(k * v, device=value.device)
-    best = ((value << 32) + (0xFFFFFFFF - place)).topk(min(count, k * v), -1).values
-    place = 0xFFFFFFFF - (best & 0xFFFFFFFF)
-    bits = (best >> 32).int()
-    total = torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits).view(torch.float32)
+        total[..., 0] = torch.where(finished, scores, total[..., 0])
+        token[..., 0].masked_fill_(finished, 0)
+    # of all beams: higher totals first, then lower beams and a beam's own order
+    total, token = total.view(b, -1), token.view(b, -1)
+    key = (_ordered(total) << 32) + (0xFFFFFFFF - torch.arange(k * each, device=x.device))
+    at = 0xFFFFFFFF - (key.topk(min(count, k * each), -1).values & 0xFFFFFFFF)
+    total = total.gather(1, at)
     none = total == -math.inf
     rank = torch.arange(total.shape[1], device=total.device).clamp(max=k - 1)
-    parents = torch.where(none, rank, place // v).int()
-    tokens = torch.where(none, 0, place % v).int()
+    parents = torch.where(none, rank, at // each).int()
+    tokens = torch.where(none, 0, token.gather(1, at)).int()
     return total, parents, tokens
 
 
@@ -457,8 +467,8 @@ def _exact_select(case, x):
                 totals.append(base[None])
                 continue
             t = base + torch.log_softmax(x["logits"][b, k].double(), -1)
-            # no more of one beam than are asked for
-            order = torch.sort(t.float(), descending=True, stable=True).indices[:case["count"]]
+            # no more of one beam than are asked for, in the order of their logits and tokens
+            order = torch.sort(x["logits"][b, k].double(), descending=True, stable=True).indices[:case["count"]]
             order = order[t[order] > -math.inf]
             names.append(order + k * case["vocab"])
             totals.append(t[order])
