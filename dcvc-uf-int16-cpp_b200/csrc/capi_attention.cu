@@ -5,7 +5,6 @@
 #include "attention.h"
 #include "capi_util.h"
 
-#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -18,12 +17,6 @@ namespace {
 constexpr int kMostKeys = 1 << 30;  // of a stream
 
 int element_size(int dtype) { return dtype == UFB_F32 ? 4 : 2; }
-
-int* current_status() {
-    int device = 0;
-    if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice")) return nullptr;
-    return device_status(device);
-}
 
 int done(cudaError_t e, const char* what) { return cuda_ok(e, what) ? UFB_OK : last_code(); }
 
@@ -80,19 +73,6 @@ bool check_outputs(const ufb_heads& a, const ufb_heads& b, int64_t tokens, int h
         for (int g = 0; g < b.heads && !meet; ++g)
             meet = rows_meet(apart + g * b.head_stride - h * a.head_stride, a.token_stride, tokens, head_dim, false);
     return !meet || fail(UFB_EINVAL, std::string(what) + " overlap");
-}
-
-// SMs of the current device; 0 with the error recorded.
-int current_sms() {
-    static std::atomic<int> known[64];
-    int device = 0;
-    if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice")) return 0;
-    int sms = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
-    if (sms == 0) {
-        if (!cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device attribute")) return 0;
-        if (device < 64) known[device].store(sms, std::memory_order_relaxed);
-    }
-    return sms;
 }
 
 bool check_cache(const ufb_kv_cache* c) {

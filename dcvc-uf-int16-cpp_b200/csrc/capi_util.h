@@ -23,6 +23,11 @@ bool cuda_ok(cudaError_t e, const char* what);     // records UFB_ECUDA on failu
 // the address cannot be resolved.
 int* device_status(int device);
 
+// The status word and the number of SMs of the current device; null and 0 with
+// the error recorded.
+int* current_status();
+int current_sms();
+
 // Argument checks of uf_conv (src/cuda/conv.cu:65-83) shared by every
 // convolution entry point; fills the output extent.
 bool check_conv(const int16_t* x, int n, int ci, int h, int w, const int16_t* weight, int co, int kh, int kw,

@@ -7,6 +7,7 @@
 
 #include "uf_b200.h"
 
+#include <atomic>
 #include <mutex>
 #include <vector>
 
@@ -41,6 +42,24 @@ int* device_status(int device) {
         g_status[device] = static_cast<int*>(p);
     }
     return g_status[device];
+}
+
+int* current_status() {
+    int device = 0;
+    if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice")) return nullptr;
+    return device_status(device);
+}
+
+int current_sms() {
+    static std::atomic<int> known[64];
+    int device = 0;
+    if (!cuda_ok(cudaGetDevice(&device), "cudaGetDevice")) return 0;
+    int sms = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+    if (sms == 0) {
+        if (!cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "device attribute")) return 0;
+        if (device < 64) known[device].store(sms, std::memory_order_relaxed);
+    }
+    return sms;
 }
 
 }  // namespace ufb

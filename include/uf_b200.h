@@ -446,6 +446,7 @@ int ufb_conv2d_noalloc(const int16_t* x, int n, int ci, int h, int w, const int1
  *   32 a slot, page or token offset out of range, or a page that is missing
  *      where tokens are to be stored (what it names is skipped)
  *   41..44 a bounded wait of the attention kernel gave up
+ *   51 a row of logits holds NaN or +infinity (its beam has no continuations)
  * ------------------------------------------------------------------------- */
 
 #define UFB_F32 0
@@ -582,6 +583,28 @@ int64_t ufb_kv_attend_workspace(void);
 /* The graph capture that `stream` is in: a number that no other capture has; 0
  * outside of one. */
 int64_t ufb_capture_id(void* stream);
+
+#define UFB_BEAM_MAX 64
+#define UFB_BEAM_COUNT_MAX 64
+
+/* The best continuations of the beams of each stream, a step of a search over
+ * sequences.  Beam k of stream b has the score s = scores[b][k] (the sum of its
+ * tokens' log probabilities) and logits l (dtype UFB_F32, UFB_F16 or UFB_BF16) at
+ * b * stream_stride + k * beam_stride, vocab of them, contiguous.  Its continuation
+ * by token v has the score
+ *   f32(s + (l[v] - ln sum_u exp l[u]))
+ * rounded once, from values good to 2^-28.  A beam marked in finished (NULL, or
+ * [streams][beams] bytes) has one continuation, token pad with score s, and its
+ * logits are not read; neither are those of a beam whose score is -infinity or NaN,
+ * which has none.  Logits of -infinity are forbidden tokens; a row that holds NaN or
+ * +infinity gives no continuations (status 51).
+ *   out_scores, parents, tokens [streams][count]: the best, falling scores; equal
+ * ones by the lower beam, of one beam by the larger logit, then the lower token.
+ * Scores of -infinity are no continuations: places i for which there are none left get
+ * score -infinity, parent min(i, beams - 1), token 0. */
+int ufb_beam_select(const void* logits, int dtype, int64_t stream_stride, int64_t beam_stride, const float* scores,
+                    const uint8_t* finished, int streams, int beams, int vocab, int count, int pad,
+                    float* out_scores, int32_t* parents, int32_t* tokens, void* stream);
 
 /* Measurement utility (no reference counterpart): launches `ctas` CTAs that
  * each issue `iters` x 4 dense tcgen05 kind::i8 M=128 N=256 K=32 MMAs from
