@@ -693,7 +693,7 @@ class StreamCodec:
 
 
 # Latent attention: rotary positions, the 8-bit paged cache and attention over it.
-from .attention import KVCache, KVForkPlan, KVPlan, Rotary  # noqa: E402,F401
+from .attention import KVBeamPlan, KVCache, KVForkPlan, KVGroups, KVPlan, Rotary  # noqa: E402,F401
 
 # A search over sequences: the best continuations of a stream's beams.
 from .beams import beam_select  # noqa: E402,F401

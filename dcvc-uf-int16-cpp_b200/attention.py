@@ -32,6 +32,10 @@ class _Cache(C.Structure):
         (n, C.c_int32) for n in ("layers", "pages", "heads", "page_tokens", "head_dim", "slots", "table_width")]
 
 
+class _Groups(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("first", "offsets", "state")] + [("groups", C.c_int32), ("max_tokens", C.c_int32)]
+
+
 def _lib():
     L = library()
     if getattr(L, "_attention_ready", False):
@@ -53,6 +57,12 @@ def _lib():
     L.ufb_kv_attend_workspace.restype = i64
     L.ufb_capture_id.restype = i64
     L.ufb_capture_id.argtypes = [vp]
+    L.ufb_kv_reorder.argtypes = [cache, vp, vp, ci, ci, vp]
+    L.ufb_kv_group_ints.restype = i64
+    L.ufb_kv_group_ints.argtypes = [ci, ci, i64]
+    L.ufb_kv_share.argtypes = [cache, vp, vp, ci, ci, i64, vp, vp]
+    L.ufb_kv_attend_groups.argtypes = [cache, ci, vp, vp, ci, ci, i64, ci, heads, heads, vp, ci, ci, ci, C.c_float, vp,
+                                       vp, vp, i64, vp]
     L.ufb_kv_attend.argtypes = [cache, ci, vp, vp, ci, ci, i64, ci, heads, heads, vp, ci, ci, ci, C.c_float, vp, i64, vp]
     L._attention_ready = True
     return L
@@ -231,6 +241,7 @@ class KVPlan:
         offsets = [0]
         for c in counts:
             offsets.append(offsets[-1] + c)
+        self._host_offsets = offsets
         ints = torch.tensor(slots + offsets, dtype=torch.int32).to(cache.device)
         self.slots, self.offsets = ints[:self.n], ints[self.n:]
         self._slots, self._offsets = self.slots.data_ptr(), self.offsets.data_ptr()
@@ -253,6 +264,48 @@ class KVForkPlan:
         self._src, self._dst = self.src.data_ptr(), self.dst.data_ptr()
 
 
+class KVBeamPlan:
+    """Groups of ``width`` streams that a search moves among (KVCache.beam_plan)."""
+
+    def __init__(self, cache, slots, width):
+        slots, width = [int(s) for s in slots], int(width)
+        if not 1 <= width <= 64 or len(slots) % width:
+            raise UfbError(-1, "beams come in whole groups of 1 to 64 slots")
+        if any(s < 0 or s >= cache.slots for s in slots):
+            raise UfbError(-1, "slot out of range")
+        if len(set(slots)) != len(slots):
+            raise UfbError(-1, "a slot may appear once in a plan")
+        self.cache, self.n, self.width = cache, len(slots), width
+        self.slots = torch.tensor(slots, dtype=torch.int32).to(cache.device)
+        self._slots = self.slots.data_ptr()
+
+
+class KVGroups:
+    """Groups of consecutive streams of a plan that may begin alike (KVCache.group_plan).
+    ``shared`` [groups] int32: the tokens they have in common, as KVCache.share found them."""
+
+    def __init__(self, plan, sizes):
+        sizes = [int(s) for s in sizes]
+        if any(s < 1 for s in sizes) or sum(sizes) != plan.n:
+            raise UfbError(-1, "groups must have one stream or more and be all of the plan's streams")
+        self.plan, self.cache, self.n = plan, plan.cache, len(sizes)
+        first = [0]
+        for s in sizes:
+            first.append(first[-1] + s)
+        host = plan._host_offsets
+        tokens = [host[f] for f in first]
+        self.max_tokens = max((b - a for a, b in zip(tokens, tokens[1:])), default=0)
+        device = plan.cache.device
+        ints = torch.tensor(first + tokens, dtype=torch.int32).to(device)
+        self.first, self.offsets = ints[:self.n + 1], ints[self.n + 1:]
+        self._state = torch.zeros(_lib().ufb_kv_group_ints(self.n, plan.n, plan.tokens), dtype=torch.int32, device=device)
+        self.shared = self._state[:self.n]
+        self._struct = _Groups(self.first.data_ptr(), self.offsets.data_ptr(), self._state.data_ptr(), self.n,
+                               self.max_tokens)
+        self._ref = C.addressof(self._struct)
+        self._at = None   # the state of the cache that share saw
+
+
 class KVCache:
     """Keys and values of many streams and layers in 8 bits, in pages of
     ``page_tokens`` tokens with one scale for each page, head and side (key or
@@ -269,6 +322,15 @@ class KVCache:
         cache.extend(plan)                    # pages for them, once a step
         cache.append(layer, plan, k, v)       # in every layer
         out = cache.attend(layer, plan, q, window=..., sinks=...)
+
+    Streams that branch off one another (fork, reorder) share pages.  A step of a
+    search over them that reads those once:
+
+        cache.reorder(beam_plan, parents)     # beam_select's choice
+        cache.extend(plan)
+        cache.share(groups)                   # group_plan(plan, sizes)
+        cache.append(layer, plan, k, v)       # in every layer
+        out = cache.attend(layer, plan, q, groups=groups)
 
     When the pages do not suffice, extend changes nothing (status 31), and append
     and attend leave out the streams that were to grow (status 31 again, zeros for
@@ -304,7 +366,8 @@ class KVCache:
                               self.table_width)
         self._ref = C.addressof(self._struct)
         self._default_scale = self.head_dim ** -0.5
-        self._append, self._attend = L.ufb_kv_append, L.ufb_kv_attend
+        self._append, self._attend, self._attend_groups = L.ufb_kv_append, L.ufb_kv_attend, L.ufb_kv_attend_groups
+        self._changes = 0   # calls that changed tables or lengths
         self._workspaces, self._captures = {}, {}
         self._spare = self._new_workspace()
 
@@ -318,6 +381,15 @@ class KVCache:
         """Branches src[i] -> dst[i]; kept over calls."""
         return KVForkPlan(self, src, dst)
 
+    def beam_plan(self, slots, width):
+        """Groups of width streams each, for reorder; kept over calls."""
+        return KVBeamPlan(self, slots, width)
+
+    def group_plan(self, plan, sizes):
+        """The plan's streams in groups of the given sizes, for share and attend; kept over
+        layers and steps."""
+        return KVGroups(self._own(plan), sizes)
+
     def _own(self, plan, kind=KVPlan):
         if not isinstance(plan, kind) or plan.cache is not self:
             raise UfbError(-1, f"a {kind.__name__} of this cache is required")
@@ -326,24 +398,53 @@ class KVCache:
     def extend(self, plan):
         """Grow the plan's streams by its counts and give them the pages for it."""
         self._own(plan)
+        self._changes += 1
         _launch(self.device, self._L.ufb_kv_extend, self._ref, plan._slots, plan._offsets, plan.n)
 
     def release(self, plan):
         """Drop the pages of the plan's streams; their lengths become 0."""
         self._own(plan)
+        self._changes += 1
         _launch(self.device, self._L.ufb_kv_release, self._ref, plan._slots, plan.n)
 
     def trim(self, plan, window, sinks=0):
         """Drop the pages that no later query of the plan's streams sees."""
         self._own(plan)
         _check_ints(0, window, sinks)
+        self._changes += 1
         _launch(self.device, self._L.ufb_kv_trim, self._ref, plan._slots, plan.n, int(window), int(sinks))
 
     def fork(self, plan):
         """Make the plan's destinations branches of its sources, whose tokens have
         been appended in every layer: full pages are shared from here on."""
         self._own(plan, KVForkPlan)
+        self._changes += 1
         _launch(self.device, self._L.ufb_kv_fork, self._ref, plan._src, plan._dst, plan.n)
+
+    def reorder(self, plan, parents):
+        """The streams of every group of a beam_plan go on, all at once, from what the
+        group's streams held: place j of group g from place ``parents[g, j]`` (int32
+        tensor [groups, width], beam_select's parents).  Full pages are shared from
+        here on; a partly filled last page stays with one of its children, the others
+        get copies, on the pages of places that nobody goes on from as far as they
+        suffice.  A parent out of range or too few pages: nothing changes (status 32, 31)."""
+        self._own(plan, KVBeamPlan)
+        if not (isinstance(parents, torch.Tensor) and parents.device == self.device and parents.dtype == torch.int32 and
+                parents.shape == (plan.n // plan.width, plan.width)):
+            raise UfbError(-1, f"parents: int32 tensor {[plan.n // plan.width, plan.width]} on {self.device} required")
+        if not parents.is_contiguous():
+            parents = parents.contiguous()
+        self._changes += 1
+        _launch(self.device, self._L.ufb_kv_reorder, self._ref, plan._slots, parents.data_ptr(), plan.n, plan.width)
+
+    def share(self, groups):
+        """Find the pages that the streams of each group begin with in common: once a
+        step, behind extend, for attend in all layers."""
+        self._own(groups, KVGroups)
+        plan = groups.plan
+        _launch(self.device, self._L.ufb_kv_share, self._ref, plan._slots, plan._offsets, plan.n, plan.max_new,
+                plan.tokens, groups._ref)
+        groups._at = self._changes
 
     def compact(self):
         """Move the live pages to the lowest ids."""
@@ -423,7 +524,7 @@ class KVCache:
             held = self._captures[key] = (capture, (t.data_ptr(), t.numel(), t))
         return held[1]
 
-    def attend(self, layer, plan, q, window=0, sinks=0, causal=True, scale=None, lse=False):
+    def attend(self, layer, plan, q, window=0, sinks=0, causal=True, scale=None, lse=False, groups=None):
         """Attention of the plan's newest tokens (q [tokens, query heads, head_dim],
         float16 or bfloat16) over their streams.  A query at position a sees key
         j when j <= a (all keys when not causal) and, with a window, j > a -
@@ -432,7 +533,11 @@ class KVCache:
         heads] float32).  Every CUDA stream has its own scratch, and so has every
         capture, in its graph's memory: graphs may be replayed beside each other
         and beside other calls.  One stream may capture without an earlier call
-        on it; others call attend once before."""
+        on it; others call attend once before.
+
+        With groups (group_plan of this plan, after share has seen the cache as it is)
+        the pages that a group's streams begin with in common are read once for all of
+        them, and its result is joined with that over each stream's own keys, in 32 bits."""
         self._own(plan)
         _check_ints(layer, window, sinks)
         device = self.device
@@ -442,6 +547,18 @@ class KVCache:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         l = torch.empty((tokens, heads), dtype=torch.float32, device=device) if lse else None
         w = self._workspace()
+        if groups is not None:
+            self._own(groups, KVGroups)
+            if groups.plan is not plan:
+                raise UfbError(-1, "groups of this plan are required")
+            if groups._at != self._changes:
+                raise UfbError(-1, "share has not seen the cache since its streams changed: call it once a step")
+            parts = torch.empty(tokens * heads * (dim + 1), dtype=torch.float32, device=device)
+            _launch(device, self._attend_groups, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new,
+                    tokens, code, _heads(qa, qts, qhs, heads), _heads(out.data_ptr(), heads * dim, dim, heads),
+                    None if l is None else l.data_ptr(), window, sinks, 1 if causal else 0,
+                    self._default_scale if scale is None else scale, groups._ref, parts.data_ptr(), w[0], w[1])
+            return (out, l) if lse else out
         _launch(device, self._attend, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new, tokens, code,
                 _heads(qa, qts, qhs, heads), _heads(out.data_ptr(), heads * dim, dim, heads),
                 None if l is None else l.data_ptr(), window, sinks, 1 if causal else 0,

@@ -35,6 +35,8 @@ cudaError_t rotary(const RotaryArgs& a, int dtype, int sms, int* status, cudaStr
 __host__ __device__ inline int32_t* kv_refused(const ufb_kv_cache& c) {
     return c.work + 16 + 3ll * c.pages + c.slots;
 }
+// Behind them, one integer for each stream of a reorder.
+__host__ __device__ inline int32_t* kv_last_entry(const ufb_kv_cache& c) { return kv_refused(c) + c.slots; }
 
 // Streams of one call: new tokens [offsets[i], offsets[i + 1]) belong to slots[i].
 struct KvBatch {
@@ -54,6 +56,8 @@ cudaError_t kv_extend(const ufb_kv_cache& c, const int32_t* slots, const int32_t
 cudaError_t kv_release(const ufb_kv_cache& c, const int32_t* slots, int n, int* status, cudaStream_t s);
 cudaError_t kv_fork(const ufb_kv_cache& c, const int32_t* src, const int32_t* dst, int n, int* status,
                     cudaStream_t s);
+cudaError_t kv_reorder(const ufb_kv_cache& c, const int32_t* slots, const int32_t* parents, int n, int width,
+                       int* status, cudaStream_t s);
 cudaError_t kv_trim(const ufb_kv_cache& c, const int32_t* slots, int n, int window, int sinks, int* status,
                     cudaStream_t s);
 cudaError_t kv_compact(const ufb_kv_cache& c, int* status, cudaStream_t s);
@@ -75,8 +79,35 @@ struct AttendArgs {
     float* lse;
     int* status;
     void* workspace;
+    // attention in two parts (kv_attend.cuh: kOwn, kCommon)
+    const int32_t* starts;           // [n] tokens of each stream that its group has in common
+    const int32_t* lows;             // [n] first and last position of a group's new tokens
+    const int32_t* highs;
+    const int32_t* positions;        // [tokens]
+    float* part_out;                 // [tokens][query heads][head_dim] of the streams' own keys
+    float* part_lse;                 // [tokens][query heads], in base 2
 };
 cudaError_t kv_attend(const AttendArgs& a, int dtype, int sms, cudaStream_t s);
+
+// What kv_share leaves of the groups of a batch (ufb_kv_groups.state).
+struct KvGroupState {
+    int32_t *shared, *slot, *low, *high;   // [groups] tokens in common, a stream that has them, positions
+    int32_t* starts;                       // [n]
+    int32_t* positions;                    // [tokens]; -1: sees no key, -2: not to be written
+};
+inline KvGroupState kv_group_state(const ufb_kv_groups& g, int n) {
+    KvGroupState s;
+    s.shared = g.state;
+    s.slot = s.shared + g.groups;
+    s.low = s.slot + g.groups;
+    s.high = s.low + g.groups;
+    s.starts = s.high + g.groups;
+    s.positions = s.starts + n;
+    return s;
+}
+cudaError_t kv_share(const ufb_kv_cache& c, const KvBatch& b, const ufb_kv_groups& g, int* status, cudaStream_t s);
+// own: attention of every stream over its own keys; common: of the groups over the keys in common
+cudaError_t kv_attend_groups(const AttendArgs& own, const AttendArgs& common, int dtype, int sms, cudaStream_t s);
 int64_t kv_attend_workspace_bytes(int sms);
 
 }  // namespace ufb

@@ -113,6 +113,15 @@ bool check_batch(const ufb_kv_cache* c, int layer, const int32_t* slots, const i
     return true;
 }
 
+// Groups of the streams of a batch that check_batch has passed.
+bool check_groups(const ufb_kv_groups* g, int n, int max_new, int64_t tokens) {
+    if (!g || g->groups < 0 || g->groups > n || (n > 0 && g->groups == 0))
+        return fail(UFB_EINVAL, "a batch has between one group and one for each stream");
+    if (g->groups > 0 && (!g->first || !g->offsets || !g->state)) return fail(UFB_EINVAL, "group tensors must be non-null");
+    if (g->max_tokens < max_new || g->max_tokens > tokens) return fail(UFB_EINVAL, "invalid token count of a group");
+    return true;
+}
+
 }  // namespace
 
 extern "C" {
@@ -194,7 +203,7 @@ int ufb_rotary(const float* table, int axes, const int32_t* pairs, const int32_t
 int64_t ufb_kv_work_ints(int32_t pages, int32_t slots) {
     clear_error();
     if (pages <= 0 || slots <= 0) return err(UFB_EINVAL, "empty cache");
-    return 16 + 3ll * pages + 2ll * slots;
+    return 16 + 3ll * pages + 3ll * slots;
 }
 
 int ufb_kv_extend(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, void* stream) {
@@ -223,6 +232,20 @@ int ufb_kv_fork(const ufb_kv_cache* c, const int32_t* src, const int32_t* dst, i
     int* status = current_status();
     if (!status) return last_code();
     return done(kv_fork(*c, src, dst, n, status, static_cast<cudaStream_t>(stream)), "kv fork");
+}
+
+int ufb_kv_reorder(const ufb_kv_cache* c, const int32_t* slots, const int32_t* parents, int n, int width,
+                   void* stream) {
+    clear_error();
+    if (!check_list(c, slots, n)) return last_code();
+    if (width < 1 || n % width) return err(UFB_EINVAL, "a reorder takes whole groups of streams");
+    if (width > UFB_BEAM_MAX) return err(UFB_ERANGE, "at most " + std::to_string(UFB_BEAM_MAX) + " streams to a group");
+    if (n == 0) return UFB_OK;
+    if (!parents) return err(UFB_EINVAL, "parent list is null");
+    if (n / width * ((c->table_width + 127ll) / 128) > (1 << 30)) return err(UFB_ERANGE, "cache exceeds grid bounds");
+    int* status = current_status();
+    if (!status) return last_code();
+    return done(kv_reorder(*c, slots, parents, n, width, status, static_cast<cudaStream_t>(stream)), "kv reorder");
 }
 
 int ufb_kv_trim(const ufb_kv_cache* c, const int32_t* slots, int n, int window, int sinks, void* stream) {
@@ -286,28 +309,48 @@ int64_t ufb_capture_id(void* stream) {
     return state == cudaStreamCaptureStatusActive ? static_cast<int64_t>(id) : 0;
 }
 
-int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
-                  int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse, int window,
-                  int sinks, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens) {
     clear_error();
-    if (!check_batch(c, layer, slots, offsets, n, max_new, tokens)) return last_code();
-    if (dtype != UFB_F16 && dtype != UFB_BF16) return err(UFB_EINVAL, "attention takes float16 or bfloat16 queries");
-    if (window < 0 || sinks < 0) return err(UFB_EINVAL, "window and sinks must not be negative");
-    if (!std::isfinite(scale)) return err(UFB_EINVAL, "softmax scale must be finite");
-    if (n == 0 || max_new == 0) return UFB_OK;
-    if (!check_heads(q, 0, c->head_dim, dtype, "queries") ||
-        !check_output(out, q->heads, tokens, c->head_dim, dtype, "attention output"))
+    if (groups < 0 || n < 0 || tokens < 0 || tokens > INT32_MAX) return err(UFB_EINVAL, "invalid counts");
+    return 4ll * groups + n + tokens;
+}
+
+int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, int max_new,
+                 int64_t tokens, const ufb_kv_groups* groups, void* stream) {
+    clear_error();
+    if (!check_batch(c, 0, slots, offsets, n, max_new, tokens) || !check_groups(groups, n, max_new, tokens))
         return last_code();
-    if (q->heads % c->heads) return err(UFB_EINVAL, "query heads must be a multiple of the cache's heads");
-    if (q->heads / c->heads > 128) return err(UFB_ERANGE, "more than 128 query heads to a key head");
-    const int sms = current_sms();
-    if (sms <= 0) return last_code();
-    const int64_t need = kv_attend_workspace_bytes(sms);
-    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)
-        return err(UFB_EINVAL, "attention needs " + std::to_string(need) + " bytes of 256-byte aligned workspace");
+    if (groups->groups == 0) return UFB_OK;
     int* status = current_status();
     if (!status) return last_code();
-    AttendArgs a{};
+    const KvBatch b{slots, offsets, n, max_new, tokens};
+    return done(kv_share(*c, b, *groups, status, static_cast<cudaStream_t>(stream)), "kv share");
+}
+
+// Checks of ufb_kv_attend and ufb_kv_attend_groups, and the kernels' arguments; nothing
+// to do: go is left false.
+static bool attend_args(AttendArgs& a, bool& go, int& sms, const ufb_kv_cache* c, int layer, const int32_t* slots,
+                        const int32_t* offsets, int n, int max_new, int64_t tokens, int dtype, const ufb_heads* q,
+                        const ufb_heads* out, float* lse, int window, int sinks, int causal, float scale,
+                        void* workspace, int64_t workspace_bytes) {
+    go = false;
+    if (!check_batch(c, layer, slots, offsets, n, max_new, tokens)) return false;
+    if (dtype != UFB_F16 && dtype != UFB_BF16) return fail(UFB_EINVAL, "attention takes float16 or bfloat16 queries");
+    if (window < 0 || sinks < 0) return fail(UFB_EINVAL, "window and sinks must not be negative");
+    if (!std::isfinite(scale)) return fail(UFB_EINVAL, "softmax scale must be finite");
+    if (n == 0 || max_new == 0) return true;
+    if (!check_heads(q, 0, c->head_dim, dtype, "queries") ||
+        !check_output(out, q->heads, tokens, c->head_dim, dtype, "attention output"))
+        return false;
+    if (q->heads % c->heads) return fail(UFB_EINVAL, "query heads must be a multiple of the cache's heads");
+    if (q->heads / c->heads > 128) return fail(UFB_ERANGE, "more than 128 query heads to a key head");
+    sms = current_sms();
+    if (sms <= 0) return false;
+    const int64_t need = kv_attend_workspace_bytes(sms);
+    if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)
+        return fail(UFB_EINVAL, "attention needs " + std::to_string(need) + " bytes of 256-byte aligned workspace");
+    int* status = current_status();
+    if (!status) return false;
     const int64_t page_heads = 2ll * c->heads * c->pages;
     a.kv = c->kv + layer * page_heads * c->page_tokens * c->head_dim;
     a.scale = c->scale + layer * page_heads;
@@ -336,7 +379,54 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
     a.lse = lse;
     a.status = status;
     a.workspace = workspace;
+    go = true;
+    return true;
+}
+
+int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n, int max_new,
+                  int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse, int window,
+                  int sinks, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+    clear_error();
+    AttendArgs a{};
+    bool go;
+    int sms;
+    if (!attend_args(a, go, sms, c, layer, slots, offsets, n, max_new, tokens, dtype, q, out, lse, window, sinks, causal,
+                     scale, workspace, workspace_bytes))
+        return last_code();
+    if (!go) return UFB_OK;
     return done(kv_attend(a, dtype, sms, static_cast<cudaStream_t>(stream)), "kv attend");
+}
+
+int ufb_kv_attend_groups(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n,
+                         int max_new, int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse,
+                         int window, int sinks, int causal, float scale, const ufb_kv_groups* groups, float* parts,
+                         void* workspace, int64_t workspace_bytes, void* stream) {
+    clear_error();
+    AttendArgs own{};
+    bool go;
+    int sms;
+    if (!attend_args(own, go, sms, c, layer, slots, offsets, n, max_new, tokens, dtype, q, out, lse, window, sinks,
+                     causal, scale, workspace, workspace_bytes) ||
+        !check_groups(groups, n, max_new, tokens))
+        return last_code();
+    if (!go || groups->groups == 0) return UFB_OK;
+    if (!parts || reinterpret_cast<uintptr_t>(parts) % 16) return err(UFB_EINVAL, "16-byte aligned parts required");
+    const KvGroupState state = kv_group_state(*groups, n);
+    own.starts = state.starts;
+    own.positions = state.positions;
+    own.part_out = parts;
+    own.part_lse = parts + tokens * q->heads * c->head_dim;
+    // the groups as streams; their queries stand behind all keys in common
+    AttendArgs common = own;
+    common.slots = state.slot;
+    common.offsets = groups->offsets;
+    common.n = groups->groups;
+    common.max_new = groups->max_tokens;
+    common.starts = state.shared;
+    common.lows = state.low;
+    common.highs = state.high;
+    common.causal = 1;
+    return done(kv_attend_groups(own, common, dtype, sms, static_cast<cudaStream_t>(stream)), "kv attend groups");
 }
 
 }  // extern "C"

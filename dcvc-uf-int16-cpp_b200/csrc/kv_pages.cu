@@ -1,4 +1,5 @@
-// Pages of the 8-bit cache: extend, release, fork, trim, compact.
+// Pages of the 8-bit cache: extend, release, fork, reorder, trim, compact, and what
+// groups of streams have in common.
 //
 // Tables, lengths and reference counts live on the device and the host never
 // waits for them.  What has to be decided in order (which free page goes to
@@ -11,16 +12,21 @@
 
 #include "capi_util.h"
 
+#include <climits>
+
 namespace ufb {
 
 namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
+constexpr int kApplyThreads = 256;
+constexpr int kColumns = 128;   // table columns of a block of reorder_apply_kernel
 
-// Scratch layout (int32): [0] moves to make, [16, 16 + pages) free pages found,
-// in order; then [pages) moves' sources / [pages) token counts; then one offset
-// per request (slots).  Behind it lie the marks of refused streams (kv_refused).
+// Scratch layout (int32): [0] moves to make, [1] whether a reorder goes ahead, [16, 16 +
+// pages) free pages found, in order; then [pages) moves' sources / [pages) token counts;
+// then one offset per request (slots).  Behind it lie the marks of refused streams
+// (kv_refused) and the entries of last pages (kv_last_entry).
 struct Work {
     int32_t* moves;
     int32_t* found;
@@ -296,10 +302,36 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 // head.  Else whole pages, and one more row of blocks (y = layers * 2) takes the
 // moved pages' new ids (rest[page]) into the tables.
 template <bool PARTIAL>
+__device__ __forceinline__ void move_page(const ufb_kv_cache& c, const Work& w, int m, int layer, int side) {
+    const int head_vecs = c.page_tokens * c.head_dim / 16;
+    const long long from = ((static_cast<long long>(layer) * c.pages + w.source[m]) * 2 + side) * c.heads;
+    const long long to = ((static_cast<long long>(layer) * c.pages + w.found[m]) * 2 + side) * c.heads;
+    const uint4* in = reinterpret_cast<const uint4*>(c.kv) + from * head_vecs;
+    uint4* out = reinterpret_cast<uint4*>(c.kv) + to * head_vecs;
+    const int vecs = PARTIAL ? w.rest[m] * c.head_dim / 16 : head_vecs;
+    const int total = vecs * c.heads;
+    constexpr int kBatch = 8;
+    for (int base = threadIdx.x; base < total; base += 256 * kBatch) {
+        uint4 v[kBatch];
+        int at[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int i = base + j * 256;
+            const int head = PARTIAL ? i / vecs : 0;
+            at[j] = PARTIAL ? head * head_vecs + i - head * vecs : i;
+            if (i < total) v[j] = __ldcs(in + at[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (base + j * 256 < total) out[at[j]] = v[j];
+    }
+    for (int h = threadIdx.x; h < c.heads; h += 256) c.scale[to + h] = c.scale[from + h];
+}
+
+template <bool PARTIAL>
 __global__ void __launch_bounds__(256) move_kernel(const ufb_kv_cache c) {
     const Work w = work_of(c);
     const int side = blockIdx.y & 1, layer = blockIdx.y >> 1;
-    const int head_vecs = c.page_tokens * c.head_dim / 16;
     wait_for_previous();
     const int moves = *w.moves;
     if (!PARTIAL && layer == c.layers) {
@@ -313,30 +345,222 @@ __global__ void __launch_bounds__(256) move_kernel(const ufb_kv_cache c) {
         }
         return;
     }
-    for (int m = blockIdx.x; m < moves; m += gridDim.x) {
-        const long long from = ((static_cast<long long>(layer) * c.pages + w.source[m]) * 2 + side) * c.heads;
-        const long long to = ((static_cast<long long>(layer) * c.pages + w.found[m]) * 2 + side) * c.heads;
-        const uint4* in = reinterpret_cast<const uint4*>(c.kv) + from * head_vecs;
-        uint4* out = reinterpret_cast<uint4*>(c.kv) + to * head_vecs;
-        const int vecs = PARTIAL ? w.rest[m] * c.head_dim / 16 : head_vecs;
-        const int total = vecs * c.heads;
-        constexpr int kBatch = 8;
-        for (int base = threadIdx.x; base < total; base += 256 * kBatch) {
-            uint4 v[kBatch];
-            int at[kBatch];
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j) {
-                const int i = base + j * 256;
-                const int head = PARTIAL ? i / vecs : 0;
-                at[j] = PARTIAL ? head * head_vecs + i - head * vecs : i;
-                if (i < total) v[j] = __ldcs(in + at[j]);
+    for (int m = blockIdx.x; m < moves; m += gridDim.x) move_page<PARTIAL>(c, w, m, layer, side);
+}
+
+// ---- reorder: stream i of the list goes on from what stream parent(i) held.
+//
+// The decision, by one CTA, writes nothing that it reads: which stream keeps its
+// parent's last page, which get a copy, and the pages for these -- first those that
+// streams without a child leave, so that the pool is looked through only where their
+// number does not suffice.  A second launch takes the rows of a group through shared
+// memory, a column of all its streams to a thread (a row may be read by several and
+// is overwritten itself), and moves the copies' bytes.
+
+// The page of a stream's last, partly filled entry; -1: it has none.
+__device__ __forceinline__ int last_page(const ufb_kv_cache& c, int slot, int length) {
+    const int full = length / c.page_tokens;
+    if (length <= 0 || length % c.page_tokens == 0 || full >= c.table_width) return -1;
+    const int page = c.table[static_cast<long long>(slot) * c.table_width + full];
+    return page < c.pages ? page : -1;
+}
+
+__global__ void __launch_bounds__(kThreads) reorder_kernel(const ufb_kv_cache c, const int32_t* slots,
+                                                           const int32_t* parents, int n, int width, int* status) {
+    __shared__ int warp_sum[kWarps];
+    __shared__ int children[kThreads], first[kThreads], page_of[kThreads], rest_of[kThreads];
+    const Work w = work_of(c);
+    int32_t* last_entry = kv_last_entry(c);
+    if (threadIdx.x == 0) w.moves[0] = w.moves[1] = 0;
+    // whole groups at a time
+    const int tile = kThreads / width * width;
+    int need = 0, left = 0, bad = 0;
+    for (int base = 0; base < n; base += tile) {
+        const int t = threadIdx.x, i = base + t, group = t / width * width;
+        const bool mine = t < tile && i < n;
+        int parent = t, page = -1, rest = 0;
+        children[t] = 0;
+        first[t] = kThreads;
+        __syncthreads();
+        if (mine) {
+            const int p = parents[i], slot = slots[i];
+            if (p < 0 || p >= width || !valid_slot(c, slot)) {
+                bad = 1;
+            } else {
+                parent = group + p;
+                const int length = c.lengths[slot];
+                page = last_page(c, slot, length);
+                rest = length % c.page_tokens;
+                last_entry[i] = page >= 0 ? length / c.page_tokens : -1;
+                atomicAdd(children + parent, 1);
+                // the parent itself comes before its other children
+                atomicMin(first + parent, parent == t ? -1 : t);
             }
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j)
-                if (base + j * 256 < total) out[at[j]] = v[j];
         }
-        for (int h = threadIdx.x; h < c.heads; h += 256) c.scale[to + h] = c.scale[from + h];
+        page_of[t] = page;
+        rest_of[t] = rest;
+        __syncthreads();
+        const bool copy = mine && !bad && page_of[parent] >= 0 && first[parent] != (parent == t ? -1 : t);
+        const bool leaves = mine && !bad && children[t] == 0 && page >= 0 && c.refs[page] == 1;
+        int copies, leavers;
+        const int at = need + block_scan(copy, warp_sum, copies), from = left + block_scan(leaves, warp_sum, leavers);
+        if (mine) w.start[i] = copy ? at : -1;
+        if (copy && at < c.pages) {
+            w.source[at] = page_of[parent];
+            w.rest[at] = rest_of[parent];
+        }
+        if (leaves && from < c.pages) w.found[from] = page;
+        need += copies;
+        left += leavers;
+        __syncthreads();
     }
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) atomicCAS(status, 0, kStatusIndex);
+        return;
+    }
+    if (need > left) {
+        const int more = need - left;
+        if (need > c.pages || find_free(c, more, w.found + left, warp_sum) != more) {
+            if (threadIdx.x == 0) atomicCAS(status, 0, kStatusPages);
+            return;
+        }
+    }
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int at = w.start[i];
+        if (at < 0) continue;
+        const int page = w.found[at];
+        // a page that a stream leaves loses that stream's count with its row
+        c.refs[page] = at < left ? 2 : 1;
+        w.start[i] = page;
+    }
+    if (threadIdx.x == 0) w.moves[0] = need, w.moves[1] = 1;
+}
+
+// Blocks below row_blocks: kColumns columns of one group's rows; the others: copies, by
+// (layer, side).
+__global__ void __launch_bounds__(kApplyThreads) reorder_apply_kernel(const ufb_kv_cache c, const int32_t* slots,
+                                                                      const int32_t* parents, int width, int row_blocks,
+                                                                      int chunks) {
+    extern __shared__ int rows[];   // [width][kColumns]
+    __shared__ int slot[UFB_BEAM_MAX], parent[UFB_BEAM_MAX], page[UFB_BEAM_MAX], entry[UFB_BEAM_MAX];
+    __shared__ int children[UFB_BEAM_MAX], length[UFB_BEAM_MAX], refused[UFB_BEAM_MAX];
+    const Work w = work_of(c);
+    wait_for_previous();
+    if (w.moves[1] == 0) return;
+    if (blockIdx.x >= row_blocks) {
+        const int moves = w.moves[0], parts = c.layers * 2;
+        for (long long j = blockIdx.x - row_blocks; j < static_cast<long long>(moves) * parts; j += gridDim.x - row_blocks)
+            move_page<true>(c, w, static_cast<int>(j / parts), static_cast<int>(j % parts) >> 1, static_cast<int>(j & 1));
+        return;
+    }
+    const int group = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    if (threadIdx.x < width) {
+        const int i = group * width + threadIdx.x;
+        slot[threadIdx.x] = slots[i];
+        parent[threadIdx.x] = parents[i];
+        page[threadIdx.x] = w.start[i];
+        entry[threadIdx.x] = kv_last_entry(c)[i];
+        children[threadIdx.x] = 0;
+        if (chunk == 0) {
+            length[threadIdx.x] = c.lengths[slots[i]];
+            refused[threadIdx.x] = kv_refused(c)[slots[i]];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < width) {
+        atomicAdd(children + parent[threadIdx.x], 1);
+        if (chunk == 0) {
+            c.lengths[slot[threadIdx.x]] = length[parent[threadIdx.x]];
+            kv_refused(c)[slot[threadIdx.x]] = refused[parent[threadIdx.x]];
+        }
+    }
+    // half of the block's threads have the even rows, the other half the odd ones
+    const int column = threadIdx.x % kColumns, half = threadIdx.x / kColumns, e = chunk * kColumns + column;
+    const bool there = e < c.table_width;
+    for (int r = half; there && r < width; r += kApplyThreads / kColumns)
+        rows[r * kColumns + column] = c.table[static_cast<long long>(slot[r]) * c.table_width + e];
+    __syncthreads();
+    if (!there) return;
+    bool same = true;   // one page in all rows: nothing changes, nor does its count
+    for (int r = 1; r < width; ++r) same &= rows[r * kColumns + column] == rows[column];
+    for (int r = 0; r < width; ++r) same &= entry[r] != e;
+    if (same) return;
+    for (int r = half; r < width; r += kApplyThreads / kColumns) {
+        const int held = rows[r * kColumns + column], p = parent[r];
+        // of a last page that is partly filled one child at most goes on with it
+        const int more = (entry[r] == e ? min(children[r], 1) : children[r]) - 1;
+        if (more != 0 && held >= 0 && held < c.pages) atomicAdd(c.refs + held, more);
+        const int now = page[r] >= 0 && entry[p] == e ? page[r] : rows[p * kColumns + column];
+        if (now != held) c.table[static_cast<long long>(slot[r]) * c.table_width + e] = now;
+    }
+}
+
+// What the streams of group blockIdx.x have in common: the leading entries that are equal
+// in all their tables, inside of every one's earlier tokens.  Streams that bring no tokens,
+// or whose extend was refused, do not count.
+__global__ void __launch_bounds__(256) share_kernel(const ufb_kv_cache c, const KvBatch b, const ufb_kv_groups g,
+                                                    const KvGroupState out, int* status) {
+    __shared__ int width, lowest, highest, members, chosen, least;
+    const int group = blockIdx.x, first = max(g.first[group], 0), end = min(g.first[group + 1], b.n);
+    if (threadIdx.x == 0) width = c.table_width, lowest = INT_MAX, highest = -1, members = 0, chosen = INT_MAX, least = 0;
+    __syncthreads();
+    for (int i = first + threadIdx.x; i < end; i += 256) {
+        const int slot = b.slots[i], o0 = b.offsets[i], o1 = b.offsets[i + 1];
+        if (!valid_slot(c, slot) || o0 < 0 || o1 < o0 || o1 > b.tokens || o1 - o0 > b.max_new) {
+            atomicCAS(status, 0, kStatusIndex);
+            continue;
+        }
+        const bool refused = kv_refused(c)[slot] != 0;
+        const int start = c.lengths[slot] - (o1 - o0);
+        if (!refused && o1 > o0 && start >= 0) {
+            atomicAdd(&members, 1);
+            atomicMin(&chosen, i);
+            atomicMin(&width, start / c.page_tokens);
+            atomicMin(&lowest, start);
+            atomicMax(&highest, c.lengths[slot] - 1);
+        } else if (o1 > o0) {
+            atomicMin(&lowest, -1);
+        }
+    }
+    // positions: a warp to a stream
+    for (int i = first + (threadIdx.x >> 5); i < end; i += 8) {
+        const int slot = b.slots[i], o0 = b.offsets[i], o1 = b.offsets[i + 1];
+        const bool ok = valid_slot(c, slot) && o0 >= 0 && o1 >= o0 && o1 <= b.tokens && o1 - o0 <= b.max_new;
+        const int start = ok ? c.lengths[slot] - (o1 - o0) : 0;
+        const bool none = ok && (start < 0 || kv_refused(c)[slot]);
+        for (int t = max(o0, 0) + (threadIdx.x & 31); t < o1 && t < b.tokens; t += 32)
+            out.positions[t] = !ok ? -2 : none ? -1 : start + t - o0;
+    }
+    __syncthreads();
+    int common = 0;
+    if (members > 1) {
+        const int most = width;
+        const int32_t* row = c.table + static_cast<long long>(b.slots[chosen]) * c.table_width;
+        bool all = true;
+        for (int e0 = 0; e0 < most && all; e0 += 256) {
+            const int e = e0 + threadIdx.x;
+            bool same = true;
+            if (e < most) {
+                const int page = row[e];
+                for (int i = chosen + 1; i < end && same; ++i) {
+                    const int slot = b.slots[i];
+                    if (!valid_slot(c, slot) || kv_refused(c)[slot] || b.offsets[i + 1] <= b.offsets[i]) continue;
+                    same = c.table[static_cast<long long>(slot) * c.table_width + e] == page;
+                }
+                if (!same) atomicMin(&width, e);
+            }
+            all = __syncthreads_and(same);
+        }
+        common = width;
+    }
+    const int shared = common * c.page_tokens;
+    if (threadIdx.x == 0) {
+        out.shared[group] = shared;
+        out.slot[group] = members ? b.slots[chosen] : first < end ? b.slots[first] : -1;
+        out.low[group] = lowest == INT_MAX ? -1 : lowest;
+        out.high[group] = highest;
+    }
+    for (int i = first + threadIdx.x; i < end; i += 256) out.starts[i] = shared;
 }
 
 template <bool PARTIAL>
@@ -378,6 +602,32 @@ cudaError_t kv_fork(const ufb_kv_cache& c, const int32_t* src, const int32_t* ds
     fork_kernel<<<1, kThreads, 0, s>>>(c, src, dst, n, status);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? move<true>(c, n, s) : e;
+}
+
+cudaError_t kv_reorder(const ufb_kv_cache& c, const int32_t* slots, const int32_t* parents, int n, int width,
+                       int* status, cudaStream_t s) {
+    reorder_kernel<<<1, kThreads, 0, s>>>(c, slots, parents, n, width, status);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    const int chunks = (c.table_width + kColumns - 1) / kColumns, row_blocks = n / width * chunks;
+    // at most a copy for each stream but one of a group; blocks take further ones in turn
+    const long long copies = static_cast<long long>(n - n / width) * c.layers * 2;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(row_blocks + static_cast<unsigned>(copies < 2368 ? copies : 2368));
+    config.blockDim = dim3(kApplyThreads);
+    config.dynamicSmemBytes = width * kColumns * sizeof(int);
+    config.stream = s;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, reorder_apply_kernel, c, slots, parents, width, row_blocks, chunks);
+}
+
+cudaError_t kv_share(const ufb_kv_cache& c, const KvBatch& b, const ufb_kv_groups& g, int* status, cudaStream_t s) {
+    share_kernel<<<g.groups, 256, 0, s>>>(c, b, g, kv_group_state(g, b.n), status);
+    return cudaGetLastError();
 }
 
 cudaError_t kv_compact(const ufb_kv_cache& c, int*, cudaStream_t s) {

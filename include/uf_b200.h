@@ -442,9 +442,10 @@ int ufb_conv2d_noalloc(const int16_t* x, int n, int ci, int h, int w, const int1
  *   31 too few free pages, or a stream longer than its table row (extend: no
  *      stream was changed; append, attend: the stream's extend was refused, its
  *      tokens are not stored and its queries see no key; fork: the destinations
- *      are left empty)
+ *      are left empty; reorder: nothing was changed)
  *   32 a slot, page or token offset out of range, or a page that is missing
- *      where tokens are to be stored (what it names is skipped)
+ *      where tokens are to be stored (what it names is skipped; reorder, with a
+ *      parent out of range too: nothing was changed)
  *   41..44 a bounded wait of the attention kernel gave up
  *   51 a row of logits holds NaN or +infinity (its beam has no continuations)
  * ------------------------------------------------------------------------- */
@@ -528,6 +529,22 @@ int ufb_kv_release(const ufb_kv_cache* c, const int32_t* slots, int n, void* str
  * shows in all its branches. */
 int ufb_kv_fork(const ufb_kv_cache* c, const int32_t* src, const int32_t* dst, int n, void* stream);
 
+#define UFB_BEAM_MAX 64
+#define UFB_BEAM_COUNT_MAX 64
+
+/* The streams of each group (`width` of the list, one group after another, width at
+ * most UFB_BEAM_MAX) go on, all at once, from what the streams of the group held:
+ * stream slots[g * width + j] from stream slots[g * width + parents[g * width + j]],
+ * parents in [0, width).  Full pages are shared.  A partly filled last page stays
+ * with one of those that go on from its stream, that stream itself if it is among
+ * them, else the first of the list; each other one gets a copy of its tokens, in every
+ * layer, on a page of its own: first the pages that streams leave from which none goes
+ * on (their partly filled last ones, in the order of the list), then the lowest free
+ * ones, in the order of the list.  Streams of one length so never need a free page.
+ * No slot twice.  The streams' tokens are stored in every layer before it. */
+int ufb_kv_reorder(const ufb_kv_cache* c, const int32_t* slots, const int32_t* parents, int n, int width,
+                   void* stream);
+
 /* Drop the pages of the listed streams that no later query sees through a
  * window (ufb_kv_attend) of `window` >= 1 keys and `sinks` first tokens. */
 int ufb_kv_trim(const ufb_kv_cache* c, const int32_t* slots, int n, int window, int sinks, void* stream);
@@ -577,15 +594,42 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
                   int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse, int window,
                   int sinks, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Groups of consecutive streams of a batch that may begin with common pages: the
+ * branches of one stream. */
+typedef struct ufb_kv_groups {
+    const int32_t* first;   /* [groups + 1] first stream of each in the batch; 0 .. n */
+    const int32_t* offsets; /* [groups + 1] their tokens: offsets[first[g]] of the batch */
+    int32_t* state;         /* [ufb_kv_group_ints()] written by ufb_kv_share */
+    int32_t groups;
+    int32_t max_tokens;     /* no less than any group's tokens */
+} ufb_kv_groups;
+
+/* int32 entries of ufb_kv_groups.state. */
+int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens);
+
+/* Find what each group has in common: the leading table entries that are equal in
+ * all its streams, as far as they lie before every stream's new tokens (streams
+ * that bring none, or whose extend was refused, do not count; none in a group of
+ * one).  state[g] are the tokens on them.  Once a step, behind ufb_kv_extend: it holds
+ * until a call changes tables or lengths. */
+int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, int max_new,
+                 int64_t tokens, const ufb_kv_groups* groups, void* stream);
+
+/* ufb_kv_attend, which reads the pages that the streams of a group have in common
+ * (ufb_kv_share) once for all of them: attention over the common keys and over the
+ * stream's own, joined by their sums of exponentials in 32 bits.  parts:
+ * tokens * q heads * (head_dim + 1) floats of scratch, 16-byte aligned. */
+int ufb_kv_attend_groups(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n,
+                         int max_new, int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse,
+                         int window, int sinks, int causal, float scale, const ufb_kv_groups* groups, float* parts,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Workspace of ufb_kv_attend on the current device, in bytes. */
 int64_t ufb_kv_attend_workspace(void);
 
 /* The graph capture that `stream` is in: a number that no other capture has; 0
  * outside of one. */
 int64_t ufb_capture_id(void* stream);
-
-#define UFB_BEAM_MAX 64
-#define UFB_BEAM_COUNT_MAX 64
 
 /* The best continuations of the beams of each stream, a step of a search over
  * sequences.  Beam k of stream b has the score s = scores[b][k] (the sum of its
