@@ -11,8 +11,11 @@ import ctypes as C
 
 import torch
 
-from . import UfbError, library
+from . import UfbError, _check, library
 from .attention import _DTYPES, _launch
+
+
+_rooms = {}   # bytes of scratch by device and sizes
 
 
 def _entry():
@@ -20,7 +23,9 @@ def _entry():
     fn = L.ufb_beam_select
     if fn.argtypes is None:
         vp, ci, i64 = C.c_void_p, C.c_int, C.c_int64
-        fn.argtypes = [vp, ci, i64, i64, vp, vp, ci, ci, ci, ci, ci, vp, vp, vp, vp]
+        fn.argtypes = [vp, ci, i64, i64, vp, vp, ci, ci, ci, ci, ci, vp, vp, vp, vp, i64, vp]
+        L.ufb_beam_select_workspace.restype = i64
+        L.ufb_beam_select_workspace.argtypes = [ci, ci, ci, ci, ci]
     return fn
 
 
@@ -56,10 +61,21 @@ def beam_select(logits, scores, count, finished=None, pad=0):
         scores = scores.contiguous()
     if finished is not None and not finished.is_contiguous():
         finished = finished.contiguous()
+    fn = _entry()
+    dtype = _DTYPES[logits.dtype]
+    key = (device.index, dtype, streams, beams, vocab, count)
+    room = _rooms.get(key)
+    if room is None:
+        with torch.cuda.device(device):
+            room = library().ufb_beam_select_workspace(dtype, streams, beams, vocab, count)
+        if room < 0:
+            _check(room)
+        _rooms[key] = room
     out = torch.empty((3, streams, count), dtype=torch.int32, device=device)
+    work = torch.empty(room, dtype=torch.uint8, device=device)
     at, step = out.data_ptr(), streams * count * 4
-    _launch(device, _entry(), logits.data_ptr(), _DTYPES[logits.dtype], ss, bs, scores.data_ptr(),
+    _launch(device, fn, logits.data_ptr(), dtype, ss, bs, scores.data_ptr(),
             None if finished is None else finished.data_ptr(), streams, beams, vocab, count, pad, at, at + step,
-            at + 2 * step)
+            at + 2 * step, work.data_ptr(), room)
     best, parents, tokens = out.unbind(0)
     return best.view(torch.float32), parents, tokens

@@ -24,7 +24,9 @@ struct BeamSelectArgs {
     int32_t* parents;
     int32_t* tokens;
     int* status;
+    void* workspace;                    // beam_select_workspace_bytes
 };
+int64_t beam_select_workspace_bytes(int streams, int beams, int vocab, int count, int dtype, int sms);
 cudaError_t beam_select(const BeamSelectArgs& a, int dtype, int sms, cudaStream_t s);
 
 }  // namespace ufb

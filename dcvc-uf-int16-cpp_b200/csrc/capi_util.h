@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -34,6 +35,21 @@ bool check_conv(const int16_t* x, int n, int ci, int h, int w, const int16_t* we
                 int bias_bits, int sh, int sw, int ph, int pw, int groups, const int16_t* out, int& oh, int& ow);
 
 inline int round_up(int v, int m) { return (v + m - 1) / m * m; }
+
+// Lets `kernel` have `bytes` of dynamic shared memory.  That is per function and
+// device: `done` holds a bit for each device where it has been set, so that a call
+// costs no more than asking for the device.
+template <class Kernel>
+cudaError_t allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // Scratch memory allocated and released in stream order (cudaMallocAsync /
 // cudaFreeAsync), so concurrent calls on different streams never share it.

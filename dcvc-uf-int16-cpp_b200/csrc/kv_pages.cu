@@ -500,9 +500,9 @@ __global__ void __launch_bounds__(kApplyThreads) reorder_apply_kernel(const ufb_
 // or whose extend was refused, do not count.
 __global__ void __launch_bounds__(256) share_kernel(const ufb_kv_cache c, const KvBatch b, const ufb_kv_groups g,
                                                     const KvGroupState out, int* status) {
-    __shared__ int width, lowest, highest, members, chosen, least;
+    __shared__ int width, lowest, highest, members, chosen;
     const int group = blockIdx.x, first = max(g.first[group], 0), end = min(g.first[group + 1], b.n);
-    if (threadIdx.x == 0) width = c.table_width, lowest = INT_MAX, highest = -1, members = 0, chosen = INT_MAX, least = 0;
+    if (threadIdx.x == 0) width = c.table_width, lowest = INT_MAX, highest = -1, members = 0, chosen = INT_MAX;
     __syncthreads();
     for (int i = first + threadIdx.x; i < end; i += 256) {
         const int slot = b.slots[i], o0 = b.offsets[i], o1 = b.offsets[i + 1];

@@ -531,6 +531,7 @@ int ufb_kv_fork(const ufb_kv_cache* c, const int32_t* src, const int32_t* dst, i
 
 #define UFB_BEAM_MAX 64
 #define UFB_BEAM_COUNT_MAX 64
+#define UFB_BEAM_VOCAB_MAX (1 << 25)
 
 /* The streams of each group (`width` of the list, one group after another, width at
  * most UFB_BEAM_MAX) go on, all at once, from what the streams of the group held:
@@ -637,7 +638,7 @@ int64_t ufb_capture_id(void* stream);
  * b * stream_stride + k * beam_stride, vocab of them, contiguous.  Its continuation
  * by token v has the score
  *   f32(s + (l[v] - ln sum_u exp l[u]))
- * rounded once, from values good to 2^-28.  A beam marked in finished (NULL, or
+ * rounded once, from values good to 2^-27.  A beam marked in finished (NULL, or
  * [streams][beams] bytes) has one continuation, token pad with score s, and its
  * logits are not read; neither are those of a beam whose score is -infinity or NaN,
  * which has none.  Logits of -infinity are forbidden tokens; a row that holds NaN or
@@ -645,10 +646,16 @@ int64_t ufb_capture_id(void* stream);
  *   out_scores, parents, tokens [streams][count]: the best, falling scores; equal
  * ones by the lower beam, of one beam by the larger logit, then the lower token.
  * Scores of -infinity are no continuations: places i for which there are none left get
- * score -infinity, parent min(i, beams - 1), token 0. */
+ * score -infinity, parent min(i, beams - 1), token 0.
+ * workspace: ufb_beam_select_workspace() bytes, 16-byte aligned; calls that may overlap
+ * need one each. */
 int ufb_beam_select(const void* logits, int dtype, int64_t stream_stride, int64_t beam_stride, const float* scores,
                     const uint8_t* finished, int streams, int beams, int vocab, int count, int pad,
-                    float* out_scores, int32_t* parents, int32_t* tokens, void* stream);
+                    float* out_scores, int32_t* parents, int32_t* tokens, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/* Workspace of ufb_beam_select on the current device, in bytes. */
+int64_t ufb_beam_select_workspace(int dtype, int streams, int beams, int vocab, int count);
 
 /* Measurement utility (no reference counterpart): launches `ctas` CTAs that
  * each issue `iters` x 4 dense tcgen05 kind::i8 M=128 N=256 K=32 MMAs from

@@ -15,7 +15,7 @@ def fn(ufb):
 
 
 BASE = dict(logits=1 << 20, dtype=2, stream_stride=400, beam_stride=100, scores=4096, finished=None, streams=3, beams=4,
-            vocab=100, count=4, pad=0, out_scores=8192, parents=8192, tokens=8192)
+            vocab=100, count=4, pad=0, out_scores=8192, parents=8192, tokens=8192, workspace=1 << 22, room=1 << 30)
 
 
 def call(fn, **over):
@@ -30,8 +30,12 @@ def test_refusals(ufb, fn):
                  dict(logits=(1 << 20) + 1), dict(logits=(1 << 20) + 2, dtype=0)):
         assert call(fn, **over) == EINVAL, over
         assert L.ufb_last_error()
-    for over in (dict(beams=65), dict(count=65), dict(vocab=(1 << 30) + 1), dict(streams=(1 << 24) + 1)):
+    for over in (dict(beams=65), dict(count=65), dict(vocab=(1 << 25) + 1), dict(streams=(1 << 24) + 1)):
         assert call(fn, **over) == ERANGE, over
+    size = dict(dtype=2, streams=3, beams=4, vocab=100, count=4)
+    for over, code in ((dict(dtype=3), EINVAL), (dict(streams=-1), EINVAL), (dict(count=0), EINVAL), (dict(beams=65), ERANGE)):
+        assert L.ufb_beam_select_workspace(*{**size, **over}.values()) == code, over
+    assert L.ufb_beam_select_workspace(*{**size, "streams": 0}.values()) == 0
     assert call(fn, streams=0, logits=None, scores=None) == 0  # nothing to do, no CUDA call
 
 
