@@ -62,7 +62,7 @@ def _lib():
     L.ufb_kv_group_ints.argtypes = [ci, ci, i64]
     L.ufb_kv_share.argtypes = [cache, vp, vp, ci, ci, i64, vp, vp]
     L.ufb_kv_attend_groups.argtypes = [cache, ci, vp, vp, ci, ci, i64, ci, heads, heads, vp, ci, ci, ci, C.c_float, vp,
-                                       vp, vp, i64, vp]
+                                       vp, i64, vp]
     L.ufb_kv_attend.argtypes = [cache, ci, vp, vp, ci, ci, i64, ci, heads, heads, vp, ci, ci, ci, C.c_float, vp, i64, vp]
     L._attention_ready = True
     return L
@@ -537,7 +537,7 @@ class KVCache:
 
         With groups (group_plan of this plan, after share has seen the cache as it is)
         the pages that a group's streams begin with in common are read once for all of
-        them, and its result is joined with that over each stream's own keys, in 32 bits."""
+        them: made for branches that go on by few tokens of their own."""
         self._own(plan)
         _check_ints(layer, window, sinks)
         device = self.device
@@ -553,11 +553,10 @@ class KVCache:
                 raise UfbError(-1, "groups of this plan are required")
             if groups._at != self._changes:
                 raise UfbError(-1, "share has not seen the cache since its streams changed: call it once a step")
-            parts = torch.empty(tokens * heads * (dim + 1), dtype=torch.float32, device=device)
             _launch(device, self._attend_groups, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new,
                     tokens, code, _heads(qa, qts, qhs, heads), _heads(out.data_ptr(), heads * dim, dim, heads),
                     None if l is None else l.data_ptr(), window, sinks, 1 if causal else 0,
-                    self._default_scale if scale is None else scale, groups._ref, parts.data_ptr(), w[0], w[1])
+                    self._default_scale if scale is None else scale, groups._ref, w[0], w[1])
             return (out, l) if lse else out
         _launch(device, self._attend, self._ref, layer, plan._slots, plan._offsets, plan.n, plan.max_new, tokens, code,
                 _heads(qa, qts, qhs, heads), _heads(out.data_ptr(), heads * dim, dim, heads),

@@ -79,35 +79,36 @@ struct AttendArgs {
     float* lse;
     int* status;
     void* workspace;
-    // attention in two parts (kv_attend.cuh: kOwn, kCommon)
-    const int32_t* starts;           // [n] tokens of each stream that its group has in common
-    const int32_t* lows;             // [n] first and last position of a group's new tokens
-    const int32_t* highs;
-    const int32_t* positions;        // [tokens]
-    float* part_out;                 // [tokens][query heads][head_dim] of the streams' own keys
-    float* part_lse;                 // [tokens][query heads], in base 2
 };
 cudaError_t kv_attend(const AttendArgs& a, int dtype, int sms, cudaStream_t s);
 
 // What kv_share leaves of the groups of a batch (ufb_kv_groups.state).
 struct KvGroupState {
-    int32_t *shared, *slot, *low, *high;   // [groups] tokens in common, a stream that has them, positions
-    int32_t* starts;                       // [n]
-    int32_t* positions;                    // [tokens]; -1: sees no key, -2: not to be written
+    int32_t *shared, *slot, *low, *high;   // [groups] tokens in common, a stream that has them, least and largest position
+    int32_t* tiles;                        // [n] tiles of own keys of the group's streams up to this one
+    int32_t* positions;                    // [tokens]; kNotWritten: its results are left alone
+    int32_t* stream;                       // [tokens] number of its stream in the batch
 };
-inline KvGroupState kv_group_state(const ufb_kv_groups& g, int n) {
+constexpr int kNotWritten = INT32_MIN;
+constexpr int kGroupTileKeys = 128;        // keys of a tile of kv_attend_groups
+struct GroupArgs {
+    const int32_t *first, *offsets;        // [groups + 1] streams, tokens
+    int groups, max_tokens;
+    KvGroupState state;
+};
+inline KvGroupState kv_group_state(const ufb_kv_groups& g, int n, long long tokens) {
     KvGroupState s;
     s.shared = g.state;
     s.slot = s.shared + g.groups;
     s.low = s.slot + g.groups;
     s.high = s.low + g.groups;
-    s.starts = s.high + g.groups;
-    s.positions = s.starts + n;
+    s.tiles = s.high + g.groups;
+    s.positions = s.tiles + n;
+    s.stream = s.positions + tokens;
     return s;
 }
 cudaError_t kv_share(const ufb_kv_cache& c, const KvBatch& b, const ufb_kv_groups& g, int* status, cudaStream_t s);
-// own: attention of every stream over its own keys; common: of the groups over the keys in common
-cudaError_t kv_attend_groups(const AttendArgs& own, const AttendArgs& common, int dtype, int sms, cudaStream_t s);
+cudaError_t kv_attend_groups(const AttendArgs& a, const GroupArgs& g, int dtype, int sms, cudaStream_t s);
 int64_t kv_attend_workspace_bytes(int sms);
 
 }  // namespace ufb

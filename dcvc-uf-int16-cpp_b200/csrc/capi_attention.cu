@@ -312,7 +312,7 @@ int64_t ufb_capture_id(void* stream) {
 int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens) {
     clear_error();
     if (groups < 0 || n < 0 || tokens < 0 || tokens > INT32_MAX) return err(UFB_EINVAL, "invalid counts");
-    return 4ll * groups + n + tokens;
+    return 4ll * groups + n + 2 * tokens;
 }
 
 int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, int max_new,
@@ -399,34 +399,19 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
 
 int ufb_kv_attend_groups(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n,
                          int max_new, int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse,
-                         int window, int sinks, int causal, float scale, const ufb_kv_groups* groups, float* parts,
+                         int window, int sinks, int causal, float scale, const ufb_kv_groups* groups,
                          void* workspace, int64_t workspace_bytes, void* stream) {
     clear_error();
-    AttendArgs own{};
+    AttendArgs a{};
     bool go;
     int sms;
-    if (!attend_args(own, go, sms, c, layer, slots, offsets, n, max_new, tokens, dtype, q, out, lse, window, sinks,
+    if (!attend_args(a, go, sms, c, layer, slots, offsets, n, max_new, tokens, dtype, q, out, lse, window, sinks,
                      causal, scale, workspace, workspace_bytes) ||
         !check_groups(groups, n, max_new, tokens))
         return last_code();
     if (!go || groups->groups == 0) return UFB_OK;
-    if (!parts || reinterpret_cast<uintptr_t>(parts) % 16) return err(UFB_EINVAL, "16-byte aligned parts required");
-    const KvGroupState state = kv_group_state(*groups, n);
-    own.starts = state.starts;
-    own.positions = state.positions;
-    own.part_out = parts;
-    own.part_lse = parts + tokens * q->heads * c->head_dim;
-    // the groups as streams; their queries stand behind all keys in common
-    AttendArgs common = own;
-    common.slots = state.slot;
-    common.offsets = groups->offsets;
-    common.n = groups->groups;
-    common.max_new = groups->max_tokens;
-    common.starts = state.shared;
-    common.lows = state.low;
-    common.highs = state.high;
-    common.causal = 1;
-    return done(kv_attend_groups(own, common, dtype, sms, static_cast<cudaStream_t>(stream)), "kv attend groups");
+    const GroupArgs g{groups->first, groups->offsets, groups->groups, groups->max_tokens, kv_group_state(*groups, n, tokens)};
+    return done(kv_attend_groups(a, g, dtype, sms, static_cast<cudaStream_t>(stream)), "kv attend groups");
 }
 
 }  // extern "C"

@@ -46,14 +46,7 @@ cudaError_t kv_attend(const AttendArgs& a, int dtype, int sms, cudaStream_t s) {
     // 16000 889 [519].  The stream with the most rows decides for the whole call: 63
     // streams of one token beside one of 32, 16000 keys each, take 500 us together, 184 and
     // 41 us in calls of their own.
-    return rows <= 32 ? attend_few(a, kAll, dtype, sms, s) : attend_many(a, kAll, dtype, sms, s);
-}
-
-cudaError_t kv_attend_groups(const AttendArgs& own, const AttendArgs& common, int dtype, int sms, cudaStream_t s) {
-    auto few = [](const AttendArgs& a) { return static_cast<long long>(a.max_new) * a.group <= 32; };
-    const cudaError_t e = few(own) ? attend_few(own, kOwn, dtype, sms, s) : attend_many(own, kOwn, dtype, sms, s);
-    if (e != cudaSuccess) return e;
-    return few(common) ? attend_few(common, kCommon, dtype, sms, s) : attend_many(common, kCommon, dtype, sms, s);
+    return rows <= 32 ? attend_few(a, dtype, sms, s) : attend_many(a, dtype, sms, s);
 }
 
 }  // namespace ufb

@@ -19,15 +19,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <atomic>
-
 namespace ufb {
-
-// What a launch covers: a call's streams, all their keys; or, of a call whose streams
-// come in groups that begin with common pages, first the streams' own keys (kOwn: the
-// results go to 32-bit parts), then for each group, as one stream with all its tokens,
-// the common keys (kCommon: joined with the parts).
-constexpr int kAll = 0, kOwn = 1, kCommon = 2;
 
 constexpr int kAttendMaxCtas = 160;     // CTAs of a launch at most (scratch is sized by the SMs)
 constexpr int kAttendManyRows = 256;    // rows of the widest tile
@@ -48,21 +40,16 @@ struct KeyRange {
     __device__ __forceinline__ bool touches(int k) const { return k < sink || (k < hi && k + kGroupKeys > low); }
 };
 
-// Positions first..last over `length` keys, those from `from` on.
+// Tokens first..last (of n_new) of a stream of `length` keys.
 template <int BK>
-__device__ __forceinline__ KeyRange key_range(const AttendArgs& a, int length, long long first, long long last,
-                                              int from = 0) {
+__device__ __forceinline__ KeyRange key_range(const AttendArgs& a, int length, int n_new, int first, int last) {
     KeyRange r;
-    const long long top = a.causal ? last + 1 : length;
+    const long long base = static_cast<long long>(length) - n_new;
+    const long long top = a.causal ? base + last + 1 : length;
     r.hi = static_cast<int>(top < 0 ? 0 : (top > length ? length : top));
-    const long long low = a.window ? first - a.window + 1 : 0;
+    const long long low = a.window ? base + first - a.window + 1 : 0;
     r.low = static_cast<int>(low < 0 ? 0 : (low > length ? length : low));
     r.sink = a.window ? min(a.sinks, min(r.low, r.hi)) : 0;
-    if (from > 0) {
-        // first tokens that reach past it are seldom: the keys between are looked at too
-        r.low = r.sink > from ? from : max(r.low, from);
-        r.sink = 0;
-    }
     const int hi_tile = (r.hi + BK - 1) / BK;
     r.low_tile = min(r.low / BK, hi_tile);
     r.sink_tiles = (r.sink + BK - 1) / BK;
@@ -78,12 +65,11 @@ struct RowTile {
     int slot, length, n_new;
     long long token0;       // the stream's first new token
     int row0, rows;         // rows of the tile
-    int low, high;          // kCommon: first and last position of the group's tokens
     KeyRange keys;
 };
 
 // false: the pair (stream, row tile) does not exist.
-template <int BK, int TM, int MODE>
+template <int BK, int TM>
 __device__ __forceinline__ bool row_tile(const AttendArgs& a, int stream, int rt, RowTile& t) {
     const int o0 = a.offsets[stream], o1 = a.offsets[stream + 1];
     t.slot = a.slots[stream];
@@ -94,22 +80,13 @@ __device__ __forceinline__ bool row_tile(const AttendArgs& a, int stream, int rt
     t.rows = min(TM, t.n_new * a.group - t.row0);
     if (!ok && rt == 0) atomicCAS(a.status, 0, kStatusIndex);
     if (t.rows <= 0) return false;
-    if (MODE == kCommon) {
-        t.length = a.starts[stream];
-        t.low = a.lows[stream];
-        t.high = a.highs[stream];
-        t.keys = key_range<BK>(a, t.length, t.low, t.high);
-        return true;
-    }
     t.length = max(a.lengths[t.slot], 0);
     if (a.refused[t.slot]) {
         // its new tokens were not taken in: no position is theirs, they see no key
         t.length = 0;
         if (rt == 0) atomicCAS(a.status, 0, kStatusPages);
     }
-    const long long base = static_cast<long long>(t.length) - t.n_new;
-    t.keys = key_range<BK>(a, t.length, base + t.row0 / a.group, base + (t.row0 + t.rows - 1) / a.group,
-                           MODE == kOwn ? min(a.starts[stream], t.length) : 0);
+    t.keys = key_range<BK>(a, t.length, t.n_new, t.row0 / a.group, (t.row0 + t.rows - 1) / a.group);
     return true;
 }
 
@@ -132,18 +109,12 @@ struct ShareSmem {
     int pair;
 };
 
-// Every thread of the block calls it.  row_tiles: row tiles of a stream at most.
-template <int BK, int TM, int THREADS, int MODE>
-__device__ __forceinline__ Share locate_share(const AttendArgs& a, int row_tiles, int min_share, ShareSmem& sm) {
+// Every thread of the block calls it.  tiles(p): the tiles of pair p.
+template <int THREADS, class Tiles>
+__device__ __forceinline__ Share share_out(int pairs, int min_share, Tiles tiles_of, ShareSmem& sm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int pairs = a.n * row_tiles;
     Share s;
-    RowTile t;
-    auto tiles = [&](int p) -> long long {
-        return p < pairs && row_tile<BK, TM, MODE>(a, p / row_tiles, p % row_tiles, t)
-                   ? static_cast<long long>(t.keys.nt) * a.heads
-                   : 0;
-    };
+    auto tiles = [&](int p) -> long long { return p < pairs ? tiles_of(p) : 0; };
     long long first = 0, sum = 0;
     for (int base = 0; base < pairs; base += THREADS) {
         const long long v = tiles(base + threadIdx.x);
@@ -188,6 +159,18 @@ __device__ __forceinline__ Share locate_share(const AttendArgs& a, int row_tiles
     return s;
 }
 
+// row_tiles: row tiles of a stream at most.
+template <int BK, int TM, int THREADS>
+__device__ __forceinline__ Share locate_share(const AttendArgs& a, int row_tiles, int min_share, ShareSmem& sm) {
+    RowTile t;
+    return share_out<THREADS>(
+        a.n * row_tiles, min_share,
+        [&](int p) -> long long {
+            return row_tile<BK, TM>(a, p / row_tiles, p % row_tiles, t) ? static_cast<long long>(t.keys.nt) * a.heads : 0;
+        },
+        sm);
+}
+
 // The part of one item that a CTA holds.
 struct Piece {
     RowTile t;
@@ -198,7 +181,7 @@ struct Piece {
 };
 
 // Walks the pieces of this CTA's share; every role of a kernel has its own.
-template <int BK, int TM, int MODE>
+template <int BK, int TM>
 struct Walker {
     int row_tiles, pair, pairs;
     long long pos, end, pair_start;
@@ -219,7 +202,7 @@ struct Walker {
         while (true) {
             if (pair >= pairs) return false;
             if (!loaded) {
-                if (!row_tile<BK, TM, MODE>(a, pair / row_tiles, pair % row_tiles, t)) {
+                if (!row_tile<BK, TM>(a, pair / row_tiles, pair % row_tiles, t)) {
                     pair = (pair / row_tiles + 1) * row_tiles;  // no further row tiles of this stream
                     continue;
                 }
@@ -317,61 +300,7 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
 // values, with TMA's 128-byte swizzle.
 bool kv_tensor_map(CUtensorMap& map, const AttendArgs& a, int keys);
 
-// Waits for the kernels before this one (and so theirs).  Launched with programmatic
-// serialization this kernel may begin before they have ended.
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Lets the next kernel begin where it fits.
-__device__ __forceinline__ void begin_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
-// The share of two parts with logarithmic weights x, y (base 2; -infinity: nothing) in
-// their sum, and its logarithm.
-struct Joined {
-    float x, y, lse;
-};
-__device__ __forceinline__ Joined join_parts(float x, float y) {
-    Joined j;
-    const float top = fmaxf(x, y);
-    if (top == -INFINITY) {
-        j.x = j.y = 0.0f;
-        j.lse = x == x && y == y ? -INFINITY : x + y;
-        if (j.lse != -INFINITY) j.x = j.y = j.lse;
-        return j;
-    }
-    const float wx = ex2(x - top), wy = ex2(y - top), sum = wx + wy;
-    j.x = wx / sum;
-    j.y = wy / sum;
-    j.lse = top + log2f(sum);
-    return j;
-}
-
-// Writes four columns from d on of a finished row (token, head): the sums v of weights
-// that add up to `weight`, with the maximum `top` (in base 2) taken out of them.
-template <typename T, int MODE>
-__device__ __forceinline__ void finish_row(const AttendArgs& a, long long token, int head, int d, float4 v, float top,
-                                           float weight) {
-    float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
-    float lse = weight == 0.0f ? -INFINITY : top + log2f(weight);
-    const long long row = token * (a.heads * a.group) + head;
-    if (MODE == kOwn) {
-        *reinterpret_cast<float4*>(a.part_out + row * a.head_dim + d) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-        if (d == 0) a.part_lse[row] = lse;
-        return;
-    }
-    if (MODE == kCommon) {
-        if (a.positions[token] < -1) return;
-        const float4 o = __ldcg(reinterpret_cast<const float4*>(a.part_out + row * a.head_dim + d));
-        const Joined j = join_parts(lse, __ldcg(a.part_lse + row));
-        inv *= j.x;
-        v = make_float4(fmaf(v.x, inv, o.x * j.y), fmaf(v.y, inv, o.y * j.y), fmaf(v.z, inv, o.z * j.y), fmaf(v.w, inv, o.w * j.y));
-        inv = 1.0f;
-        lse = j.lse;
-    }
-    T* to = static_cast<T*>(a.out.data) + token * a.out.token_stride + head * a.out.head_stride + d;
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
-    if (a.lse && d == 0) a.lse[row] = lse * 0.6931471805599453f;
-}
-
-cudaError_t attend_few(const AttendArgs& a, int mode, int dtype, int sms, cudaStream_t s);
-cudaError_t attend_many(const AttendArgs& a, int mode, int dtype, int sms, cudaStream_t s);
+cudaError_t attend_few(const AttendArgs& a, int dtype, int sms, cudaStream_t s);
+cudaError_t attend_many(const AttendArgs& a, int dtype, int sms, cudaStream_t s);
 
 }  // namespace ufb

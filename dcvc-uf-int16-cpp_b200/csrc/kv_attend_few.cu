@@ -111,7 +111,7 @@ __device__ __forceinline__ int value_dim(int n) {
 // The key (of 8) that lane row n of a score tile stands for.
 __device__ __forceinline__ int key_of(int n) { return ((n & 1) << 2) | (n >> 1); }
 
-template <typename T, int D, int NT, int MODE>
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
     few_kernel(const __grid_constant__ CUtensorMap map, const AttendArgs a, int row_tiles, int min_share) {
     constexpr int kWarps = consumers(NT), kRows = 8 * NT, kThreads = 32 * (kWarps + kProducers), kStages = stages(NT);
@@ -128,9 +128,8 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
         fence_mbar_init();
         sm.dead = 0;
     }
-    if (MODE == kOwn) begin_next();
-    const Share share = locate_share<kKeys, kRows, kThreads, MODE>(a, row_tiles, min_share, sm.share);
-    Walker<kKeys, kRows, MODE> walk(a, share, row_tiles);
+    const Share share = locate_share<kKeys, kRows, kThreads>(a, row_tiles, min_share, sm.share);
+    Walker<kKeys, kRows> walk(a, share, row_tiles);
     volatile int* dead = &sm.dead;
 
     if (warp >= kWarps) {
@@ -286,9 +285,7 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
                 q[n][t][1] = pack2(y.x * mul, y.y * mul, __half());
             }
             const float f = unit_inverse(u) * a.scale_log2;
-            // rows behind the last stand where the tile's first does
-            const int at = MODE == kCommon ? (real ? a.positions[p.t.token0 + token] : p.t.low)
-                                           : p.t.length - p.t.n_new + token;
+            const int at = p.t.length - p.t.n_new + token;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int from = (2 * c + r) * 4;
@@ -304,8 +301,8 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
             for (int j = 0; j < kTiles; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.0f;
             m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
         }
-        const int last_pos = MODE == kCommon ? p.t.high : p.t.length - p.t.n_new + (p.t.row0 + p.t.rows - 1) / a.group;
-        const int first_pos = MODE == kCommon ? p.t.low : p.t.length - p.t.n_new + p.t.row0 / a.group;
+        const int last_pos = p.t.length - p.t.n_new + (p.t.row0 + p.t.rows - 1) / a.group;
+        const int first_pos = p.t.length - p.t.n_new + p.t.row0 / a.group;
 
         // steps of 32 keys go round the warps
         const int steps_before = it * (kKeys / kWarpKeys);
@@ -519,12 +516,15 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
         consumers_sync<kWarps>();
         const bool whole = p.whole();
         const int part = 2 * blockIdx.x + (p.first > 0 ? 0 : 1);
-        // the parts of the streams' own keys are there, and the scratch is free
-        if (MODE == kCommon) wait_for_previous();
         auto finish = [&](int row, int d, float4 v, float top, float weight) {
             const int in_stream = p.t.row0 + row, token = in_stream / a.group;
             const int head = p.head * a.group + in_stream - token * a.group;
-            finish_row<T, MODE>(a, p.t.token0 + token, head, d, v, top - kShift, weight);
+            const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+            T* to = static_cast<T*>(a.out.data) + (p.t.token0 + token) * a.out.token_stride + head * a.out.head_stride + d;
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
+            if (a.lse && d == 0)
+                a.lse[(p.t.token0 + token) * (a.heads * a.group) + head] =
+                    weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
         };
         // as many warps as there is to sum; the others go on to the next piece
         const int joiners = min(kWarps, (p.t.rows * (D / 4) + 31) / 32);
@@ -593,9 +593,9 @@ __global__ void __launch_bounds__(32 * (consumers(NT) + kProducers), 1)
     }
 }
 
-template <typename T, int D, int NT, int MODE>
+template <typename T, int D, int NT>
 cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
-    auto kernel = few_kernel<T, D, NT, MODE>;
+    auto kernel = few_kernel<T, D, NT>;
     const int smem = sizeof(Smem<D, NT>) + 1024;
     static std::atomic<uint64_t> allowed;
     const cudaError_t attr = allow_smem(kernel, smem, allowed);
@@ -604,44 +604,22 @@ cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     // boxes of the keys that lie together in a page, 64 at most
     if (!kv_tensor_map(map, a, kKeys)) return cudaErrorInvalidValue;
     const int row_tiles = static_cast<int>((static_cast<long long>(a.max_new) * a.group + 8 * NT - 1) / (8 * NT));
-    const int ctas = sms < kAttendMaxCtas ? sms : kAttendMaxCtas;
-    if (MODE != kCommon) {
-        // own keys are few: every item on a CTA of its own where there are enough
-        kernel<<<ctas, 32 * (consumers(NT) + kProducers), smem, s>>>(map, a, row_tiles, MODE == kOwn ? 1 : kMinShare);
-        return cudaGetLastError();
-    }
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(ctas);
-    config.blockDim = dim3(32 * (consumers(NT) + kProducers));
-    config.dynamicSmemBytes = smem;
-    config.stream = s;
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, map, a, row_tiles, kMinShare);
+    kernel<<<sms < kAttendMaxCtas ? sms : kAttendMaxCtas, 32 * (consumers(NT) + kProducers), smem, s>>>(map, a, row_tiles, kMinShare);
+    return cudaGetLastError();
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D>
 cudaError_t launch_rows(const AttendArgs& a, int sms, cudaStream_t s) {
     const long long rows = static_cast<long long>(a.max_new) * a.group;
-    return rows <= 8 ? launch<T, D, 1, MODE>(a, sms, s) : launch<T, D, 2, MODE>(a, sms, s);
-}
-
-template <int MODE>
-cudaError_t launch_type(const AttendArgs& a, int dtype, int sms, cudaStream_t s) {
-    if (a.head_dim == 64)
-        return dtype == UFB_F16 ? launch_rows<__half, 64, MODE>(a, sms, s) : launch_rows<__nv_bfloat16, 64, MODE>(a, sms, s);
-    return dtype == UFB_F16 ? launch_rows<__half, 128, MODE>(a, sms, s) : launch_rows<__nv_bfloat16, 128, MODE>(a, sms, s);
+    return rows <= 8 ? launch<T, D, 1>(a, sms, s) : launch<T, D, 2>(a, sms, s);
 }
 
 }  // namespace
 
-cudaError_t attend_few(const AttendArgs& a, int mode, int dtype, int sms, cudaStream_t s) {
-    return mode == kAll   ? launch_type<kAll>(a, dtype, sms, s)
-           : mode == kOwn ? launch_type<kOwn>(a, dtype, sms, s)
-                          : launch_type<kCommon>(a, dtype, sms, s);
+cudaError_t attend_few(const AttendArgs& a, int dtype, int sms, cudaStream_t s) {
+    if (a.head_dim == 64)
+        return dtype == UFB_F16 ? launch_rows<__half, 64>(a, sms, s) : launch_rows<__nv_bfloat16, 64>(a, sms, s);
+    return dtype == UFB_F16 ? launch_rows<__half, 128>(a, sms, s) : launch_rows<__nv_bfloat16, 128>(a, sms, s);
 }
 
 }  // namespace ufb

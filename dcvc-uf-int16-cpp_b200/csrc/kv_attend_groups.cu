@@ -1,0 +1,866 @@
+// Attention of groups of streams that begin with common pages (ufb_kv_attend_groups):
+// the branches of one stream, which go on by few tokens of their own.
+//
+//   S = Q K^T,  P = 2^(S f + log2 vs - M),  O = P V,  l = sum P / vs,  out = O / l
+//
+// as in kv_attend_many.cu, in tiles of 128 rows x 128 keys on the fifth-generation tensor
+// cores.  The rows of a group -- all its streams' new tokens times the query heads of a
+// key head -- go through the common keys once; then, in the same accumulators, through
+// each stream's own keys, which only that stream's rows see.  Nothing has to be joined
+// but what CTAs share, and a step of a search is one launch and its join.
+//
+// One CTA an SM, five roles:
+//   walker (1 warp)      says of each tile ahead where its keys are and who sees them
+//   converter (8 warps)  integers from global memory through registers to float16 in
+//                        shared memory, keys and values double buffered
+//   MMA (1 warp)         S of the next tile before P V of this one: two tiles of scores
+//                        in tensor memory, one of sums
+//   softmax (2 x 4 warps) two threads to a row, 64 columns each, which stay in registers
+//                        between the maximum and the weights; the two exchange maxima
+//                        through shared memory.  P goes back over S in float16.
+// Rows are few here, so a tile's time is the way through its steps, and two threads to a
+// row make the longest of them half as long as one does.  Warps whose rows are padding
+// skip the softmax.
+#include "kv_attend.cuh"
+#include "umma.cuh"
+
+#include <type_traits>
+
+namespace ufb {
+
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kKeys = kGroupTileKeys;
+constexpr int kGroups = kKeys / kGroupKeys;
+constexpr int kMmaWarp = 16, kWalkWarp = 17;
+constexpr int kThreads = 640;         // warps: softmax 0-7, converter 8-15, MMA 16, walker 17; 18, 19 idle
+constexpr int kPieces = 4;            // pieces announced ahead
+constexpr int kTiles = 8;             // tiles announced ahead
+constexpr int kScaleRing = 4;
+constexpr int kCode = 45;
+// As in kv_attend_many.cu: a running maximum stays while it grows by less than 2^kSlack, P is
+// taken times 2^kShift, rows with scores beyond kFar round the score before the maximum is
+// taken off.
+constexpr float kSlack = 2.0f, kShift = 13.0f;
+constexpr float kFar = 1048576.0f;   // 2^20
+
+struct alignas(16) GroupScales {
+    float key, log2_value, inv_value, pad;   // log2_value -inf: the 16 keys are not there
+};
+
+// One row tile of a group.
+struct GroupTile {
+    int token0;             // the group's first token
+    int row0, rows;
+    int low, high;          // first and last position of the group's tokens
+    int shared, slot;       // common keys, and a stream that has them
+    KeyRange keys;          // of the common ones
+    int common, nt;         // tiles of common keys, of all
+    int stream, last, own;  // the row tile's streams; of their own tiles the first's place in the group's
+};
+
+// A piece of an item as the walker announces it; rows 0: there is none any more.
+struct Announced {
+    int rows, row0, token0, head, parts, part;
+};
+// A tile of a piece.
+struct Tile {
+    int slot, key0, head;
+    int limit;              // keys below it are there
+    int row_low, row_high;  // rows that may see it
+    int groups;             // 16-key groups that are looked at, a bit each
+    int flags;              // kFirst, kLast of the piece; kClear: all its rows see all of it; kOwnKeys
+};
+constexpr int kFirst = 1, kLast = 2, kClear = 4, kOwnKeys = 8, kNone = 16;
+
+template <int D>
+struct Smem {
+    alignas(1024) uint8_t q[kRows * D * 2];        // [64 dims][row][128 bytes]
+    alignas(1024) uint8_t k[2][kKeys * D * 2];
+    alignas(1024) uint8_t v[2][kKeys * D * 2];
+    GroupScales scales[kScaleRing][kGroups];
+    float top[2][2][kRows];                        // by tile parity, half
+    float row[2][2][kRows];                        // of a piece: largest |q| and what is not finite; weights
+    alignas(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2];
+    uint64_t q_full, o_full, drained, pair[4];
+    uint64_t piece_full[kPieces], piece_empty[kPieces], tile_full[kTiles], tile_empty[kTiles];
+    Announced pieces[kPieces];
+    Tile tiles[kTiles];
+    ShareSmem share;
+    uint32_t tmem;
+    int dead;
+};
+
+template <int D>
+struct Tmem {
+    __device__ static constexpr uint32_t s(int b) { return b * 128; }
+    static constexpr uint32_t kO = 256;
+};
+
+// Address of row `row`, 16-byte chunk `chunk` (8 float16) of a [D / 64][128][128 bytes] tile.
+__device__ __forceinline__ uint32_t tile_at(int row, int chunk) {
+    return (chunk >> 3) * (128 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// The lowest n bits (none below 0, all from 32 on).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u); }
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// Two 32-bit multiply-adds (x, y) = (x, y) f + add, two additions (a, b) += (x, y).
+__device__ __forceinline__ void fma2(float& x, float& y, float f, float add) {
+    asm("{\n\t.reg .b64 v, m, c;\n\t"
+        "mov.b64 v, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 c, {%3, %3};\n\t"
+        "fma.rn.f32x2 v, v, m, c;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(f), "f"(add));
+}
+__device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
+    asm("{\n\t.reg .b64 v, w;\n\t"
+        "mov.b64 v, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\t"
+        "add.rn.f32x2 v, v, w;\n\tmov.b64 {%0, %1}, v;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(x), "f"(y));
+}
+
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// false: the pair (group, row tile) does not exist.
+__device__ __forceinline__ bool group_tile(const AttendArgs& a, const GroupArgs& g, int group, int rt, GroupTile& t) {
+    const int o0 = g.offsets[group], o1 = g.offsets[group + 1];
+    const bool ok = o0 >= 0 && o1 >= o0 && o1 <= a.tokens && o1 - o0 <= g.max_tokens;
+    if (!ok && rt == 0) atomicCAS(a.status, 0, kStatusIndex);
+    t.token0 = o0;
+    t.row0 = rt * kRows;
+    t.rows = min(kRows, ok ? (o1 - o0) * a.group - t.row0 : 0);
+    if (t.rows <= 0) return false;
+    t.shared = g.state.shared[group];
+    t.slot = g.state.slot[group];
+    t.low = g.state.low[group];
+    t.high = g.state.high[group];
+    const int first = g.first[group];
+    const int s0 = g.state.stream[o0 + t.row0 / a.group], s1 = g.state.stream[o0 + (t.row0 + t.rows - 1) / a.group];
+    t.stream = s0;
+    t.last = s1;
+    t.own = s0 > first ? g.state.tiles[s0 - 1] : 0;
+    t.keys = key_range<kKeys>(a, t.shared, 0, t.low - t.shared, t.high - t.shared);
+    t.common = t.keys.hi > 0 ? t.keys.nt : 0;
+    // rows that see nothing are still written: one tile, all of it hidden
+    t.nt = max(t.common + g.state.tiles[s1] - t.own, 1);
+    return true;
+}
+
+// Walks the pieces of this CTA's share.
+struct GroupWalker {
+    int row_tiles, pair, pairs;
+    long long pos, end, pair_start;
+    bool loaded;
+    GroupTile t;
+    int head, first, last;      // the piece: key head, key tiles [first, last)
+    long long item_start;
+
+    __device__ __forceinline__ bool next(const AttendArgs& a, const GroupArgs& g) {
+        if (pos >= end) return false;
+        while (true) {
+            if (pair >= pairs) return false;
+            if (!loaded) {
+                if (!group_tile(a, g, pair / row_tiles, pair % row_tiles, t)) {
+                    pair = (pair / row_tiles + 1) * row_tiles;
+                    continue;
+                }
+                loaded = true;
+            }
+            const long long size = static_cast<long long>(t.nt) * a.heads;
+            if (pos < pair_start + size) break;
+            pair_start += size;
+            ++pair;
+            loaded = false;
+        }
+        head = static_cast<int>(quotient(pos - pair_start, t.nt));
+        item_start = pair_start + static_cast<long long>(head) * t.nt;
+        first = static_cast<int>(pos - item_start);
+        last = static_cast<int>(min(static_cast<long long>(t.nt), end - item_start));
+        pos = item_start + last;
+        return true;
+    }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a, const GroupArgs g, int row_tiles) {
+    // aligned by declaration, so that descriptors are constants (checked below)
+    extern __shared__ __align__(1024) uint8_t raw[];
+    Smem<D>& sm = *reinterpret_cast<Smem<D>*>(raw);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.k_full[i], 128);
+            mbar_init(&sm.v_full[i], 128);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_empty[i], 1);
+            mbar_init(&sm.p_full[i][0], 128);
+            mbar_init(&sm.p_full[i][1], 128);
+            mbar_init(&sm.s_full[i], 1);
+        }
+        mbar_init(&sm.q_full, 256);
+        mbar_init(&sm.o_full, 1);
+        mbar_init(&sm.drained, 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&sm.pair[i], 64);
+        for (int i = 0; i < kPieces; ++i) {
+            mbar_init(&sm.piece_full[i], 1);
+            mbar_init(&sm.piece_empty[i], 8);
+        }
+        for (int i = 0; i < kTiles; ++i) {
+            mbar_init(&sm.tile_full[i], 1);
+            mbar_init(&sm.tile_empty[i], 17);
+        }
+        fence_mbar_init();
+        sm.dead = (smem_u32(raw) & 1023) != 0;
+        if (sm.dead) atomicCAS(a.status, 0, kCode);
+    }
+    if (warp == kMmaWarp) {
+        tmem_alloc(&sm.tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    GroupTile scratch_tile;
+    const int pairs = g.groups * row_tiles;
+    const Share share = share_out<kThreads>(
+        pairs, 1, [&](int p) -> long long {
+            return group_tile(a, g, p / row_tiles, p % row_tiles, scratch_tile) ? static_cast<long long>(scratch_tile.nt) * a.heads : 0;
+        },
+        sm.share);
+    tc_fence_after();
+    // all 512 columns are this CTA's: its tensor memory begins at 0
+    constexpr uint32_t tmem = 0;
+    volatile int* dead = &sm.dead;
+    // after a wait gave up nobody waits any more, and no further tile is begun
+    auto wait = [&](uint64_t* bar, int phase) {
+        if (mbar_try_wait(bar, phase & 1)) return;
+        if (!*dead && !mbar_wait(bar, phase & 1, a.status, kCode)) *dead = 1;
+    };
+    // Tiles one after another; a reader gives each back when it is done with it.
+    auto tile_info = [&](int n) -> const Tile& {
+        wait(&sm.tile_full[n % kTiles], n / kTiles);
+        __syncwarp();
+        return sm.tiles[n % kTiles];
+    };
+    auto tile_done = [&](int n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.tile_empty[n % kTiles]);
+    };
+
+    // the registers of 640 threads at 96: 2 x 128 + 2 x 72 + 80 = 5 x 96
+    if (warp < 8) {
+        regs_inc<128>();
+        // ---- softmax: row of the tile = lane of tensor memory, half of the columns
+        const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
+        if (threadIdx.x == 0) scratch.items[blockIdx.x * 8] = 0;
+        // the two warps that share rows meet, in tensor memory too
+        int met = 0;
+        auto pair_sync = [&] {
+            tc_fence_before();
+            mbar_arrive(&sm.pair[quarter]);
+            wait(&sm.pair[quarter], met++);
+            __syncwarp();
+            tc_fence_after();
+        };
+        int pieces = -1, pos = 0, head = 0, token = 0;
+        bool real = false, busy = false, write = false;   // this row, a row of this warp: of the piece
+        bool far = false;
+        float unit = 0.0f, m = -INFINITY, l = 0.0f;
+        for (int n = 0;; ++n) {
+            const Tile& tile = tile_info(n);
+            const int flags = tile.flags, b = n & 1;
+            if ((flags & kNone) || *dead) break;
+            if (flags & kFirst) {
+                ++pieces;
+                wait(&sm.piece_full[pieces % kPieces], pieces / kPieces);
+                __syncwarp();
+                const Announced& p = sm.pieces[pieces % kPieces];
+                real = row < p.rows;
+                busy = quarter * 32 < p.rows;
+                const int in_group = p.row0 + (real ? row : 0);
+                token = in_group / a.group;
+                head = p.head * a.group + in_group - token * a.group;
+                token += p.token0;
+                pos = real ? g.state.positions[token] : -1;
+                write = real && pos != kNotWritten;
+                if (!write) pos = -1;
+                m = -INFINITY, l = 0.0f;
+                far = false;
+                if (busy) {
+                    // half of the row's dims to [2^15, 2^16) and float16; the softmax scale's sign goes with it
+                    const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + static_cast<long long>(token) * a.q.token_stride +
+                                                                      head * a.q.head_stride) + half * (D / 16);
+                    uint4 v[D / 16];
+                    float top = 0.0f, odd = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) v[i] = real ? vec[i] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 f = unpack2(x[j], T());
+                            top = max3(top, fabsf(f.x), fabsf(f.y));
+                            odd += (f.x - f.x) + (f.y - f.y);  // NaN for what is not finite
+                        }
+                    }
+                    sm.row[0][half][row] = odd == odd ? top : odd;
+                    pair_sync();
+                    const float other = sm.row[0][half ^ 1][row];
+                    const float u = row_unit(odd == odd && other == other ? fmaxf(top, other) : __int_as_float(0x7fffffff));
+                    unit = unit_inverse(u) * fabsf(a.scale_log2);
+                    const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                        uint32_t y[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 f = unpack2(x[j], T());
+                            y[j] = pack2(f.x * mul, f.y * mul, __half());
+                        }
+                        *reinterpret_cast<uint4*>(sm.q + tile_at(row, half * (D / 16) + i)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&sm.q_full);
+            }
+            wait(&sm.s_full[b], n >> 1);
+            __syncwarp();
+            tc_fence_after();
+            const int key0 = tile.key0;
+            const uint32_t ts = tmem + lanes + Tmem<D>::s(b), tp = ts + half * 32;
+            // rows of this warp that the tile is for
+            const bool mine = busy && tile.row_low < quarter * 32 + 32 && tile.row_high > quarter * 32;
+            if (mine) {
+                const GroupScales* sc = sm.scales[n % kScaleRing] + half * 4;
+                uint32_t s0[32], s1[32];
+                tmem_ld32(ts + half * 64, s0);
+                tmem_ld32(ts + half * 64 + 32, s1);
+                // columns [0, high) that are from low on or below sink are seen by this row
+                const bool ours = row >= tile.row_low && row < tile.row_high;
+                const int limit = tile.limit;
+                const int high = ours ? min(limit, a.causal || !(flags & kOwnKeys) ? pos + 1 : limit) - key0 - half * 64 : 0;
+                const int low = a.window ? max(pos - a.window + 1, 0) - key0 - half * 64 : 0;
+                const int sink = a.window ? a.sinks - key0 - half * 64 : 0;
+                auto seen = [&](int c) {   // of 32 columns, a bit each
+                    return bits_below(high - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
+                };
+                tmem_wait_ld();
+                tmem_tie32(s0);
+                tmem_tie32(s1);
+                float top = -INFINITY;
+                auto maximum = [&](auto masked) {
+                    auto chunk = [&](int c, const uint32_t (&s)[32]) {
+                        const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            auto f = [&](int j) {
+                                return decltype(masked)::value && !(bits & (1u << (h * 16 + j))) ? -INFINITY : __uint_as_float(s[h * 16 + j]);
+                            };
+                            float y = max3(f(0), f(1), f(2)), z = max3(f(3), f(4), f(5));
+                            y = max3(y, f(6), f(7)), z = max3(z, f(8), f(9));
+                            y = max3(y, f(10), f(11)), z = max3(z, f(12), f(13));
+                            y = max3(y, f(14), f(15));
+                            y = fmaxf(y, z);
+                            const GroupScales gs = sc[c * 2 + h];
+                            const float v = fmaf(y, unit * gs.key, gs.log2_value);
+                            // -infinity: nothing of the group is seen
+                            top = fmaxf(top, decltype(masked)::value && y == -INFINITY ? y : v);
+                        }
+                    };
+                    chunk(0, s0);
+                    chunk(1, s1);
+                };
+                const bool clear = flags & kClear;
+                if (clear) maximum(std::false_type());
+                else maximum(std::true_type());
+                // all scores of these rows are in registers behind this: P may go over them
+                sm.top[b][half][row] = top;
+                pair_sync();
+                top = fmaxf(top, sm.top[b][half ^ 1][row]);
+                // the maximum stays while it is within 2^kSlack
+                const bool grow = top > __fadd_rd(m, kSlack);
+                if (__any_sync(0xffffffffu, grow)) {
+                    if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
+                        const float keep = grow && m != -INFINITY ? ex2(m - top) : 1.0f;
+                        // the product before this has to be in the sums
+                        if (!(flags & kFirst)) {
+                            wait(&sm.v_empty[(n - 1) & 1], (n - 1) >> 1);
+                            __syncwarp();
+                            tc_fence_after();
+                        }
+#pragma unroll 1
+                        for (int c = half * (D / 32); c < (half + 1) * (D / 32); ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(tmem + lanes + Tmem<D>::kO + c * 16, o);
+                            tmem_wait_ld_regs(o);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
+                            tmem_st16(tmem + lanes + Tmem<D>::kO + c * 16, o);
+                        }
+                        l *= keep;
+                    }
+                    if (grow) m = top;
+                    far = __any_sync(0xffffffffu, fabsf(m) >= kFar && m != -INFINITY);
+                }
+                const float base = m == -INFINITY ? 0.0f : __fsub_ru(m, kShift);
+                auto weights = [&](auto masked) {
+                    auto chunk = [&](int c, uint32_t (&s)[32]) {
+                        const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
+                        uint32_t w[16];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const GroupScales gs = sc[c * 2 + h];
+                            const float f = unit * gs.key, add = decltype(masked)::value ? gs.log2_value : gs.log2_value - base;
+                            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+                            for (int j = 0; j < 16; j += 2) {
+                                float x = __uint_as_float(s[h * 16 + j]), y = __uint_as_float(s[h * 16 + j + 1]);
+                                fma2(x, y, f, add);
+                                if (decltype(masked)::value) {
+                                    add2(x, y, -base, -base);
+                                    if (!(bits & (1u << (h * 16 + j)))) x = -INFINITY;
+                                    if (!(bits & (1u << (h * 16 + j + 1)))) y = -INFINITY;
+                                }
+                                x = ex2(x);
+                                y = ex2(y);
+                                add2(sum[0], sum[1], x, y);
+                                w[h * 8 + j / 2] = pack2(x, y, __half());
+                            }
+                            sum[0] += sum[1];
+                            if (sum[0] != 0.0f) l = fmaf(sum[0], gs.inv_value, l);
+                        }
+                        tmem_st16(tp + c * 16, w);
+                    };
+                    chunk(0, s0);
+                    chunk(1, s1);
+                };
+                if (clear && !far) weights(std::false_type());
+                else weights(std::true_type());
+                tmem_wait_st();
+            } else if (busy) {
+                // rows of other streams: no weight.  (Padding's weights do not matter.)
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = 0;
+                tmem_st16(tp, w);
+                tmem_st16(tp + 16, w);
+                tmem_wait_st();
+            }
+            tc_fence_before();
+            mbar_arrive(&sm.p_full[b][half]);
+            tile_done(n);
+            if (!(flags & kLast)) continue;
+
+            // ---- the piece's rows
+            if (busy) sm.row[1][half][row] = l;
+            wait(&sm.o_full, pieces);
+            __syncwarp();
+            tc_fence_after();
+            const Announced& p = sm.pieces[pieces % kPieces];
+            if (busy) {
+                pair_sync();
+                l = sm.row[1][0][row] + sm.row[1][1][row];
+                const bool whole = p.part < 0;
+                const int part = 2 * blockIdx.x + p.part;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                T* out = static_cast<T*>(a.out.data) + static_cast<long long>(token) * a.out.token_stride + head * a.out.head_stride;
+                float* sums = scratch.sums + (static_cast<long long>(part) * kRows + row) * D;
+#pragma unroll 1
+                for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(tmem + lanes + Tmem<D>::kO + c * 32, o);
+                    tmem_wait_ld();
+                    tmem_tie32(o);
+                    if (write && whole) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[i] = pack2(__uint_as_float(o[j + 2 * i]) * inv, __uint_as_float(o[j + 2 * i + 1]) * inv, T());
+                            reinterpret_cast<uint4*>(out)[c * 4 + j / 8] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else if (real && !whole) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            __stcg(reinterpret_cast<uint4*>(sums + c * 32 + j), make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+                    }
+                    __syncwarp();
+                }
+                if (half == 0 && write && whole && a.lse)
+                    a.lse[static_cast<long long>(token) * (a.heads * a.group) + head] =
+                        l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * 0.6931471805599453f;
+                if (half == 0 && real && !whole) {
+                    __stcg(scratch.stats + (part * 2) * kRows + row, m);
+                    __stcg(scratch.stats + (part * 2 + 1) * kRows + row, l);
+                }
+            }
+            if (p.parts && threadIdx.x == 0) {
+                int32_t* item = scratch.items + blockIdx.x * 8;
+                item[1] = p.token0;
+                item[2] = p.row0;
+                item[3] = p.rows;
+                item[4] = p.head;
+                item[0] = p.parts;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.piece_empty[pieces % kPieces]);
+            tc_fence_before();
+        }
+    } else if (warp < kMmaWarp) {
+        regs_dec<72>();
+        // ---- converter: warps 8-11 the keys and the scales, 12-15 the values, 32 keys each
+        constexpr int kLoads = D / 16;   // 16-byte loads of a thread for a tile
+        const int side = (warp - 8) >> 2, w = warp & 3;
+        const int chunk = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;
+        const int sub = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) & 1) * 2 : lane >> 2;
+        constexpr int kStep = D == 128 ? 4 : 8;   // rows of one load of a warp
+        uint64_t* full = side ? sm.v_full : sm.k_full;
+        uint64_t* empty = side ? sm.v_empty : sm.k_empty;
+        uint8_t* tiles = side ? sm.v[0] : sm.k[0];
+        // this thread's two 16-byte pieces of its first row; row & 7 repeats every kStep * 2 rows
+        uint32_t at0[2], at1[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            at0[i] = tile_at(w * 32 + i * kStep + sub, chunk * 2);
+            at1[i] = tile_at(w * 32 + i * kStep + sub, chunk * 2 + 1);
+        }
+        struct Next {
+            int page[2], row[2], head;   // of this warp's two groups of 16 keys
+            bool tile;                   // false: no further tile
+        };
+        int looked = 0;
+        bool have = true;
+        auto fetch = [&](Next& n) {
+            n.tile = false;
+            n.page[0] = n.page[1] = -1;
+            if (!have) return;
+            const Tile& t = tile_info(looked);
+            have = !(t.flags & kNone) && !*dead;
+            if (!have) return;
+            n.tile = true;
+            n.head = t.head;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int key = t.key0 + w * 32 + i * kGroupKeys, entry = key >> a.page_shift;
+                n.row[i] = key & (a.page_tokens - 1);
+                if ((t.groups >> (w * 2 + i) & 1) && entry < a.table_width)
+                    n.page[i] = a.table[static_cast<long long>(t.slot) * a.table_width + entry];
+            }
+            tile_done(looked++);
+        };
+        uint4 buf[kLoads];
+        float key_scale = 0.0f, value_scale = -1.0f;   // of the warp's group `lane` (0, 1); -1: not there
+        auto load = [&](const Next& n) {
+            if (!n.tile) return;
+            const int8_t* from[2];
+            bool there[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                there[i] = n.page[i] >= 0 && n.page[i] < a.pages;
+                const long long tile = (static_cast<long long>(n.page[i]) * 2 + side) * a.heads + n.head;
+                from[i] = a.kv + ((tile << a.page_shift) + n.row[i] + sub) * D + chunk * 16;
+            }
+            if (there[0] && there[1]) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i)  // sub < kStep, a divisor of 16
+                    buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    buf[i] = make_uint4(0, 0, 0, 0);
+                    if (there[(i * kStep) >> 4])
+                        buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
+                }
+            }
+            if (side == 0 && lane < 2) {
+                key_scale = 0.0f, value_scale = -1.0f;
+                if (lane == 0 ? there[0] : there[1]) {
+                    const int page = lane == 0 ? n.page[0] : n.page[1];
+                    const float* s = a.scale + static_cast<long long>(page) * 2 * a.heads + n.head;
+                    key_scale = s[0];
+                    value_scale = s[a.heads];
+                    if (value_scale < kTinyScale) value_scale = kTinyScale;
+                }
+            }
+        };
+        Next now, next;
+        fetch(now);
+        load(now);
+        fetch(next);
+        for (int n = 0; now.tile; ++n) {
+            const int b = n & 1;
+            if (n >= 2) wait(&empty[b], (n >> 1) - 1);
+            uint8_t* to = tiles + b * (kKeys * D * 2);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const uint32_t x[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
+                uint32_t y[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) int8x4_to_half(x[j], y[2 * j], y[2 * j + 1]);
+                const int step = (i / 2) * 2 * kStep * 128;
+                *reinterpret_cast<uint4*>(to + at0[i & 1] + step) = make_uint4(y[0], y[1], y[2], y[3]);
+                *reinterpret_cast<uint4*>(to + at1[i & 1] + step) = make_uint4(y[4], y[5], y[6], y[7]);
+            }
+            if (side == 0 && lane < 2) {
+                GroupScales s;
+                s.key = key_scale;
+                s.log2_value = value_scale == -1.0f ? -INFINITY : log2f(value_scale);
+                s.inv_value = value_scale == -1.0f ? 0.0f : 1.0f / value_scale;
+                s.pad = 0.0f;
+                sm.scales[n % kScaleRing][w * 2 + lane] = s;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&full[b]);
+            load(next);
+            now = next;
+            fetch(next);
+        }
+    } else {
+        regs_dec<80>();
+        if (warp == kWalkWarp) {
+            // ---- walker: announces this CTA's pieces and their tiles
+            GroupWalker walk;
+            walk.row_tiles = row_tiles;
+            walk.pairs = pairs;
+            walk.pos = share.per * blockIdx.x;
+            walk.end = min(walk.pos + share.per, share.total);
+            walk.pair = share.pair;
+            walk.pair_start = share.pair_start;
+            walk.loaded = false;
+            int n = 0;
+            for (int piece = 0; !*dead && walk.next(a, g); ++piece) {
+                const GroupTile& t = walk.t;
+                if (piece >= kPieces) wait(&sm.piece_empty[piece % kPieces], piece / kPieces - 1);
+                if (lane == 0) {
+                    Announced& o = sm.pieces[piece % kPieces];
+                    o.rows = t.rows;
+                    o.row0 = t.row0;
+                    o.token0 = t.token0;
+                    o.head = walk.head;
+                    // the part of a shared item: 0 where an earlier CTA began it, 1 where this
+                    // one does, which then tells how many parts there are
+                    const bool whole = walk.first == 0 && walk.last == t.nt;
+                    o.part = whole ? -1 : (walk.first > 0 ? 0 : 1);
+                    o.parts = o.part == 1 ? static_cast<int>(quotient(walk.item_start + t.nt - 1, share.per)) - static_cast<int>(blockIdx.x) + 1 : 0;
+                    mbar_arrive(&sm.piece_full[piece % kPieces]);
+                }
+                // own tiles: of stream `s`, whose first is number `from` of the group's
+                int s = t.stream, from = t.own, until = g.state.tiles[s];
+                for (int i = walk.first; i < walk.last; ++i, ++n) {
+                    Tile o;
+                    o.head = walk.head;
+                    o.flags = (i == walk.first ? kFirst : 0) | (i + 1 == walk.last ? kLast : 0);
+                    o.row_low = 0;
+                    o.row_high = kRows;
+                    if (i < t.common) {
+                        o.slot = t.slot;
+                        o.key0 = t.keys.tile(i) * kKeys;
+                        o.limit = t.shared;
+                        o.groups = 0;
+                        for (int k = 0; k < kGroups; ++k) o.groups |= t.keys.touches(o.key0 + k * kGroupKeys) << k;
+                        if (o.key0 + kKeys - 1 <= t.low && o.key0 + kKeys <= t.shared &&
+                            (!a.window || t.high - o.key0 < a.window || o.key0 + kKeys <= a.sinks))
+                            o.flags |= kClear;
+                    } else {
+                        const int own = t.own + i - t.common;
+                        while (own >= until && s < t.last) from = until, until = g.state.tiles[++s];
+                        const bool there = own < until;      // else the tile of rows that see nothing
+                        o.slot = there ? a.slots[s] : 0;
+                        o.key0 = there ? t.shared + (own - from) * kKeys : 0;
+                        o.limit = there ? a.lengths[o.slot] : 0;
+                        o.groups = 0;
+                        for (int k = 0; k < kGroups; ++k) o.groups |= (o.key0 + k * kGroupKeys < o.limit) << k;
+                        o.row_low = (a.offsets[s] - t.token0) * a.group - t.row0;
+                        o.row_high = (a.offsets[s + 1] - t.token0) * a.group - t.row0;
+                        o.flags |= kOwnKeys;
+                        if (!there) o.row_low = 0, o.row_high = kRows;
+                    }
+                    if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
+                    if (lane == 0) {
+                        sm.tiles[n % kTiles] = o;
+                        mbar_arrive(&sm.tile_full[n % kTiles]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
+            if (lane == 0) {
+                sm.tiles[n % kTiles].flags = kNone;
+                mbar_arrive(&sm.tile_full[n % kTiles]);
+            }
+            __syncwarp();
+        }
+        // ---- MMA: the warp waits together, one lane issues
+        if (warp == kMmaWarp) {
+            constexpr uint32_t qk = f16_idesc(128, kKeys, false), pv = f16_idesc(128, D, true);
+            constexpr uint64_t kTile = (kKeys * D * 2) >> 4;   // descriptor step between the two buffers
+            const uint64_t q_desc = sw128_desc(smem_u32(sm.q)), k_desc = sw128_desc(smem_u32(sm.k[0]));
+            const uint64_t v_desc = sw128_n_major_desc(smem_u32(sm.v[0]), 128 * 128);
+            const uint32_t issue = lane == 0;
+            int piece = 0, held = 0;   // held: the flags of the tile whose P V is outstanding
+            auto sums = [&](int n) {
+                const int b = n & 1;
+                wait(&sm.v_full[b], n >> 1);
+                const uint64_t vd = v_desc + b * kTile;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    wait(&sm.p_full[b][h], n >> 1);
+                    __syncwarp();
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = h * 4; k < h * 4 + 4; ++k)
+                        mma_f16_ts(tmem + Tmem<D>::kO, tmem + Tmem<D>::s(b) + k * 8, vd + k * (16 * 128 >> 4), pv,
+                                   !(held & kFirst) || k > 0, issue);
+                }
+                mma_commit_if(&sm.v_empty[b], issue);
+                if (held & kLast) mma_commit_if(&sm.o_full, issue);
+            };
+            bool outstanding = false;
+            int n = 0;
+            for (;; ++n) {
+                const int flags = tile_info(n).flags, b = n & 1;
+                tile_done(n);
+                if ((flags & kNone) || *dead) break;
+                if (flags & kFirst) {
+                    // the queries' place is free once the piece before is through
+                    if (outstanding) sums(n - 1);
+                    outstanding = false;
+                    wait(&sm.q_full, piece++);
+                }
+                wait(&sm.k_full[b], n >> 1);
+                __syncwarp();
+                tc_fence_after();
+                const uint64_t kd = k_desc + b * kTile;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const int off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                    mma_f16(tmem + Tmem<D>::s(b), q_desc + off, kd + off, qk, k > 0, issue);
+                }
+                mma_commit_if(&sm.s_full[b], issue);
+                mma_commit_if(&sm.k_empty[b], issue);
+                if (outstanding) sums(n - 1);
+                outstanding = true;
+                held = flags;
+            }
+            if (outstanding && !*dead) sums(n - 1);
+            // nothing may be in flight when tensor memory is given back
+            if (lane == 0) {
+                mma_commit(&sm.drained);
+                mbar_wait(&sm.drained, 0, a.status, kCode);
+            }
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(sm.tmem, 512);
+    }
+}
+
+// Rows that several CTAs share: the item that CTA x's share ends in, a block's rows
+// from kJoinRows * y on.  The parts' maxima and weights come first, once a row, by a
+// warp; then a thread adds the parts of four columns, in the order of the CTAs.
+constexpr int kJoinThreads = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) groups_join_kernel(const AttendArgs a, const GroupArgs g, int ctas) {
+    constexpr int kJoinRows = kJoinThreads / (D / 4);
+    __shared__ float share[kAttendMaxCtas][kJoinRows];   // of a part in a row's sum
+    __shared__ float tops[kJoinRows], weights[kJoinRows];
+    const AttendScratch scratch = scratch_of(a.workspace, ctas, kRows);
+    const int c0 = blockIdx.x, first = blockIdx.y * kJoinRows;
+    wait_for_previous();
+    const int32_t* item = scratch.items + c0 * 8;
+    const int parts = item[0], rows = min(item[3] - first, kJoinRows);
+    if (parts == 0 || rows <= 0) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int r = warp; r < rows; r += kJoinThreads / 32) {
+        float top = -INFINITY;
+        for (int i = lane; i < parts; i += 32)
+            top = fmaxf(top, scratch.stats[(2 * (c0 + i) + (i == 0)) * 2 * kRows + first + r]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float weight = 0.0f;
+        for (int i = lane; i < parts; i += 32) {
+            const int from = 2 * (c0 + i) + (i == 0);
+            const float m = scratch.stats[from * 2 * kRows + first + r], l = scratch.stats[(from * 2 + 1) * kRows + first + r];
+            const float mul = m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2(m - top);
+            share[i][r] = mul;
+            weight += l * mul;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) weight += __shfl_xor_sync(0xffffffffu, weight, o);
+        if (lane == 0) tops[r] = top, weights[r] = weight;
+    }
+    __syncthreads();
+    const int r = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    if (r >= rows) return;
+    const int row = first + r;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) {
+        const int from = 2 * (c0 + i) + (i == 0);
+        const float4 x = *reinterpret_cast<const float4*>(scratch.sums + (static_cast<long long>(from) * kRows + row) * D + d);
+        const float mul = share[i][r];
+        v.x += x.x * mul, v.y += x.y * mul, v.z += x.z * mul, v.w += x.w * mul;
+    }
+    const int in_group = item[2] + row;
+    int token = in_group / a.group;
+    const int head = item[4] * a.group + in_group - token * a.group;
+    token += item[1];
+    if (g.state.positions[token] == kNotWritten) return;
+    const float top = tops[r], weight = weights[r];
+    const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+    T* to = static_cast<T*>(a.out.data) + static_cast<long long>(token) * a.out.token_stride + head * a.out.head_stride + d;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
+    if (a.lse && d == 0)
+        a.lse[static_cast<long long>(token) * (a.heads * a.group) + head] =
+            weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
+}
+
+template <typename T, int D>
+cudaError_t launch(const AttendArgs& a, const GroupArgs& g, int sms, cudaStream_t s) {
+    auto kernel = groups_kernel<T, D>;
+    const int smem = sizeof(Smem<D>);
+    static std::atomic<uint64_t> allowed;
+    const cudaError_t attr = allow_smem(kernel, smem, allowed);
+    if (attr != cudaSuccess) return attr;
+    const long long row_tiles = (static_cast<long long>(g.max_tokens) * a.group + kRows - 1) / kRows;
+    if (row_tiles * g.groups > 0x3fffffff) return cudaErrorInvalidValue;
+    const int ctas = sms < kAttendMaxCtas ? sms : kAttendMaxCtas;
+    kernel<<<ctas, kThreads, smem, s>>>(a, g, static_cast<int>(row_tiles));
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    // its blocks may start once the CTAs have exited, before that kernel's end is signalled
+    // (it gives no earlier trigger): they wait for that
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(ctas, kRows * (D / 4) / kJoinThreads);
+    config.blockDim = dim3(kJoinThreads);
+    config.stream = s;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, groups_join_kernel<T, D>, a, g, ctas);
+}
+
+}  // namespace
+
+cudaError_t kv_attend_groups(const AttendArgs& a, const GroupArgs& g, int dtype, int sms, cudaStream_t s) {
+    if (a.head_dim == 64)
+        return dtype == UFB_F16 ? launch<__half, 64>(a, g, sms, s) : launch<__nv_bfloat16, 64>(a, g, sms, s);
+    return dtype == UFB_F16 ? launch<__half, 128>(a, g, sms, s) : launch<__nv_bfloat16, 128>(a, g, sms, s);
+}
+
+}  // namespace ufb

@@ -67,7 +67,6 @@ struct alignas(16) GroupScales {
 struct Announced {
     KeyRange keys;
     int rows, row0, first, end, slot, length, start, token0, head, parts, part;  // start: where token 0 stands
-    int low, high;   // kCommon
 };
 
 template <int D>
@@ -117,7 +116,7 @@ __device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
         : "f"(x), "f"(y));
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, int row_tiles, int min_share) {
     // aligned by declaration, so that descriptors are constants (checked below)
     extern __shared__ __align__(1024) uint8_t raw[];
@@ -149,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
         tmem_relinquish();
     }
     tc_fence_before();
-    const Share share = locate_share<kKeys, kRows, kThreads, MODE>(a, row_tiles, min_share, sm.share);
+    const Share share = locate_share<kKeys, kRows, kThreads>(a, row_tiles, min_share, sm.share);
     tc_fence_after();
     // all 512 columns are this CTA's: its tensor memory begins at 0
     constexpr uint32_t tmem = 0;
@@ -192,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             const bool real = r < p.rows;
             const int in_stream = p.row0 + (real ? r : 0);
             const int token = in_stream / a.group, head = p.head * a.group + in_stream - token * a.group;
-            const int pos = MODE == kCommon ? a.positions[p.token0 + token] : p.start + token;
+            const int pos = p.start + token;
             const long long out_row = p.token0 + static_cast<long long>(token);
             float unit;
             {
@@ -232,8 +231,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             }
             float m = -INFINITY, l = 0.0f;
             bool far = false;   // a row of the warp has scores beyond kFar
-            const int first_pos = MODE == kCommon ? p.low : p.start + (p.row0 + t * kHalf) / a.group;
-            const int last_pos = MODE == kCommon ? p.high : p.start + (p.row0 + min(p.rows, (t + 1) * kHalf) - 1) / a.group;
+            const int first_pos = p.start + (p.row0 + t * kHalf) / a.group;
+            const int last_pos = p.start + (p.row0 + min(p.rows, (t + 1) * kHalf) - 1) / a.group;
             const int length = p.length, end = p.end;
             for (int tile = p.first; tile < end; ++tile, ++tiles) {
                 wait(&sm.s_full[t], s_n++);
@@ -361,8 +360,6 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
             tc_fence_after();
             const bool whole = p.part < 0;
             const int part = 2 * blockIdx.x + p.part;
-            // the parts of the streams' own keys are there, and the scratch is free
-            if (MODE == kCommon) wait_for_previous();
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             T* out = static_cast<T*>(a.out.data) + out_row * a.out.token_stride + head * a.out.head_stride;
             float* sums = scratch.sums + (static_cast<long long>(part) * kRows + r) * D;
@@ -371,14 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 uint32_t o[32];
                 tmem_ld32(to + c * 32, o);
                 tmem_wait_ld();
-                if (MODE != kAll && real && whole) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        finish_row<T, MODE>(a, out_row, head, c * 32 + j,
-                                            make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]),
-                                                        __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3])),
-                                            m - kShift, l);
-                } else if (real && whole) {
+                if (real && whole) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) {
                         uint32_t w[4];
@@ -396,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                 }
                 __syncwarp();
             }
-            if (MODE == kAll && real && whole && a.lse)
+            if (real && whole && a.lse)
                 a.lse[out_row * (a.heads * a.group) + head] =
                     l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * 0.6931471805599453f;
             if (real && !whole) {
@@ -532,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
         regs_dec<80>();
         if (warp == kWalkWarp) {
             // ---- walker: announces this CTA's pieces
-            Walker<kKeys, kRows, MODE> walk(a, share, row_tiles);
+            Walker<kKeys, kRows> walk(a, share, row_tiles);
             Piece p;
             bool more = true;
             for (int n = 0; more; ++n) {
@@ -549,7 +539,6 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
                         o.slot = p.t.slot;
                         o.length = p.t.length;
                         o.start = p.t.length - p.t.n_new;
-                        if (MODE == kCommon) o.low = p.t.low, o.high = p.t.high;
                         o.token0 = static_cast<int>(p.t.token0);
                         o.head = p.head;
                         // the part of a shared item: 0 where an earlier CTA began it, 1 where this
@@ -647,14 +636,14 @@ __global__ void __launch_bounds__(kThreads, 1) many_kernel(const AttendArgs a, i
 // warp; then a thread adds the parts of four columns, in the order of the CTAs.
 constexpr int kJoinThreads = 256;
 
-template <typename T, int D, int MODE>
+template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendArgs a, int ctas) {
     constexpr int kJoinRows = kJoinThreads / (D / 4);
     __shared__ float share[kAttendMaxCtas][kJoinRows];   // of a part in a row's sum
     __shared__ float tops[kJoinRows], weights[kJoinRows];
     const AttendScratch scratch = scratch_of(a.workspace, ctas, kRows);
     const int c0 = blockIdx.x, first = blockIdx.y * kJoinRows;
-    wait_for_previous();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int32_t* item = scratch.items + c0 * 8;
     const int parts = item[0], rows = min(item[3] - first, kJoinRows);
     if (parts == 0 || rows <= 0) return;
@@ -691,12 +680,19 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendArgs a, 
     }
     const int in_stream = item[2] + row, token = in_stream / a.group;
     const int head = item[4] * a.group + in_stream - token * a.group;
-    finish_row<T, MODE>(a, item[1] + static_cast<long long>(token), head, d, v, tops[r] - kShift, weights[r]);
+    const float top = tops[r], weight = weights[r];
+    const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
+    const long long out_row = item[1] + static_cast<long long>(token);
+    T* to = static_cast<T*>(a.out.data) + out_row * a.out.token_stride + head * a.out.head_stride + d;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
+    if (a.lse && d == 0)
+        a.lse[out_row * (a.heads * a.group) + head] =
+            weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
 }
 
-template <typename T, int D, int MODE>
+template <typename T, int D>
 cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
-    auto kernel = many_kernel<T, D, MODE>;
+    auto kernel = many_kernel<T, D>;
     const int smem = sizeof(Smem<D>);
     static std::atomic<uint64_t> allowed;
     const cudaError_t attr = allow_smem(kernel, smem, allowed);
@@ -704,40 +700,29 @@ cudaError_t launch(const AttendArgs& a, int sms, cudaStream_t s) {
     const long long row_tiles = (static_cast<long long>(a.max_new) * a.group + kRows - 1) / kRows;
     if (row_tiles * a.n > 0x3fffffff) return cudaErrorInvalidValue;
     const int ctas = sms < kAttendMaxCtas ? sms : kAttendMaxCtas;
+    many_kernel<T, D><<<ctas, kThreads, smem, s>>>(a, static_cast<int>(row_tiles), 1);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    // its blocks may start once the CTAs have exited, before that kernel's end is signalled
+    // (it gives no earlier trigger): they wait for that
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(ctas);
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = smem;
+    config.gridDim = dim3(ctas, kRows * (D / 4) / kJoinThreads);
+    config.blockDim = dim3(kJoinThreads);
     config.stream = s;
     cudaLaunchAttribute early;
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
-    config.numAttrs = MODE == kCommon ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a, static_cast<int>(row_tiles), 1);
-    if (e != cudaSuccess) return e;
-    // its blocks may start once the CTAs have exited, before that kernel's end is signalled
-    // (it gives no earlier trigger): they wait for that
-    config.gridDim = dim3(ctas, kRows * (D / 4) / kJoinThreads);
-    config.blockDim = dim3(kJoinThreads);
-    config.dynamicSmemBytes = 0;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, join_kernel<T, D, MODE>, a, ctas);
-}
-
-template <int MODE>
-cudaError_t launch_type(const AttendArgs& a, int dtype, int sms, cudaStream_t s) {
-    if (a.head_dim == 64)
-        return dtype == UFB_F16 ? launch<__half, 64, MODE>(a, sms, s) : launch<__nv_bfloat16, 64, MODE>(a, sms, s);
-    return dtype == UFB_F16 ? launch<__half, 128, MODE>(a, sms, s) : launch<__nv_bfloat16, 128, MODE>(a, sms, s);
+    return cudaLaunchKernelEx(&config, join_kernel<T, D>, a, ctas);
 }
 
 }  // namespace
 
-cudaError_t attend_many(const AttendArgs& a, int mode, int dtype, int sms, cudaStream_t s) {
-    return mode == kAll   ? launch_type<kAll>(a, dtype, sms, s)
-           : mode == kOwn ? launch_type<kOwn>(a, dtype, sms, s)
-                          : launch_type<kCommon>(a, dtype, sms, s);
+cudaError_t attend_many(const AttendArgs& a, int dtype, int sms, cudaStream_t s) {
+    if (a.head_dim == 64)
+        return dtype == UFB_F16 ? launch<__half, 64>(a, sms, s) : launch<__nv_bfloat16, 64>(a, sms, s);
+    return dtype == UFB_F16 ? launch<__half, 128>(a, sms, s) : launch<__nv_bfloat16, 128>(a, sms, s);
 }
 
 }  // namespace ufb

@@ -497,70 +497,83 @@ __global__ void __launch_bounds__(kApplyThreads) reorder_apply_kernel(const ufb_
 
 // What the streams of group blockIdx.x have in common: the leading entries that are equal
 // in all their tables, inside of every one's earlier tokens.  Streams that bring no tokens,
-// or whose extend was refused, do not count.
-__global__ void __launch_bounds__(256) share_kernel(const ufb_kv_cache c, const KvBatch b, const ufb_kv_groups g,
-                                                    const KvGroupState out, int* status) {
+// or whose extend was refused, do not count.  Then how many tiles of own keys the streams
+// have, summed up over the group.
+__global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, const KvBatch b, const ufb_kv_groups g,
+                                                         const KvGroupState out, int* status) {
+    __shared__ int warp_sum[kWarps];
     __shared__ int width, lowest, highest, members, chosen;
     const int group = blockIdx.x, first = max(g.first[group], 0), end = min(g.first[group + 1], b.n);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) width = c.table_width, lowest = INT_MAX, highest = -1, members = 0, chosen = INT_MAX;
     __syncthreads();
-    for (int i = first + threadIdx.x; i < end; i += 256) {
+    // of stream i: its slot, -1 when something is out of range, -2 when it does not count
+    int start = 0, count = 0;
+    auto look = [&](int i) {
         const int slot = b.slots[i], o0 = b.offsets[i], o1 = b.offsets[i + 1];
-        if (!valid_slot(c, slot) || o0 < 0 || o1 < o0 || o1 > b.tokens || o1 - o0 > b.max_new) {
+        if (!valid_slot(c, slot) || o0 < 0 || o1 < o0 || o1 > b.tokens || o1 - o0 > b.max_new) return -1;
+        count = o1 - o0;
+        start = c.lengths[slot] - count;
+        return kv_refused(c)[slot] != 0 || count == 0 ? -2 : slot;
+    };
+    for (int i = first + threadIdx.x; i < end; i += kThreads) {
+        const int slot = look(i);
+        if (slot == -1) {
             atomicCAS(status, 0, kStatusIndex);
-            continue;
-        }
-        const bool refused = kv_refused(c)[slot] != 0;
-        const int start = c.lengths[slot] - (o1 - o0);
-        if (!refused && o1 > o0 && start >= 0) {
+        } else if (slot >= 0) {
             atomicAdd(&members, 1);
             atomicMin(&chosen, i);
-            atomicMin(&width, start / c.page_tokens);
+            atomicMin(&width, max(start, 0) / c.page_tokens);
             atomicMin(&lowest, start);
-            atomicMax(&highest, c.lengths[slot] - 1);
-        } else if (o1 > o0) {
+            atomicMax(&highest, start + count - 1);
+        } else if (count > 0) {
             atomicMin(&lowest, -1);
+            atomicCAS(status, 0, kStatusPages);
         }
-    }
-    // positions: a warp to a stream
-    for (int i = first + (threadIdx.x >> 5); i < end; i += 8) {
-        const int slot = b.slots[i], o0 = b.offsets[i], o1 = b.offsets[i + 1];
-        const bool ok = valid_slot(c, slot) && o0 >= 0 && o1 >= o0 && o1 <= b.tokens && o1 - o0 <= b.max_new;
-        const int start = ok ? c.lengths[slot] - (o1 - o0) : 0;
-        const bool none = ok && (start < 0 || kv_refused(c)[slot]);
-        for (int t = max(o0, 0) + (threadIdx.x & 31); t < o1 && t < b.tokens; t += 32)
-            out.positions[t] = !ok ? -2 : none ? -1 : start + t - o0;
     }
     __syncthreads();
-    int common = 0;
-    if (members > 1) {
-        const int most = width;
-        const int32_t* row = c.table + static_cast<long long>(b.slots[chosen]) * c.table_width;
-        bool all = true;
-        for (int e0 = 0; e0 < most && all; e0 += 256) {
-            const int e = e0 + threadIdx.x;
-            bool same = true;
-            if (e < most) {
-                const int page = row[e];
-                for (int i = chosen + 1; i < end && same; ++i) {
-                    const int slot = b.slots[i];
-                    if (!valid_slot(c, slot) || kv_refused(c)[slot] || b.offsets[i + 1] <= b.offsets[i]) continue;
-                    same = c.table[static_cast<long long>(slot) * c.table_width + e] == page;
-                }
-                if (!same) atomicMin(&width, e);
-            }
-            all = __syncthreads_and(same);
+    const int most = width;
+    // a warp to a stream: its positions, and where its table first differs from the chosen one's
+    for (int i = first + warp; i < end; i += kWarps) {
+        const int slot = look(i), o0 = b.offsets[i], o1 = b.offsets[i + 1];
+        for (int t = max(o0, 0) + lane; t < o1 && t < b.tokens; t += 32) {
+            out.positions[t] = slot == -1 ? kNotWritten : slot == -2 ? -1 : start + t - o0;
+            out.stream[t] = i;
         }
-        common = width;
+        if (slot < 0 || members < 2 || i == chosen) continue;
+        const int32_t* own = c.table + static_cast<long long>(slot) * c.table_width;
+        const int32_t* other = c.table + static_cast<long long>(b.slots[chosen]) * c.table_width;
+        for (int e0 = 0; e0 < most; e0 += 128) {
+            int differs = INT_MAX;
+#pragma unroll
+            for (int j = 3; j >= 0; --j) {
+                const int e = e0 + j * 32 + lane;
+                if (e < most && own[e] != other[e]) differs = e;
+            }
+            differs = __reduce_min_sync(0xffffffffu, differs);
+            if (differs != INT_MAX) {
+                if (lane == 0) atomicMin(&width, differs);
+                break;
+            }
+        }
     }
-    const int shared = common * c.page_tokens;
+    __syncthreads();
+    const int shared = members > 1 ? width * c.page_tokens : 0;
+    int sum = 0;
+    for (int i0 = first; i0 < end; i0 += kThreads) {
+        const int i = i0 + threadIdx.x, slot = i < end ? look(i) : -1;
+        int total;
+        const int tiles = slot >= 0 ? (start + count - shared + kGroupTileKeys - 1) / kGroupTileKeys : 0;
+        const int before = block_scan(tiles, warp_sum, total);
+        if (i < end) out.tiles[i] = sum + before + tiles;
+        sum += total;
+    }
     if (threadIdx.x == 0) {
         out.shared[group] = shared;
-        out.slot[group] = members ? b.slots[chosen] : first < end ? b.slots[first] : -1;
+        out.slot[group] = members ? b.slots[chosen] : 0;
         out.low[group] = lowest == INT_MAX ? -1 : lowest;
         out.high[group] = highest;
     }
-    for (int i = first + threadIdx.x; i < end; i += 256) out.starts[i] = shared;
 }
 
 template <bool PARTIAL>
@@ -626,7 +639,7 @@ cudaError_t kv_reorder(const ufb_kv_cache& c, const int32_t* slots, const int32_
 }
 
 cudaError_t kv_share(const ufb_kv_cache& c, const KvBatch& b, const ufb_kv_groups& g, int* status, cudaStream_t s) {
-    share_kernel<<<g.groups, 256, 0, s>>>(c, b, g, kv_group_state(g, b.n), status);
+    share_kernel<<<g.groups, kThreads, 0, s>>>(c, b, g, kv_group_state(g, b.n, b.tokens), status);
     return cudaGetLastError();
 }
 

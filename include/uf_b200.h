@@ -446,7 +446,7 @@ int ufb_conv2d_noalloc(const int16_t* x, int n, int ci, int h, int w, const int1
  *   32 a slot, page or token offset out of range, or a page that is missing
  *      where tokens are to be stored (what it names is skipped; reorder, with a
  *      parent out of range too: nothing was changed)
- *   41..44 a bounded wait of the attention kernel gave up
+ *   41..45 a bounded wait of the attention kernels gave up
  *   51 a row of logits holds NaN or +infinity (its beam has no continuations)
  * ------------------------------------------------------------------------- */
 
@@ -611,18 +611,18 @@ int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens);
 /* Find what each group has in common: the leading table entries that are equal in
  * all its streams, as far as they lie before every stream's new tokens (streams
  * that bring none, or whose extend was refused, do not count; none in a group of
- * one).  state[g] are the tokens on them.  Once a step, behind ufb_kv_extend: it holds
+ * one; status 31 for one whose extend was refused: its queries see no key).  state[g]
+ * are the tokens on them.  Once a step, behind ufb_kv_extend: it holds
  * until a call changes tables or lengths. */
 int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, int max_new,
                  int64_t tokens, const ufb_kv_groups* groups, void* stream);
 
 /* ufb_kv_attend, which reads the pages that the streams of a group have in common
- * (ufb_kv_share) once for all of them: attention over the common keys and over the
- * stream's own, joined by their sums of exponentials in 32 bits.  parts:
- * tokens * q heads * (head_dim + 1) floats of scratch, 16-byte aligned. */
+ * (ufb_kv_share) once for all of them: made for branches that go on by few tokens of
+ * their own (every own key takes the work that 128 rows take). */
 int ufb_kv_attend_groups(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n,
                          int max_new, int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse,
-                         int window, int sinks, int causal, float scale, const ufb_kv_groups* groups, float* parts,
+                         int window, int sinks, int causal, float scale, const ufb_kv_groups* groups,
                          void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Workspace of ufb_kv_attend on the current device, in bytes. */

@@ -33,9 +33,9 @@ def test_group_refusals(att):  # noqa: F811
     def share(g, n=4, max_new=2, tokens=5, slots=4096, offsets=4096):
         return L.ufb_kv_share(c, slots, offsets, n, max_new, tokens, C.byref(g) if g else None, None)
 
-    def attend(g, parts=4096, workspace=None, room=0, layer=0, window=0):
+    def attend(g, workspace=None, room=0, layer=0, window=0):
         return L.ufb_kv_attend_groups(c, layer, 4096, 4096, 4, 2, 5, 1, C.byref(q), C.byref(q), None, window, 0, 1, 1.0,
-                                      C.byref(g) if g else None, parts, workspace, room, None)
+                                      C.byref(g) if g else None, workspace, room, None)
 
     for g in (None, groups(first=None), groups(offsets=None), groups(state=None), groups(n=-1), groups(n=0), groups(n=5),
               groups(most=1), groups(most=6)):
@@ -46,6 +46,6 @@ def test_group_refusals(att):  # noqa: F811
     assert share(groups(n=0, first=None, most=0), n=0, max_new=0, tokens=0) == 0
     for over in (dict(layer=2), dict(layer=-1), dict(window=-1)):
         assert attend(groups(), **over) == EINVAL, over
-    assert L.ufb_kv_group_ints(2, 4, 5) == 4 * 2 + 4 + 5
+    assert L.ufb_kv_group_ints(2, 4, 5) == 4 * 2 + 4 + 2 * 5
     for args in ((-1, 4, 5), (2, -1, 5), (2, 4, -1), (2, 4, 1 << 31)):
         assert L.ufb_kv_group_ints(*args) == EINVAL
