@@ -9,18 +9,18 @@
 // each stream's own keys, which only that stream's rows see.  Nothing has to be joined
 // but what CTAs share, and a step of a search is one launch and its join.
 //
-// One CTA an SM, five roles:
-//   walker (1 warp)      says of each tile ahead where its keys are and who sees them
+// One CTA an SM, six roles:
+//   walker (1 warp)      says of each tile ahead which pages hold its keys and who sees them
 //   converter (8 warps)  integers from global memory through registers to float16 in
 //                        shared memory, keys and values double buffered
 //   MMA (1 warp)         S of the next tile before P V of this one: two tiles of scores
-//                        in tensor memory, one of sums
-//   softmax (2 x 4 warps) two threads to a row, 64 columns each, which stay in registers
-//                        between the maximum and the weights; the two exchange maxima
-//                        through shared memory.  P goes back over S in float16.
-// Rows are few here, so a tile's time is the way through its steps, and two threads to a
-// row make the longest of them half as long as one does.  Warps whose rows are padding
-// skip the softmax.
+//                        in tensor memory, two of sums
+//   softmax (2 x 4 warps) a thread to a row; the two sets take every other tile, each
+//                        with a maximum and sums of its own, so that one exponentiates
+//                        while the other loads or waits.  P goes back over S in float16.
+//   scales (1 warp)      of each 16 keys, a tile ahead
+// The two sums of a row become one at a piece's end.  Warps whose rows are padding, or no
+// rows of an own tile's stream, skip the softmax.
 #include "kv_attend.cuh"
 #include "umma.cuh"
 
@@ -33,12 +33,16 @@ namespace {
 constexpr int kRows = 128;
 constexpr int kKeys = kGroupTileKeys;
 constexpr int kGroups = kKeys / kGroupKeys;
-constexpr int kMmaWarp = 16, kWalkWarp = 17;
-constexpr int kThreads = 640;         // warps: softmax 0-7, converter 8-15, MMA 16, walker 17; 18, 19 idle
+constexpr int kMmaWarp = 16, kWalkWarp = 17, kScaleWarp = 18;
+constexpr int kThreads = 640;         // warps: softmax 0-7, converter 8-15, MMA 16, walker 17, scales 18; 19 idle
 constexpr int kPieces = 4;            // pieces announced ahead
 constexpr int kTiles = 8;             // tiles announced ahead
 constexpr int kScaleRing = 4;
 constexpr int kCode = 45;
+// A wait gives up after so many looks at its barrier; the hardware holds each for about 300
+// cycles, so that is a second or so.  (A clock in every wait took three times the instructions,
+// and the roles share the instruction caches.)
+constexpr int kPolls = 1 << 22;
 // As in kv_attend_many.cu: a running maximum stays while it grows by less than 2^kSlack, P is
 // taken times 2^kShift, rows with scores beyond kFar round the score before the maximum is
 // taken off.
@@ -63,13 +67,14 @@ struct GroupTile {
 // A piece of an item as the walker announces it; rows 0: there is none any more.
 struct Announced {
     int rows, row0, token0, head, parts, part;
+    int count;              // its tiles
 };
 // A tile of a piece.
 struct Tile {
     int slot, key0, head;
     int limit;              // keys below it are there
     int row_low, row_high;  // rows that may see it
-    int groups;             // 16-key groups that are looked at, a bit each
+    int page[kGroups];      // of each 16 keys; -1: not looked at, or not there
     int flags;              // kFirst, kLast of the piece; kClear: all its rows see all of it; kOwnKeys
 };
 constexpr int kFirst = 1, kLast = 2, kClear = 4, kOwnKeys = 8, kNone = 16;
@@ -80,8 +85,7 @@ struct Smem {
     alignas(1024) uint8_t k[2][kKeys * D * 2];
     alignas(1024) uint8_t v[2][kKeys * D * 2];
     GroupScales scales[kScaleRing][kGroups];
-    float top[2][2][kRows];                        // by tile parity, half
-    float row[2][2][kRows];                        // of a piece: largest |q| and what is not finite; weights
+    float row[2][2][kRows];                        // by parity: largest |q|, then maxima; weights
     alignas(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2];
     uint64_t q_full, o_full, drained, pair[4];
     uint64_t piece_full[kPieces], piece_empty[kPieces], tile_full[kTiles], tile_empty[kTiles];
@@ -95,7 +99,7 @@ struct Smem {
 template <int D>
 struct Tmem {
     __device__ static constexpr uint32_t s(int b) { return b * 128; }
-    static constexpr uint32_t kO = 256;
+    __device__ static constexpr uint32_t o(int b) { return 256 + b * D; }
 };
 
 // Address of row `row`, 16-byte chunk `chunk` (8 float16) of a [D / 64][128][128 bytes] tile.
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sm.k_full[i], 128);
+            mbar_init(&sm.k_full[i], 129);
             mbar_init(&sm.v_full[i], 128);
             mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         }
         for (int i = 0; i < kTiles; ++i) {
             mbar_init(&sm.tile_full[i], 1);
-            mbar_init(&sm.tile_empty[i], 17);
+            mbar_init(&sm.tile_empty[i], 14);
         }
         fence_mbar_init();
         sm.dead = (smem_u32(raw) & 1023) != 0;
@@ -236,8 +240,13 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     volatile int* dead = &sm.dead;
     // after a wait gave up nobody waits any more, and no further tile is begun
     auto wait = [&](uint64_t* bar, int phase) {
-        if (mbar_try_wait(bar, phase & 1)) return;
-        if (!*dead && !mbar_wait(bar, phase & 1, a.status, kCode)) *dead = 1;
+        for (int polls = 0; !mbar_try_wait(bar, phase & 1); ++polls) {
+            if (*dead) return;
+            if (polls == kPolls) {
+                atomicCAS(a.status, 0, kCode);
+                *dead = 1;
+            }
+        }
     };
     // Tiles one after another; a reader gives each back when it is done with it.
     auto tile_info = [&](int n) -> const Tile& {
@@ -245,17 +254,20 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         __syncwarp();
         return sm.tiles[n % kTiles];
     };
-    auto tile_done = [&](int n) {
+    // what the warp's lanes did before is seen by those that wait
+    auto arrive = [&](uint64_t* bar) {
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.tile_empty[n % kTiles]);
+        if (lane == 0) mbar_arrive(bar);
     };
+    auto tile_done = [&](int n) { arrive(&sm.tile_empty[n % kTiles]); };
 
     // the registers of 640 threads at 96: 2 x 128 + 2 x 72 + 80 = 5 x 96
     if (warp < 8) {
         regs_inc<128>();
-        // ---- softmax: row of the tile = lane of tensor memory, half of the columns
-        const int half = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        // ---- softmax: the tiles of parity t, each into sums of its own; row = lane of tensor memory
+        const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t ts = tmem + lanes + Tmem<D>::s(t), to = tmem + lanes + Tmem<D>::o(t);
         const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
         if (threadIdx.x == 0) scratch.items[blockIdx.x * 8] = 0;
         // the two warps that share rows meet, in tensor memory too
@@ -267,93 +279,97 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             __syncwarp();
             tc_fence_after();
         };
-        int pieces = -1, pos = 0, head = 0, token = 0;
-        bool real = false, busy = false, write = false;   // this row, a row of this warp: of the piece
-        bool far = false;
-        float unit = 0.0f, m = -INFINITY, l = 0.0f;
-        for (int n = 0;; ++n) {
-            const Tile& tile = tile_info(n);
-            const int flags = tile.flags, b = n & 1;
-            if ((flags & kNone) || *dead) break;
-            if (flags & kFirst) {
-                ++pieces;
-                wait(&sm.piece_full[pieces % kPieces], pieces / kPieces);
-                __syncwarp();
-                const Announced& p = sm.pieces[pieces % kPieces];
-                real = row < p.rows;
-                busy = quarter * 32 < p.rows;
-                const int in_group = p.row0 + (real ? row : 0);
-                token = in_group / a.group;
-                head = p.head * a.group + in_group - token * a.group;
-                token += p.token0;
-                pos = real ? g.state.positions[token] : -1;
-                write = real && pos != kNotWritten;
-                if (!write) pos = -1;
-                m = -INFINITY, l = 0.0f;
-                far = false;
-                if (busy) {
-                    // half of the row's dims to [2^15, 2^16) and float16; the softmax scale's sign goes with it
-                    const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + static_cast<long long>(token) * a.q.token_stride +
-                                                                      head * a.q.head_stride) + half * (D / 16);
-                    uint4 v[D / 16];
-                    float top = 0.0f, odd = 0.0f;
+        int first = 0;   // number of the piece's first tile among this CTA's
+        for (int piece = 0;; ++piece) {
+            wait(&sm.piece_full[piece % kPieces], piece / kPieces);
+            __syncwarp();
+            const Announced& p = sm.pieces[piece % kPieces];
+            if (p.rows == 0 || *dead) break;
+            const int count = p.count;
+            const bool real = row < p.rows;
+            const bool busy = quarter * 32 < p.rows;
+            const int in_group = p.row0 + (real ? row : 0);
+            int token = in_group / a.group;
+            const int head = p.head * a.group + in_group - token * a.group;
+            token += p.token0;
+            int pos = real ? g.state.positions[token] : -1;
+            const bool write = real && pos != kNotWritten;
+            if (!write) pos = -1;
+            float unit = 0.0f, m = -INFINITY, l = 0.0f;
+            bool far = false;   // a row of the warp has scores beyond kFar
+            if (busy) {
+                // half of the row's dims to [2^15, 2^16) and float16; the softmax scale's sign goes with it
+                const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + static_cast<long long>(token) * a.q.token_stride +
+                                                                  head * a.q.head_stride) + t * (D / 16);
+                uint4 v[D / 16];
+                float top = 0.0f, odd = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) v[i] = real ? vec[i] : make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < D / 16; ++i) v[i] = real ? vec[i] : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 f = unpack2(x[j], T());
-                            top = max3(top, fabsf(f.x), fabsf(f.y));
-                            odd += (f.x - f.x) + (f.y - f.y);  // NaN for what is not finite
-                        }
-                    }
-                    sm.row[0][half][row] = odd == odd ? top : odd;
-                    pair_sync();
-                    const float other = sm.row[0][half ^ 1][row];
-                    const float u = row_unit(odd == odd && other == other ? fmaxf(top, other) : __int_as_float(0x7fffffff));
-                    unit = unit_inverse(u) * fabsf(a.scale_log2);
-                    const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                        uint32_t y[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 f = unpack2(x[j], T());
-                            y[j] = pack2(f.x * mul, f.y * mul, __half());
-                        }
-                        *reinterpret_cast<uint4*>(sm.q + tile_at(row, half * (D / 16) + i)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = unpack2(x[j], T());
+                        top = max3(top, fabsf(f.x), fabsf(f.y));
+                        odd += (f.x - f.x) + (f.y - f.y);  // NaN for what is not finite
                     }
                 }
-                fence_proxy_async_smem();
-                mbar_arrive(&sm.q_full);
+                sm.row[0][t][row] = odd == odd ? top : odd;
+                pair_sync();
+                const float other = sm.row[0][t ^ 1][row];
+                const float u = row_unit(odd == odd && other == other ? fmaxf(top, other) : __int_as_float(0x7fffffff));
+                unit = unit_inverse(u) * fabsf(a.scale_log2);
+                const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                    uint32_t y[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = unpack2(x[j], T());
+                        y[j] = pack2(f.x * mul, f.y * mul, __half());
+                    }
+                    *reinterpret_cast<uint4*>(sm.q + tile_at(row, t * (D / 16) + i)) = make_uint4(y[0], y[1], y[2], y[3]);
+                }
             }
-            wait(&sm.s_full[b], n >> 1);
-            __syncwarp();
-            tc_fence_after();
-            const int key0 = tile.key0;
-            const uint32_t ts = tmem + lanes + Tmem<D>::s(b), tp = ts + half * 32;
-            // rows of this warp that the tile is for
-            const bool mine = busy && tile.row_low < quarter * 32 + 32 && tile.row_high > quarter * 32;
-            if (mine) {
-                const GroupScales* sc = sm.scales[n % kScaleRing] + half * 4;
-                uint32_t s0[32], s1[32];
-                tmem_ld32(ts + half * 64, s0);
-                tmem_ld32(ts + half * 64 + 32, s1);
+            fence_proxy_async_smem();
+            mbar_arrive(&sm.q_full);
+            for (int n = first + ((first ^ t) & 1); n < first + count; n += 2) {
+                const Tile& tile = tile_info(n);
+                const int key0 = tile.key0, limit = tile.limit, flags = tile.flags, row_low = tile.row_low, row_high = tile.row_high;
+                wait(&sm.s_full[t], n >> 1);
+                __syncwarp();
+                tc_fence_after();
+                tile_done(n);
+                // rows of this warp that the tile is for
+                const bool mine = busy && row_low < quarter * 32 + 32 && row_high > quarter * 32;
+                if (!mine) {
+                    // rows of other streams: no weight.  (Padding's weights do not matter.)
+                    if (busy) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) w[j] = 0;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) tmem_st16(ts + c * 16, w);
+                        tmem_wait_st();
+                    }
+                    tc_fence_before();
+                    mbar_arrive(&sm.p_full[t][0]);
+                    mbar_arrive(&sm.p_full[t][1]);
+                    continue;
+                }
+                const GroupScales* sc = sm.scales[n % kScaleRing];
                 // columns [0, high) that are from low on or below sink are seen by this row
-                const bool ours = row >= tile.row_low && row < tile.row_high;
-                const int limit = tile.limit;
-                const int high = ours ? min(limit, a.causal || !(flags & kOwnKeys) ? pos + 1 : limit) - key0 - half * 64 : 0;
-                const int low = a.window ? max(pos - a.window + 1, 0) - key0 - half * 64 : 0;
-                const int sink = a.window ? a.sinks - key0 - half * 64 : 0;
+                const bool ours = row >= row_low && row < row_high;
+                const int high = ours ? min(limit, a.causal || !(flags & kOwnKeys) ? pos + 1 : limit) - key0 : 0;
+                const int low = a.window ? max(pos - a.window + 1, 0) - key0 : 0;
+                const int sink = a.window ? a.sinks - key0 : 0;
                 auto seen = [&](int c) {   // of 32 columns, a bit each
                     return bits_below(high - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
                 };
-                tmem_wait_ld();
-                tmem_tie32(s0);
-                tmem_tie32(s1);
+                // 64 columns at a time, the later ones first: the others stay for their weights
+                uint32_t s0[32], s1[32];
                 float top = -INFINITY;
                 auto maximum = [&](auto masked) {
                     auto chunk = [&](int c, const uint32_t (&s)[32]) {
@@ -374,35 +390,33 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                             top = fmaxf(top, decltype(masked)::value && y == -INFINITY ? y : v);
                         }
                     };
-                    chunk(0, s0);
-                    chunk(1, s1);
+#pragma unroll 1
+                    for (int c = 2; c >= 0; c -= 2) {
+                        tmem_ld32(ts + c * 32, s0);
+                        tmem_ld32(ts + c * 32 + 32, s1);
+                        tmem_wait_ld();
+                        tmem_tie32(s0);
+                        tmem_tie32(s1);
+                        chunk(c, s0);
+                        chunk(c + 1, s1);
+                    }
                 };
                 const bool clear = flags & kClear;
                 if (clear) maximum(std::false_type());
                 else maximum(std::true_type());
-                // all scores of these rows are in registers behind this: P may go over them
-                sm.top[b][half][row] = top;
-                pair_sync();
-                top = fmaxf(top, sm.top[b][half ^ 1][row]);
-                // the maximum stays while it is within 2^kSlack
+                // the maximum stays while it is within 2^kSlack; these sums' last product was before these scores
                 const bool grow = top > __fadd_rd(m, kSlack);
                 if (__any_sync(0xffffffffu, grow)) {
                     if (__any_sync(0xffffffffu, grow && m != -INFINITY)) {
                         const float keep = grow && m != -INFINITY ? ex2(m - top) : 1.0f;
-                        // the product before this has to be in the sums
-                        if (!(flags & kFirst)) {
-                            wait(&sm.v_empty[(n - 1) & 1], (n - 1) >> 1);
-                            __syncwarp();
-                            tc_fence_after();
-                        }
 #pragma unroll 1
-                        for (int c = half * (D / 32); c < (half + 1) * (D / 32); ++c) {
+                        for (int c = 0; c < D / 16; ++c) {
                             uint32_t o[16];
-                            tmem_ld16(tmem + lanes + Tmem<D>::kO + c * 16, o);
+                            tmem_ld16(to + c * 16, o);
                             tmem_wait_ld_regs(o);
 #pragma unroll
                             for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-                            tmem_st16(tmem + lanes + Tmem<D>::kO + c * 16, o);
+                            tmem_st16(to + c * 16, o);
                         }
                         l *= keep;
                     }
@@ -411,6 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 }
                 const float base = m == -INFINITY ? 0.0f : __fsub_ru(m, kShift);
                 auto weights = [&](auto masked) {
+                    // 32 columns: P, the row's weight
                     auto chunk = [&](int c, uint32_t (&s)[32]) {
                         const uint32_t bits = decltype(masked)::value ? seen(c) : 0u;
                         uint32_t w[16];
@@ -436,71 +451,86 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                             sum[0] += sum[1];
                             if (sum[0] != 0.0f) l = fmaf(sum[0], gs.inv_value, l);
                         }
-                        tmem_st16(tp + c * 16, w);
+                        tmem_st16(ts + c * 16, w);
                     };
-                    chunk(0, s0);
-                    chunk(1, s1);
+                    // the next columns are on their way while these are worked on
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        tmem_wait_ld();
+                        tmem_tie32(s0);
+                        tmem_tie32(s1);
+                        chunk(half * 2, s0);
+                        if (half == 0) tmem_ld32(ts + 64, s0);
+                        chunk(half * 2 + 1, s1);
+                        if (half == 0) tmem_ld32(ts + 96, s1);
+                        // P V starts on the first 64 keys while the others are in the works
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(&sm.p_full[t][half]);
+                    }
                 };
                 if (clear && !far) weights(std::false_type());
                 else weights(std::true_type());
-                tmem_wait_st();
-            } else if (busy) {
-                // rows of other streams: no weight.  (Padding's weights do not matter.)
-                uint32_t w[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) w[j] = 0;
-                tmem_st16(tp, w);
-                tmem_st16(tp + 16, w);
-                tmem_wait_st();
             }
-            tc_fence_before();
-            mbar_arrive(&sm.p_full[b][half]);
-            tile_done(n);
-            if (!(flags & kLast)) continue;
+            first += count;
 
-            // ---- the piece's rows
-            if (busy) sm.row[1][half][row] = l;
-            wait(&sm.o_full, pieces);
+            // ---- the piece's rows: both sums, half of the dims each
+            if (busy) {
+                sm.row[0][t][row] = m;
+                sm.row[1][t][row] = l;
+            }
+            wait(&sm.o_full, piece);
             __syncwarp();
             tc_fence_after();
-            const Announced& p = sm.pieces[pieces % kPieces];
             if (busy) {
                 pair_sync();
-                l = sm.row[1][0][row] + sm.row[1][1][row];
+                const float m0 = sm.row[0][0][row], m1 = sm.row[0][1][row], l0 = sm.row[1][0][row], l1 = sm.row[1][1][row];
+                const float top = fmaxf(m0, m1);
+                // a part that saw nothing has no weight; one that is not finite spoils its row
+                const float e0 = m0 == -INFINITY ? (l0 == 0.0f ? 0.0f : 1.0f) : ex2(m0 - top);
+                const float e1 = m1 == -INFINITY ? (l1 == 0.0f ? 0.0f : 1.0f) : ex2(m1 - top);
+                const float weight = (e0 == 0.0f ? 0.0f : l0 * e0) + (e1 == 0.0f ? 0.0f : l1 * e1);
                 const bool whole = p.part < 0;
                 const int part = 2 * blockIdx.x + p.part;
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const float inv = !whole ? 1.0f : weight == 0.0f ? 0.0f : 1.0f / weight;
                 T* out = static_cast<T*>(a.out.data) + static_cast<long long>(token) * a.out.token_stride + head * a.out.head_stride;
                 float* sums = scratch.sums + (static_cast<long long>(part) * kRows + row) * D;
 #pragma unroll 1
-                for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
-                    uint32_t o[32];
-                    tmem_ld32(tmem + lanes + Tmem<D>::kO + c * 32, o);
-                    tmem_wait_ld();
-                    tmem_tie32(o);
+                for (int c = t * (D / 32); c < (t + 1) * (D / 32); ++c) {
+                    uint32_t x[16], y[16];
+                    tmem_ld16(tmem + lanes + Tmem<D>::o(0) + c * 16, x);
+                    tmem_ld16(tmem + lanes + Tmem<D>::o(1) + c * 16, y);
+                    tmem_wait_ld_regs(x);
+                    tmem_wait_ld_regs(y);
+                    float o[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        // sums that hold nothing of this piece are not looked at
+                        const float u = e0 == 0.0f ? 0.0f : __uint_as_float(x[j]) * e0;
+                        o[j] = (e1 == 0.0f ? u : fmaf(__uint_as_float(y[j]), e1, u)) * inv;
+                    }
                     if (write && whole) {
+                        uint32_t w[8];
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                w[i] = pack2(__uint_as_float(o[j + 2 * i]) * inv, __uint_as_float(o[j + 2 * i + 1]) * inv, T());
-                            reinterpret_cast<uint4*>(out)[c * 4 + j / 8] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        for (int i = 0; i < 8; ++i) w[i] = pack2(o[2 * i], o[2 * i + 1], T());
+                        reinterpret_cast<uint4*>(out)[c * 2] = make_uint4(w[0], w[1], w[2], w[3]);
+                        reinterpret_cast<uint4*>(out)[c * 2 + 1] = make_uint4(w[4], w[5], w[6], w[7]);
                     } else if (real && !whole) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            __stcg(reinterpret_cast<uint4*>(sums + c * 32 + j), make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+                        for (int j = 0; j < 16; j += 4)
+                            __stcg(reinterpret_cast<float4*>(sums + c * 16 + j), make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
                     }
                     __syncwarp();
                 }
-                if (half == 0 && write && whole && a.lse)
+                if (t == 0 && write && whole && a.lse)
                     a.lse[static_cast<long long>(token) * (a.heads * a.group) + head] =
-                        l == 0.0f ? -INFINITY : (m - kShift + log2f(l)) * 0.6931471805599453f;
-                if (half == 0 && real && !whole) {
-                    __stcg(scratch.stats + (part * 2) * kRows + row, m);
-                    __stcg(scratch.stats + (part * 2 + 1) * kRows + row, l);
+                        weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
+                if (t == 0 && real && !whole) {
+                    __stcg(scratch.stats + (part * 2) * kRows + row, top);
+                    __stcg(scratch.stats + (part * 2 + 1) * kRows + row, weight);
                 }
+                // the next piece's queries and sums wait until both warps have read these
+                pair_sync();
             }
             if (p.parts && threadIdx.x == 0) {
                 int32_t* item = scratch.items + blockIdx.x * 8;
@@ -510,8 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 item[4] = p.head;
                 item[0] = p.parts;
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.piece_empty[pieces % kPieces]);
+            arrive(&sm.piece_empty[piece % kPieces]);
             tc_fence_before();
         }
     } else if (warp < kMmaWarp) {
@@ -549,22 +578,19 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             n.head = t.head;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int key = t.key0 + w * 32 + i * kGroupKeys, entry = key >> a.page_shift;
-                n.row[i] = key & (a.page_tokens - 1);
-                if ((t.groups >> (w * 2 + i) & 1) && entry < a.table_width)
-                    n.page[i] = a.table[static_cast<long long>(t.slot) * a.table_width + entry];
+                n.row[i] = (t.key0 + w * 32 + i * kGroupKeys) & (a.page_tokens - 1);
+                n.page[i] = t.page[w * 2 + i];
             }
             tile_done(looked++);
         };
         uint4 buf[kLoads];
-        float key_scale = 0.0f, value_scale = -1.0f;   // of the warp's group `lane` (0, 1); -1: not there
         auto load = [&](const Next& n) {
             if (!n.tile) return;
             const int8_t* from[2];
             bool there[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                there[i] = n.page[i] >= 0 && n.page[i] < a.pages;
+                there[i] = n.page[i] >= 0;
                 const long long tile = (static_cast<long long>(n.page[i]) * 2 + side) * a.heads + n.head;
                 from[i] = a.kv + ((tile << a.page_shift) + n.row[i] + sub) * D + chunk * 16;
             }
@@ -578,16 +604,6 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     buf[i] = make_uint4(0, 0, 0, 0);
                     if (there[(i * kStep) >> 4])
                         buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
-                }
-            }
-            if (side == 0 && lane < 2) {
-                key_scale = 0.0f, value_scale = -1.0f;
-                if (lane == 0 ? there[0] : there[1]) {
-                    const int page = lane == 0 ? n.page[0] : n.page[1];
-                    const float* s = a.scale + static_cast<long long>(page) * 2 * a.heads + n.head;
-                    key_scale = s[0];
-                    value_scale = s[a.heads];
-                    if (value_scale < kTinyScale) value_scale = kTinyScale;
                 }
             }
         };
@@ -609,14 +625,6 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 *reinterpret_cast<uint4*>(to + at0[i & 1] + step) = make_uint4(y[0], y[1], y[2], y[3]);
                 *reinterpret_cast<uint4*>(to + at1[i & 1] + step) = make_uint4(y[4], y[5], y[6], y[7]);
             }
-            if (side == 0 && lane < 2) {
-                GroupScales s;
-                s.key = key_scale;
-                s.log2_value = value_scale == -1.0f ? -INFINITY : log2f(value_scale);
-                s.inv_value = value_scale == -1.0f ? 0.0f : 1.0f / value_scale;
-                s.pad = 0.0f;
-                sm.scales[n % kScaleRing][w * 2 + lane] = s;
-            }
             fence_proxy_async_smem();
             mbar_arrive(&full[b]);
             load(next);
@@ -635,8 +643,8 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             walk.pair = share.pair;
             walk.pair_start = share.pair_start;
             walk.loaded = false;
-            int n = 0;
-            for (int piece = 0; !*dead && walk.next(a, g); ++piece) {
+            int n = 0, piece = 0;
+            for (; !*dead && walk.next(a, g); ++piece) {
                 const GroupTile& t = walk.t;
                 if (piece >= kPieces) wait(&sm.piece_empty[piece % kPieces], piece / kPieces - 1);
                 if (lane == 0) {
@@ -645,6 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     o.row0 = t.row0;
                     o.token0 = t.token0;
                     o.head = walk.head;
+                    o.count = walk.last - walk.first;
                     // the part of a shared item: 0 where an earlier CTA began it, 1 where this
                     // one does, which then tells how many parts there are
                     const bool whole = walk.first == 0 && walk.last == t.nt;
@@ -656,6 +665,8 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 int s = t.stream, from = t.own, until = g.state.tiles[s];
                 for (int i = walk.first; i < walk.last; ++i, ++n) {
                     Tile o;
+                    bool looked_at;          // lane's 16 keys
+                    const int my_key = (lane % kGroups) * kGroupKeys;
                     o.head = walk.head;
                     o.flags = (i == walk.first ? kFirst : 0) | (i + 1 == walk.last ? kLast : 0);
                     o.row_low = 0;
@@ -664,8 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                         o.slot = t.slot;
                         o.key0 = t.keys.tile(i) * kKeys;
                         o.limit = t.shared;
-                        o.groups = 0;
-                        for (int k = 0; k < kGroups; ++k) o.groups |= t.keys.touches(o.key0 + k * kGroupKeys) << k;
+                        looked_at = t.keys.touches(o.key0 + my_key);
                         if (o.key0 + kKeys - 1 <= t.low && o.key0 + kKeys <= t.shared &&
                             (!a.window || t.high - o.key0 < a.window || o.key0 + kKeys <= a.sinks))
                             o.flags |= kClear;
@@ -676,27 +686,68 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                         o.slot = there ? a.slots[s] : 0;
                         o.key0 = there ? t.shared + (own - from) * kKeys : 0;
                         o.limit = there ? a.lengths[o.slot] : 0;
-                        o.groups = 0;
-                        for (int k = 0; k < kGroups; ++k) o.groups |= (o.key0 + k * kGroupKeys < o.limit) << k;
+                        looked_at = o.key0 + my_key < o.limit;
                         o.row_low = (a.offsets[s] - t.token0) * a.group - t.row0;
                         o.row_high = (a.offsets[s + 1] - t.token0) * a.group - t.row0;
                         o.flags |= kOwnKeys;
                         if (!there) o.row_low = 0, o.row_high = kRows;
                     }
-                    if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
-                    if (lane == 0) {
-                        sm.tiles[n % kTiles] = o;
-                        mbar_arrive(&sm.tile_full[n % kTiles]);
+                    int page = -1;
+                    const int entry = (o.key0 + my_key) >> a.page_shift;
+                    if (looked_at && entry < a.table_width) {
+                        page = a.table[static_cast<long long>(o.slot) * a.table_width + entry];
+                        if (page >= a.pages) page = -1;
                     }
-                    __syncwarp();
+                    if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
+                    Tile& to = sm.tiles[n % kTiles];
+                    if (lane < kGroups) to.page[lane] = page;
+                    if (lane == 0) {
+                        to.slot = o.slot, to.key0 = o.key0, to.head = o.head, to.limit = o.limit;
+                        to.row_low = o.row_low, to.row_high = o.row_high, to.flags = o.flags;
+                    }
+                    arrive(&sm.tile_full[n % kTiles]);
                 }
             }
             if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
+            if (piece >= kPieces) wait(&sm.piece_empty[piece % kPieces], piece / kPieces - 1);
             if (lane == 0) {
                 sm.tiles[n % kTiles].flags = kNone;
                 mbar_arrive(&sm.tile_full[n % kTiles]);
+                sm.pieces[piece % kPieces].rows = 0;
+                mbar_arrive(&sm.piece_full[piece % kPieces]);
             }
             __syncwarp();
+        }
+        if (warp == kScaleWarp) {
+            // ---- scales: a lane to 16 keys, one tile ahead of what is written
+            float key = 0.0f, value = -1.0f;   // -1: not there
+            auto fetch = [&](int n) {
+                const Tile& t = tile_info(n);
+                const bool have = !(t.flags & kNone) && !*dead;
+                key = 0.0f, value = -1.0f;
+                if (have && lane < kGroups && t.page[lane] >= 0) {
+                    const float* s = a.scale + static_cast<long long>(t.page[lane]) * 2 * a.heads + t.head;
+                    key = s[0];
+                    value = s[a.heads];
+                }
+                if (have) tile_done(n);
+                return have;
+            };
+            bool have = fetch(0);
+            for (int n = 0; have; ++n) {
+                const float key_now = key, value_now = value;
+                have = fetch(n + 1);
+                GroupScales s;
+                const float v = value_now == -1.0f || !(value_now < kTinyScale) ? value_now : kTinyScale;
+                s.key = key_now;
+                s.log2_value = v == -1.0f ? -INFINITY : log2f(v);
+                s.inv_value = v == -1.0f ? 0.0f : 1.0f / v;
+                s.pad = 0.0f;
+                // the scores two tiles back are made, so the weights four tiles back are: their place is free
+                if (n >= 2) wait(&sm.k_empty[n & 1], (n >> 1) - 1);
+                if (lane < kGroups) sm.scales[n % kScaleRing][lane] = s;
+                arrive(&sm.k_full[n & 1]);
+            }
         }
         // ---- MMA: the warp waits together, one lane issues
         if (warp == kMmaWarp) {
@@ -706,6 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             const uint64_t v_desc = sw128_n_major_desc(smem_u32(sm.v[0]), 128 * 128);
             const uint32_t issue = lane == 0;
             int piece = 0, held = 0;   // held: the flags of the tile whose P V is outstanding
+            int begun = 0;             // sums of each parity, in this piece: a bit each
             auto sums = [&](int n) {
                 const int b = n & 1;
                 wait(&sm.v_full[b], n >> 1);
@@ -717,9 +769,10 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     tc_fence_after();
 #pragma unroll
                     for (int k = h * 4; k < h * 4 + 4; ++k)
-                        mma_f16_ts(tmem + Tmem<D>::kO, tmem + Tmem<D>::s(b) + k * 8, vd + k * (16 * 128 >> 4), pv,
-                                   !(held & kFirst) || k > 0, issue);
+                        mma_f16_ts(tmem + Tmem<D>::o(b), tmem + Tmem<D>::s(b) + k * 8, vd + k * (16 * 128 >> 4), pv,
+                                   (begun >> b & 1) || k > 0, issue);
                 }
+                begun |= 1 << b;
                 mma_commit_if(&sm.v_empty[b], issue);
                 if (held & kLast) mma_commit_if(&sm.o_full, issue);
             };
@@ -733,6 +786,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     // the queries' place is free once the piece before is through
                     if (outstanding) sums(n - 1);
                     outstanding = false;
+                    begun = 0;
                     wait(&sm.q_full, piece++);
                 }
                 wait(&sm.k_full[b], n >> 1);
