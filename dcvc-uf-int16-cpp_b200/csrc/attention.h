@@ -84,7 +84,12 @@ cudaError_t kv_attend(const AttendArgs& a, int dtype, int sms, cudaStream_t s);
 
 // What kv_share leaves of the groups of a batch (ufb_kv_groups.state).
 struct KvGroupState {
-    int32_t *shared, *slot, *low, *high;   // [groups] tokens in common, a stream that has them, least and largest position
+    int32_t* shared;                       // [groups] tokens in common
+    struct Group {
+        int32_t token0, tokens, stream0, streams;
+        int32_t shared, slot, low, high;   // slot: of a stream that has them; least and largest position
+    };
+    Group* group;                          // [groups], 16-byte aligned
     int32_t* tiles;                        // [n] tiles of own keys of the group's streams up to this one
     int32_t* positions;                    // [tokens]; kNotWritten: its results are left alone
     int32_t* stream;                       // [tokens] number of its stream in the batch
@@ -92,17 +97,14 @@ struct KvGroupState {
 constexpr int kNotWritten = INT32_MIN;
 constexpr int kGroupTileKeys = 128;        // keys of a tile of kv_attend_groups
 struct GroupArgs {
-    const int32_t *first, *offsets;        // [groups + 1] streams, tokens
     int groups, max_tokens;
     KvGroupState state;
 };
 inline KvGroupState kv_group_state(const ufb_kv_groups& g, int n, long long tokens) {
     KvGroupState s;
     s.shared = g.state;
-    s.slot = s.shared + g.groups;
-    s.low = s.slot + g.groups;
-    s.high = s.low + g.groups;
-    s.tiles = s.high + g.groups;
+    s.group = reinterpret_cast<KvGroupState::Group*>(s.shared + (g.groups + 3) / 4 * 4);
+    s.tiles = reinterpret_cast<int32_t*>(s.group + g.groups);
     s.positions = s.tiles + n;
     s.stream = s.positions + tokens;
     return s;

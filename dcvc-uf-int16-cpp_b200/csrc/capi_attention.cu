@@ -118,6 +118,7 @@ bool check_groups(const ufb_kv_groups* g, int n, int max_new, int64_t tokens) {
     if (!g || g->groups < 0 || g->groups > n || (n > 0 && g->groups == 0))
         return fail(UFB_EINVAL, "a batch has between one group and one for each stream");
     if (g->groups > 0 && (!g->first || !g->offsets || !g->state)) return fail(UFB_EINVAL, "group tensors must be non-null");
+    if (reinterpret_cast<uintptr_t>(g->state) % 16) return fail(UFB_EINVAL, "group state must be 16-byte aligned");
     if (g->max_tokens < max_new || g->max_tokens > tokens) return fail(UFB_EINVAL, "invalid token count of a group");
     return true;
 }
@@ -312,7 +313,7 @@ int64_t ufb_capture_id(void* stream) {
 int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens) {
     clear_error();
     if (groups < 0 || n < 0 || tokens < 0 || tokens > INT32_MAX) return err(UFB_EINVAL, "invalid counts");
-    return 4ll * groups + n + 2 * tokens;
+    return (groups + 3ll) / 4 * 4 + 8ll * groups + n + 2 * tokens;
 }
 
 int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, int max_new,
@@ -410,7 +411,7 @@ int ufb_kv_attend_groups(const ufb_kv_cache* c, int layer, const int32_t* slots,
         !check_groups(groups, n, max_new, tokens))
         return last_code();
     if (!go || groups->groups == 0) return UFB_OK;
-    const GroupArgs g{groups->first, groups->offsets, groups->groups, groups->max_tokens, kv_group_state(*groups, n, tokens)};
+    const GroupArgs g{groups->groups, groups->max_tokens, kv_group_state(*groups, n, tokens)};
     return done(kv_attend_groups(a, g, dtype, sms, static_cast<cudaStream_t>(stream)), "kv attend groups");
 }
 

@@ -132,26 +132,30 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 
 // false: the pair (group, row tile) does not exist.
 __device__ __forceinline__ bool group_tile(const AttendArgs& a, const GroupArgs& g, int group, int rt, GroupTile& t) {
-    const int o0 = g.offsets[group], o1 = g.offsets[group + 1];
-    const bool ok = o0 >= 0 && o1 >= o0 && o1 <= a.tokens && o1 - o0 <= g.max_tokens;
-    if (!ok && rt == 0) atomicCAS(a.status, 0, kStatusIndex);
-    t.token0 = o0;
+    const int4* record = reinterpret_cast<const int4*>(g.state.group + group);
+    const int4 place = record[0], keys = record[1];   // KvGroupState::Group
+    t.token0 = place.x;
     t.row0 = rt * kRows;
-    t.rows = min(kRows, ok ? (o1 - o0) * a.group - t.row0 : 0);
+    const int rows = place.y * a.group;
+    t.rows = min(kRows, rows - t.row0);
     if (t.rows <= 0) return false;
-    t.shared = g.state.shared[group];
-    t.slot = g.state.slot[group];
-    t.low = g.state.low[group];
-    t.high = g.state.high[group];
-    const int first = g.first[group];
-    const int s0 = g.state.stream[o0 + t.row0 / a.group], s1 = g.state.stream[o0 + (t.row0 + t.rows - 1) / a.group];
-    t.stream = s0;
-    t.last = s1;
-    t.own = s0 > first ? g.state.tiles[s0 - 1] : 0;
+    t.shared = keys.x;
+    t.slot = keys.y;
+    t.low = keys.z;
+    t.high = keys.w;
+    t.stream = place.z;
+    t.last = place.z + place.w - 1;
+    t.own = 0;
+    if (rows > kRows) {
+        // the streams of these rows only
+        t.stream = g.state.stream[t.token0 + t.row0 / a.group];
+        t.last = g.state.stream[t.token0 + (t.row0 + t.rows - 1) / a.group];
+        if (t.stream > place.z) t.own = g.state.tiles[t.stream - 1];
+    }
     t.keys = key_range<kKeys>(a, t.shared, 0, t.low - t.shared, t.high - t.shared);
     t.common = t.keys.hi > 0 ? t.keys.nt : 0;
     // rows that see nothing are still written: one tile, all of it hidden
-    t.nt = max(t.common + g.state.tiles[s1] - t.own, 1);
+    t.nt = max(t.common + g.state.tiles[t.last] - t.own, 1);
     return true;
 }
 
@@ -898,7 +902,9 @@ cudaError_t launch(const AttendArgs& a, const GroupArgs& g, int sms, cudaStream_
     // its blocks may start once the CTAs have exited, before that kernel's end is signalled
     // (it gives no earlier trigger): they wait for that
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(ctas, kRows * (D / 4) / kJoinThreads);
+    const long long rows = static_cast<long long>(g.max_tokens) * a.group;
+    constexpr int kJoinRows = kJoinThreads / (D / 4);
+    config.gridDim = dim3(ctas, static_cast<unsigned>(((rows < kRows ? rows : kRows) + kJoinRows - 1) / kJoinRows));
     config.blockDim = dim3(kJoinThreads);
     config.stream = s;
     cudaLaunchAttribute early;

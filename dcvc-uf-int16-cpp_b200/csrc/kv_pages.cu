@@ -570,9 +570,14 @@ __global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, c
     }
     if (threadIdx.x == 0) {
         out.shared[group] = shared;
-        out.slot[group] = members ? b.slots[chosen] : 0;
-        out.low[group] = lowest == INT_MAX ? -1 : lowest;
-        out.high[group] = highest;
+        const int o0 = g.offsets[group], o1 = g.offsets[group + 1];
+        const bool ok = o0 >= 0 && o1 >= o0 && o1 <= b.tokens && o1 - o0 <= g.max_tokens && first <= end;
+        if (!ok) atomicCAS(status, 0, kStatusIndex);
+        KvGroupState::Group r;
+        r.token0 = o0, r.tokens = ok ? o1 - o0 : 0, r.stream0 = first, r.streams = end - first;
+        r.shared = shared, r.slot = members ? b.slots[chosen] : 0;
+        r.low = lowest == INT_MAX ? -1 : lowest, r.high = highest;
+        out.group[group] = r;
     }
 }
 

@@ -600,7 +600,7 @@ int ufb_kv_attend(const ufb_kv_cache* c, int layer, const int32_t* slots, const 
 typedef struct ufb_kv_groups {
     const int32_t* first;   /* [groups + 1] first stream of each in the batch; 0 .. n */
     const int32_t* offsets; /* [groups + 1] their tokens: offsets[first[g]] of the batch */
-    int32_t* state;         /* [ufb_kv_group_ints()] written by ufb_kv_share */
+    int32_t* state;         /* [ufb_kv_group_ints()] written by ufb_kv_share; 16-byte aligned */
     int32_t groups;
     int32_t max_tokens;     /* no less than any group's tokens */
 } ufb_kv_groups;

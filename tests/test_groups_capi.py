@@ -37,7 +37,7 @@ def test_group_refusals(att):  # noqa: F811
         return L.ufb_kv_attend_groups(c, layer, 4096, 4096, 4, 2, 5, 1, C.byref(q), C.byref(q), None, window, 0, 1, 1.0,
                                       C.byref(g) if g else None, workspace, room, None)
 
-    for g in (None, groups(first=None), groups(offsets=None), groups(state=None), groups(n=-1), groups(n=0), groups(n=5),
+    for g in (None, groups(first=None), groups(offsets=None), groups(state=None), groups(state=4100), groups(n=-1), groups(n=0), groups(n=5),
               groups(most=1), groups(most=6)):
         assert share(g) == EINVAL
         assert L.ufb_last_error()
@@ -46,6 +46,6 @@ def test_group_refusals(att):  # noqa: F811
     assert share(groups(n=0, first=None, most=0), n=0, max_new=0, tokens=0) == 0
     for over in (dict(layer=2), dict(layer=-1), dict(window=-1)):
         assert attend(groups(), **over) == EINVAL, over
-    assert L.ufb_kv_group_ints(2, 4, 5) == 4 * 2 + 4 + 2 * 5
+    assert L.ufb_kv_group_ints(2, 4, 5) == 4 + 8 * 2 + 4 + 2 * 5
     for args in ((-1, 4, 5), (2, -1, 5), (2, 4, -1), (2, 4, 1 << 31)):
         assert L.ufb_kv_group_ints(*args) == EINVAL
