@@ -38,6 +38,7 @@ constexpr int kThreads = 640;         // warps: softmax 0-7, converter 8-15, MMA
 constexpr int kPieces = 4;            // pieces announced ahead
 constexpr int kTiles = 8;             // tiles announced ahead
 constexpr int kScaleRing = 4;
+constexpr int kWarpPairs = 128;       // (group, row tile) pairs up to which one warp divides the work
 constexpr int kCode = 45;
 // A wait gives up after so many looks at its barrier; the hardware holds each for about 300
 // cycles, so that is a second or so.  (A clock in every wait took three times the instructions,
@@ -75,9 +76,9 @@ struct Tile {
     int limit;              // keys below it are there
     int row_low, row_high;  // rows that may see it
     int page[kGroups];      // of each 16 keys; -1: not looked at, or not there
-    int flags;              // kFirst, kLast of the piece; kClear: all its rows see all of it; kOwnKeys
+    int flags;              // kClear: all its rows see all of it; kOwnKeys; kNone: there is no further tile
 };
-constexpr int kFirst = 1, kLast = 2, kClear = 4, kOwnKeys = 8, kNone = 16;
+constexpr int kClear = 1, kOwnKeys = 2, kNone = 4;
 
 template <int D>
 struct Smem {
@@ -86,8 +87,8 @@ struct Smem {
     alignas(1024) uint8_t v[2][kKeys * D * 2];
     GroupScales scales[kScaleRing][kGroups];
     float row[2][2][kRows];                        // by parity: largest |q|, then maxima; weights
-    alignas(8) uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2];
-    uint64_t q_full, o_full, drained, pair[4];
+    alignas(8) uint64_t k_full[2], v_empty[2], s_full[2], p_full[2][2];   // s_full: and the keys' place is free
+    uint64_t q_full, o_full, drained, pair[4], all;
     uint64_t piece_full[kPieces], piece_empty[kPieces], tile_full[kTiles], tile_empty[kTiles];
     Announced pieces[kPieces];
     Tile tiles[kTiles];
@@ -126,6 +127,25 @@ __device__ __forceinline__ void add2(float& a, float& b, float x, float y) {
         "add.rn.f32x2 v, v, w;\n\tmov.b64 {%0, %1}, v;\n\t}"
         : "+f"(a), "+f"(b)
         : "f"(x), "f"(y));
+}
+
+// (x, y) = (x, y) f + (u, v) g
+__device__ __forceinline__ void weigh2(float& x, float& y, float f, float u, float v, float g) {
+    asm("{\n\t.reg .b64 a, b, m, n;\n\t"
+        "mov.b64 a, {%0, %1};\n\tmov.b64 m, {%2, %2};\n\tmov.b64 b, {%3, %4};\n\tmov.b64 n, {%5, %5};\n\t"
+        "mul.rn.f32x2 b, b, n;\n\tfma.rn.f32x2 a, a, m, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(f), "f"(u), "f"(v), "f"(g));
+}
+
+// The larger of two pairs, entry by entry, of their absolute values; NaN if there is one.
+__device__ __forceinline__ uint32_t top2(uint32_t a, uint32_t b, __half) {
+    const __half2 m = __hmax2_nan(__habs2(*reinterpret_cast<const __half2*>(&a)), __habs2(*reinterpret_cast<const __half2*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t top2(uint32_t a, uint32_t b, __nv_bfloat16) {
+    const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
+    return *reinterpret_cast<const uint32_t*>(&m);
 }
 
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -194,6 +214,43 @@ struct GroupWalker {
     }
 };
 
+// share_out by one warp, which needs no other: for few pairs (lanes take 32 at a time).
+template <class Tiles>
+__device__ __forceinline__ Share share_of_warp(int pairs, Tiles tiles_of) {
+    const int lane = threadIdx.x & 31;
+    Share s;
+    long long first = 0;
+    s.total = 0;
+    for (int base = 0; base < pairs; base += 32) {
+        const long long v = base + lane < pairs ? tiles_of(base + lane) : 0;
+        if (base == 0) first = v;
+        s.total += v;
+    }
+#pragma unroll 1
+    for (int o = 16; o; o >>= 1) s.total += __shfl_xor_sync(0xffffffffu, s.total, o);
+    s.per = max(quotient(s.total + gridDim.x - 1, gridDim.x), 1ll);
+    s.pair = pairs, s.pair_start = 0;
+    const long long start = s.per * blockIdx.x;
+    long long before = 0;
+    for (int base = 0; base < pairs && before <= start; base += 32) {
+        const long long v = base == 0 ? first : base + lane < pairs ? tiles_of(base + lane) : 0;
+        long long at = before + v;
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += u - before;
+        }
+        before = __shfl_sync(0xffffffffu, at, 31);
+        at -= v;
+        const uint32_t hit = __ballot_sync(0xffffffffu, at <= start && start < at + v);
+        if (hit) {
+            s.pair = base + __ffs(hit) - 1;
+            s.pair_start = __shfl_sync(0xffffffffu, at, __ffs(hit) - 1);
+        }
+    }
+    return s;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a, const GroupArgs g, int row_tiles) {
     // aligned by declaration, so that descriptors are constants (checked below)
@@ -203,10 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.k_full[i], 129);
-            mbar_init(&sm.v_full[i], 128);
-            mbar_init(&sm.k_empty[i], 1);
             mbar_init(&sm.v_empty[i], 1);
-            mbar_init(&sm.p_full[i][0], 128);
+            mbar_init(&sm.p_full[i][0], 256);   // the first half of the weights, and the values
             mbar_init(&sm.p_full[i][1], 128);
             mbar_init(&sm.s_full[i], 1);
         }
@@ -214,13 +269,14 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         mbar_init(&sm.o_full, 1);
         mbar_init(&sm.drained, 1);
         for (int i = 0; i < 4; ++i) mbar_init(&sm.pair[i], 64);
+        mbar_init(&sm.all, 256);
         for (int i = 0; i < kPieces; ++i) {
             mbar_init(&sm.piece_full[i], 1);
-            mbar_init(&sm.piece_empty[i], 8);
+            mbar_init(&sm.piece_empty[i], 9);
         }
         for (int i = 0; i < kTiles; ++i) {
             mbar_init(&sm.tile_full[i], 1);
-            mbar_init(&sm.tile_empty[i], 14);
+            mbar_init(&sm.tile_empty[i], 13);
         }
         fence_mbar_init();
         sm.dead = (smem_u32(raw) & 1023) != 0;
@@ -231,13 +287,17 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         tmem_relinquish();
     }
     tc_fence_before();
-    GroupTile scratch_tile;
     const int pairs = g.groups * row_tiles;
-    const Share share = share_out<kThreads>(
-        pairs, 1, [&](int p) -> long long {
-            return group_tile(a, g, p / row_tiles, p % row_tiles, scratch_tile) ? static_cast<long long>(scratch_tile.nt) * a.heads : 0;
-        },
-        sm.share);
+    auto tiles_of = [&](int p) -> long long {
+        GroupTile t;
+        return group_tile(a, g, p / row_tiles, p % row_tiles, t) ? static_cast<long long>(t.nt) * a.heads : 0;
+    };
+    __syncthreads();
+    wait_for_previous();
+    // Only the walker needs to know this CTA's share.  One warp finds it in 1 us where it takes
+    // all the block's 2 us; from some hundred pairs on the block is faster.
+    Share share;
+    if (pairs > kWarpPairs) share = share_out<kThreads>(pairs, 1, tiles_of, sm.share);
     tc_fence_after();
     // all 512 columns are this CTA's: its tensor memory begins at 0
     constexpr uint32_t tmem = 0;
@@ -268,21 +328,23 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     // the registers of 640 threads at 96: 2 x 128 + 2 x 72 + 80 = 5 x 96
     if (warp < 8) {
         regs_inc<128>();
-        // ---- softmax: the tiles of parity t, each into sums of its own; row = lane of tensor memory
-        const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        // ---- softmax: the tiles of parity t, each into sums of its own
+        const int t = warp >> 2, quarter = warp & 3, line = quarter * 32 + lane;   // line: of tensor memory
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t ts = tmem + lanes + Tmem<D>::s(t), to = tmem + lanes + Tmem<D>::o(t);
         const AttendScratch scratch = scratch_of(a.workspace, gridDim.x, kRows);
         if (threadIdx.x == 0) scratch.items[blockIdx.x * 8] = 0;
-        // the two warps that share rows meet, in tensor memory too
-        int met = 0;
-        auto pair_sync = [&] {
+        // the two warps that share lines meet, in tensor memory too; all eight
+        auto meet = [&](uint64_t* bar, int& met) {
             tc_fence_before();
-            mbar_arrive(&sm.pair[quarter]);
-            wait(&sm.pair[quarter], met++);
+            mbar_arrive(bar);
+            wait(bar, met++);
             __syncwarp();
             tc_fence_after();
         };
+        int pair_met = 0, all_met = 0;
+        auto pair_sync = [&] { meet(&sm.pair[quarter], pair_met); };
+        auto all_sync = [&] { meet(&sm.all, all_met); };
         int first = 0;   // number of the piece's first tile among this CTA's
         for (int piece = 0;; ++piece) {
             wait(&sm.piece_full[piece % kPieces], piece / kPieces);
@@ -290,8 +352,13 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             const Announced& p = sm.pieces[piece % kPieces];
             if (p.rows == 0 || *dead) break;
             const int count = p.count;
+            // up to 64 rows lie in the tile two times, up to 32 four times: copy `copy` takes
+            // `wide` of each tile's chunks of 32 keys
+            const int wide = p.rows > 64 ? 4 : p.rows > 32 ? 2 : 1;
+            const int copy = wide == 4 ? 0 : wide == 2 ? quarter >> 1 : quarter;
+            const int row0 = (quarter - copy * wide) * 32, row = row0 + lane;
             const bool real = row < p.rows;
-            const bool busy = quarter * 32 < p.rows;
+            const bool busy = row0 < p.rows;
             const int in_group = p.row0 + (real ? row : 0);
             int token = in_group / a.group;
             const int head = p.head * a.group + in_group - token * a.group;
@@ -306,23 +373,18 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + static_cast<long long>(token) * a.q.token_stride +
                                                                   head * a.q.head_stride) + t * (D / 16);
                 uint4 v[D / 16];
-                float top = 0.0f, odd = 0.0f;
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i) v[i] = real ? vec[i] : make_uint4(0, 0, 0, 0);
+                uint32_t largest = 0;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                    const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 f = unpack2(x[j], T());
-                        top = max3(top, fabsf(f.x), fabsf(f.y));
-                        odd += (f.x - f.x) + (f.y - f.y);  // NaN for what is not finite
-                    }
-                }
-                sm.row[0][t][row] = odd == odd ? top : odd;
+                for (int i = 0; i < D / 16; ++i)
+                    largest = top2(top2(top2(largest, v[i].x, T()), v[i].y, T()), top2(v[i].z, v[i].w, T()), T());
+                const float2 f = unpack2(largest, T());
+                const float top = f.x == f.x && f.y == f.y ? fmaxf(f.x, f.y) : __int_as_float(0x7fffffff);
+                sm.row[0][t][line] = top;
                 pair_sync();
-                const float other = sm.row[0][t ^ 1][row];
-                const float u = row_unit(odd == odd && other == other ? fmaxf(top, other) : __int_as_float(0x7fffffff));
+                const float other = sm.row[0][t ^ 1][line];
+                const float u = row_unit(top == top && other == other ? fmaxf(top, other) : __int_as_float(0x7fffffff));
                 unit = unit_inverse(u) * fabsf(a.scale_log2);
                 const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
 #pragma unroll
@@ -334,20 +396,28 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                         const float2 f = unpack2(x[j], T());
                         y[j] = pack2(f.x * mul, f.y * mul, __half());
                     }
-                    *reinterpret_cast<uint4*>(sm.q + tile_at(row, t * (D / 16) + i)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4*>(sm.q + tile_at(line, t * (D / 16) + i)) = make_uint4(y[0], y[1], y[2], y[3]);
                 }
             }
             fence_proxy_async_smem();
             mbar_arrive(&sm.q_full);
             for (int n = first + ((first ^ t) & 1); n < first + count; n += 2) {
                 const Tile& tile = tile_info(n);
-                const int key0 = tile.key0, limit = tile.limit, flags = tile.flags, row_low = tile.row_low, row_high = tile.row_high;
+                const int flags = tile.flags;
+                // columns [0, high) that are from low on or below sink are seen by this row
+                int high = 0, low = 0, sink = 0;
+                bool mine = busy;   // rows of this warp that the tile is for
+                if (!(flags & kClear)) {
+                    const int key0 = tile.key0, limit = tile.limit, row_low = tile.row_low, row_high = tile.row_high;
+                    mine = busy && row_low < row0 + 32 && row_high > row0;
+                    if (row >= row_low && row < row_high)
+                        high = min(limit, a.causal || !(flags & kOwnKeys) ? pos + 1 : limit) - key0;
+                    if (a.window) low = max(pos - a.window + 1, 0) - key0, sink = a.sinks - key0;
+                }
+                tile_done(n);
                 wait(&sm.s_full[t], n >> 1);
                 __syncwarp();
                 tc_fence_after();
-                tile_done(n);
-                // rows of this warp that the tile is for
-                const bool mine = busy && row_low < quarter * 32 + 32 && row_high > quarter * 32;
                 if (!mine) {
                     // rows of other streams: no weight.  (Padding's weights do not matter.)
                     if (busy) {
@@ -364,11 +434,6 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     continue;
                 }
                 const GroupScales* sc = sm.scales[n % kScaleRing];
-                // columns [0, high) that are from low on or below sink are seen by this row
-                const bool ours = row >= row_low && row < row_high;
-                const int high = ours ? min(limit, a.causal || !(flags & kOwnKeys) ? pos + 1 : limit) - key0 : 0;
-                const int low = a.window ? max(pos - a.window + 1, 0) - key0 : 0;
-                const int sink = a.window ? a.sinks - key0 : 0;
                 auto seen = [&](int c) {   // of 32 columns, a bit each
                     return bits_below(high - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
                 };
@@ -395,19 +460,28 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                         }
                     };
 #pragma unroll 1
-                    for (int c = 2; c >= 0; c -= 2) {
+                    for (int c = wide == 4 ? 2 : copy * wide; c >= copy * wide; c -= 2) {
                         tmem_ld32(ts + c * 32, s0);
-                        tmem_ld32(ts + c * 32 + 32, s1);
+                        if (wide > 1) tmem_ld32(ts + c * 32 + 32, s1);
                         tmem_wait_ld();
                         tmem_tie32(s0);
                         tmem_tie32(s1);
                         chunk(c, s0);
-                        chunk(c + 1, s1);
+                        if (wide > 1) chunk(c + 1, s1);
                     }
                 };
                 const bool clear = flags & kClear;
                 if (clear) maximum(std::false_type());
                 else maximum(std::true_type());
+                if (wide < 4) {
+                    // the keys of the other copies have no weight in this one
+                    uint32_t w[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) w[j] = 0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (c < copy * wide || c >= copy * wide + wide) tmem_st16(ts + c * 16, w);
+                }
                 // the maximum stays while it is within 2^kSlack; these sums' last product was before these scores
                 const bool grow = top > __fadd_rd(m, kSlack);
                 if (__any_sync(0xffffffffu, grow)) {
@@ -459,82 +533,128 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     };
                     // the next columns are on their way while these are worked on
 #pragma unroll 1
-                    for (int half = 0; half < 2; ++half) {
+                    for (int c = copy * wide; c < copy * wide + wide; c += 2) {
+                        const bool more = wide == 4 && c == 0;
                         tmem_wait_ld();
                         tmem_tie32(s0);
                         tmem_tie32(s1);
-                        chunk(half * 2, s0);
-                        if (half == 0) tmem_ld32(ts + 64, s0);
-                        chunk(half * 2 + 1, s1);
-                        if (half == 0) tmem_ld32(ts + 96, s1);
+                        chunk(c, s0);
+                        if (more) tmem_ld32(ts + 64, s0);
+                        if (wide > 1) chunk(c + 1, s1);
+                        if (more) tmem_ld32(ts + 96, s1);
                         // P V starts on the first 64 keys while the others are in the works
                         tmem_wait_st();
                         tc_fence_before();
-                        mbar_arrive(&sm.p_full[t][half]);
+                        if (more || wide < 4) mbar_arrive(&sm.p_full[t][0]);
+                        if (!more) mbar_arrive(&sm.p_full[t][1]);
                     }
                 };
                 if (clear && !far) weights(std::false_type());
                 else weights(std::true_type());
             }
+            // sets that had no tile have no sums
+            const int sums0 = count > 1 || !(first & 1) ? 0 : 1, sums1 = count > 1 || (first & 1) ? 1 : 0;
             first += count;
 
-            // ---- the piece's rows: both sums, half of the dims each
+            // ---- the piece's rows: the sums of both sets and all copies, half of the dims each
             if (busy) {
-                sm.row[0][t][row] = m;
-                sm.row[1][t][row] = l;
+                sm.row[0][t][line] = m;
+                sm.row[1][t][line] = l;
             }
             wait(&sm.o_full, piece);
             __syncwarp();
             tc_fence_after();
             if (busy) {
-                pair_sync();
-                const float m0 = sm.row[0][0][row], m1 = sm.row[0][1][row], l0 = sm.row[1][0][row], l1 = sm.row[1][1][row];
-                const float top = fmaxf(m0, m1);
+                if (wide == 4) pair_sync();
+                else all_sync();
+                float top = -INFINITY;
+                for (int i = row; i < kRows; i += wide * 32) top = max3(top, sm.row[0][0][i], sm.row[0][1][i]);
                 // a part that saw nothing has no weight; one that is not finite spoils its row
-                const float e0 = m0 == -INFINITY ? (l0 == 0.0f ? 0.0f : 1.0f) : ex2(m0 - top);
-                const float e1 = m1 == -INFINITY ? (l1 == 0.0f ? 0.0f : 1.0f) : ex2(m1 - top);
-                const float weight = (e0 == 0.0f ? 0.0f : l0 * e0) + (e1 == 0.0f ? 0.0f : l1 * e1);
+                auto part_of = [&](int u, int i) {
+                    const float m = sm.row[0][u][i];
+                    return m == -INFINITY ? (sm.row[1][u][i] == 0.0f ? 0.0f : 1.0f) : ex2(m - top);
+                };
+                float weight = 0.0f;
+                for (int i = row; i < kRows; i += wide * 32)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float e = part_of(u, i);
+                        if (e != 0.0f) weight += sm.row[1][u][i] * e;
+                    }
+                const float e0 = part_of(0, line), e1 = part_of(1, line);
                 const bool whole = p.part < 0;
                 const int part = 2 * blockIdx.x + p.part;
                 const float inv = !whole ? 1.0f : weight == 0.0f ? 0.0f : 1.0f / weight;
                 T* out = static_cast<T*>(a.out.data) + static_cast<long long>(token) * a.out.token_stride + head * a.out.head_stride;
                 float* sums = scratch.sums + (static_cast<long long>(part) * kRows + row) * D;
-#pragma unroll 1
-                for (int c = t * (D / 32); c < (t + 1) * (D / 32); ++c) {
+                // 16 dims of this line
+                auto sum16 = [&](int c, float (&o)[16]) {
                     uint32_t x[16], y[16];
-                    tmem_ld16(tmem + lanes + Tmem<D>::o(0) + c * 16, x);
-                    tmem_ld16(tmem + lanes + Tmem<D>::o(1) + c * 16, y);
+                    tmem_ld16(tmem + lanes + Tmem<D>::o(0) + sums0 * D + c * 16, x);
+                    tmem_ld16(tmem + lanes + Tmem<D>::o(0) + sums1 * D + c * 16, y);
                     tmem_wait_ld_regs(x);
                     tmem_wait_ld_regs(y);
-                    float o[16];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        // sums that hold nothing of this piece are not looked at
-                        const float u = e0 == 0.0f ? 0.0f : __uint_as_float(x[j]) * e0;
-                        o[j] = (e1 == 0.0f ? u : fmaf(__uint_as_float(y[j]), e1, u)) * inv;
+                    for (int j = 0; j < 16; j += 2) {
+                        o[j] = __uint_as_float(x[j]), o[j + 1] = __uint_as_float(x[j + 1]);
+                        weigh2(o[j], o[j + 1], e0, __uint_as_float(y[j]), __uint_as_float(y[j + 1]), e1);
                     }
-                    if (write && whole) {
-                        uint32_t w[8];
+                };
+                auto store4 = [&](int dim, float4 v) {
+                    if (write && whole)
+                        *reinterpret_cast<uint2*>(out + dim) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
+                    else if (real && !whole)
+                        __stcg(reinterpret_cast<float4*>(sums + dim), v);
+                };
+                if (wide == 4) {
+#pragma unroll 1
+                    for (int c = t * (D / 32); c < (t + 1) * (D / 32); ++c) {
+                        float o[16];
+                        sum16(c, o);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) w[i] = pack2(o[2 * i], o[2 * i + 1], T());
-                        reinterpret_cast<uint4*>(out)[c * 2] = make_uint4(w[0], w[1], w[2], w[3]);
-                        reinterpret_cast<uint4*>(out)[c * 2 + 1] = make_uint4(w[4], w[5], w[6], w[7]);
-                    } else if (real && !whole) {
-#pragma unroll
-                        for (int j = 0; j < 16; j += 4)
-                            __stcg(reinterpret_cast<float4*>(sums + c * 16 + j), make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+                        for (int j = 0; j < 16; j += 4) store4(c * 16 + j, make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+                        __syncwarp();
                     }
-                    __syncwarp();
+                } else {
+                    // a quarter of the dims of all lines at a time through the queries' place, a
+                    // copy's threads then add up their share of it
+                    constexpr int kChunks = D / 16;   // of 4 dims, in a step of a set
+                    float4* place = reinterpret_cast<float4*>(sm.q) + t * kRows * kChunks;
+#pragma unroll 1
+                    for (int step = 0; step < 2; ++step) {
+                        const int dim0 = t * (D / 2) + step * (D / 4);
+#pragma unroll 1
+                        for (int c = 0; c < D / 64; ++c) {
+                            float o[16];
+                            sum16(dim0 / 16 + c, o);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                place[line * kChunks + ((c * 4 + j) ^ (line & (kChunks - 1)))] =
+                                    make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                        }
+                        all_sync();
+                        const int mine = kChunks * wide / 4;
+                        for (int c = copy * mine; c < copy * mine + mine; ++c) {
+                            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            for (int i = row; i < kRows; i += wide * 32) {
+                                const float4 x = place[i * kChunks + (c ^ (line & (kChunks - 1)))];
+                                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                            }
+                            store4(dim0 + c * 4, v);
+                        }
+                        if (step == 0) all_sync();
+                    }
                 }
-                if (t == 0 && write && whole && a.lse)
+                if (t == 0 && copy == 0 && write && whole && a.lse)
                     a.lse[static_cast<long long>(token) * (a.heads * a.group) + head] =
                         weight == 0.0f ? -INFINITY : (top - kShift + log2f(weight)) * 0.6931471805599453f;
-                if (t == 0 && real && !whole) {
+                if (t == 0 && copy == 0 && real && !whole) {
                     __stcg(scratch.stats + (part * 2) * kRows + row, top);
                     __stcg(scratch.stats + (part * 2 + 1) * kRows + row, weight);
                 }
-                // the next piece's queries and sums wait until both warps have read these
-                pair_sync();
+                // the next piece's queries and sums wait until all have read these
+                if (wide == 4) pair_sync();
+                else all_sync();
             }
             if (p.parts && threadIdx.x == 0) {
                 int32_t* item = scratch.items + blockIdx.x * 8;
@@ -555,8 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         const int chunk = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;
         const int sub = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) & 1) * 2 : lane >> 2;
         constexpr int kStep = D == 128 ? 4 : 8;   // rows of one load of a warp
-        uint64_t* full = side ? sm.v_full : sm.k_full;
-        uint64_t* empty = side ? sm.v_empty : sm.k_empty;
+        uint64_t* empty = side ? sm.v_empty : sm.s_full;
         uint8_t* tiles = side ? sm.v[0] : sm.k[0];
         // this thread's two 16-byte pieces of its first row; row & 7 repeats every kStep * 2 rows
         uint32_t at0[2], at1[2];
@@ -588,35 +707,31 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             tile_done(looked++);
         };
         uint4 buf[kLoads];
-        auto load = [&](const Next& n) {
-            if (!n.tile) return;
-            const int8_t* from[2];
-            bool there[2];
+        const uint8_t* from[2];
+        auto source = [&](const Next& n) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                there[i] = n.page[i] >= 0;
                 const long long tile = (static_cast<long long>(n.page[i]) * 2 + side) * a.heads + n.head;
-                from[i] = a.kv + ((tile << a.page_shift) + n.row[i] + sub) * D + chunk * 16;
+                from[i] = reinterpret_cast<const uint8_t*>(a.kv) + ((tile << a.page_shift) + n.row[i] + sub) * D + chunk * 16;
             }
-            if (there[0] && there[1]) {
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i)  // sub < kStep, a divisor of 16
-                    buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
-            } else {
-#pragma unroll
-                for (int i = 0; i < kLoads; ++i) {
-                    buf[i] = make_uint4(0, 0, 0, 0);
-                    if (there[(i * kStep) >> 4])
-                        buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
-                }
-            }
+        };
+        // what is not there keeps what was: its weights are 0
+        auto load = [&](int i, const Next& n) {
+            if (n.page[(i * kStep) >> 4] >= 0)   // sub < kStep, a divisor of 16
+                buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
         };
         Next now, next;
         fetch(now);
-        load(now);
+        source(now);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            buf[i] = make_uint4(0, 0, 0, 0);
+            load(i, now);
+        }
         fetch(next);
         for (int n = 0; now.tile; ++n) {
             const int b = n & 1;
+            source(next);
             if (n >= 2) wait(&empty[b], (n >> 1) - 1);
             uint8_t* to = tiles + b * (kKeys * D * 2);
 #pragma unroll
@@ -628,10 +743,11 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 const int step = (i / 2) * 2 * kStep * 128;
                 *reinterpret_cast<uint4*>(to + at0[i & 1] + step) = make_uint4(y[0], y[1], y[2], y[3]);
                 *reinterpret_cast<uint4*>(to + at1[i & 1] + step) = make_uint4(y[4], y[5], y[6], y[7]);
+                // a tile's time until it is looked at
+                load(i, next);
             }
             fence_proxy_async_smem();
-            mbar_arrive(&full[b]);
-            load(next);
+            mbar_arrive(side ? &sm.p_full[b][0] : &sm.k_full[b]);
             now = next;
             fetch(next);
         }
@@ -639,6 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         regs_dec<80>();
         if (warp == kWalkWarp) {
             // ---- walker: announces this CTA's pieces and their tiles
+            if (pairs <= kWarpPairs) share = share_of_warp(pairs, tiles_of);
             GroupWalker walk;
             walk.row_tiles = row_tiles;
             walk.pairs = pairs;
@@ -665,14 +782,16 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     o.parts = o.part == 1 ? static_cast<int>(quotient(walk.item_start + t.nt - 1, share.per)) - static_cast<int>(blockIdx.x) + 1 : 0;
                     mbar_arrive(&sm.piece_full[piece % kPieces]);
                 }
+                // four tiles at a time, a lane to 16 keys of one
+                const int my_tile = lane / kGroups, my_key = (lane % kGroups) * kGroupKeys;
                 // own tiles: of stream `s`, whose first is number `from` of the group's
                 int s = t.stream, from = t.own, until = g.state.tiles[s];
-                for (int i = walk.first; i < walk.last; ++i, ++n) {
+                for (int i0 = walk.first; i0 < walk.last; i0 += 4) {
+                    const int i = min(i0 + my_tile, walk.last - 1);
                     Tile o;
                     bool looked_at;          // lane's 16 keys
-                    const int my_key = (lane % kGroups) * kGroupKeys;
                     o.head = walk.head;
-                    o.flags = (i == walk.first ? kFirst : 0) | (i + 1 == walk.last ? kLast : 0);
+                    o.flags = 0;
                     o.row_low = 0;
                     o.row_high = kRows;
                     if (i < t.common) {
@@ -702,14 +821,19 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                         page = a.table[static_cast<long long>(o.slot) * a.table_width + entry];
                         if (page >= a.pages) page = -1;
                     }
-                    if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
-                    Tile& to = sm.tiles[n % kTiles];
-                    if (lane < kGroups) to.page[lane] = page;
-                    if (lane == 0) {
-                        to.slot = o.slot, to.key0 = o.key0, to.head = o.head, to.limit = o.limit;
-                        to.row_low = o.row_low, to.row_high = o.row_high, to.flags = o.flags;
+                    const int tiles = min(walk.last - i0, 4);
+                    for (int j = 0; j < tiles; ++j, ++n) {
+                        if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
+                        Tile& to = sm.tiles[n % kTiles];
+                        if (my_tile == j) {
+                            to.page[lane % kGroups] = page;
+                            if (lane % kGroups == 0) {
+                                to.slot = o.slot, to.key0 = o.key0, to.head = o.head, to.limit = o.limit;
+                                to.row_low = o.row_low, to.row_high = o.row_high, to.flags = o.flags;
+                            }
+                        }
+                        arrive(&sm.tile_full[n % kTiles]);
                     }
-                    arrive(&sm.tile_full[n % kTiles]);
                 }
             }
             if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
@@ -723,34 +847,46 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             __syncwarp();
         }
         if (warp == kScaleWarp) {
-            // ---- scales: a lane to 16 keys, one tile ahead of what is written
-            float key = 0.0f, value = -1.0f;   // -1: not there
-            auto fetch = [&](int n) {
+            // ---- scales: a lane to 16 keys, kAhead tiles ahead of what is written
+            constexpr int kAhead = 3;
+            float key[kAhead + 1], value[kAhead + 1];
+            bool have[kAhead + 1] = {};
+            bool more = true;
+            auto fetch = [&](int n, float& k, float& v, bool& got) {
+                got = false;
+                if (!more) return;
                 const Tile& t = tile_info(n);
-                const bool have = !(t.flags & kNone) && !*dead;
-                key = 0.0f, value = -1.0f;
-                if (have && lane < kGroups && t.page[lane] >= 0) {
+                more = got = !(t.flags & kNone) && !*dead;
+                k = 0.0f, v = -1.0f;   // -1: not there
+                if (!got) return;
+                if (lane < kGroups && t.page[lane] >= 0) {
                     const float* s = a.scale + static_cast<long long>(t.page[lane]) * 2 * a.heads + t.head;
-                    key = s[0];
-                    value = s[a.heads];
+                    k = s[0];
+                    v = s[a.heads];
                 }
-                if (have) tile_done(n);
-                return have;
+                tile_done(n);
             };
-            bool have = fetch(0);
-            for (int n = 0; have; ++n) {
-                const float key_now = key, value_now = value;
-                have = fetch(n + 1);
-                GroupScales s;
-                const float v = value_now == -1.0f || !(value_now < kTinyScale) ? value_now : kTinyScale;
-                s.key = key_now;
-                s.log2_value = v == -1.0f ? -INFINITY : log2f(v);
-                s.inv_value = v == -1.0f ? 0.0f : 1.0f / v;
-                s.pad = 0.0f;
-                // the scores two tiles back are made, so the weights four tiles back are: their place is free
-                if (n >= 2) wait(&sm.k_empty[n & 1], (n >> 1) - 1);
-                if (lane < kGroups) sm.scales[n % kScaleRing][lane] = s;
-                arrive(&sm.k_full[n & 1]);
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) fetch(j, key[j], value[j], have[j]);
+            bool going = true;
+            for (int n0 = 0; going; n0 += kAhead + 1) {
+#pragma unroll
+                for (int j = 0; j <= kAhead; ++j) {
+                    const int n = n0 + j, then = (j + kAhead) % (kAhead + 1);
+                    going = have[j];
+                    if (!going) break;
+                    fetch(n + kAhead, key[then], value[then], have[then]);
+                    GroupScales s;
+                    const float v = value[j] == -1.0f || !(value[j] < kTinyScale) ? value[j] : kTinyScale;
+                    s.key = key[j];
+                    s.log2_value = v == -1.0f ? -INFINITY : log2f(v);
+                    s.inv_value = v == -1.0f ? 0.0f : 1.0f / v;
+                    s.pad = 0.0f;
+                    // the scores two tiles back are made, so the weights four tiles back are: their place is free
+                    if (n >= 2) wait(&sm.s_full[n & 1], (n >> 1) - 1);
+                    if (lane < kGroups) sm.scales[n % kScaleRing][lane] = s;
+                    arrive(&sm.k_full[n & 1]);
+                }
             }
         }
         // ---- MMA: the warp waits together, one lane issues
@@ -760,55 +896,49 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             const uint64_t q_desc = sw128_desc(smem_u32(sm.q)), k_desc = sw128_desc(smem_u32(sm.k[0]));
             const uint64_t v_desc = sw128_n_major_desc(smem_u32(sm.v[0]), 128 * 128);
             const uint32_t issue = lane == 0;
-            int piece = 0, held = 0;   // held: the flags of the tile whose P V is outstanding
-            int begun = 0;             // sums of each parity, in this piece: a bit each
-            auto sums = [&](int n) {
-                const int b = n & 1;
-                wait(&sm.v_full[b], n >> 1);
-                const uint64_t vd = v_desc + b * kTile;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    wait(&sm.p_full[b][h], n >> 1);
-                    __syncwarp();
-                    tc_fence_after();
-#pragma unroll
-                    for (int k = h * 4; k < h * 4 + 4; ++k)
-                        mma_f16_ts(tmem + Tmem<D>::o(b), tmem + Tmem<D>::s(b) + k * 8, vd + k * (16 * 128 >> 4), pv,
-                                   (begun >> b & 1) || k > 0, issue);
-                }
-                begun |= 1 << b;
-                mma_commit_if(&sm.v_empty[b], issue);
-                if (held & kLast) mma_commit_if(&sm.o_full, issue);
-            };
-            bool outstanding = false;
-            int n = 0;
-            for (;; ++n) {
-                const int flags = tile_info(n).flags, b = n & 1;
-                tile_done(n);
-                if ((flags & kNone) || *dead) break;
-                if (flags & kFirst) {
-                    // the queries' place is free once the piece before is through
-                    if (outstanding) sums(n - 1);
-                    outstanding = false;
-                    begun = 0;
-                    wait(&sm.q_full, piece++);
-                }
-                wait(&sm.k_full[b], n >> 1);
+            int n = 0;   // the piece's first tile
+            for (int piece = 0;; ++piece) {
+                wait(&sm.piece_full[piece % kPieces], piece / kPieces);
                 __syncwarp();
-                tc_fence_after();
-                const uint64_t kd = k_desc + b * kTile;
+                const int count = sm.pieces[piece % kPieces].rows ? sm.pieces[piece % kPieces].count : 0;
+                arrive(&sm.piece_empty[piece % kPieces]);
+                if (count == 0 || *dead) break;
+                // the queries' place is free once the piece before is through
+                wait(&sm.q_full, piece);
+#pragma unroll 1
+                for (int i = 0; i <= count; ++i) {
+                    if (i < count) {
+                        const int b = (n + i) & 1;
+                        wait(&sm.k_full[b], (n + i) >> 1);
+                        __syncwarp();
+                        tc_fence_after();
+                        const uint64_t kd = k_desc + b * kTile;
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const int off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-                    mma_f16(tmem + Tmem<D>::s(b), q_desc + off, kd + off, qk, k > 0, issue);
+                        for (int k = 0; k < D / 16; ++k) {
+                            const int off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                            mma_f16(tmem + Tmem<D>::s(b), q_desc + off, kd + off, qk, k > 0, issue);
+                        }
+                        mma_commit_if(&sm.s_full[b], issue);
+                    }
+                    if (i > 0) {
+                        const int b = (n + i - 1) & 1;
+                        const uint64_t vd = v_desc + b * kTile;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            wait(&sm.p_full[b][h], (n + i - 1) >> 1);
+                            __syncwarp();
+                            tc_fence_after();
+#pragma unroll
+                            for (int k = h * 4; k < h * 4 + 4; ++k)
+                                mma_f16_ts(tmem + Tmem<D>::o(b), tmem + Tmem<D>::s(b) + k * 8, vd + k * (16 * 128 >> 4), pv,
+                                           i > 2 || k > 0, issue);   // a piece's first two tiles begin their sums
+                        }
+                        mma_commit_if(&sm.v_empty[b], issue);
+                    }
                 }
-                mma_commit_if(&sm.s_full[b], issue);
-                mma_commit_if(&sm.k_empty[b], issue);
-                if (outstanding) sums(n - 1);
-                outstanding = true;
-                held = flags;
+                mma_commit_if(&sm.o_full, issue);
+                n += count;
             }
-            if (outstanding && !*dead) sums(n - 1);
             // nothing may be in flight when tensor memory is given back
             if (lane == 0) {
                 mma_commit(&sm.drained);
@@ -896,22 +1026,25 @@ cudaError_t launch(const AttendArgs& a, const GroupArgs& g, int sms, cudaStream_
     const long long row_tiles = (static_cast<long long>(g.max_tokens) * a.group + kRows - 1) / kRows;
     if (row_tiles * g.groups > 0x3fffffff) return cudaErrorInvalidValue;
     const int ctas = sms < kAttendMaxCtas ? sms : kAttendMaxCtas;
-    kernel<<<ctas, kThreads, smem, s>>>(a, g, static_cast<int>(row_tiles));
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-    // its blocks may start once the CTAs have exited, before that kernel's end is signalled
-    // (it gives no earlier trigger): they wait for that
+    // both kernels: the blocks may start once the CTAs before have exited, ahead of the signal
+    // that they have ended (nothing gives an earlier trigger); they wait for that
     cudaLaunchConfig_t config = {};
-    const long long rows = static_cast<long long>(g.max_tokens) * a.group;
-    constexpr int kJoinRows = kJoinThreads / (D / 4);
-    config.gridDim = dim3(ctas, static_cast<unsigned>(((rows < kRows ? rows : kRows) + kJoinRows - 1) / kJoinRows));
-    config.blockDim = dim3(kJoinThreads);
-    config.stream = s;
     cudaLaunchAttribute early;
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     config.attrs = &early;
     config.numAttrs = 1;
+    config.stream = s;
+    config.gridDim = dim3(ctas);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = smem;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a, g, static_cast<int>(row_tiles));
+    if (e != cudaSuccess) return e;
+    config.dynamicSmemBytes = 0;
+    const long long rows = static_cast<long long>(g.max_tokens) * a.group;
+    constexpr int kJoinRows = kJoinThreads / (D / 4);
+    config.gridDim = dim3(ctas, static_cast<unsigned>(((rows < kRows ? rows : kRows) + kJoinRows - 1) / kJoinRows));
+    config.blockDim = dim3(kJoinThreads);
     return cudaLaunchKernelEx(&config, groups_join_kernel<T, D>, a, g, ctas);
 }
 
