@@ -86,6 +86,7 @@ struct Smem {
     alignas(1024) uint8_t k[2][kKeys * D * 2];
     alignas(1024) uint8_t v[2][kKeys * D * 2];
     GroupScales scales[kScaleRing][kGroups];
+    float2 stored[kTiles][kGroups];                // scales of keys and values as the pages have them
     float row[2][2][kRows];                        // by parity: largest |q|, then maxima; weights
     alignas(8) uint64_t k_full[2], v_empty[2], s_full[2], p_full[2][2];   // s_full: and the keys' place is free
     uint64_t q_full, o_full, drained, pair[4], all;
@@ -146,6 +147,10 @@ __device__ __forceinline__ uint32_t top2(uint32_t a, uint32_t b, __half) {
 __device__ __forceinline__ uint32_t top2(uint32_t a, uint32_t b, __nv_bfloat16) {
     const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&b)));
     return *reinterpret_cast<const uint32_t*>(&m);
+}
+
+__device__ __forceinline__ void cp_async4(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
 }
 
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -280,7 +285,6 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         }
         fence_mbar_init();
         sm.dead = (smem_u32(raw) & 1023) != 0;
-        if (sm.dead) atomicCAS(a.status, 0, kCode);
     }
     if (warp == kMmaWarp) {
         tmem_alloc(&sm.tmem, 512);
@@ -306,10 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     auto wait = [&](uint64_t* bar, int phase) {
         for (int polls = 0; !mbar_try_wait(bar, phase & 1); ++polls) {
             if (*dead) return;
-            if (polls == kPolls) {
-                atomicCAS(a.status, 0, kCode);
-                *dead = 1;
-            }
+            if (polls == kPolls) *dead = 1;   // reported at the end
         }
     };
     // Tiles one after another; a reader gives each back when it is done with it.
@@ -849,44 +850,43 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         if (warp == kScaleWarp) {
             // ---- scales: a lane to 16 keys, kAhead tiles ahead of what is written
             constexpr int kAhead = 3;
-            float key[kAhead + 1], value[kAhead + 1];
-            bool have[kAhead + 1] = {};
             bool more = true;
-            auto fetch = [&](int n, float& k, float& v, bool& got) {
-                got = false;
-                if (!more) return;
-                const Tile& t = tile_info(n);
-                more = got = !(t.flags & kNone) && !*dead;
-                k = 0.0f, v = -1.0f;   // -1: not there
-                if (!got) return;
-                if (lane < kGroups && t.page[lane] >= 0) {
-                    const float* s = a.scale + static_cast<long long>(t.page[lane]) * 2 * a.heads + t.head;
-                    k = s[0];
-                    v = s[a.heads];
+            int known = 0;
+            auto fetch = [&](int n) {
+                const Tile* t = more ? &tile_info(n) : nullptr;
+                more = more && !(t->flags & kNone) && !*dead;
+                if (more) {
+                    if (lane < kGroups) {
+                        float2* to = &sm.stored[n % kTiles][lane];
+                        if (t->page[lane] >= 0) {
+                            const float* s = a.scale + static_cast<long long>(t->page[lane]) * 2 * a.heads + t->head;
+                            cp_async4(&to->x, s);
+                            cp_async4(&to->y, s + a.heads);
+                        } else {
+                            *to = make_float2(0.0f, -1.0f);   // -1: not there
+                        }
+                    }
+                    ++known;
+                    tile_done(n);
                 }
-                tile_done(n);
+                asm volatile("cp.async.commit_group;" ::: "memory");
             };
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) fetch(j, key[j], value[j], have[j]);
-            bool going = true;
-            for (int n0 = 0; going; n0 += kAhead + 1) {
-#pragma unroll
-                for (int j = 0; j <= kAhead; ++j) {
-                    const int n = n0 + j, then = (j + kAhead) % (kAhead + 1);
-                    going = have[j];
-                    if (!going) break;
-                    fetch(n + kAhead, key[then], value[then], have[then]);
-                    GroupScales s;
-                    const float v = value[j] == -1.0f || !(value[j] < kTinyScale) ? value[j] : kTinyScale;
-                    s.key = key[j];
-                    s.log2_value = v == -1.0f ? -INFINITY : log2f(v);
-                    s.inv_value = v == -1.0f ? 0.0f : 1.0f / v;
-                    s.pad = 0.0f;
-                    // the scores two tiles back are made, so the weights four tiles back are: their place is free
-                    if (n >= 2) wait(&sm.s_full[n & 1], (n >> 1) - 1);
-                    if (lane < kGroups) sm.scales[n % kScaleRing][lane] = s;
-                    arrive(&sm.k_full[n & 1]);
-                }
+#pragma unroll 1
+            for (int n = -kAhead; n < known; ++n) {
+                fetch(n + kAhead);
+                if (n < 0) continue;
+                asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+                const float2 got = sm.stored[n % kTiles][lane % kGroups];
+                GroupScales s;
+                const float v = got.y == -1.0f || !(got.y < kTinyScale) ? got.y : kTinyScale;
+                s.key = got.x;
+                s.log2_value = v == -1.0f ? -INFINITY : log2f(v);
+                s.inv_value = v == -1.0f ? 0.0f : 1.0f / v;
+                s.pad = 0.0f;
+                // the scores two tiles back are made, so the weights four tiles back are: their place is free
+                if (n >= 2) wait(&sm.s_full[n & 1], (n >> 1) - 1);
+                if (lane < kGroups) sm.scales[n % kScaleRing][lane] = s;
+                arrive(&sm.k_full[n & 1]);
             }
         }
         // ---- MMA: the warp waits together, one lane issues
@@ -949,6 +949,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *dead) atomicCAS(a.status, 0, kCode);
     if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(sm.tmem, 512);
