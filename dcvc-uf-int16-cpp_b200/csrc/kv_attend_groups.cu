@@ -149,6 +149,29 @@ __device__ __forceinline__ uint32_t top2(uint32_t a, uint32_t b, __nv_bfloat16) 
     return *reinterpret_cast<const uint32_t*>(&m);
 }
 
+// One lane of a whole warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+// Products by the elected lane; a descriptor's address is in its lower word.
+__device__ __forceinline__ void product(uint32_t d, uint32_t a, uint32_t a_high, uint32_t b, uint32_t b_high, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n\t}" ::"r"(d), "r"(a), "r"(a_high), "r"(b), "r"(b_high), "r"(idesc),
+        "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+// A in tensor memory.
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t b_high, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tmov.b64 y, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(b_high), "r"(idesc),
+        "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+
 __device__ __forceinline__ void cp_async4(void* to, const void* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(to)), "l"(from) : "memory");
 }
@@ -685,54 +708,37 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             at0[i] = tile_at(w * 32 + i * kStep + sub, chunk * 2);
             at1[i] = tile_at(w * 32 + i * kStep + sub, chunk * 2 + 1);
         }
-        struct Next {
-            int page[2], row[2], head;   // of this warp's two groups of 16 keys
-            bool tile;                   // false: no further tile
-        };
-        int looked = 0;
-        bool have = true;
-        auto fetch = [&](Next& n) {
-            n.tile = false;
-            n.page[0] = n.page[1] = -1;
-            if (!have) return;
-            const Tile& t = tile_info(looked);
-            have = !(t.flags & kNone) && !*dead;
-            if (!have) return;
-            n.tile = true;
-            n.head = t.head;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                n.row[i] = (t.key0 + w * 32 + i * kGroupKeys) & (a.page_tokens - 1);
-                n.page[i] = t.page[w * 2 + i];
-            }
-            tile_done(looked++);
-        };
         uint4 buf[kLoads];
-        const uint8_t* from[2];
-        auto source = [&](const Next& n) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const long long tile = (static_cast<long long>(n.page[i]) * 2 + side) * a.heads + n.head;
-                from[i] = reinterpret_cast<const uint8_t*>(a.kv) + ((tile << a.page_shift) + n.row[i] + sub) * D + chunk * 16;
-            }
-        };
+        const uint8_t* from[2] = {};   // of this warp's two groups of 16 keys
+        int page[2] = {-1, -1};
         // what is not there keeps what was: its weights are 0
-        auto load = [&](int i, const Next& n) {
-            if (n.page[(i * kStep) >> 4] >= 0)   // sub < kStep, a divisor of 16
+        auto load = [&](int i) {
+            if (page[(i * kStep) >> 4] >= 0)   // sub < kStep, a divisor of 16
                 buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
         };
-        Next now, next;
-        fetch(now);
-        source(now);
+        bool more = true;
+        // tile n from its registers, which then take tile n + 1: a tile's time until it is looked at
+#pragma unroll 1
+        for (int n = -1; more; ++n) {
+            const Tile& t = tile_info(n + 1);
+            more = !(t.flags & kNone) && !*dead;
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            buf[i] = make_uint4(0, 0, 0, 0);
-            load(i, now);
-        }
-        fetch(next);
-        for (int n = 0; now.tile; ++n) {
+            for (int i = 0; i < 2; ++i) {
+                page[i] = more ? t.page[w * 2 + i] : -1;
+                const int row = ((t.key0 + w * 32 + i * kGroupKeys) & (a.page_tokens - 1)) + sub;
+                const long long tile = (static_cast<long long>(page[i]) * 2 + side) * a.heads + t.head;
+                from[i] = reinterpret_cast<const uint8_t*>(a.kv) + ((tile << a.page_shift) + row) * D + chunk * 16;
+            }
+            if (more) tile_done(n + 1);
+            if (n < 0) {
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) {
+                    buf[i] = make_uint4(0, 0, 0, 0);
+                    load(i);
+                }
+                continue;
+            }
             const int b = n & 1;
-            source(next);
             if (n >= 2) wait(&empty[b], (n >> 1) - 1);
             uint8_t* to = tiles + b * (kKeys * D * 2);
 #pragma unroll
@@ -744,13 +750,10 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 const int step = (i / 2) * 2 * kStep * 128;
                 *reinterpret_cast<uint4*>(to + at0[i & 1] + step) = make_uint4(y[0], y[1], y[2], y[3]);
                 *reinterpret_cast<uint4*>(to + at1[i & 1] + step) = make_uint4(y[4], y[5], y[6], y[7]);
-                // a tile's time until it is looked at
-                load(i, next);
+                load(i);
             }
             fence_proxy_async_smem();
             mbar_arrive(side ? &sm.p_full[b][0] : &sm.k_full[b]);
-            now = next;
-            fetch(next);
         }
     } else {
         regs_dec<80>();
@@ -892,10 +895,11 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         // ---- MMA: the warp waits together, one lane issues
         if (warp == kMmaWarp) {
             constexpr uint32_t qk = f16_idesc(128, kKeys, false), pv = f16_idesc(128, D, true);
-            constexpr uint64_t kTile = (kKeys * D * 2) >> 4;   // descriptor step between the two buffers
+            constexpr uint32_t kTile = (kKeys * D * 2) >> 4;   // descriptor step between the two buffers
             const uint64_t q_desc = sw128_desc(smem_u32(sm.q)), k_desc = sw128_desc(smem_u32(sm.k[0]));
             const uint64_t v_desc = sw128_n_major_desc(smem_u32(sm.v[0]), 128 * 128);
-            const uint32_t issue = lane == 0;
+            const uint32_t q_low = static_cast<uint32_t>(q_desc), q_high = static_cast<uint32_t>(q_desc >> 32);
+            const uint32_t v_high = static_cast<uint32_t>(v_desc >> 32);
             int n = 0;   // the piece's first tile
             for (int piece = 0;; ++piece) {
                 wait(&sm.piece_full[piece % kPieces], piece / kPieces);
@@ -912,38 +916,47 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                         wait(&sm.k_full[b], (n + i) >> 1);
                         __syncwarp();
                         tc_fence_after();
-                        const uint64_t kd = k_desc + b * kTile;
+                        if (elect_one()) {
+                            const uint32_t kd = static_cast<uint32_t>(k_desc) + b * kTile;
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            const int off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-                            mma_f16(tmem + Tmem<D>::s(b), q_desc + off, kd + off, qk, k > 0, issue);
+                            for (int k = 0; k < D / 16; ++k) {
+                                const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                                product(tmem + Tmem<D>::s(b), q_low + off, q_high, kd + off, q_high, qk, k > 0);
+                            }
+                            mma_commit(&sm.s_full[b]);
                         }
-                        mma_commit_if(&sm.s_full[b], issue);
+                        __syncwarp();
                     }
                     if (i > 0) {
                         const int b = (n + i - 1) & 1;
-                        const uint64_t vd = v_desc + b * kTile;
+                        const uint32_t vd = static_cast<uint32_t>(v_desc) + b * kTile;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             wait(&sm.p_full[b][h], (n + i - 1) >> 1);
                             __syncwarp();
                             tc_fence_after();
+                            if (elect_one()) {
 #pragma unroll
-                            for (int k = h * 4; k < h * 4 + 4; ++k)
-                                mma_f16_ts(tmem + Tmem<D>::o(b), tmem + Tmem<D>::s(b) + k * 8, vd + k * (16 * 128 >> 4), pv,
-                                           i > 2 || k > 0, issue);   // a piece's first two tiles begin their sums
+                                for (int k = h * 4; k < h * 4 + 4; ++k)
+                                    product_ts(tmem + Tmem<D>::o(b), tmem + Tmem<D>::s(b) + k * 8, vd + k * (16 * 128 >> 4), v_high, pv,
+                                               i > 2 || k > 0);   // a piece's first two tiles begin their sums
+                                if (h == 1) {
+                                    mma_commit(&sm.v_empty[b]);
+                                    if (i == count) mma_commit(&sm.o_full);
+                                }
+                            }
+                            __syncwarp();
                         }
-                        mma_commit_if(&sm.v_empty[b], issue);
                     }
                 }
-                mma_commit_if(&sm.o_full, issue);
                 n += count;
             }
             // nothing may be in flight when tensor memory is given back
-            if (lane == 0) {
+            if (elect_one()) {
                 mma_commit(&sm.drained);
                 mbar_wait(&sm.drained, 0, a.status, kCode);
             }
+            __syncwarp();
         }
         __syncwarp();
     }
