@@ -591,21 +591,27 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             if (busy) {
                 if (wide == 4) pair_sync();
                 else all_sync();
-                float top = -INFINITY;
-                for (int i = row; i < kRows; i += wide * 32) top = max3(top, sm.row[0][0][i], sm.row[0][1][i]);
-                // a part that saw nothing has no weight; one that is not finite spoils its row
-                auto part_of = [&](int u, int i) {
-                    const float m = sm.row[0][u][i];
-                    return m == -INFINITY ? (sm.row[1][u][i] == 0.0f ? 0.0f : 1.0f) : ex2(m - top);
-                };
-                float weight = 0.0f;
-                for (int i = row; i < kRows; i += wide * 32)
+                // of the lines that have this row
+                auto copy_of = [&](int i) { return ((i ^ quarter) & (wide - 1)) == 0; };
+                float tops[4][2], top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const float e = part_of(u, i);
-                        if (e != 0.0f) weight += sm.row[1][u][i] * e;
+                        tops[i][u] = copy_of(i) ? sm.row[0][u][i * 32 + lane] : -INFINITY;
+                        top = fmaxf(top, tops[i][u]);
                     }
-                const float e0 = part_of(0, line), e1 = part_of(1, line);
+                float weight = 0.0f, e0 = 0.0f, e1 = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float l = copy_of(i) ? sm.row[1][u][i * 32 + lane] : 0.0f;
+                        // a part that saw nothing has no weight; one that is not finite spoils its row
+                        const float e = tops[i][u] == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : ex2(tops[i][u] - top);
+                        if (e != 0.0f) weight += l * e;
+                        if (i == quarter) (u ? e1 : e0) = e;
+                    }
                 const bool whole = p.part < 0;
                 const int part = 2 * blockIdx.x + p.part;
                 const float inv = !whole ? 1.0f : weight == 0.0f ? 0.0f : 1.0f / weight;
@@ -653,17 +659,20 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                             sum16(dim0 / 16 + c, o);
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                place[line * kChunks + ((c * 4 + j) ^ (line & (kChunks - 1)))] =
+                                place[line * kChunks + ((c * 4 + j) ^ (lane & (kChunks - 1)))] =
                                     make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                         }
                         all_sync();
                         const int mine = kChunks * wide / 4;
+#pragma unroll 1
                         for (int c = copy * mine; c < copy * mine + mine; ++c) {
                             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            for (int i = row; i < kRows; i += wide * 32) {
-                                const float4 x = place[i * kChunks + (c ^ (line & (kChunks - 1)))];
-                                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-                            }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (copy_of(i)) {
+                                    const float4 x = place[(i * 32 + lane) * kChunks + (c ^ (lane & (kChunks - 1)))];
+                                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                                }
                             store4(dim0 + c * 4, v);
                         }
                         if (step == 0) all_sync();
