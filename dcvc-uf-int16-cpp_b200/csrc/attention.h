@@ -88,6 +88,7 @@ struct KvGroupState {
     struct Group {
         int32_t token0, tokens, stream0, streams;
         int32_t shared, slot, low, high;   // slot: of a stream that has them; least and largest position
+        int32_t own, pad[3];               // tiles of own keys of all its streams
     };
     Group* group;                          // [groups], 16-byte aligned
     int32_t* tiles;                        // [n] tiles of own keys of the group's streams up to this one

@@ -87,7 +87,8 @@ struct Smem {
     alignas(1024) uint8_t v[2][kKeys * D * 2];
     GroupScales scales[kScaleRing][kGroups];
     float2 stored[kTiles][kGroups];                // scales of keys and values as the pages have them
-    float row[2][2][kRows];                        // by parity: largest |q|, then maxima; weights
+    float row[2][2][kRows];                        // maxima, weights: by parity
+    float unit[kRows];                             // what a line's products count
     alignas(8) uint64_t k_full[2], v_empty[2], s_full[2], p_full[2][2];   // s_full: and the keys' place is free
     uint64_t q_full, o_full, drained, pair[4], all;
     uint64_t piece_full[kPieces], piece_empty[kPieces], tile_full[kTiles], tile_empty[kTiles];
@@ -182,6 +183,7 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 __device__ __forceinline__ bool group_tile(const AttendArgs& a, const GroupArgs& g, int group, int rt, GroupTile& t) {
     const int4* record = reinterpret_cast<const int4*>(g.state.group + group);
     const int4 place = record[0], keys = record[1];   // KvGroupState::Group
+    int own = g.state.group[group].own;
     t.token0 = place.x;
     t.row0 = rt * kRows;
     const int rows = place.y * a.group;
@@ -199,11 +201,12 @@ __device__ __forceinline__ bool group_tile(const AttendArgs& a, const GroupArgs&
         t.stream = g.state.stream[t.token0 + t.row0 / a.group];
         t.last = g.state.stream[t.token0 + (t.row0 + t.rows - 1) / a.group];
         if (t.stream > place.z) t.own = g.state.tiles[t.stream - 1];
+        own = g.state.tiles[t.last];
     }
     t.keys = key_range<kKeys>(a, t.shared, 0, t.low - t.shared, t.high - t.shared);
     t.common = t.keys.hi > 0 ? t.keys.nt : 0;
     // rows that see nothing are still written: one tile, all of it hidden
-    t.nt = max(t.common + g.state.tiles[t.last] - t.own, 1);
+    t.nt = max(t.common + own - t.own, 1);
     return true;
 }
 
@@ -243,15 +246,17 @@ struct GroupWalker {
 };
 
 // share_out by one warp, which needs no other: for few pairs (lanes take 32 at a time).
+// item: the tile that the share begins in.  tiles_of(p, t): the tiles of pair p, which is t.
 template <class Tiles>
-__device__ __forceinline__ Share share_of_warp(int pairs, Tiles tiles_of) {
+__device__ __forceinline__ Share share_of_warp(int pairs, Tiles tiles_of, GroupTile& item) {
     const int lane = threadIdx.x & 31;
     Share s;
-    long long first = 0;
+    GroupTile t;
+    long long v = 0;
     s.total = 0;
+#pragma unroll 1
     for (int base = 0; base < pairs; base += 32) {
-        const long long v = base + lane < pairs ? tiles_of(base + lane) : 0;
-        if (base == 0) first = v;
+        v = base + lane < pairs ? tiles_of(base + lane, t) : 0;
         s.total += v;
     }
 #pragma unroll 1
@@ -260,21 +265,29 @@ __device__ __forceinline__ Share share_of_warp(int pairs, Tiles tiles_of) {
     s.pair = pairs, s.pair_start = 0;
     const long long start = s.per * blockIdx.x;
     long long before = 0;
-    for (int base = 0; base < pairs && before <= start; base += 32) {
-        const long long v = base == 0 ? first : base + lane < pairs ? tiles_of(base + lane) : 0;
-        long long at = before + v;
+#pragma unroll 1
+    for (int base = 0; base < pairs; base += 32) {
+        if (pairs > 32) v = base + lane < pairs ? tiles_of(base + lane, t) : 0;
+        long long at = v;
 #pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
             const long long u = __shfl_up_sync(0xffffffffu, at, o);
-            if (lane >= o) at += u - before;
+            if (lane >= o) at += u;
         }
-        before = __shfl_sync(0xffffffffu, at, 31);
-        at -= v;
+        const long long sum = __shfl_sync(0xffffffffu, at, 31);
+        at += before - v;
         const uint32_t hit = __ballot_sync(0xffffffffu, at <= start && start < at + v);
         if (hit) {
-            s.pair = base + __ffs(hit) - 1;
-            s.pair_start = __shfl_sync(0xffffffffu, at, __ffs(hit) - 1);
+            const int from = __ffs(hit) - 1;
+            s.pair = base + from;
+            s.pair_start = __shfl_sync(0xffffffffu, at, from);
+            static_assert(sizeof(GroupTile) % 4 == 0, "words");
+#pragma unroll
+            for (int i = 0; i < static_cast<int>(sizeof(GroupTile) / 4); ++i)
+                reinterpret_cast<int*>(&item)[i] = __shfl_sync(0xffffffffu, reinterpret_cast<const int*>(&t)[i], from);
+            break;
         }
+        before += sum;
     }
     return s;
 }
@@ -315,16 +328,23 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     }
     tc_fence_before();
     const int pairs = g.groups * row_tiles;
-    auto tiles_of = [&](int p) -> long long {
-        GroupTile t;
-        return group_tile(a, g, p / row_tiles, p % row_tiles, t) ? static_cast<long long>(t.nt) * a.heads : 0;
+    auto tiles_of = [&](int p, GroupTile& t) -> long long {
+        const int group = row_tiles == 1 ? p : p / row_tiles;
+        return group_tile(a, g, group, p - group * row_tiles, t) ? static_cast<long long>(t.nt) * a.heads : 0;
     };
     __syncthreads();
     wait_for_previous();
     // Only the walker needs to know this CTA's share.  One warp finds it in 1 us where it takes
     // all the block's 2 us; from some hundred pairs on the block is faster.
     Share share;
-    if (pairs > kWarpPairs) share = share_out<kThreads>(pairs, 1, tiles_of, sm.share);
+    if (pairs > kWarpPairs)
+        share = share_out<kThreads>(
+            pairs, 1,
+            [&](int p) {
+                GroupTile t;
+                return tiles_of(p, t);
+            },
+            sm.share);
     tc_fence_after();
     // all 512 columns are this CTA's: its tensor memory begins at 0
     constexpr uint32_t tmem = 0;
@@ -390,37 +410,42 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             int pos = real ? g.state.positions[token] : -1;
             const bool write = real && pos != kNotWritten;
             if (!write) pos = -1;
-            float unit = 0.0f, m = -INFINITY, l = 0.0f;
+            float m = -INFINITY, l = 0.0f;
             bool far = false;   // a row of the warp has scores beyond kFar
-            if (busy) {
-                // half of the row's dims to [2^15, 2^16) and float16; the softmax scale's sign goes with it
-                const uint4* vec = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + static_cast<long long>(token) * a.q.token_stride +
-                                                                  head * a.q.head_stride) + t * (D / 16);
-                uint4 v[D / 16];
+            // The queries: a warp takes 16 lines, D / 8 lanes to a line.  To [2^15, 2^16) and
+            // float16; the softmax scale's sign goes with it.
+            {
+                constexpr int kLanes = D / 8, kLines = 32 / kLanes;
+                const int mine = (warp * 16 + (lane & 15)) & (wide * 32 - 1);   // a row for each lane's sake
+                const uint32_t there = __ballot_sync(0xffffffffu, mine < p.rows);
+                const int of_group = p.row0 + mine, of_token = of_group / a.group;
+                const long long at = (p.token0 + of_token) * a.q.token_stride + (p.head * a.group + of_group - of_token * a.group) * a.q.head_stride;
+                uint4 v[16 / kLines];
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) v[i] = real ? vec[i] : make_uint4(0, 0, 0, 0);
-                uint32_t largest = 0;
+                for (int i = 0; i < 16 / kLines; ++i) {
+                    const int j = i * kLines + lane / kLanes;
+                    const long long from = __shfl_sync(0xffffffffu, at, j);
+                    v[i] = make_uint4(0, 0, 0, 0);
+                    if (there >> j & 1) v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + from + lane % kLanes * 8);
+                }
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    largest = top2(top2(top2(largest, v[i].x, T()), v[i].y, T()), top2(v[i].z, v[i].w, T()), T());
-                const float2 f = unpack2(largest, T());
-                const float top = f.x == f.x && f.y == f.y ? fmaxf(f.x, f.y) : __int_as_float(0x7fffffff);
-                sm.row[0][t][line] = top;
-                pair_sync();
-                const float other = sm.row[0][t ^ 1][line];
-                const float u = row_unit(top == top && other == other ? fmaxf(top, other) : __int_as_float(0x7fffffff));
-                unit = unit_inverse(u) * fabsf(a.scale_log2);
-                const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
+                for (int i = 0; i < 16 / kLines; ++i) {
+                    const int j = warp * 16 + i * kLines + lane / kLanes;
+                    uint32_t largest = top2(top2(v[i].x, v[i].y, T()), top2(v[i].z, v[i].w, T()), T());
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
+                    for (int o = 1; o < kLanes; o <<= 1) largest = top2(largest, __shfl_xor_sync(0xffffffffu, largest, o), T());
+                    const float2 f = unpack2(largest, T());
+                    const float u = row_unit(f.x == f.x && f.y == f.y ? fmaxf(f.x, f.y) : __int_as_float(0x7fffffff));
+                    const float mul = u == u ? (a.scale_log2 < 0.0f ? -u : u) : 0.0f;
                     const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
                     uint32_t y[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 f = unpack2(x[j], T());
-                        y[j] = pack2(f.x * mul, f.y * mul, __half());
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 d = unpack2(x[k], T());
+                        y[k] = pack2(d.x * mul, d.y * mul, __half());
                     }
-                    *reinterpret_cast<uint4*>(sm.q + tile_at(line, t * (D / 16) + i)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    *reinterpret_cast<uint4*>(sm.q + tile_at(j, lane % kLanes)) = make_uint4(y[0], y[1], y[2], y[3]);
+                    if (lane % kLanes == 0) sm.unit[j] = unit_inverse(u) * fabsf(a.scale_log2);
                 }
             }
             fence_proxy_async_smem();
@@ -458,6 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     continue;
                 }
                 const GroupScales* sc = sm.scales[n % kScaleRing];
+                const float unit = sm.unit[line];
                 auto seen = [&](int c) {   // of 32 columns, a bit each
                     return bits_below(high - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
                 };
@@ -615,8 +641,9 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 const bool whole = p.part < 0;
                 const int part = 2 * blockIdx.x + p.part;
                 const float inv = !whole ? 1.0f : weight == 0.0f ? 0.0f : 1.0f / weight;
-                T* out = static_cast<T*>(a.out.data) + static_cast<long long>(token) * a.out.token_stride + head * a.out.head_stride;
-                float* sums = scratch.sums + (static_cast<long long>(part) * kRows + row) * D;
+                e0 *= inv, e1 *= inv;
+                T* out = static_cast<T*>(a.out.data) + head * a.out.head_stride;   // of a row: behind its token
+                float* sums = scratch.sums + static_cast<long long>(part) * kRows * D;
                 // 16 dims of this line
                 auto sum16 = [&](int c, float (&o)[16]) {
                     uint32_t x[16], y[16];
@@ -630,24 +657,24 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                         weigh2(o[j], o[j + 1], e0, __uint_as_float(y[j]), __uint_as_float(y[j + 1]), e1);
                     }
                 };
-                auto store4 = [&](int dim, float4 v) {
-                    if (write && whole)
-                        *reinterpret_cast<uint2*>(out + dim) = make_uint2(pack2(v.x * inv, v.y * inv, T()), pack2(v.z * inv, v.w * inv, T()));
-                    else if (real && !whole)
-                        __stcg(reinterpret_cast<float4*>(sums + dim), v);
-                };
+                auto store4 = [&](T* to, float4 v) { *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v.x, v.y, T()), pack2(v.z, v.w, T())); };
                 if (wide == 4) {
+                    T* to = out + static_cast<long long>(token) * a.out.token_stride;
 #pragma unroll 1
                     for (int c = t * (D / 32); c < (t + 1) * (D / 32); ++c) {
                         float o[16];
                         sum16(c, o);
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4) store4(c * 16 + j, make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]));
+                        for (int j = 0; j < 16; j += 4) {
+                            const float4 v = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                            if (write && whole) store4(to + c * 16 + j, v);
+                            else if (real && !whole) __stcg(reinterpret_cast<float4*>(sums + row * D + c * 16 + j), v);
+                        }
                         __syncwarp();
                     }
                 } else {
-                    // a quarter of the dims of all lines at a time through the queries' place, a
-                    // copy's threads then add up their share of it
+                    // a quarter of the dims of all lines at a time through the queries' place, where
+                    // neighbouring threads then add up neighbouring dims of a row
                     constexpr int kChunks = D / 16;   // of 4 dims, in a step of a set
                     float4* place = reinterpret_cast<float4*>(sm.q) + t * kRows * kChunks;
 #pragma unroll 1
@@ -663,17 +690,25 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                                     make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                         }
                         all_sync();
-                        const int mine = kChunks * wide / 4;
 #pragma unroll 1
-                        for (int c = copy * mine; c < copy * mine + mine; ++c) {
+                        for (int i = line; i < wide * 32 * kChunks; i += kRows) {
+                            const int r = i / kChunks, c = i % kChunks;
+                            if (r >= p.rows) break;
                             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (copy_of(i)) {
-                                    const float4 x = place[(i * 32 + lane) * kChunks + (c ^ (lane & (kChunks - 1)))];
+                            for (int k = 0; k < 4; ++k)
+                                if (k * wide < 4) {
+                                    const float4 x = place[(k * wide * 32 + r) * kChunks + (c ^ (r & (kChunks - 1)))];
                                     v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
                                 }
-                            store4(dim0 + c * 4, v);
+                            if (!whole) {
+                                __stcg(reinterpret_cast<float4*>(sums + r * D + dim0 + c * 4), v);
+                            } else {
+                                const int of_group = p.row0 + r, of_token = of_group / a.group;
+                                if (g.state.positions[p.token0 + of_token] != kNotWritten)
+                                    store4(static_cast<T*>(a.out.data) + (p.token0 + of_token) * a.out.token_stride +
+                                               (p.head * a.group + of_group - of_token * a.group) * a.out.head_stride + dim0 + c * 4, v);
+                            }
                         }
                         if (step == 0) all_sync();
                     }
@@ -768,15 +803,15 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         regs_dec<80>();
         if (warp == kWalkWarp) {
             // ---- walker: announces this CTA's pieces and their tiles
-            if (pairs <= kWarpPairs) share = share_of_warp(pairs, tiles_of);
             GroupWalker walk;
+            if (pairs <= kWarpPairs) share = share_of_warp(pairs, tiles_of, walk.t);
             walk.row_tiles = row_tiles;
             walk.pairs = pairs;
             walk.pos = share.per * blockIdx.x;
             walk.end = min(walk.pos + share.per, share.total);
             walk.pair = share.pair;
             walk.pair_start = share.pair_start;
-            walk.loaded = false;
+            walk.loaded = pairs <= kWarpPairs;
             int n = 0, piece = 0;
             for (; !*dead && walk.next(a, g); ++piece) {
                 const GroupTile& t = walk.t;

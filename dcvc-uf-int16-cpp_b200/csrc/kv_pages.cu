@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, c
         r.token0 = o0, r.tokens = ok ? o1 - o0 : 0, r.stream0 = first, r.streams = end - first;
         r.shared = shared, r.slot = members ? b.slots[chosen] : 0;
         r.low = lowest == INT_MAX ? -1 : lowest, r.high = highest;
+        r.own = sum, r.pad[0] = r.pad[1] = r.pad[2] = 0;
         out.group[group] = r;
     }
 }
