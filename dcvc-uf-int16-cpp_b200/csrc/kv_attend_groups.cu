@@ -1017,6 +1017,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
 // from kJoinRows * y on.  The parts' maxima and weights come first, once a row, by a
 // warp; then a thread adds the parts of four columns, in the order of the CTAs.
 constexpr int kJoinThreads = 256;
+constexpr int kJoinAhead = 8;   // parts
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) groups_join_kernel(const AttendArgs a, const GroupArgs g, int ctas) {
@@ -1030,6 +1031,16 @@ __global__ void __launch_bounds__(kJoinThreads) groups_join_kernel(const AttendA
     const int parts = item[0], rows = min(item[3] - first, kJoinRows);
     if (parts == 0 || rows <= 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4, row = first + r;
+    auto part_sums = [&](int i) {
+        const int from = 2 * (c0 + i) + (i == 0);
+        return __ldcg(reinterpret_cast<const float4*>(scratch.sums + (static_cast<long long>(from) * kRows + row) * D + d));
+    };
+    // the first parts are on their way while the weights are worked out
+    float4 ahead[kJoinAhead];
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i)
+        if (i < parts && r < rows) ahead[i] = part_sums(i);
     for (int r = warp; r < rows; r += kJoinThreads / 32) {
         float top = -INFINITY;
         for (int i = lane; i < parts; i += 32)
@@ -1049,17 +1060,17 @@ __global__ void __launch_bounds__(kJoinThreads) groups_join_kernel(const AttendA
         if (lane == 0) tops[r] = top, weights[r] = weight;
     }
     __syncthreads();
-    const int r = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
     if (r >= rows) return;
-    const int row = first + r;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-        const int from = 2 * (c0 + i) + (i == 0);
-        const float4 x = *reinterpret_cast<const float4*>(scratch.sums + (static_cast<long long>(from) * kRows + row) * D + d);
+    auto add = [&](int i, float4 x) {
         const float mul = share[i][r];
         v.x += x.x * mul, v.y += x.y * mul, v.z += x.z * mul, v.w += x.w * mul;
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kJoinAhead; ++i)
+        if (i < parts) add(i, ahead[i]);
+#pragma unroll 8
+    for (int i = kJoinAhead; i < parts; ++i) add(i, part_sums(i));
     const int in_group = item[2] + row;
     int token = in_group / a.group;
     const int head = item[4] * a.group + in_group - token * a.group;
