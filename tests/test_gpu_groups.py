@@ -2,7 +2,7 @@
 against plain implementations, and a search that runs them all.
 
 Attention is held to the tolerances of the plain attention (test_gpu_attention.py).
-The join of the two parts adds to a weight what its logarithms (base 2, at most a few
+The join of a row's parts adds to a weight what its logarithms (base 2, at most a few
 units beyond the scores, whose own rounding is counted there) and two exponentials lose:
 below 2^-19 of it.
 """
@@ -410,6 +410,56 @@ def test_groups_on_streams_and_in_graphs(ufb, dev):
         want, _, tol, _ = attend_ref(cache, 0, list(range(4, 24)), [1] * 20, q, 0, 0, True, 64 ** -0.5)
         full = tol * (1 + 2.0 ** -8) + ULP[torch.float16] * want.abs() + F16_TINY
         assert bool(((out.double() - want).abs() <= full).all())
+    _clean(ufb)
+
+
+@pytest.mark.parametrize("groups", [33, 70, 150])
+def test_groups_of_any_number(ufb, dev, groups):
+    """The work is divided by one warp, 32 (group, row tile) pairs at a time, or by a block where there are many."""
+    made = [((i * 37) % 300, [1 + i % 3] * (1 + i % 4)) for i in range(groups)]
+    cache, lengths, sizes = make_groups(ufb, dev, made, 2, 64, 16, seed=groups)
+    for dtype in (torch.float16, torch.bfloat16):
+        check_groups(ufb, cache, list(range(len(lengths))), [1] * len(lengths), sizes, 10, dtype)
+
+
+@pytest.mark.parametrize("rows", [31, 32, 33, 64, 65, 96, 97, 128, 129, 161])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_groups_row_counts(ufb, dev, rows, dim):
+    """Rows around the numbers that lie in a tile four times, two times and once; short items that no
+    other block shares, and long ones."""
+    cache, lengths, sizes = make_groups(ufb, dev, [(70, [3] * rows), (2500, [3] * rows)], 1, dim, 32, seed=rows)
+    check_groups(ufb, cache, list(range(rows)), [1] * rows, [rows], 1, torch.float16)
+    check_groups(ufb, cache, list(range(2 * rows)), [1] * (2 * rows), sizes, 1, torch.bfloat16)
+
+
+def test_groups_captured_behind_other_work(ufb, dev):
+    """In a graph the attention follows a copy, a fill, or what another stream did."""
+    cache, lengths, sizes = make_groups(ufb, dev, [(500, [9] * 6)], 2, 128, 32)
+    plan = cache.plan(list(range(6)), [1] * 6)
+    group = cache.group_plan(plan, [6])
+    cache.share(group)
+    source = [randn(dev, (6, 4, 128), i, torch.float16) for i in range(3)]
+    want = [cache.attend(0, plan, q, groups=group) for q in source]
+    given, q = torch.empty_like(source[0]), torch.empty_like(source[0])
+    main, side = torch.cuda.Stream(dev), torch.cuda.Stream(dev)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize(dev)
+    with torch.cuda.graph(graph, stream=main):
+        q.copy_(given)
+        after_copy = cache.attend(0, plan, q, groups=group)
+        q.zero_()
+        after_fill = cache.attend(0, plan, q, groups=group)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            q.copy_(given)
+        main.wait_stream(side)
+        after_side = cache.attend(0, plan, q, groups=group)
+    zero = cache.attend(0, plan, torch.zeros_like(q), groups=group)
+    for x, w in zip(source, want):
+        given.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        assert torch.equal(after_copy, w) and torch.equal(after_side, w) and torch.equal(after_fill, zero)
     _clean(ufb)
 
 
