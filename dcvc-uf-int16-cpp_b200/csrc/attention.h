@@ -88,26 +88,29 @@ struct KvGroupState {
     struct Group {
         int32_t token0, tokens, stream0, streams;
         int32_t shared, slot, low, high;   // slot: of a stream that has them; least and largest position
-        int32_t own, pad[3];               // tiles of own keys of all its streams
+        int32_t own, pad[3];               // of all its streams' own keys: `units`
     };
     Group* group;                          // [groups], 16-byte aligned
-    int32_t* tiles;                        // [n] tiles of own keys of the group's streams up to this one
-    int32_t* positions;                    // [tokens]; kNotWritten: its results are left alone
-    int32_t* stream;                       // [tokens] number of its stream in the batch
+    struct Token {
+        int32_t position;                  // kNotWritten: its results are left alone
+        int32_t own, end;                  // of the group's own keys, one after another: its stream's first, and the end
+        int32_t stream;                    // number in the batch
+    };
+    Token* token;                          // [tokens], 16-byte aligned
+    int32_t* units;                        // [n] kGroupUnit own keys each, of the group's streams up to this one
 };
 constexpr int kNotWritten = INT32_MIN;
-constexpr int kGroupTileKeys = 128;        // keys of a tile of kv_attend_groups
+constexpr int kGroupUnit = 16;             // own keys that begin together in a tile of kv_attend_groups
 struct GroupArgs {
     int groups, max_tokens;
     KvGroupState state;
 };
-inline KvGroupState kv_group_state(const ufb_kv_groups& g, int n, long long tokens) {
+inline KvGroupState kv_group_state(const ufb_kv_groups& g, long long tokens) {
     KvGroupState s;
     s.shared = g.state;
     s.group = reinterpret_cast<KvGroupState::Group*>(s.shared + (g.groups + 3) / 4 * 4);
-    s.tiles = reinterpret_cast<int32_t*>(s.group + g.groups);
-    s.positions = s.tiles + n;
-    s.stream = s.positions + tokens;
+    s.token = reinterpret_cast<KvGroupState::Token*>(s.group + g.groups);
+    s.units = reinterpret_cast<int32_t*>(s.token + tokens);
     return s;
 }
 cudaError_t kv_share(const ufb_kv_cache& c, const KvBatch& b, const ufb_kv_groups& g, int* status, cudaStream_t s);

@@ -313,7 +313,7 @@ int64_t ufb_capture_id(void* stream) {
 int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens) {
     clear_error();
     if (groups < 0 || n < 0 || tokens < 0 || tokens > INT32_MAX) return err(UFB_EINVAL, "invalid counts");
-    return (groups + 3ll) / 4 * 4 + 12ll * groups + n + 2 * tokens;
+    return (groups + 3ll) / 4 * 4 + 12ll * groups + n + 4 * tokens;
 }
 
 int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, int max_new,
@@ -411,7 +411,7 @@ int ufb_kv_attend_groups(const ufb_kv_cache* c, int layer, const int32_t* slots,
         !check_groups(groups, n, max_new, tokens))
         return last_code();
     if (!go || groups->groups == 0) return UFB_OK;
-    const GroupArgs g{groups->groups, groups->max_tokens, kv_group_state(*groups, n, tokens)};
+    const GroupArgs g{groups->groups, groups->max_tokens, kv_group_state(*groups, tokens)};
     return done(kv_attend_groups(a, g, dtype, sms, static_cast<cudaStream_t>(stream)), "kv attend groups");
 }
 

@@ -6,8 +6,11 @@
 // as in kv_attend_many.cu, in tiles of 128 rows x 128 keys on the fifth-generation tensor
 // cores.  The rows of a group -- all its streams' new tokens times the query heads of a
 // key head -- go through the common keys once; then, in the same accumulators, through
-// each stream's own keys, which only that stream's rows see.  Nothing has to be joined
-// but what CTAs share, and a step of a search is one launch and its join.
+// the streams' own keys, which only that stream's rows see.  Own keys lie in the tiles one
+// stream's behind the other's, from every 16th key on: 19 branches with 9 own tokens each
+// fill 3 tiles, not 19 (10 such groups, 8 heads of 128, 1324 common keys, 2 layers: 78 us
+// where a tile to each stream took 98).  Nothing has to be joined but what CTAs share, and
+// a step of a search is one launch and its join.
 //
 // One CTA an SM, six roles:
 //   walker (1 warp)      divides the work, and says of the tiles ahead (four at a time, a
@@ -27,7 +30,7 @@
 // become one at a piece's end.  Warps whose rows are padding, or no rows of an own tile's
 // stream, skip the softmax.
 //
-// Measured on 148 SMs: 64 branches x 65320 keys, 64 query heads over 8 of 128: 221 us, 610
+// Measured on 148 SMs: 64 branches x 65320 keys, 64 query heads over 8 of 128: 219 us, 620
 // TFLOP/s, 3200 cycles a tile; 8 streams x 8 branches, to 16381 keys, 4 heads of 128: 41 us
 // a layer, 2700 cycles a tile.  The products of a tile take 1300 alone, its exponentials
 // 1024, its integers 1400 from HBM.  What bounds a tile is the chain S -> softmax -> P V ->
@@ -46,8 +49,9 @@ namespace ufb {
 namespace {
 
 constexpr int kRows = 128;
-constexpr int kKeys = kGroupTileKeys;
+constexpr int kKeys = 128;
 constexpr int kGroups = kKeys / kGroupKeys;
+static_assert(kGroupUnit == kGroupKeys, "own keys begin where pages and scales are looked up");
 constexpr int kMmaWarp = 16, kWalkWarp = 17, kScaleWarp = 18;
 constexpr int kThreads = 640;         // warps: softmax 0-7, converter 8-15, MMA 16, walker 17, scales 18; 19 idle
 constexpr int kPieces = 4;            // pieces announced ahead
@@ -77,20 +81,20 @@ struct GroupTile {
     int shared, slot;       // common keys, and a stream that has them
     KeyRange keys;          // of the common ones
     int common, nt;         // tiles of common keys, of all
-    int stream, last, own;  // the row tile's streams; of their own tiles the first's place in the group's
+    int stream, last, own;  // the row tile's streams, their first tile among the group's of own keys
+    int before;             // units of own keys of the streams before
 };
 
 // A piece of an item as the walker announces it; rows 0: there is none any more.
 struct Announced {
-    int rows, row0, token0, head, parts, part;
+    int rows, row0, token0, head, parts, part, shared;
     int count;              // its tiles
 };
 // A tile of a piece.
 struct Tile {
-    int slot, key0, head;
-    int limit;              // keys below it are there
+    int key0, head;         // key0: of the common keys, or of the group's own ones
     int row_low, row_high;  // rows that may see it
-    int page[kGroups];      // of each 16 keys; -1: not looked at, or not there
+    int place[kGroups];     // of each 16 keys among the pool's; -1: not looked at, or not there
     int flags;              // kClear: all its rows see all of it; kOwnKeys; kNone: there is no further tile
 };
 constexpr int kClear = 1, kOwnKeys = 2, kNone = 4;
@@ -210,18 +214,19 @@ __device__ __forceinline__ bool group_tile(const AttendArgs& a, const GroupArgs&
     t.high = keys.w;
     t.stream = place.z;
     t.last = place.z + place.w - 1;
-    t.own = 0;
+    t.before = 0;
     if (rows > kRows) {
         // the streams of these rows only
-        t.stream = g.state.stream[t.token0 + t.row0 / a.group];
-        t.last = g.state.stream[t.token0 + (t.row0 + t.rows - 1) / a.group];
-        if (t.stream > place.z) t.own = g.state.tiles[t.stream - 1];
-        own = g.state.tiles[t.last];
+        t.stream = g.state.token[t.token0 + t.row0 / a.group].stream;
+        t.last = g.state.token[t.token0 + (t.row0 + t.rows - 1) / a.group].stream;
+        if (t.stream > place.z) t.before = g.state.units[t.stream - 1];
+        own = g.state.units[t.last];
     }
+    t.own = t.before / kGroups;
     t.keys = key_range<kKeys>(a, t.shared, 0, t.low - t.shared, t.high - t.shared);
     t.common = t.keys.hi > 0 ? t.keys.nt : 0;
     // rows that see nothing are still written: one tile, all of it hidden
-    t.nt = max(t.common + own - t.own, 1);
+    t.nt = max(t.common + (own > t.before ? (own + kGroups - 1) / kGroups - t.own : 0), 1);
     return true;
 }
 
@@ -422,9 +427,10 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             int token = in_group / a.group;
             const int head = p.head * a.group + in_group - token * a.group;
             token += p.token0;
-            int pos = real ? g.state.positions[token] : -1;
-            const bool write = real && pos != kNotWritten;
-            if (!write) pos = -1;
+            int4 seat = make_int4(-1, 0, 0, 0);   // KvGroupState::Token
+            if (real) seat = reinterpret_cast<const int4*>(g.state.token)[token];
+            const bool write = real && seat.x != kNotWritten;
+            const int pos = write ? seat.x : -1;
             float m = -INFINITY, l = 0.0f;
             bool far = false;   // a row of the warp has scores beyond kFar
             // The queries: a warp takes 16 lines, D / 8 lanes to a line.  To [2^15, 2^16) and
@@ -468,15 +474,19 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             for (int n = first + ((first ^ t) & 1); n < first + count; n += 2) {
                 const Tile& tile = tile_info(n);
                 const int flags = tile.flags;
-                // columns [0, high) that are from low on or below sink are seen by this row
-                int high = 0, low = 0, sink = 0;
+                // columns below high are seen by this row that are from low on, or from first on and below sink
+                int high = 0, low = 0, sink = 0, begin = 0;
                 bool mine = busy;   // rows of this warp that the tile is for
                 if (!(flags & kClear)) {
-                    const int key0 = tile.key0, limit = tile.limit, row_low = tile.row_low, row_high = tile.row_high;
+                    const int row_low = tile.row_low, row_high = tile.row_high;
                     mine = busy && row_low < row0 + 32 && row_high > row0;
-                    if (row >= row_low && row < row_high)
-                        high = min(limit, a.causal || !(flags & kOwnKeys) ? pos + 1 : limit) - key0;
-                    if (a.window) low = max(pos - a.window + 1, 0) - key0, sink = a.sinks - key0;
+                    // column of key 0
+                    const int zero = (flags & kOwnKeys ? seat.y - p.shared : 0) - tile.key0;
+                    begin = flags & kOwnKeys ? seat.y - tile.key0 : 0;
+                    const int end = flags & kOwnKeys ? seat.z - tile.key0 : p.shared - tile.key0;
+                    high = a.causal || !(flags & kOwnKeys) ? min(end, pos + 1 + zero) : end;
+                    low = begin;
+                    if (a.window) low = max(begin, pos - a.window + 1 + zero), sink = a.sinks + zero;
                 }
                 tile_done(n);
                 wait(&sm.s_full[t], n >> 1);
@@ -500,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 const GroupScales* sc = sm.scales[n % kScaleRing];
                 const float unit = sm.unit[line];
                 auto seen = [&](int c) {   // of 32 columns, a bit each
-                    return bits_below(high - c * 32) & (~bits_below(low - c * 32) | bits_below(sink - c * 32));
+                    return bits_below(high - c * 32) & (~bits_below(low - c * 32) | (bits_below(sink - c * 32) & ~bits_below(begin - c * 32)));
                 };
                 // 64 columns at a time, the later ones first: the others stay for their weights
                 uint32_t s0[32], s1[32];
@@ -720,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                                 __stcg(reinterpret_cast<float4*>(sums + r * D + dim0 + c * 4), v);
                             } else {
                                 const int of_group = p.row0 + r, of_token = of_group / a.group;
-                                if (g.state.positions[p.token0 + of_token] != kNotWritten)
+                                if (g.state.token[p.token0 + of_token].position != kNotWritten)
                                     store4(static_cast<T*>(a.out.data) + (p.token0 + of_token) * a.out.token_stride +
                                                (p.head * a.group + of_group - of_token * a.group) * a.out.head_stride + dim0 + c * 4, v);
                             }
@@ -769,10 +779,10 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
         }
         uint4 buf[kLoads];
         const uint8_t* from[2] = {};   // of this warp's two groups of 16 keys
-        int page[2] = {-1, -1};
+        int place[2] = {-1, -1};
         // what is not there keeps what was: its weights are 0
         auto load = [&](int i) {
-            if (page[(i * kStep) >> 4] >= 0)   // sub < kStep, a divisor of 16
+            if (place[(i * kStep) >> 4] >= 0)   // sub < kStep, a divisor of 16
                 buf[i] = __ldg(reinterpret_cast<const uint4*>(from[(i * kStep) >> 4] + ((i * kStep) & 15) * D));
         };
         bool more = true;
@@ -783,9 +793,9 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
             more = !(t.flags & kNone) && !*dead;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                page[i] = more ? t.page[w * 2 + i] : -1;
-                const int row = ((t.key0 + w * 32 + i * kGroupKeys) & (a.page_tokens - 1)) + sub;
-                const long long tile = (static_cast<long long>(page[i]) * 2 + side) * a.heads + t.head;
+                place[i] = more ? t.place[w * 2 + i] : -1;
+                const int row = (place[i] & (a.page_tokens / 16 - 1)) * 16 + sub;
+                const long long tile = (static_cast<long long>(place[i] >> (a.page_shift - 4)) * 2 + side) * a.heads + t.head;
                 from[i] = reinterpret_cast<const uint8_t*>(a.kv) + ((tile << a.page_shift) + row) * D + chunk * 16;
             }
             if (more) tile_done(n + 1);
@@ -836,6 +846,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     o.rows = t.rows;
                     o.row0 = t.row0;
                     o.token0 = t.token0;
+                    o.shared = t.shared;
                     o.head = walk.head;
                     o.count = walk.last - walk.first;
                     // the part of a shared item: 0 where an earlier CTA began it, 1 where this
@@ -847,52 +858,58 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 }
                 // four tiles at a time, a lane to 16 keys of one
                 const int my_tile = lane / kGroups, my_key = (lane % kGroups) * kGroupKeys;
-                // own tiles: of stream `s`, whose first is number `from` of the group's
-                int s = t.stream, from = t.own, until = g.state.tiles[s];
+                // own keys: of stream `s`, whose units are [from, until) of the group's
+                int s = t.stream, from = t.before, until = g.state.units[s];
                 for (int i0 = walk.first; i0 < walk.last; i0 += 4) {
                     const int i = min(i0 + my_tile, walk.last - 1);
                     Tile o;
-                    bool looked_at;          // lane's 16 keys
                     o.head = walk.head;
                     o.flags = 0;
                     o.row_low = 0;
                     o.row_high = kRows;
+                    int slot = t.slot, key = -1;          // lane's 16 keys; -1: not looked at
                     if (i < t.common) {
-                        o.slot = t.slot;
                         o.key0 = t.keys.tile(i) * kKeys;
-                        o.limit = t.shared;
-                        looked_at = t.keys.touches(o.key0 + my_key);
+                        if (t.keys.touches(o.key0 + my_key)) key = o.key0 + my_key;
                         if (o.key0 + kKeys - 1 <= t.low && o.key0 + kKeys <= t.shared &&
                             (!a.window || t.high - o.key0 < a.window || o.key0 + kKeys <= a.sinks))
                             o.flags |= kClear;
                     } else {
-                        const int own = t.own + i - t.common;
-                        while (own >= until && s < t.last) from = until, until = g.state.tiles[++s];
-                        const bool there = own < until;      // else the tile of rows that see nothing
-                        o.slot = there ? a.slots[s] : 0;
-                        o.key0 = there ? t.shared + (own - from) * kKeys : 0;
-                        o.limit = there ? a.lengths[o.slot] : 0;
-                        looked_at = o.key0 + my_key < o.limit;
-                        o.row_low = (a.offsets[s] - t.token0) * a.group - t.row0;
-                        o.row_high = (a.offsets[s + 1] - t.token0) * a.group - t.row0;
+                        o.key0 = (t.own + i - t.common) * kKeys;
                         o.flags |= kOwnKeys;
-                        if (!there) o.row_low = 0, o.row_high = kRows;
+                        const int unit = (o.key0 + my_key) / kGroupUnit;
+                        while (unit >= until && s < t.last) from = until, until = g.state.units[++s];
+                        if (unit >= from && unit < until) {
+                            slot = a.slots[s];
+                            key = t.shared + (unit - from) * kGroupUnit;
+                            o.row_low = (a.offsets[s] - t.token0) * a.group - t.row0;
+                            o.row_high = (a.offsets[s + 1] - t.token0) * a.group - t.row0;
+                        } else {
+                            o.row_low = kRows, o.row_high = 0;
+                        }
                     }
-                    int page = -1;
-                    const int entry = (o.key0 + my_key) >> a.page_shift;
-                    if (looked_at && entry < a.table_width) {
-                        page = a.table[static_cast<long long>(o.slot) * a.table_width + entry];
-                        if (page >= a.pages) page = -1;
+                    // all its streams' rows
+#pragma unroll
+                    for (int d = 1; d < kGroups; d <<= 1) {
+                        o.row_low = min(o.row_low, __shfl_xor_sync(0xffffffffu, o.row_low, d));
+                        o.row_high = max(o.row_high, __shfl_xor_sync(0xffffffffu, o.row_high, d));
+                    }
+                    int place = -1;
+                    const int entry = key >> a.page_shift;
+                    if (key >= 0 && entry < a.table_width) {
+                        const int page = a.table[static_cast<long long>(slot) * a.table_width + entry];
+                        if (page >= 0 && page < a.pages)
+                            place = (page << (a.page_shift - 4)) + ((key & (a.page_tokens - 1)) >> 4);
                     }
                     const int tiles = min(walk.last - i0, 4);
                     for (int j = 0; j < tiles; ++j, ++n) {
                         if (n >= kTiles) wait(&sm.tile_empty[n % kTiles], n / kTiles - 1);
                         Tile& to = sm.tiles[n % kTiles];
                         if (my_tile == j) {
-                            to.page[lane % kGroups] = page;
+                            to.place[lane % kGroups] = place;
                             if (lane % kGroups == 0) {
-                                to.slot = o.slot, to.key0 = o.key0, to.head = o.head, to.limit = o.limit;
-                                to.row_low = o.row_low, to.row_high = o.row_high, to.flags = o.flags;
+                                to.key0 = o.key0, to.head = o.head, to.flags = o.flags;
+                                to.row_low = o.row_low, to.row_high = o.row_high;
                             }
                         }
                         arrive(&sm.tile_full[n % kTiles]);
@@ -920,8 +937,8 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 if (more) {
                     if (lane < kGroups) {
                         float2* to = &sm.stored[n % kTiles][lane];
-                        if (t->page[lane] >= 0) {
-                            const float* s = a.scale + static_cast<long long>(t->page[lane]) * 2 * a.heads + t->head;
+                        if (t->place[lane] >= 0) {
+                            const float* s = a.scale + static_cast<long long>(t->place[lane] >> (a.page_shift - 4)) * 2 * a.heads + t->head;
                             cp_async4(&to->x, s);
                             cp_async4(&to->y, s + a.heads);
                         } else {
@@ -1090,7 +1107,7 @@ __global__ void __launch_bounds__(kJoinThreads) groups_join_kernel(const AttendA
     int token = in_group / a.group;
     const int head = item[4] * a.group + in_group - token * a.group;
     token += item[1];
-    if (g.state.positions[token] == kNotWritten) return;
+    if (g.state.token[token].position == kNotWritten) return;
     const float top = tops[r], weight = weights[r];
     const float inv = weight == 0.0f ? 0.0f : 1.0f / weight;
     T* to = static_cast<T*>(a.out.data) + static_cast<long long>(token) * a.out.token_stride + head * a.out.head_stride + d;

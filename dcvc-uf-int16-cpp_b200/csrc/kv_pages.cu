@@ -501,14 +501,15 @@ __global__ void __launch_bounds__(kApplyThreads) reorder_apply_kernel(const ufb_
 
 // What the streams of group blockIdx.x have in common: the leading entries that are equal
 // in all their tables, inside of every one's earlier tokens.  Streams that bring no tokens,
-// or whose extend was refused, do not count.  Then how many tiles of own keys the streams
-// have, summed up over the group.  Latency of three passes over the streams: 3.5 us for 4
-// streams of 1769 tokens, 4.9 for 8 groups of 8, 9.6 for 64 streams of 65320 (2 a warp, 511
-// entries each).
+// or whose extend was refused, do not count.  Then where each stream's own keys lie among
+// the group's, one stream's behind the other's in units of kGroupUnit, and the tokens'
+// positions.  Latency of three passes over the streams: 4.0 us for 4 streams of 1769 tokens,
+// 5.7 for 8 groups of 8, 14 for 64 streams of 65320 (2 a warp, 511 entries each).
 __global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, const KvBatch b, const ufb_kv_groups g,
                                                          const KvGroupState out, int* status) {
     __shared__ int warp_sum[kWarps];
     __shared__ int width, lowest, highest, members, chosen;
+    __shared__ long long warp_units[kWarps];
     const int group = blockIdx.x, first = max(g.first[group], 0), end = min(g.first[group + 1], b.n);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) width = c.table_width, lowest = INT_MAX, highest = -1, members = 0, chosen = INT_MAX;
@@ -539,13 +540,9 @@ __global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, c
     }
     __syncthreads();
     const int most = width;
-    // a warp to a stream: its positions, and where its table first differs from the chosen one's
+    // a warp to a stream: where its table first differs from the chosen one's
     for (int i = first + warp; i < end; i += kWarps) {
-        const int slot = look(i), o0 = b.offsets[i], o1 = b.offsets[i + 1];
-        for (int t = max(o0, 0) + lane; t < o1 && t < b.tokens; t += 32) {
-            out.positions[t] = slot == -1 ? kNotWritten : slot == -2 ? -1 : start + t - o0;
-            out.stream[t] = i;
-        }
+        const int slot = look(i);
         if (slot < 0 || members < 2 || i == chosen) continue;
         const int32_t* own = c.table + static_cast<long long>(slot) * c.table_width;
         const int32_t* other = c.table + static_cast<long long>(b.slots[chosen]) * c.table_width;
@@ -565,19 +562,46 @@ __global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, c
     }
     __syncthreads();
     const int shared = members > 1 ? width * c.page_tokens : 0;
+    // tokens from..., `step` apart, of stream i, whose own keys are behind `before` units
+    auto seat = [&](int i, int slot, int before, int from, int step) {
+        KvGroupState::Token r;
+        r.own = before * kGroupUnit;
+        r.end = slot >= 0 ? r.own + start + count - shared : r.own;
+        r.stream = i;
+        const int o0 = b.offsets[i], o1 = min(b.offsets[i + 1], static_cast<int>(min(b.tokens, static_cast<long long>(INT_MAX))));
+        for (int t = max(o0, 0) + from; t < o1; t += step) {
+            r.position = slot == -1 ? kNotWritten : slot == -2 ? -1 : start + t - o0;
+            out.token[t] = r;
+        }
+    };
+    const bool few = b.max_new <= 4;   // tokens of a stream: its thread writes them, else a warp
     int sum = 0;
+    long long many = 0;
     for (int i0 = first; i0 < end; i0 += kThreads) {
         const int i = i0 + threadIdx.x, slot = i < end ? look(i) : -1;
         int total;
-        const int tiles = slot >= 0 ? (start + count - shared + kGroupTileKeys - 1) / kGroupTileKeys : 0;
-        const int before = block_scan(tiles, warp_sum, total);
-        if (i < end) out.tiles[i] = sum + before + tiles;
+        const int units = slot >= 0 ? (start + count - shared + kGroupUnit - 1) / kGroupUnit : 0;
+        many += units;
+        const int before = block_scan(units, warp_sum, total);
+        if (i < end) out.units[i] = sum + before + units;
+        if (i < end && few) seat(i, slot, sum + before, 0, 1);
         sum += total;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) many += __shfl_xor_sync(0xffffffffu, many, o);
+    if (lane == 0) warp_units[warp] = many;
+    __syncthreads();
+    for (int i = first + warp; !few && i < end; i += kWarps) seat(i, look(i), i > first ? out.units[i - 1] : 0, lane, 32);
+    if (warp == 0) {
+        many = warp_units[lane];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) many += __shfl_xor_sync(0xffffffffu, many, o);
     }
     if (threadIdx.x == 0) {
         out.shared[group] = shared;
         const int o0 = g.offsets[group], o1 = g.offsets[group + 1];
-        const bool ok = o0 >= 0 && o1 >= o0 && o1 <= b.tokens && o1 - o0 <= g.max_tokens && first <= end;
+        const bool ok = o0 >= 0 && o1 >= o0 && o1 <= b.tokens && o1 - o0 <= g.max_tokens && first <= end &&
+                        many <= INT_MAX / kGroupUnit - 8;
         if (!ok) atomicCAS(status, 0, kStatusIndex);
         KvGroupState::Group r;
         r.token0 = o0, r.tokens = ok ? o1 - o0 : 0, r.stream0 = first, r.streams = end - first;
@@ -651,7 +675,7 @@ cudaError_t kv_reorder(const ufb_kv_cache& c, const int32_t* slots, const int32_
 }
 
 cudaError_t kv_share(const ufb_kv_cache& c, const KvBatch& b, const ufb_kv_groups& g, int* status, cudaStream_t s) {
-    share_kernel<<<g.groups, kThreads, 0, s>>>(c, b, g, kv_group_state(g, b.n, b.tokens), status);
+    share_kernel<<<g.groups, kThreads, 0, s>>>(c, b, g, kv_group_state(g, b.tokens), status);
     return cudaGetLastError();
 }
 

@@ -611,7 +611,8 @@ int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens);
 /* Find what each group has in common: the leading table entries that are equal in
  * all its streams, as far as they lie before every stream's new tokens (streams
  * that bring none, or whose extend was refused, do not count; none in a group of
- * one; status 31 for one whose extend was refused: its queries see no key).  state[g]
+ * one; status 31 for one whose extend was refused: its queries see no key; 32 for a
+ * group with 2^31 - 144 own keys or more, whose results are left alone).  state[g]
  * are the tokens on them.  Once a step, behind ufb_kv_extend: it holds
  * until a call changes tables or lengths. */
 int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, int max_new,

@@ -46,6 +46,6 @@ def test_group_refusals(att):  # noqa: F811
     assert share(groups(n=0, first=None, most=0), n=0, max_new=0, tokens=0) == 0
     for over in (dict(layer=2), dict(layer=-1), dict(window=-1)):
         assert attend(groups(), **over) == EINVAL, over
-    assert L.ufb_kv_group_ints(2, 4, 5) == 4 + 12 * 2 + 4 + 2 * 5
+    assert L.ufb_kv_group_ints(2, 4, 5) == 4 + 12 * 2 + 4 + 4 * 5
     for args in ((-1, 4, 5), (2, -1, 5), (2, 4, -1), (2, 4, 1 << 31)):
         assert L.ufb_kv_group_ints(*args) == EINVAL
