@@ -600,8 +600,9 @@ __global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, c
     if (threadIdx.x == 0) {
         out.shared[group] = shared;
         const int o0 = g.offsets[group], o1 = g.offsets[group + 1];
-        const bool ok = o0 >= 0 && o1 >= o0 && o1 <= b.tokens && o1 - o0 <= g.max_tokens && first <= end &&
-                        many <= INT_MAX / kGroupUnit - 8;
+        // the tokens are those of the streams: every one of them has its record
+        const bool ok = first <= end && o0 == b.offsets[first] && o1 == b.offsets[end] && o0 >= 0 && o1 >= o0 && o1 <= b.tokens &&
+                        o1 - o0 <= g.max_tokens && many <= INT_MAX / kGroupUnit - 8;
         if (!ok) atomicCAS(status, 0, kStatusIndex);
         KvGroupState::Group r;
         r.token0 = o0, r.tokens = ok ? o1 - o0 : 0, r.stream0 = first, r.streams = end - first;

@@ -372,6 +372,25 @@ def test_groups_refusals(ufb, dev):
     _clean(ufb)
 
 
+@pytest.mark.parametrize("which", ["first", "offsets"])
+def test_groups_that_are_not_the_streams(ufb, dev, which):
+    """Group bounds that do not belong to the batch: reported, the group's results left alone."""
+    cache, lengths, sizes = make_groups(ufb, dev, [(100, [5] * 3), (200, [5] * 2)], 2, 64, 16)
+    plan = cache.plan(list(range(5)), [2] * 5)
+    groups = cache.group_plan(plan, sizes)
+    q = randn(dev, (10, 4, 64), 1, torch.float16)
+    cache.share(groups)
+    want = cache.attend(0, plan, q, groups=groups)
+    _clean(ufb)
+    getattr(groups, which)[1] -= 1   # the border between the groups
+    cache.share(groups)
+    assert ufb.device_status(0) == 32
+    getattr(groups, which)[1] += 1
+    cache.share(groups)
+    assert torch.equal(cache.attend(0, plan, q, groups=groups), want)
+    _clean(ufb)
+
+
 def test_groups_on_streams_and_in_graphs(ufb, dev):
     """Calls side by side do not share scratch; a captured step follows tables and lengths."""
     cache, lengths, sizes = make_groups(ufb, dev, [(3000, [9] * 4), (2000, [9] * 20)], 2, 64, 32, spare=80)
