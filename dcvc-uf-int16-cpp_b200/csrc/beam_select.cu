@@ -39,6 +39,7 @@ constexpr int kBatch = 4;         // vectors of a thread that are loaded togethe
 constexpr int kStretches = 8;     // of a thread's batches, whose largest values are kept
 constexpr int kFound = 1024;      // candidates that are counted against each other
 constexpr int kMostParts = 32;    // of a row
+constexpr int kAhead = 4;         // candidates of a thread in the join that are loaded beside the sums
 constexpr int kPartCost = 900;    // of a part in warp instructions: threshold, gather, ranks (700 to 900 counted)
 // Sums are of exp itself while the part's largest logit is inside this, else of exp(x - largest).
 constexpr float kPlain = 600.0f;
@@ -559,23 +560,42 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
     const unsigned char* work = static_cast<const unsigned char*>(a.workspace) + static_cast<long long>(stream) * a.beams * parts * bytes;
     if (tid == 0) lives = endeds = finds = 0;
     __syncthreads();
-    bool live = false;
-    float mine = 0.0f;
     if (tid < a.beams) {
         // the inputs are older than the launch before
         const long long row = static_cast<long long>(stream) * a.beams + tid;
-        mine = a.scores[row];
-        live = row_is_read(a, row);
-        if (mine > -INFINITY && !live) ended[atomicAdd(&endeds, 1)] = static_cast<unsigned long long>(ordered(mine)) << 32 | (0xffffffffu - tid);
+        const float mine = a.scores[row];
+        if (row_is_read(a, row)) {
+            const int place = atomicAdd(&lives, 1);
+            alive[place] = tid;
+            score[place] = mine;
+        } else if (mine > -INFINITY) {
+            ended[atomicAdd(&endeds, 1)] = static_cast<unsigned long long>(ordered(mine)) << 32 | (0xffffffffu - tid);
+        }
     }
+    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (live) {
+    // candidates of a row lie one after another, all[parts * count] of each
+    const int each = parts * count, all = lives * each;
+    auto key_of = [&](int c, int& row) {   // (ordered logit, ~token)
+        row = c / each;
+        const int in_row = c - row * each, part = in_row / count;
+        return reinterpret_cast<const unsigned long long*>(work + (alive[row] * parts + part) * bytes + sizeof(Part))[in_row - part * count];
+    };
+    // a thread's first ones are on their way while the sums are worked out
+    unsigned long long keys[kAhead];
+    int rows[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+        keys[k] = 0, rows[k] = 0;
+        if (tid + k * kThreads < all) keys[k] = key_of(tid + k * kThreads, rows[k]);
+    }
+    if (tid < lives) {
         // the row's sum, its parts in order
         double ref = -INFINITY, sum = 0.0;
         bool bad = false;
 #pragma unroll 4
         for (int c = 0; c < parts; ++c) {
-            const Part r = *reinterpret_cast<const Part*>(work + (tid * parts + c) * bytes);
+            const Part r = *reinterpret_cast<const Part*>(work + (alive[tid] * parts + c) * bytes);
             bad |= !(r.sum < INFINITY);
             if (!(r.sum > 0.0)) continue;
             // sums of one reference, as most are, are just added
@@ -586,29 +606,31 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
         }
         // NaN or +infinity in the row: no candidates of it
         if (bad) atomicCAS(a.status, 0, kStatusLogits);
-        if (!bad && sum > 0.0) {
-            const int place = atomicAdd(&lives, 1);
-            alive[place] = tid;
-            lse[place] = ref + log(sum);
-            score[place] = mine;
-        }
+        lse[tid] = !bad && sum > 0.0 ? ref + log(sum) : NAN;
     }
     __syncthreads();
-    // candidates of a row lie one after another, all[parts * count] of each
-    const int each = parts * count, all = lives * each;
-    auto candidate = [&](int c) {
-        const int row = c / each, in_row = c - row * each, part = in_row / count, beam = alive[row];
+    auto candidate_of = [&](unsigned long long key, int row) {
         Candidate x;
-        x.low = reinterpret_cast<const unsigned long long*>(work + (beam * parts + part) * bytes + sizeof(Part))[in_row - part * count];
-        const float logit = unordered(static_cast<uint32_t>(x.low >> 32));
+        x.low = key;
+        const float logit = unordered(static_cast<uint32_t>(key >> 32));
         const float t = static_cast<float>(score[row] + (static_cast<double>(logit) - lse[row]));
-        x.high = x.low && t > -INFINITY ? static_cast<unsigned long long>(ordered(t)) << 32 | (0xffffffffu - beam) : 0;
+        x.high = key && t > -INFINITY ? static_cast<unsigned long long>(ordered(t)) << 32 | (0xffffffffu - alive[row]) : 0;
         return x;
     };
+    auto candidate = [&](int c) {
+        int row;
+        const unsigned long long key = key_of(c, row);
+        return candidate_of(key, row);
+    };
+    uint32_t totals[kAhead];   // ordered; 0: none
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) totals[k] = keys[k] ? static_cast<uint32_t>(candidate_of(keys[k], rows[k]).high >> 32) : 0;
     // a threshold on the totals as in the parts, from each thread's largest
     uint32_t best = 0;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) best = max(best, totals[k]);
 #pragma unroll 4
-    for (int c = tid; c < all; c += kThreads) best = max(best, static_cast<uint32_t>(candidate(c).high >> 32));
+    for (int c = tid + kAhead * kThreads; c < all; c += kThreads) best = max(best, static_cast<uint32_t>(candidate(c).high >> 32));
     const int warps = min(all / 32, kWarps);
     const int rounds = warps ? (count + warps - 1) / warps : 33;
     uint32_t least = rounds > 32 ? 0 : 0xffffffffu;
@@ -625,12 +647,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) least = min(least, limit[w]);
     least = max(least, 1u);
-#pragma unroll 4
-    for (int c = tid; c < all; c += kThreads) {
-        const Candidate x = candidate(c);
-        if (static_cast<uint32_t>(x.high >> 32) < least) continue;
+    auto keep = [&](const Candidate& x) {
         const int place = atomicAdd(&finds, 1);
         if (place < kFound - kBeamMax) found[place] = x;
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+        if (totals[k] >= least)
+            keep(Candidate{static_cast<unsigned long long>(totals[k]) << 32 | (0xffffffffu - alive[rows[k]]), keys[k]});
+#pragma unroll 4
+    for (int c = tid + kAhead * kThreads; c < all; c += kThreads) {
+        const Candidate x = candidate(c);
+        if (static_cast<uint32_t>(x.high >> 32) >= least) keep(x);
     }
     __syncthreads();
     if (finds > kFound - kBeamMax) {
