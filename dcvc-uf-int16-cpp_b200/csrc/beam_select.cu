@@ -574,13 +574,20 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
     }
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // Candidates by their place in a part's list, then the part, then the row, dealt out to the
-    // warps one by one: every warp has as many of the first places and of every row, and the
-    // threshold below is near what it has to be.  (A row to a warp, as they lie, let hundreds
-    // through where rows differ: 18 us for 9 of 32 streams x 16 beams x 32.)
+    // Candidates are numbered by their place in a part's list, then the part, then the row, and
+    // dealt out by an odd multiple: neighbouring threads, and a thread's own, have different
+    // places and rows, and the threshold below lets few more through than it has to.  (As they
+    // lie, a row to a warp, hundreds pass where rows differ: 18 us for 9 of 32 streams x 16
+    // beams x 32; with the rows in turn, where their number and the warps' have a factor in
+    // common.)
     const int all = lives * parts * count;
-    const int warps = min((all + 31) / 32, kWarps), stride = warps * 32;   // no more than have something to do
-    const int e0 = warp < warps ? lane * warps + warp : all;
+    const int deals = all > 32 ? 1 << (32 - __clz(all - 1)) : 32;   // a power of two, all or more
+    const int each = max(deals / kThreads, 1);                       // of a thread
+    auto dealt = [&](int k) {   // the thread's k-th; all: none
+        const uint32_t e = tid * each + k;
+        return k < each && e < deals ? static_cast<int>(e * 0x9e3779b1u & (deals - 1)) : all;
+    };
+    const int warps = min(deals / 32, kWarps);
     const float lives_inv = 1.0f / lives, parts_inv = 1.0f / parts;
     static_assert(UFB_BEAM_MAX * UFB_BEAM_COUNT_MAX * kMostParts <= 1 << 17, "candidates of a stream");
     auto key_of = [&](int c, int& row) {   // (ordered logit, ~token)
@@ -595,7 +602,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
         keys[k] = 0, rows[k] = 0;
-        if (e0 + k * stride < all) keys[k] = key_of(e0 + k * stride, rows[k]);
+        const int c = dealt(k);
+        if (c < all) keys[k] = key_of(c, rows[k]);
     }
     if (tid < lives) {
         // the row's sum, its parts in order
@@ -638,7 +646,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) best = max(best, totals[k]);
 #pragma unroll 4
-    for (int c = e0 + kAhead * stride; c < all; c += stride) best = max(best, static_cast<uint32_t>(candidate(c).high >> 32));
+    for (int k = kAhead; k < each; ++k)
+        if (dealt(k) < all) best = max(best, static_cast<uint32_t>(candidate(dealt(k)).high >> 32));
     uint32_t least = warp < warps ? 0 : 0xffffffffu;
     for (int r = 0; warp < warps && r * warps < count; ++r) {
         least = __reduce_max_sync(0xffffffffu, best);
@@ -660,8 +669,9 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
         if (totals[k] >= least)
             keep(Candidate{static_cast<unsigned long long>(totals[k]) << 32 | (0xffffffffu - alive[rows[k]]), keys[k]});
 #pragma unroll 4
-    for (int c = e0 + kAhead * stride; c < all; c += stride) {
-        const Candidate x = candidate(c);
+    for (int k = kAhead; k < each; ++k) {
+        if (dealt(k) >= all) continue;
+        const Candidate x = candidate(dealt(k));
         if (static_cast<uint32_t>(x.high >> 32) >= least) keep(x);
     }
     __syncthreads();
