@@ -40,7 +40,7 @@ constexpr int kStretches = 8;     // of a thread's batches, whose largest values
 constexpr int kFound = 1024;      // candidates that are counted against each other
 constexpr int kMostParts = 32;    // of a row
 constexpr int kAhead = 4;         // candidates of a thread in the join that are loaded beside the sums
-constexpr int kPartCost = 900;    // of a part in warp instructions: threshold, gather, ranks (700 to 900 counted)
+constexpr int kPartCost = 28;     // of a part, in values of a thread
 // Sums are of exp itself while the part's largest logit is inside this, else of exp(x - largest).
 constexpr float kPlain = 600.0f;
 
@@ -725,29 +725,36 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
     }
 }
 
-// Parts of a row: the number with the least time, in instructions of a warp: a vector of a
-// thread takes about 18 for each of its values, and a part kPartCost besides; what does not
-// fit on the GPU at a time comes after.
+// Parts of a row: the number with the least time of the SM that has the most CTAs.  An SM
+// takes about as long for each value whether one CTA or four are on it (a row of 65537 floats
+// alone 10 us; the pipes bound it), so what counts is how evenly the work lies, against what
+// a part costs besides.  Measured with other numbers of parts: 64 streams x 8 beams x 32768
+// 24 us (2 parts 31, 4: 40), 48 x 8 x 50257 27.5 (2: 30, 3: 34), 32 x 16 x 131072 with a
+// fifth of the beams ended 61 (1: 69, 4: 74), 8 x 8 x 131072 18 (1: 25, 4: 19), 1 x 8 x 131072
+// 12 (1: 23, 4: 14), 16 x 4 x 50000 floats 11.4 (1: 14.4, 3: 13.2), 24 x 5 x 65537 floats 17.3
+// (3: 18.7, 6: 23.6).  No more candidates than the join's threads have at hand (17 parts of the
+// 8 rows take 15.7 us, 13 12.2).
 struct Division {
     int parts, vecs;
 };
 template <typename T>
-Division divide(int streams, int beams, int vocab, int sms) {
+Division divide(int streams, int beams, int vocab, int count, int sms) {
     constexpr int elements = kElems<T>;
     const int row_vecs = (vocab + 2 * elements - 2) / elements;    // of any alignment
-    const long long rows = static_cast<long long>(streams) * beams, slots = static_cast<long long>(sms) * kCtas<T>;
+    const long long rows = static_cast<long long>(streams) * beams;
     Division d{1, row_vecs};
     double least = 1e300;
     for (int parts = 1; parts <= kMostParts && (parts == 1 || row_vecs / parts >= kThreads / 2); ++parts) {
         // whole sweeps of a CTA's threads, unless the row has less than one
         int vecs = (row_vecs + parts - 1) / parts;
         if (vecs > kThreads) vecs = (vecs + kThreads - 1) / kThreads * kThreads;
-        const double cost = static_cast<double>((rows * parts + slots - 1) / slots) *
-                            (static_cast<double>((vecs + kThreads - 1) / kThreads) * elements * 18 + kPartCost);
-        if (cost < least) {
+        const double cost = static_cast<double>((rows * parts + sms - 1) / sms) *
+                            (static_cast<double>((vecs + kThreads - 1) / kThreads) * elements + kPartCost);
+        const int made = (row_vecs + vecs - 1) / vecs;
+        if (cost < least && (made == 1 || beams * made * count <= kAhead * kThreads)) {
             least = cost;
             d.vecs = vecs;
-            d.parts = (row_vecs + vecs - 1) / vecs;
+            d.parts = made;
         }
     }
     return d;
@@ -755,7 +762,7 @@ Division divide(int streams, int beams, int vocab, int sms) {
 
 template <typename T>
 cudaError_t launch(const BeamSelectArgs& a, int sms, cudaStream_t s) {
-    const Division d = divide<T>(a.streams, a.beams, a.vocab, sms);
+    const Division d = divide<T>(a.streams, a.beams, a.vocab, a.count, sms);
     static std::atomic<uint64_t> allowed;
     cudaError_t e = allow_smem(part_kernel<T>, sizeof(Shared), allowed);
     if (e != cudaSuccess) return e;
@@ -777,7 +784,7 @@ cudaError_t launch(const BeamSelectArgs& a, int sms, cudaStream_t s) {
 }  // namespace
 
 int64_t beam_select_workspace_bytes(int streams, int beams, int vocab, int count, int dtype, int sms) {
-    const Division d = dtype == UFB_F32 ? divide<float>(streams, beams, vocab, sms) : divide<__half>(streams, beams, vocab, sms);
+    const Division d = dtype == UFB_F32 ? divide<float>(streams, beams, vocab, count, sms) : divide<__half>(streams, beams, vocab, count, sms);
     return static_cast<int64_t>(streams) * beams * d.parts * part_bytes(count);
 }
 
