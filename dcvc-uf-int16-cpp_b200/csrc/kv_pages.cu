@@ -503,9 +503,10 @@ __global__ void __launch_bounds__(kApplyThreads) reorder_apply_kernel(const ufb_
 // in all their tables, inside of every one's earlier tokens.  Streams that bring no tokens,
 // or whose extend was refused, do not count.  Then where each stream's own keys lie among
 // the group's, one stream's behind the other's in units of kGroupUnit, and the tokens'
-// positions.  Latency of three passes over the streams: 4.0 us for 4 streams of 1769 tokens,
-// 5.7 for 8 groups of 8, 14 for 64 streams of 65320 (2 a warp, 511 entries each).
-__global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, const KvBatch b, const ufb_kv_groups g,
+// positions.  Latency of three passes over the streams: 4.2 us for 4 streams of 1769 tokens,
+// 5.1 for 8 groups of 8, 8.9 for 64 streams of 65320 (2 a warp, 511 entries each; 14 where
+// 32 registers made the loads of a row wait for one another).
+__global__ void __launch_bounds__(kThreads, 1) share_kernel(const ufb_kv_cache c, const KvBatch b, const ufb_kv_groups g,
                                                          const KvGroupState out, int* status) {
     __shared__ int warp_sum[kWarps];
     __shared__ int width, lowest, highest, members, chosen;
@@ -546,13 +547,18 @@ __global__ void __launch_bounds__(kThreads) share_kernel(const ufb_kv_cache c, c
         if (slot < 0 || members < 2 || i == chosen) continue;
         const int32_t* own = c.table + static_cast<long long>(slot) * c.table_width;
         const int32_t* other = c.table + static_cast<long long>(b.slots[chosen]) * c.table_width;
-        for (int e0 = 0; e0 < most; e0 += 128) {
+        for (int e0 = 0; e0 < most; e0 += 256) {
+            // all loads before the first comparison
+            int a[8], d[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int e = min(e0 + j * 32 + lane, most - 1);
+                a[j] = own[e], d[j] = other[e];
+            }
             int differs = INT_MAX;
 #pragma unroll
-            for (int j = 3; j >= 0; --j) {
-                const int e = e0 + j * 32 + lane;
-                if (e < most && own[e] != other[e]) differs = e;
-            }
+            for (int j = 7; j >= 0; --j)
+                if (a[j] != d[j]) differs = min(e0 + j * 32 + lane, most - 1);
             differs = __reduce_min_sync(0xffffffffu, differs);
             if (differs != INT_MAX) {
                 if (lane == 0) atomicMin(&width, differs);
