@@ -197,6 +197,8 @@ __device__ __forceinline__ void cp_async4(void* to, const void* from) {
 }
 
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Once all blocks have said so the next launch's may take what room there is; they wait for this one's end.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // false: the pair (group, row tile) does not exist.
 __device__ __forceinline__ bool group_tile(const AttendArgs& a, const GroupArgs& g, int group, int rt, GroupTile& t) {
@@ -354,6 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     };
     __syncthreads();
     wait_for_previous();
+    let_next_start();
     // Only the walker needs to know this CTA's share.  One warp finds it in 1 us where it takes
     // all the block's 2 us; from some hundred pairs on the block is faster.
     Share share;
@@ -1058,6 +1061,7 @@ __global__ void __launch_bounds__(kJoinThreads) groups_join_kernel(const AttendA
     __shared__ float tops[kJoinRows], weights[kJoinRows];
     const AttendScratch scratch = scratch_of(a.workspace, ctas, kRows);
     const int c0 = blockIdx.x, first = blockIdx.y * kJoinRows;
+    let_next_start();
     wait_for_previous();
     const int32_t* item = scratch.items + c0 * 8;
     const int parts = item[0], rows = min(item[3] - first, kJoinRows);
@@ -1127,8 +1131,8 @@ cudaError_t launch(const AttendArgs& a, const GroupArgs& g, int sms, cudaStream_
     const long long row_tiles = (static_cast<long long>(g.max_tokens) * a.group + kRows - 1) / kRows;
     if (row_tiles * g.groups > 0x3fffffff) return cudaErrorInvalidValue;
     const int ctas = sms < kAttendMaxCtas ? sms : kAttendMaxCtas;
-    // both kernels: the blocks may start once the CTAs before have exited, ahead of the signal
-    // that they have ended (nothing gives an earlier trigger); they wait for that
+    // Both kernels may start before the one ahead of them has ended (each waits for that before it
+    // reads anything): 16 branches 76.3 us for 78.8, a window 30.2 for 31.6.
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute early;
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
