@@ -512,6 +512,8 @@ __global__ void __launch_bounds__(kThreads, 1) share_kernel(const ufb_kv_cache c
     __shared__ int width, lowest, highest, members, chosen;
     __shared__ long long warp_units[kWarps];
     const int group = blockIdx.x, first = max(g.first[group], 0), end = min(g.first[group + 1], b.n);
+    // attention over the groups may start; it waits for this launch's end
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) width = c.table_width, lowest = INT_MAX, highest = -1, members = 0, chosen = INT_MAX;
     __syncthreads();
