@@ -357,9 +357,10 @@ __global__ void __launch_bounds__(256) move_kernel(const ufb_kv_cache c) {
 // memory, a column of all its streams to a thread (a row may be read by several and
 // is overwritten itself), and moves the copies' bytes.
 //
-// Bound by the latency of the two launches: 4 branches of one stream, 2 layers, 6.8 us on
-// the device (4.0 and 2.7); 16 streams x 8 branches, 8 layers of 4 heads of 128, 11.1 us, of
-// which the copies (29 MB read and written) would take 4.5 from memory.
+// Bound by the latency of the two launches, of which the second reads its rows while the
+// first decides (4 branches of one stream, 2 layers: 5.5 us on the device, 6.8 one after the
+// other); 16 streams x 8 branches, 8 layers of 4 heads of 128, 10.8 us, of which the copies
+// (29 MB read and written) would take 4.5 from memory.
 
 // The page of a stream's last, partly filled entry; -1: it has none.
 __device__ __forceinline__ int last_page(const ufb_kv_cache& c, int slot, int length) {
@@ -373,6 +374,7 @@ __global__ void __launch_bounds__(kThreads) reorder_kernel(const ufb_kv_cache c,
                                                            const int32_t* parents, int n, int width, int* status) {
     __shared__ int warp_sum[kWarps];
     __shared__ int children[kThreads], first[kThreads], page_of[kThreads], rest_of[kThreads];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const Work w = work_of(c);
     int32_t* last_entry = kv_last_entry(c);
     if (threadIdx.x == 0) w.moves[0] = w.moves[1] = 0;
@@ -449,40 +451,44 @@ __global__ void __launch_bounds__(kApplyThreads) reorder_apply_kernel(const ufb_
     __shared__ int slot[UFB_BEAM_MAX], parent[UFB_BEAM_MAX], page[UFB_BEAM_MAX], entry[UFB_BEAM_MAX];
     __shared__ int children[UFB_BEAM_MAX], length[UFB_BEAM_MAX], refused[UFB_BEAM_MAX];
     const Work w = work_of(c);
-    wait_for_previous();
-    if (w.moves[1] == 0) return;
     if (blockIdx.x >= row_blocks) {
+        wait_for_previous();
+        if (w.moves[1] == 0) return;
         const int moves = w.moves[0], parts = c.layers * 2;
         for (long long j = blockIdx.x - row_blocks; j < static_cast<long long>(moves) * parts; j += gridDim.x - row_blocks)
             move_page<true>(c, w, static_cast<int>(j / parts), static_cast<int>(j % parts) >> 1, static_cast<int>(j & 1));
         return;
     }
     const int group = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    const int i = group * width + threadIdx.x;
+    // the decision writes none of this: it is read while that is made
     if (threadIdx.x < width) {
-        const int i = group * width + threadIdx.x;
-        slot[threadIdx.x] = slots[i];
+        const int from = slots[i];
+        slot[threadIdx.x] = valid_slot(c, from) ? from : 0;   // out of range: the call is refused
         parent[threadIdx.x] = parents[i];
-        page[threadIdx.x] = w.start[i];
-        entry[threadIdx.x] = kv_last_entry(c)[i];
         children[threadIdx.x] = 0;
         if (chunk == 0) {
-            length[threadIdx.x] = c.lengths[slots[i]];
-            refused[threadIdx.x] = kv_refused(c)[slots[i]];
+            length[threadIdx.x] = c.lengths[slot[threadIdx.x]];
+            refused[threadIdx.x] = kv_refused(c)[slot[threadIdx.x]];
         }
     }
     __syncthreads();
+    // half of the block's threads have the even rows, the other half the odd ones
+    const int column = threadIdx.x % kColumns, half = threadIdx.x / kColumns, e = chunk * kColumns + column;
+    const bool there = e < c.table_width;
+    for (int r = half; there && r < width; r += kApplyThreads / kColumns)
+        rows[r * kColumns + column] = c.table[static_cast<long long>(slot[r]) * c.table_width + e];
+    wait_for_previous();
+    if (w.moves[1] == 0) return;
     if (threadIdx.x < width) {
+        page[threadIdx.x] = w.start[i];
+        entry[threadIdx.x] = kv_last_entry(c)[i];
         atomicAdd(children + parent[threadIdx.x], 1);
         if (chunk == 0) {
             c.lengths[slot[threadIdx.x]] = length[parent[threadIdx.x]];
             kv_refused(c)[slot[threadIdx.x]] = refused[parent[threadIdx.x]];
         }
     }
-    // half of the block's threads have the even rows, the other half the odd ones
-    const int column = threadIdx.x % kColumns, half = threadIdx.x / kColumns, e = chunk * kColumns + column;
-    const bool there = e < c.table_width;
-    for (int r = half; there && r < width; r += kApplyThreads / kColumns)
-        rows[r * kColumns + column] = c.table[static_cast<long long>(slot[r]) * c.table_width + e];
     __syncthreads();
     if (!there) return;
     bool same = true;   // one page in all rows: nothing changes, nor does its count
