@@ -861,8 +861,14 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 }
                 // four tiles at a time, a lane to 16 keys of one
                 const int my_tile = lane / kGroups, my_key = (lane % kGroups) * kGroupKeys;
-                // own keys: of stream `s`, whose units are [from, until) of the group's
-                int s = t.stream, from = t.before, until = g.state.units[s];
+                // own keys: 32 streams at a time, from `seen` on, a lane to each; before: units ahead of them
+                int seen = t.stream - 32, before = t.before, units = t.before, slot_of = 0, low_of = 0, high_of = 0;
+                auto look_on = [&] {
+                    before = __shfl_sync(0xffffffffu, units, 31);
+                    seen += 32;
+                    const int s = min(seen + lane, t.last);
+                    units = g.state.units[s], slot_of = a.slots[s], low_of = a.offsets[s], high_of = a.offsets[s + 1];
+                };
                 for (int i0 = walk.first; i0 < walk.last; i0 += 4) {
                     const int i = min(i0 + my_tile, walk.last - 1);
                     Tile o;
@@ -871,7 +877,8 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     o.row_low = 0;
                     o.row_high = kRows;
                     int slot = t.slot, key = -1;          // lane's 16 keys; -1: not looked at
-                    if (i < t.common) {
+                    const bool own = i >= t.common;
+                    if (!own) {
                         o.key0 = t.keys.tile(i) * kKeys;
                         if (t.keys.touches(o.key0 + my_key)) key = o.key0 + my_key;
                         if (o.key0 + kKeys - 1 <= t.low && o.key0 + kKeys <= t.shared &&
@@ -880,16 +887,32 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     } else {
                         o.key0 = (t.own + i - t.common) * kKeys;
                         o.flags |= kOwnKeys;
-                        const int unit = (o.key0 + my_key) / kGroupUnit;
-                        while (unit >= until && s < t.last) from = until, until = g.state.units[++s];
-                        if (unit >= from && unit < until) {
-                            slot = a.slots[s];
-                            key = t.shared + (unit - from) * kGroupUnit;
-                            o.row_low = (a.offsets[s] - t.token0) * a.group - t.row0;
-                            o.row_high = (a.offsets[s + 1] - t.token0) * a.group - t.row0;
-                        } else {
-                            o.row_low = kRows, o.row_high = 0;
+                        o.row_low = kRows, o.row_high = 0;
+                    }
+                    const int unit = own ? (o.key0 + my_key) / kGroupUnit : INT_MAX;
+                    bool wanted = own;
+                    if (__any_sync(0xffffffffu, own) && seen < t.stream) look_on();
+                    while (__any_sync(0xffffffffu, wanted)) {
+                        // the first stream whose units reach beyond this one
+                        int k = 0;
+#pragma unroll
+                        for (int d = 16; d; d >>= 1)
+                            if (__shfl_sync(0xffffffffu, units, k + d - 1) <= unit) k += d;
+                        const int until = __shfl_sync(0xffffffffu, units, k), ahead = __shfl_sync(0xffffffffu, units, max(k - 1, 0));
+                        const int found = __shfl_sync(0xffffffffu, slot_of, k);
+                        const int low = __shfl_sync(0xffffffffu, low_of, k), high = __shfl_sync(0xffffffffu, high_of, k);
+                        const int from = k > 0 ? ahead : before;
+                        if (wanted && unit < until) {
+                            wanted = false;
+                            if (unit >= from) {   // else of a stream before this row tile's
+                                slot = found;
+                                key = t.shared + (unit - from) * kGroupUnit;
+                                o.row_low = (low - t.token0) * a.group - t.row0;
+                                o.row_high = (high - t.token0) * a.group - t.row0;
+                            }
                         }
+                        if (seen + 32 > t.last || !__any_sync(0xffffffffu, wanted)) break;
+                        look_on();
                     }
                     // all its streams' rows
 #pragma unroll
