@@ -8,7 +8,7 @@
 // key head -- go through the common keys once; then, in the same accumulators, through
 // the streams' own keys, which only that stream's rows see.  Own keys lie in the tiles one
 // stream's behind the other's, from every 16th key on: 19 branches with 9 own tokens each
-// fill 3 tiles, not 19 (10 such groups, 8 heads of 128, 1324 common keys, 2 layers: 78 us
+// fill 3 tiles, not 19 (10 such groups, 8 heads of 128, 1324 common keys, 2 layers: 74 us
 // where a tile to each stream took 98).  Nothing has to be joined but what CTAs share, and
 // a step of a search is one launch and its join.
 //
@@ -30,8 +30,8 @@
 // become one at a piece's end.  Warps whose rows are padding, or no rows of an own tile's
 // stream, skip the softmax.
 //
-// Measured on 148 SMs: 64 branches x 65320 keys, 64 query heads over 8 of 128: 219 us, 620
-// TFLOP/s, 3200 cycles a tile; 8 streams x 8 branches, to 16381 keys, 4 heads of 128: 41 us
+// Measured on 148 SMs: 64 branches x 65320 keys, 64 query heads over 8 of 128: 213 us, 640
+// TFLOP/s, 3100 cycles a tile; 8 streams x 8 branches, to 16381 keys, 4 heads of 128: 40 us
 // a layer, 2700 cycles a tile.  The products of a tile take 1300 alone, its exponentials
 // 1024, its integers 1400 from HBM.  What bounds a tile is the chain S -> softmax -> P V ->
 // S of a set (S and P share their columns; tensor memory is full), half a period each: of
@@ -357,8 +357,9 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
     __syncthreads();
     wait_for_previous();
     let_next_start();
-    // Only the walker needs to know this CTA's share.  One warp finds it in 1 us where it takes
-    // all the block's 2 us; from some hundred pairs on the block is faster.
+    // Only the walker needs to know this CTA's share.  For few pairs its warp alone has the first
+    // piece 5300 cycles after the start, where with the block's scan it had it after 7400; beyond
+    // four rounds of 32 loads the block divides.
     Share share;
     if (pairs > kWarpPairs)
         share = share_out<kThreads>(
