@@ -490,7 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                     const int end = flags & kOwnKeys ? seat.z - tile.key0 : p.shared - tile.key0;
                     high = a.causal || !(flags & kOwnKeys) ? min(end, pos + 1 + zero) : end;
                     low = begin;
-                    if (a.window) low = max(begin, pos - a.window + 1 + zero), sink = a.sinks + zero;
+                    // sinks that reach past the end act as the end: of any number of them the sum stays in 32 bits
+                    if (a.window) low = max(begin, pos - a.window + 1 + zero), sink = min(a.sinks, end - zero) + zero;
                 }
                 tile_done(n);
                 wait(&sm.s_full[t], n >> 1);
