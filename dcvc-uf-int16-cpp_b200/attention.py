@@ -303,7 +303,7 @@ class KVGroups:
         self._struct = _Groups(self.first.data_ptr(), self.offsets.data_ptr(), self._state.data_ptr(), self.n,
                                self.max_tokens)
         self._ref = C.addressof(self._struct)
-        self._at = None   # the state of the cache that share saw
+        self._at = None   # calls on the cache when share was called; the device counts those that ran
 
 
 class KVCache:
@@ -537,7 +537,10 @@ class KVCache:
 
         With groups (group_plan of this plan, after share has seen the cache as it is)
         the pages that a group's streams begin with in common are read once for all of
-        them: made for branches that go on by few tokens of their own."""
+        them: made for branches that go on by few tokens of their own.  A call that
+        follows a change without a share is refused; where only the device can tell (a
+        replayed graph that changes streams, a share that was captured and has not run)
+        the status is 33 and the queries see no key."""
         self._own(plan)
         _check_ints(layer, window, sinks)
         device = self.device

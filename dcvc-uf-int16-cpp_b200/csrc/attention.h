@@ -13,6 +13,7 @@ namespace ufb {
 constexpr int kStatusPosition = 21;
 constexpr int kStatusPages = 31;
 constexpr int kStatusIndex = 32;
+constexpr int kStatusShare = 33;
 
 constexpr int kRotaryMaxPairs = 128;
 
@@ -35,7 +36,9 @@ cudaError_t rotary(const RotaryArgs& a, int dtype, int sms, int* status, cudaStr
 __host__ __device__ inline int32_t* kv_refused(const ufb_kv_cache& c) {
     return c.work + 16 + 3ll * c.pages + c.slots;
 }
-// Behind them, one integer for each stream of a reorder.
+// How many calls changed tables or lengths (the page operators' scratch begins with words of its own).
+__host__ __device__ inline int32_t* kv_changes(const ufb_kv_cache& c) { return c.work + 2; }
+// Behind the marks, one integer for each stream of a reorder.
 __host__ __device__ inline int32_t* kv_last_entry(const ufb_kv_cache& c) { return kv_refused(c) + c.slots; }
 
 // Streams of one call: new tokens [offsets[i], offsets[i + 1]) belong to slots[i].
@@ -88,7 +91,9 @@ struct KvGroupState {
     struct Group {
         int32_t token0, tokens, stream0, streams;
         int32_t shared, slot, low, high;   // slot: of a stream that has them; least and largest position
-        int32_t own, pad[3];               // of all its streams' own keys: `units`
+        int32_t own;                       // of all its streams' own keys: `units`
+        int32_t seen;                      // kv_changes when it was written, and 1
+        int32_t pad[2];
     };
     Group* group;                          // [groups], 16-byte aligned
     struct Token {
@@ -103,6 +108,9 @@ constexpr int kNotWritten = INT32_MIN;
 constexpr int kGroupUnit = 16;             // own keys that begin together in a tile of kv_attend_groups
 struct GroupArgs {
     int groups, max_tokens;
+    const int32_t* first;                  // as in ufb_kv_groups
+    const int32_t* offsets;
+    const int32_t* changes;                // kv_changes
     KvGroupState state;
 };
 inline KvGroupState kv_group_state(const ufb_kv_groups& g, long long tokens) {

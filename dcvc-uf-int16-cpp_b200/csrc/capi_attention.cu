@@ -411,7 +411,8 @@ int ufb_kv_attend_groups(const ufb_kv_cache* c, int layer, const int32_t* slots,
         !check_groups(groups, n, max_new, tokens))
         return last_code();
     if (!go || groups->groups == 0) return UFB_OK;
-    const GroupArgs g{groups->groups, groups->max_tokens, kv_group_state(*groups, tokens)};
+    const GroupArgs g{groups->groups, groups->max_tokens, groups->first, groups->offsets, kv_changes(*c),
+                      kv_group_state(*groups, tokens)};
     return done(kv_attend_groups(a, g, dtype, sms, static_cast<cudaStream_t>(stream)), "kv attend groups");
 }
 

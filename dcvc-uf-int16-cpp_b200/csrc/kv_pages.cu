@@ -23,8 +23,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kApplyThreads = 256;
 constexpr int kColumns = 128;   // table columns of a block of reorder_apply_kernel
 
-// Scratch layout (int32): [0] moves to make, [1] whether a reorder goes ahead, [16, 16 +
-// pages) free pages found, in order; then [pages) moves' sources / [pages) token counts;
+// Scratch layout (int32): [0] moves to make, [1] whether a reorder goes ahead, [2] the
+// calls that changed tables or lengths (kv_changes), [16, 16 + pages) free pages found, in order; then [pages) moves' sources / [pages) token counts;
 // then one offset per request (slots).  Behind it lie the marks of refused streams
 // (kv_refused) and the entries of last pages (kv_last_entry).
 struct Work {
@@ -100,6 +100,12 @@ __device__ int find_free(const ufb_kv_cache& c, int need, int32_t* found, int* w
     return min(have, need);
 }
 
+// By one thread of a kernel that changes tables, lengths or marks (page ids apart): what
+// ufb_kv_share found before holds no more.
+__device__ __forceinline__ void count_change(const ufb_kv_cache& c) {
+    *kv_changes(c) = static_cast<int32_t>(static_cast<uint32_t>(*kv_changes(c)) + 1u);
+}
+
 __device__ __forceinline__ bool valid_slot(const ufb_kv_cache& c, int slot) { return slot >= 0 && slot < c.slots; }
 
 __global__ void __launch_bounds__(kThreads) extend_kernel(const ufb_kv_cache c, const int32_t* slots,
@@ -107,6 +113,7 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const ufb_kv_cache c, 
     __shared__ int warp_sum[kWarps];
     const Work w = work_of(c);
     const int P = c.page_tokens;
+    if (threadIdx.x == 0) count_change(c);
     long long need = 0;
     int bad = 0;
     for (int base = 0; base < n; base += kThreads) {
@@ -176,6 +183,7 @@ __device__ __forceinline__ void drop_row(const ufb_kv_cache& c, int slot, long l
 __global__ void __launch_bounds__(128) drop_kernel(const ufb_kv_cache c, const int32_t* slots, int n, int window,
                                                    int sinks, int* status) {
     const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (blockIdx.x == 0 && threadIdx.x == 0) count_change(c);
     if (i >= n) return;
     const int slot = slots[i];
     if (!valid_slot(c, slot)) {
@@ -200,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) fork_kernel(const ufb_kv_cache c, co
     const Work w = work_of(c);
     const int P = c.page_tokens;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) *w.moves = 0;
+    if (threadIdx.x == 0) *w.moves = 0, count_change(c);
     int bad = 0;
     for (int i = threadIdx.x; i < n; i += kThreads) bad |= !valid_slot(c, src[i]) || !valid_slot(c, dst[i]);
     if (__syncthreads_or(bad)) {
@@ -439,7 +447,7 @@ __global__ void __launch_bounds__(kThreads) reorder_kernel(const ufb_kv_cache c,
         c.refs[page] = at < left ? 2 : 1;
         w.start[i] = page;
     }
-    if (threadIdx.x == 0) w.moves[0] = need, w.moves[1] = 1;
+    if (threadIdx.x == 0) w.moves[0] = need, w.moves[1] = 1, count_change(c);
 }
 
 // Blocks below row_blocks: kColumns columns of one group's rows; the others: copies, by
@@ -622,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) share_kernel(const ufb_kv_cache c
         r.token0 = o0, r.tokens = ok ? o1 - o0 : 0, r.stream0 = first, r.streams = end - first;
         r.shared = shared, r.slot = members ? b.slots[chosen] : 0;
         r.low = lowest == INT_MAX ? -1 : lowest, r.high = highest;
-        r.own = sum, r.pad[0] = r.pad[1] = r.pad[2] = 0;
+        r.own = sum, r.seen = *kv_changes(c) + 1, r.pad[0] = r.pad[1] = 0;
         out.group[group] = r;
     }
 }

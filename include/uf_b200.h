@@ -446,6 +446,8 @@ int ufb_conv2d_noalloc(const int16_t* x, int n, int ci, int h, int w, const int1
  *   32 a slot, page or token offset out of range, or a page that is missing
  *      where tokens are to be stored (what it names is skipped; reorder, with a
  *      parent out of range too: nothing was changed)
+ *   33 attention over groups that ufb_kv_share has not seen since tables or lengths
+ *      changed (their queries see no key)
  *   41..45 a bounded wait of the attention kernels gave up
  *   51 a row of logits holds NaN or +infinity (its beam has no continuations)
  * ------------------------------------------------------------------------- */
@@ -614,7 +616,9 @@ int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens);
  * one; status 31 for one whose extend was refused: its queries see no key; 32 for a
  * group with 2^31 - 144 own keys or more, whose results are left alone).  state[g]
  * are the tokens on them.  Once a step, behind ufb_kv_extend: it holds
- * until a call changes tables or lengths. */
+ * until an extend, release, fork, reorder or trim of the cache, in a replayed graph
+ * or not (ufb_kv_attend_groups refuses then, status 33); what the caller writes into
+ * tables and lengths directly is not noticed. */
 int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* offsets, int n, int max_new,
                  int64_t tokens, const ufb_kv_groups* groups, void* stream);
 

@@ -1,9 +1,12 @@
 """GPU: the ends of what attention over groups takes -- sinks and windows up to the type's
-largest.
+largest, groups that share has not seen as they are.
 
 Attention is held to the tolerances of test_gpu_groups.py."""
+import math
+
 import pytest
 import torch
+from test_gpu_attention import _clean, randn
 from test_gpu_groups import check_groups, make_groups
 
 pytestmark = pytest.mark.gpu
@@ -21,3 +24,65 @@ def test_sinks_and_windows_of_any_size(ufb, dev, window, sinks):
             for causal in (True, False):
                 check_groups(ufb, cache, list(range(7)), counts, sizes, 2 * group, torch.float16, window=window, sinks=sinks,
                              causal=causal)
+
+
+# ------------------------------------- groups that share has not seen as they are ----
+
+def refused(ufb, cache, plan, groups, q, status):
+    """Their queries see no key, and the status says so."""
+    out, lse = cache.attend(0, plan, q, groups=groups, lse=True)
+    assert ufb.device_status(0) == status
+    assert not bool(out.any()) and bool((lse == -math.inf).all())
+
+
+def test_attend_between_capture_and_replay(ufb, dev):
+    """A captured share has not run: attention before the first replay is refused by the device."""
+    cache, lengths, sizes = make_groups(ufb, dev, [(300, [9] * 4), (64, [3] * 2)], 2, 64, 16, spare=40)
+    plan = cache.plan(list(range(6)), [2] * 6)
+    groups = cache.group_plan(plan, sizes)
+    q, k = randn(dev, (12, 6, 64), 1, torch.float16), randn(dev, (12, 2, 64), 2, torch.float16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.extend(plan)
+        cache.share(groups)
+        cache.append(0, plan, k, -k)
+        out = cache.attend(0, plan, q, groups=groups)
+    refused(ufb, cache, plan, groups, q, 33)
+    for step in range(2):
+        graph.replay()
+        assert torch.equal(cache.attend(0, plan, q, groups=groups), out)
+        assert cache.lengths.tolist() == [n + 2 * step + 2 for n in lengths]
+    _clean(ufb)
+    check_groups(ufb, cache, list(range(6)), [2] * 6, sizes, 6, torch.float16)
+
+
+@pytest.mark.parametrize("change", ["extend", "refused extend", "trim", "release", "fork", "reorder"])
+def test_attend_after_replayed_changes(ufb, dev, change):
+    """A replay changes tables or lengths behind share: refused until share has seen them, moved pages are not."""
+    cache, lengths, sizes = make_groups(ufb, dev, [(300, [9] * 4), (64, [3] * 2), (40, [5])], 2, 64, 16, spare=40)
+    plan = cache.plan(list(range(6)), [1] * 6)
+    groups = cache.group_plan(plan, sizes[:2])
+    beams, fork, last = cache.beam_plan(range(4), 4), cache.fork_plan([0], [6]), cache.plan([6], [0])
+    parents = torch.tensor([[1, 1, 0, 0]], dtype=torch.int32, device=dev)
+    much = cache.plan([6], [16 * 60])
+    calls = {"extend": lambda: cache.extend(plan), "refused extend": lambda: cache.extend(much),
+             "trim": lambda: cache.trim(plan, 50), "release": lambda: cache.release(last),
+             "fork": lambda: cache.fork(fork), "reorder": lambda: cache.reorder(beams, parents)}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls[change]()
+    q = randn(dev, (6, 6, 64), 1, torch.float16)
+    cache.share(groups)
+    before = cache.attend(0, plan, q, groups=groups)
+    cache.compact()   # new ids, the same pages
+    assert torch.equal(cache.attend(0, plan, q, groups=groups), before)
+    _clean(ufb)
+    graph.replay()
+    assert ufb.device_status(0) == (31 if change == "refused extend" else 0)
+    refused(ufb, cache, plan, groups, q, 33)
+    cache.share(groups)
+    got = cache.attend(0, plan, q, groups=groups)
+    _clean(ufb)
+    check_groups(ufb, cache, list(range(6)), [1] * 6, sizes[:2], 6, torch.float16)
+    if change in ("refused extend", "release", "fork"):   # streams of no group here
+        assert torch.equal(got, before)
