@@ -12,7 +12,7 @@
 // where a tile to each stream took 98).  Nothing has to be joined but what CTAs share, and
 // a step of a search is one launch and its join.
 //
-// One CTA an SM, seven roles:
+// One CTA an SM, six roles:
 //   walker (1 warp)      divides the work, and says of the tiles ahead (four at a time, a
 //                        lane to 16 keys) which pages hold their keys and who sees them
 //   converter (8 warps)  integers from global memory through registers to float16 in
@@ -24,7 +24,6 @@
 //                        with a maximum and sums of its own, so that one exponentiates
 //                        while the other loads or waits.  P goes back over S in float16.
 //   scales (1 warp)      of each 16 keys, three tiles ahead
-//   checker (1 warp)     groups that ufb_kv_share has not seen as they are: the status, zeros
 // Up to 64 rows are in the tile two times, up to 32 four times: a copy takes a half or a
 // quarter of each tile's keys, its other weights are zeros, so all softmax warps work and
 // a thread has 32 scores where it had 128.  The sums of both sets and all copies of a row
@@ -53,8 +52,8 @@ constexpr int kRows = 128;
 constexpr int kKeys = 128;
 constexpr int kGroups = kKeys / kGroupKeys;
 static_assert(kGroupUnit == kGroupKeys, "own keys begin where pages and scales are looked up");
-constexpr int kMmaWarp = 16, kWalkWarp = 17, kScaleWarp = 18, kCheckWarp = 19;
-constexpr int kThreads = 640;         // warps: softmax 0-7, converter 8-15, MMA 16, walker 17, scales 18, checker 19
+constexpr int kMmaWarp = 16, kWalkWarp = 17, kScaleWarp = 18;
+constexpr int kThreads = 640;         // warps: softmax 0-7, converter 8-15, MMA 16, walker 17, scales 18; 19 idle
 constexpr int kPieces = 4;            // pieces announced ahead
 constexpr int kTiles = 8;             // tiles announced ahead
 constexpr int kScaleRing = 4;
@@ -955,6 +954,25 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 mbar_arrive(&sm.piece_full[piece % kPieces]);
             }
             __syncwarp();
+            // No tile is made of groups that share has not seen as they are: their rows see no key.  Here,
+            // while the others work on the last tiles, it costs 0 to 0.3 us; a warp of its own, which
+            // looks beside the first look-ups, took 0.7 us of each call, the join 0.3.
+            const int heads = a.heads * a.group;
+            for (int group = blockIdx.x; group < g.groups; group += gridDim.x) {
+                if (g.state.group[group].seen == *g.changes + 1) continue;
+                if (lane == 0) atomicCAS(a.status, 0, kStatusShare);
+                const int first = max(g.first[group], 0), end = min(g.first[group + 1], a.n);
+                const int o0 = g.offsets[group], o1 = g.offsets[group + 1];
+                // of the streams' tokens alone
+                if (first > end || o0 < 0 || o1 > a.tokens || o0 != a.offsets[first] || o1 != a.offsets[end]) continue;
+                for (long long token = o0; token < o1; ++token) {
+                    T* to = static_cast<T*>(a.out.data) + token * a.out.token_stride;
+                    for (int i = lane; i < heads * (D / 8); i += 32)
+                        *reinterpret_cast<uint4*>(to + i / (D / 8) * a.out.head_stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+                    for (int h = lane; a.lse && h < heads; h += 32) a.lse[token * heads + h] = -INFINITY;
+                }
+            }
+            __syncwarp();
         }
         if (warp == kScaleWarp) {
             // ---- scales: a lane to 16 keys, kAhead tiles ahead of what is written
@@ -997,25 +1015,6 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 if (lane < kGroups) sm.scales[n % kScaleRing][lane] = s;
                 arrive(&sm.k_full[n & 1]);
             }
-        }
-        if (warp == kCheckWarp) {
-            // ---- checker: no tile is made of a group that share has not seen; its rows see no key
-            const int heads = a.heads * a.group;
-            for (int group = blockIdx.x; group < g.groups; group += gridDim.x) {
-                if (g.state.group[group].seen == *g.changes + 1) continue;
-                if (lane == 0) atomicCAS(a.status, 0, kStatusShare);
-                const int first = max(g.first[group], 0), end = min(g.first[group + 1], a.n);
-                const int o0 = g.offsets[group], o1 = g.offsets[group + 1];
-                // of the streams' tokens alone
-                if (first > end || o0 < 0 || o1 > a.tokens || o0 != a.offsets[first] || o1 != a.offsets[end]) continue;
-                for (long long token = o0; token < o1; ++token) {
-                    T* to = static_cast<T*>(a.out.data) + token * a.out.token_stride;
-                    for (int i = lane; i < heads * (D / 8); i += 32)
-                        *reinterpret_cast<uint4*>(to + i / (D / 8) * a.out.head_stride + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
-                    for (int h = lane; a.lse && h < heads; h += 32) a.lse[token * heads + h] = -INFINITY;
-                }
-            }
-            __syncwarp();
         }
         // ---- MMA: the warp waits together, one lane issues
         if (warp == kMmaWarp) {

@@ -529,6 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1) share_kernel(const ufb_kv_cache c
     // attention over the groups may start; it waits for this launch's end
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int seen = *kv_changes(c) + 1;
     if (threadIdx.x == 0) width = c.table_width, lowest = INT_MAX, highest = -1, members = 0, chosen = INT_MAX;
     __syncthreads();
     // of stream i: its slot, -1 when something is out of range, -2 when it does not count
@@ -630,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) share_kernel(const ufb_kv_cache c
         r.token0 = o0, r.tokens = ok ? o1 - o0 : 0, r.stream0 = first, r.streams = end - first;
         r.shared = shared, r.slot = members ? b.slots[chosen] : 0;
         r.low = lowest == INT_MAX ? -1 : lowest, r.high = highest;
-        r.own = sum, r.seen = *kv_changes(c) + 1, r.pad[0] = r.pad[1] = 0;
+        r.own = sum, r.seen = seen, r.pad[0] = r.pad[1] = 0;
         out.group[group] = r;
     }
 }
