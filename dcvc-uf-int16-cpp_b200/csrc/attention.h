@@ -92,7 +92,7 @@ struct KvGroupState {
         int32_t token0, tokens, stream0, streams;
         int32_t shared, slot, low, high;   // slot: of a stream that has them; least and largest position
         int32_t own;                       // of all its streams' own keys: `units`
-        int32_t seen;                      // kv_changes when it was written, and 1
+        int32_t seen;                      // kv_changes when it was written, and 1; its complement: turned away
         int32_t pad[2];
     };
     Group* group;                          // [groups], 16-byte aligned

@@ -200,7 +200,8 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 // Once all blocks have said so the next launch's may take what room there is; they wait for this one's end.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// false: the pair (group, row tile) does not exist, or ufb_kv_share has not seen the group as it is.
+// false: the pair (group, row tile) does not exist, or ufb_kv_share has turned the group away or not
+// seen it as it is.
 __device__ __forceinline__ bool group_tile(const AttendArgs& a, const GroupArgs& g, int group, int rt, GroupTile& t) {
     const int4* record = reinterpret_cast<const int4*>(g.state.group + group);
     const int4 place = record[0], keys = record[1], rest = record[2];   // KvGroupState::Group
@@ -954,16 +955,17 @@ __global__ void __launch_bounds__(kThreads, 1) groups_kernel(const AttendArgs a,
                 mbar_arrive(&sm.piece_full[piece % kPieces]);
             }
             __syncwarp();
-            // No tile is made of groups that share has not seen as they are: their rows see no key.  Here,
-            // while the others work on the last tiles, it costs 0 to 0.3 us; a warp of its own, which
-            // looks beside the first look-ups, took 0.7 us of each call, the join 0.3.
+            // No tile is made of groups that share has turned away or not seen as they are: their rows see
+            // no key.  Here, while the others work on the last tiles, it costs 0 to 0.3 us; a warp of its
+            // own, which looks beside the first look-ups, took 0.7 us of each call, the join 0.3.
             const int heads = a.heads * a.group;
             for (int group = blockIdx.x; group < g.groups; group += gridDim.x) {
-                if (g.state.group[group].seen == *g.changes + 1) continue;
-                if (lane == 0) atomicCAS(a.status, 0, kStatusShare);
+                const int seen = g.state.group[group].seen, now = *g.changes + 1;
+                if (seen == now) continue;
+                if (lane == 0) atomicCAS(a.status, 0, seen == ~now ? kStatusIndex : kStatusShare);
                 const int first = max(g.first[group], 0), end = min(g.first[group + 1], a.n);
                 const int o0 = g.offsets[group], o1 = g.offsets[group + 1];
-                // of the streams' tokens alone
+                // of the streams' tokens alone: where the bounds are not the batch's, rows may be another group's
                 if (first > end || o0 < 0 || o1 > a.tokens || o0 != a.offsets[first] || o1 != a.offsets[end]) continue;
                 for (long long token = o0; token < o1; ++token) {
                     T* to = static_cast<T*>(a.out.data) + token * a.out.token_stride;

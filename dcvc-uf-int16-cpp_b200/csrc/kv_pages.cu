@@ -631,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) share_kernel(const ufb_kv_cache c
         r.token0 = o0, r.tokens = ok ? o1 - o0 : 0, r.stream0 = first, r.streams = end - first;
         r.shared = shared, r.slot = members ? b.slots[chosen] : 0;
         r.low = lowest == INT_MAX ? -1 : lowest, r.high = highest;
-        r.own = sum, r.seen = seen, r.pad[0] = r.pad[1] = 0;
+        r.own = sum, r.seen = ok ? seen : ~seen, r.pad[0] = r.pad[1] = 0;
         out.group[group] = r;
     }
 }

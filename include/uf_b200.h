@@ -614,7 +614,9 @@ int64_t ufb_kv_group_ints(int groups, int n, int64_t tokens);
  * all its streams, as far as they lie before every stream's new tokens (streams
  * that bring none, or whose extend was refused, do not count; none in a group of
  * one; status 31 for one whose extend was refused: its queries see no key; 32 for a
- * group with 2^31 - 144 own keys or more, whose results are left alone).  state[g]
+ * group with 2^31 - 144 own keys or more, whose queries see no key, and for one whose
+ * bounds are not the batch's, whose results are left alone -- by ufb_kv_attend_groups,
+ * which gives status 32 for them too).  state[g]
  * are the tokens on them.  Once a step, behind ufb_kv_extend: it holds
  * until an extend, release, fork, reorder or trim of the cache, in a replayed graph
  * or not (ufb_kv_attend_groups refuses then, status 33); what the caller writes into

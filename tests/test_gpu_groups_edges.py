@@ -1,8 +1,10 @@
 """GPU: the ends of what attention over groups takes -- sinks and windows up to the type's
-largest, groups that share has not seen as they are.
+largest, groups that share has not seen as they are, groups that it turned away.
 
 Attention is held to the tolerances of test_gpu_groups.py."""
+import ctypes as C
 import math
+import struct
 
 import pytest
 import torch
@@ -86,3 +88,60 @@ def test_attend_after_replayed_changes(ufb, dev, change):
     check_groups(ufb, cache, list(range(6)), [1] * 6, sizes[:2], 6, torch.float16)
     if change in ("refused extend", "release", "fork"):   # streams of no group here
         assert torch.equal(got, before)
+
+
+# ------------------------------------------------------ groups that are turned away ----
+
+def call_groups(cache, plan, groups, q, out, lse):
+    """ufb_kv_attend_groups into given results."""
+    heads = lambda t: C.create_string_buffer(struct.pack("@Pqqi4x", t.data_ptr(), t.stride(0), t.stride(1), t.shape[1]))  # noqa: E731
+    room = cache._L.ufb_kv_attend_workspace()
+    work = torch.zeros(room, dtype=torch.uint8, device=q.device)
+    rc = cache._L.ufb_kv_attend_groups(cache._ref, 0, plan._slots, plan._offsets, plan.n, plan.max_new, plan.tokens, 1,
+                                       heads(q), heads(out), lse.data_ptr(), 0, 0, 1, 0.125, groups._ref,
+                                       work.data_ptr(), room, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0
+
+
+@pytest.mark.parametrize("which", ["first", "offsets"])
+def test_attend_over_groups_that_are_not_the_streams(ufb, dev, which):
+    """Bounds that do not belong to the batch: attention reports them too, leaves these groups' results alone
+    and answers the others."""
+    cache, lengths, sizes = make_groups(ufb, dev, [(100, [5] * 3), (200, [5] * 2), (70, [9] * 4)], 2, 64, 16)
+    plan = cache.plan(list(range(9)), [2] * 9)
+    groups = cache.group_plan(plan, sizes)
+    q = randn(dev, (18, 4, 64), 1, torch.float16)
+    cache.share(groups)
+    want, wl = cache.attend(0, plan, q, groups=groups, lse=True)
+    getattr(groups, which)[1] -= 1   # the border between the first two
+    cache.share(groups)
+    assert ufb.device_status(0) == 32
+    out, lse = torch.full_like(want, 7.0), torch.full_like(wl, 7.0)
+    call_groups(cache, plan, groups, q, out, lse)
+    assert ufb.device_status(0) == 32
+    assert bool((out[:10] == 7).all()) and bool((lse[:10] == 7).all())
+    assert torch.equal(out[10:], want[10:]) and torch.equal(lse[10:], wl[10:])
+    getattr(groups, which)[1] += 1
+    cache.share(groups)
+    call_groups(cache, plan, groups, q, out, lse)
+    assert torch.equal(out, want) and torch.equal(lse, wl)
+    _clean(ufb)
+
+
+def test_attend_over_groups_of_too_many_keys(ufb, dev):
+    """2^31 own keys and more: status of share and of attention, queries that see no key; the others' are right."""
+    cache, lengths, sizes = make_groups(ufb, dev, [(100, [5] * 3), (70, [9] * 4)], 2, 64, 16)
+    plan = cache.plan(list(range(7)), [2] * 7)
+    groups = cache.group_plan(plan, sizes)
+    q = randn(dev, (14, 4, 64), 1, torch.float16)
+    cache.share(groups)
+    want, wl = cache.attend(0, plan, q, groups=groups, lse=True)
+    cache.lengths[:3] = 2 ** 30   # no table has that many: share alone looks at them
+    cache.share(groups)
+    assert ufb.device_status(0) == 32
+    out, lse = cache.attend(0, plan, q, groups=groups, lse=True)
+    assert ufb.device_status(0) == 32
+    assert not bool(out[:6].any()) and bool((lse[:6] == -math.inf).all())
+    assert torch.equal(out[6:], want[6:]) and torch.equal(lse[6:], wl[6:])
+    _clean(ufb)
