@@ -537,7 +537,10 @@ class KVCache:
 
         With groups (group_plan of this plan, after share has seen the cache as it is)
         the pages that a group's streams begin with in common are read once for all of
-        them: made for branches that go on by few tokens of their own.  A call that
+        them: made for branches that go on by few tokens of their own.  It is the faster
+        call for one token or a few of four branches or more when the common keys,
+        counted in every stream, are 2^16 or more and three quarters of a stream's;
+        the one without is for shorter streams and for tokens by the dozen.  A call that
         follows a change without a share is refused; where only the device can tell (a
         replayed graph that changes streams, a share that was captured and has not run)
         the status is 33 and the queries see no key."""

@@ -5,7 +5,7 @@
 // the `count` best of a stream by total, then lower beam, larger logit, lower token.
 //
 // Bound by the bytes of the logits, which are read once from memory, and for 16-bit
-// logits by the instructions of their exponentials.  Two launches.  In the first a CTA
+// logits by the loop's instructions and what its warps wait for.  Two launches.  In the first a CTA
 // takes a part of one row: it sums exp and finds the part's `count` largest logits.  With
 // nothing between the loads but arithmetic every thread keeps its largest value and where
 // it was; from these a threshold follows that at least `count` values reach and few more
@@ -727,13 +727,16 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const BeamSelectArgs a, 
 
 // Parts of a row: the number with the least time of the SM that has the most CTAs.  An SM
 // takes about as long for each value whether one CTA or four are on it (a row of 65537 floats
-// alone 10 us; the pipes bound it), so what counts is how evenly the work lies, against what
-// a part costs besides.  Measured with other numbers of parts: 64 streams x 8 beams x 32768
+// alone 10 us, 3.3 values a cycle; the exponentials alone reach 6.7, and what the warps wait for
+// besides was not told apart), so what counts is how evenly the work lies, against what a part costs
+// besides.  Measured with other numbers of parts: 64 streams x 8 beams x 32768
 // 24 us (2 parts 31, 4: 40), 48 x 8 x 50257 27.5 (2: 30, 3: 34), 32 x 16 x 131072 with a
 // fifth of the beams ended 61 (1: 69, 4: 74), 8 x 8 x 131072 18 (1: 25, 4: 19), 1 x 8 x 131072
 // 12 (1: 23, 4: 14), 16 x 4 x 50000 floats 11.4 (1: 14.4, 3: 13.2), 24 x 5 x 65537 floats 17.3
 // (3: 18.7, 6: 23.6).  No more candidates than the join's threads have at hand (17 parts of the
-// 8 rows take 15.7 us, 13 12.2).
+// 8 rows take 15.7 us, 13 12.2), unless the rows are whole: x 131072, 1 x 16 beams, 32 best 20.5 us in
+// the 2 parts that this leaves (1: 26.8, 4: 20.9), 2 x 20, 25 best 21.4 in 2 (4: 24.5), 1 x 64, 64
+// best 40 in 1 (2: 43, 4: 70); 1 x 32, 32 best 27.4 in 1, where 2 would take 24.2 (4: 26.2).
 struct Division {
     int parts, vecs;
 };

@@ -28,15 +28,17 @@
 // quarter of each tile's keys, its other weights are zeros, so all softmax warps work and
 // a thread has 32 scores where it had 128.  The sums of both sets and all copies of a row
 // become one at a piece's end.  Warps whose rows are padding, or no rows of an own tile's
-// stream, skip the softmax.
+// stream, skip the softmax.  A window leaves out tiles of common keys only; own keys behind
+// it are loaded and masked.
 //
-// Measured on 148 SMs: 64 branches x 65320 keys, 64 query heads over 8 of 128: 213 us, 640
-// TFLOP/s, 3100 cycles a tile; 8 streams x 8 branches, to 16381 keys, 4 heads of 128: 40 us
-// a layer, 2700 cycles a tile.  The products of a tile take 1300 alone, its exponentials
-// 1024, its integers 1400 from HBM.  What bounds a tile is the chain S -> softmax -> P V ->
-// S of a set (S and P share their columns; tensor memory is full), half a period each: of
-// 128 scores a thread the softmax takes 4800 cycles, of 32 still 2800, in which a warp issues
-// every 5 to 7 cycles.  The roles share the instruction caches, and code counts: 126 KB of
+// Measured on 148 SMs: 64 branches x 65320 keys, 64 query heads over 8 of 128: 213 us among
+// calls of its own kind, 640 TFLOP/s, 3100 cycles a tile (217 to 228 us with its share, 600
+// TFLOP/s); 8 streams x 8 branches, to 16381 keys, 4 heads of 128: 40 us a layer, 2700 cycles
+// a tile.  The products of a tile take 1300 alone, its exponentials 1024, its integers 1400
+// from HBM.  What bounds a tile is the chain S -> softmax -> P V -> S of a set (S and P share
+// their columns; at 128 dims tensor memory is full), half a period each: of 128 scores a
+// thread the softmax takes 4800 cycles, of 32 still 2800, in which a warp issues every 5 to 7
+// cycles.  The roles share the instruction caches, and code counts: 126 KB of
 // it ran 240 us where 108 KB take 226.  A call's start takes 6 us (division, look-ups of
 // pages, the first loads), its end 3, the join 3 to 4.
 #include "kv_attend.cuh"

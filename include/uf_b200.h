@@ -626,7 +626,10 @@ int ufb_kv_share(const ufb_kv_cache* c, const int32_t* slots, const int32_t* off
 
 /* ufb_kv_attend, which reads the pages that the streams of a group have in common
  * (ufb_kv_share) once for all of them: made for branches that go on by few tokens of
- * their own (every own key takes the work that 128 rows take). */
+ * their own (every own key takes the work that 128 rows take, also one behind the
+ * window).  It is the faster call for one token or a few of four branches or more when
+ * the common keys, counted in every stream, are 2^16 or more and three quarters of a
+ * stream's keys; ufb_kv_attend is for shorter streams and for tokens by the dozen. */
 int ufb_kv_attend_groups(const ufb_kv_cache* c, int layer, const int32_t* slots, const int32_t* offsets, int n,
                          int max_new, int64_t tokens, int dtype, const ufb_heads* q, const ufb_heads* out, float* lse,
                          int window, int sinks, int causal, float scale, const ufb_kv_groups* groups,
